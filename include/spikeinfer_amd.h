@@ -51,8 +51,8 @@ const char *spk_last_error(void);
 
 /* ABI version, bumped on any signature change and any new entry point (2: spk_decode_advance
  * draws; 3: spk_decode_attn_combine takes the partials size, spk_norm_* GEMMs; 4: spk_prefill_attn,
- * spk_qkv_rope_lif_pack_kv). */
-#define SPK_ABI_VERSION 4
+ * spk_qkv_rope_lif_pack_kv; 5: spk_tree_attn, spk_tree_masks, spk_accept_tree, spk_key_mass, spk_evict). */
+#define SPK_ABI_VERSION 5
 int spk_abi_version(void);
 
 /*
@@ -604,6 +604,128 @@ int spk_sample_ws(const void *logits, int logits_dtype, int64_t row_stride, int 
                   void *workspace, size_t workspace_bytes, int stages, void *stream);
 
 
+/* ------------------------------------------------------------------------
+ * Trees of drafted tokens, and eviction from the cache.  No counterpart in the
+ * reference, which decodes one token a step and keeps every token.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Attention of drafted tokens.  The rows of sequence n (n < N) are
+ * [row_starts[n], row_starts[n + 1]) of q and out, at most max_nodes of them; a row
+ * attends, per timestep and query head, to the context_lens[n] tokens of its
+ * sequence's cache and to the rows i of its own sequence whose bit i % 64 of word
+ * i / 64 is set in its mask:
+ *   out = sum_j w_j bits(v_j) / sum_j w_j,  w_j = exp(popcount(q & k_j) * scale)
+ * A row that sees nothing gets zeros; rows of no sequence are left as they were.
+ *
+ *   q        int32 words of (t, row, query head) at q_strides, W words contiguous
+ *   k_tree, v_tree int32 words of (t, row, kv head) at tree_strides: the rows' own
+ *            keys and values
+ *   k_cache, v_cache int32 words of (t, kv head, slot) at cache_strides; position j in
+ *            slot block_tables[n][j/bs]*bs + j%bs; blocks outside the cache read as
+ *            zero spikes
+ *   context_lens int32 [N], at most max_blocks * block_size
+ *   row_starts int32 [N + 1], not decreasing
+ *   masks    int64 [rows, mask_words] contiguous, mask_words >= ceil(max_nodes / 64)
+ *   out      out_dtype (F32/F16/BF16) [t, row, query head, channel] at out_strides,
+ *            channel stride 1
+ * Lengths, starts and masks are read on the device, so a captured call takes another
+ * batch's.  head_dim <= 128, max_nodes <= 1024 (SPK_EUNSUPPORTED beyond),
+ * scale * head_dim <= 12.  A sequence's rows do not depend on the batch around it.
+ * workspace: spk_tree_attn_workspace_bytes(...) bytes, NULL when that is 0.
+ */
+size_t spk_tree_attn_workspace_bytes(int T, int N, int Hq, int Hkv, int head_dim, int max_nodes,
+                                     int block_size, int max_blocks);
+int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const int32_t *k_tree,
+                  const int32_t *v_tree, const int64_t tree_strides[3], const int32_t *k_cache,
+                  const int32_t *v_cache, const int64_t cache_strides[3], int64_t num_slots,
+                  const int32_t *block_tables, int64_t bt_stride0, int64_t bt_stride1,
+                  const int32_t *context_lens, const int32_t *row_starts, const int64_t *masks,
+                  int mask_words, void *out, int out_dtype, const int64_t out_strides[3],
+                  int64_t rows, int N, int max_nodes, int T, int Hq, int Hkv, int head_dim,
+                  int block_size, int max_blocks, float scale, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/*
+ * Masks and depths of trees given by parents (int32 [rows], a row of the same
+ * sequence numbered from 0; below 0: none): masks[row] has the bits of the row and
+ * its ancestors, depths[row] counts the ancestors.  A parent is numbered below its
+ * children; a number that is not ends the row's chain.  Rows of no sequence are left
+ * as they were.
+ */
+int spk_tree_masks(const int32_t *parents, const int32_t *row_starts, int64_t rows, int N,
+                   int max_nodes, int64_t *masks, int mask_words, int32_t *depths, void *stream);
+
+/*
+ * The accepted path of every tree, and its words into the caches, one launch (64
+ * layers a launch).  Row 0 of a tree is its sequence's last token; from a row the walk
+ * goes to its lowest-numbered child whose token is targets[row], and ends where there
+ * is none.
+ *   tokens, targets int64 [rows], parents int32 [rows] as spk_tree_masks
+ *   path     int32 [N, max_nodes]: the path's rows, -1 behind it
+ *   count    int32 [N]: rows of the path (0 for a sequence without rows)
+ *   next_tokens int64 [N]: targets of the path's last row (-1 without rows)
+ *   layers   host array: each layer's new words (t, row, kv head) at new_strides and
+ *            caches (t, kv head, slot) at cache_strides; step i of the path goes to
+ *            position context_lens[n] + i of the block table (dropped where the table
+ *            or the cache ends); nlayers 0: the walk alone
+ * max_nodes <= 1024.
+ */
+typedef struct SpkCommitLayer {
+  const int32_t *k_new, *v_new;
+  int32_t *k_cache, *v_cache;
+} SpkCommitLayer;
+int spk_accept_tree(const int64_t *tokens, const int32_t *parents, const int64_t *targets,
+                    const int32_t *row_starts, int64_t rows, int N, int max_nodes, int32_t *path,
+                    int32_t *count, int64_t *next_tokens, const SpkCommitLayer *layers, int nlayers,
+                    const int64_t new_strides[3], const int64_t cache_strides[3], int64_t num_slots,
+                    const int32_t *block_tables, int64_t bt_stride0, int64_t bt_stride1,
+                    const int32_t *context_lens, int T, int Hkv, int head_dim, int block_size,
+                    int max_blocks, void *stream);
+
+/*
+ * Attention weight of the cached tokens.  Row i of sequence n's m rows
+ * ([row_starts[n], row_starts[n + 1]) of q, at most max_rows; row_starts NULL: row n)
+ * is the token at position seq_lens[n] - m + i and sees positions up to its own;
+ *   mass[n][g][j] = sum over t, query heads of kv head g, rows: the row's softmax
+ *                   weight of position j
+ * for j < seq_lens[n], 0 behind (j < cap); with `accumulate` the sums are added and
+ * the rest is left as it was.  Keys as spk_tree_attn reads them.  The sums' order
+ * depends on the sequence alone.  mass float at mass_strides {sequence, kv head}.
+ */
+size_t spk_key_mass_workspace_bytes(int T, int64_t rows, int Hq, int block_size, int max_blocks);
+int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const int32_t *k_cache,
+                 const int64_t cache_strides[3], int64_t num_slots, const int32_t *block_tables,
+                 int64_t bt_stride0, int64_t bt_stride1, const int32_t *seq_lens,
+                 const int32_t *row_starts, float *mass, const int64_t mass_strides[2], int64_t cap,
+                 int accumulate, int64_t rows, int N, int max_rows, int T, int Hq, int Hkv,
+                 int head_dim, int block_size, int max_blocks, float scale, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/*
+ * Eviction: per (layer, sequence, kv head) a sequence of more than `budget` tokens keeps
+ * its first `sinks`, its last `recent` and, of the others, the tokens of largest mass
+ * (equal: the lowest positions; NaN: last), `budget` in all; a shorter one keeps all.
+ * The kept words move, in order, to positions 0, 1, ... of dst_tables, or of
+ * block_tables themselves (dst_tables NULL; no other sequence may use those blocks).
+ * dst_tables' blocks must be none that the call reads.
+ *   layers   host array of each layer's caches (t, kv head, slot) at cache_strides
+ *   mass, mass_out float (layer, sequence, kv head) at their strides, cap entries each;
+ *            kept masses move likewise, 0 behind; the same array or separate ones.
+ *            Tokens at cap and behind are dropped.
+ *   keep     int32 [nlayers, N, Hkv, budget]: the kept positions, -1 behind
+ *   new_lens int32 [N]: min(seq_lens, budget)
+ */
+typedef struct SpkCacheLayer {
+  int32_t *k, *v;
+} SpkCacheLayer;
+int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_strides[3],
+              int64_t num_slots, const float *mass, const int64_t mass_strides[3], float *mass_out,
+              const int64_t mass_out_strides[3], int64_t cap, const int32_t *block_tables,
+              int64_t bt_stride0, int64_t bt_stride1, int max_blocks, const int32_t *dst_tables,
+              int64_t dt_stride0, int64_t dt_stride1, int max_dst_blocks, const int32_t *seq_lens,
+              int32_t *new_lens, int32_t *keep, int budget, int sinks, int recent, int T, int N,
+              int Hkv, int head_dim, int block_size, void *stream);
 
 #ifdef __cplusplus
 }

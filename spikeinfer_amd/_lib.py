@@ -29,7 +29,7 @@ _DTYPE_CODES = {
     torch.int32: SPK_I32,
 }
 
-ABI_VERSION = 4  # SPK_ABI_VERSION
+ABI_VERSION = 5  # SPK_ABI_VERSION
 DECODE_ATTN_SCRATCH_BYTES = 16 << 20  # SPK_DECODE_ATTN_SCRATCH_BYTES
 
 _i64p = ctypes.POINTER(ctypes.c_int64)
@@ -63,6 +63,13 @@ _CHUNK_FORMAT = struct.Struct("<qQqiiii")  # SpkPrefillChunk, field by field (no
 def pack_prefill_chunk(start, table, table_stride, n_table, q_len, ctx) -> bytes:
     """The bytes of one SpkPrefillChunk (``table`` 0: contiguous keys)."""
     return _CHUNK_FORMAT.pack(start, table, table_stride, n_table, q_len, ctx, 0)
+
+
+def pack_pointers(layers) -> bytes:
+    """The bytes of an SpkCommitLayer or SpkCacheLayer array: the tensors' addresses
+    in order, layer by layer."""
+    flat = [t.data_ptr() for layer in layers for t in layer]
+    return struct.pack(f"<{len(flat)}Q", *flat)
 
 
 # name -> (restype, argtypes); mirrors include/spikeinfer_amd.h
@@ -130,6 +137,21 @@ _SIGNATURES = {
     "spk_sample_ws": (_i32, [
         _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64,
         _vp, _vp, _vp, _sz, _i32, _vp]),
+    "spk_tree_attn_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "spk_tree_attn": (_i32, [
+        _vp, _i64p, _vp, _vp, _i64p, _vp, _vp, _i64p, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _vp,
+        _i32, _i64p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "spk_tree_masks": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _vp]),
+    "spk_accept_tree": (_i32, [
+        _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_char_p, _i32, _i64p, _i64p, _i64,
+        _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "spk_key_mass_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
+    "spk_key_mass": (_i32, [
+        _vp, _i64p, _vp, _i64p, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64p, _i64, _i32, _i64, _i32,
+        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),
+    "spk_evict": (_i32, [
+        ctypes.c_char_p, _i32, _i64p, _i64, _vp, _i64p, _vp, _i64p, _i64, _vp, _i64, _i64, _i32, _vp,
+        _i64, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -237,6 +259,16 @@ def stream_of(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(name: str, dev: torch.device, *args) -> int:
+    """Calls entry point ``name`` on ``dev`` and its current stream (the last
+    argument), whatever the current device is."""
+    fn = getattr(load(), name)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return fn(*args, stream_of(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, stream_of(dev))
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -3,8 +3,16 @@
 The operators launch HIP kernels on gfx950 through the C ABI in
 include/spikeinfer_amd.h and have no CPU fallback.  The ``*_ref`` /
 ``*_cpu`` names (reference_paths.py) are the reference's eager-torch paths,
-restated; the operators never call them.
+restated; the operators never call them.  draft_tree.py and eviction.py go beyond
+the reference: drafted trees, and a cache kept within a budget.
 """
+from .draft_tree import (
+    accept_draft_tree,
+    draft_tree_masks,
+    paged_spike_attn_tree,
+    tree_attn_workspace_bytes,
+)
+from .eviction import evict_cache, key_mass_workspace_bytes, paged_spike_attn_key_mass
 from .lif import lif_multistep, lif_pack_write, lif_pack_write_sites, validate_thresholds
 from .packing import (
     BITS_PER_WORD,
@@ -52,4 +60,11 @@ __all__ = [
     "gather_kv_unpacked_pair",
     "paged_spike_attn_decode_partials",
     "combine_partitions",
+    "paged_spike_attn_tree",
+    "tree_attn_workspace_bytes",
+    "draft_tree_masks",
+    "accept_draft_tree",
+    "paged_spike_attn_key_mass",
+    "key_mass_workspace_bytes",
+    "evict_cache",
 ]
