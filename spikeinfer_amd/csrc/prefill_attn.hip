@@ -50,28 +50,18 @@
 // lookups under this one's products: 175).  Against unpack + SDPA (one layer, LIF
 // included, bf16): that prompt 8,693 -> 142 us; 32 decodes with chunks of 509 and
 // 472 behind 1,024 and 923 cached tokens 1,035 -> 59 us.
-#include <cmath>
-#include <cstring>
 #include <type_traits>
 
-#include "common.hpp"
+#include "spike_tiles.hpp"
 
 namespace spk {
 namespace prefill {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
-
-#define SPK_LDS __attribute__((address_space(3)))
+using namespace tiles;
 
 constexpr int kWaves = 4;
 constexpr int kKeys = 32;       // keys per tile
 constexpr int kMaxChunks = 32;  // chunks per launch (kernel arguments)
-constexpr int kTab = 129;       // weights of scores 0..head_dim (<= 128)
 
 struct Chunk {
   int64_t start;         // first batch row
@@ -96,47 +86,6 @@ struct Params {
   uint32_t tab[kTab];
   Chunk c[kMaxChunks];
 };
-
-// The value of x in the lane whose number differs by J (1, 2, 4, 8 or 16).
-template <int J>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
-  const int v = static_cast<int>(x);
-  if constexpr (J == 1) return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
-  else if constexpr (J == 2) return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
-  else if constexpr (J == 8)  // rotation by 8 within a row of 16
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false));
-  else return static_cast<uint32_t>(__builtin_amdgcn_ds_swizzle(v, (J << 10) | 0x1f));
-}
-
-// One step of the 32 x 32 bit transpose within each 32-lane half (lane = row,
-// bit = column): lanes without bit J trade their J-columns for the partner's
-// others.
-template <int J>
-__device__ __forceinline__ uint32_t transpose_step(uint32_t x, int lane) {
-  constexpr uint32_t m = J == 16 ? 0x0000ffffu : J == 8 ? 0x00ff00ffu : J == 4 ? 0x0f0f0f0fu
-                         : J == 2 ? 0x33333333u : 0x55555555u;
-  const uint32_t y = lane_xor<J>(x);
-  const bool up = lane & J;
-  const uint32_t keep = up ? ~m : m;
-  const uint32_t r = __builtin_amdgcn_alignbit(y, y, up ? J : 32 - J);  // rotate right
-  return (x & keep) | (r & ~keep);
-}
-
-__device__ __forceinline__ uint32_t transpose32(uint32_t x, int lane) {
-  x = transpose_step<16>(x, lane);
-  x = transpose_step<8>(x, lane);
-  x = transpose_step<4>(x, lane);
-  x = transpose_step<2>(x, lane);
-  return transpose_step<1>(x, lane);
-}
-
-// 32 bits as 32 fp4 values of 0.5: nibble n of word i is bit 4n + i.
-__device__ __forceinline__ v8i fp4_bits(uint32_t w) {
-  v8i r = {};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = static_cast<int>((w >> i) & 0x11111111u);
-  return r;
-}
 
 // QT row tiles of 32 rows a workgroup; NC = channel tiles of 32 (ceil(D / 32)).
 // F32: the outputs are fp32.
@@ -446,27 +395,6 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2))
   }
 }
 
-// (hi, lo) f16 pairs of exp(s * scale) * 2^15 / exp(D * scale), s = 0..D.
-static void build_table(float scale, int D, uint32_t *tab) {
-  static thread_local float last_scale = -1.f;
-  static thread_local int last_d = 0;
-  static thread_local uint32_t last[kTab];
-  if (scale != last_scale || D != last_d) {
-    for (int s = 0; s <= D; ++s) {
-      const double w = std::ldexp(std::exp((s - D) * static_cast<double>(scale)), 15);
-      const _Float16 hi = static_cast<_Float16>(w);
-      const _Float16 lo = static_cast<_Float16>(w - static_cast<double>(hi));
-      uint16_t a, b;
-      std::memcpy(&a, &hi, 2);
-      std::memcpy(&b, &lo, 2);
-      last[s] = a | (static_cast<uint32_t>(b) << 16);
-    }
-    last_scale = scale;
-    last_d = D;
-  }
-  std::memcpy(tab, last, sizeof(uint32_t) * (D + 1));
-}
-
 // Row tiles a workgroup takes of the `qt` asked for: as many as its sums leave
 // registers for (fp32 outputs have two accumulators a tile).
 constexpr int row_tiles(int qt, int NC, bool f32) {
@@ -535,7 +463,7 @@ extern "C" int spk_prefill_attn(const int32_t *q, const int64_t q_strides[3], co
   p.bs_log2 = ilog2(block_size);
   // ceil(2^32 / nrep): its product with r is off by less than r * nrep <= 2^32
   p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + nrep - 1) / nrep);
-  prefill::build_table(scale, head_dim, p.tab);
+  tiles::build_table(scale, head_dim, p.tab);
   // Row tiles per workgroup: four share a key tile's V operands; fewer while
   // that leaves under two workgroups a CU, and where their sums would not fit
   // the registers (head_dim 128, 2,000 tokens: one 60 us, two 77).  The sums do
