@@ -5,22 +5,29 @@
 //   out = sum_j w_j bits(v_j) / sum_j w_j,  w_j = exp(popc(q & k_j) * scale).
 //
 // MI355X design, on the tiles of the prefill attention (spike_tiles.hpp):
-//   * A workgroup owns 32 * QT rows of one (t, kv head): row r = node r / n_rep, query
-//     head r % n_rep.  Its four waves take the 32-key tiles round-robin: first the
-//     context's, then the tree's own, which start on a tile of their own, so that a
-//     row's mask word is the tile's.
-//   * Scores, weights and values as there: one fp4 product per 64 channels leaves the
-//     score's table offset in the accumulator's bits, the weight is a look-up, and f16
-//     products over two keys a register add bits(v) times the weight.  bf16 outputs take
-//     the weights' 11-bit high halves alone (each off by at most 2^-11, and the
-//     denominator sums the same halves, where an output's own rounding is 2^-8): half the
-//     products.  fp32 and fp16 outputs take both halves, to accumulators of their own,
-//     added and divided in fp64.
-//   * The context is cut into parts of kPart tokens, the tree's tiles belonging to the
-//     last; a part's sums are added over the waves, and parts in their order.  One
-//     workgroup takes the parts one after the other, or, where rows are few, a workgroup
-//     a part leaves its sums in the workspace and a second launch adds them: the same
-//     additions, so a sequence's outputs depend neither on that choice nor on the batch.
+//   * Rows: node r / n_rep, query head r % n_rep of one (t, kv head), in tiles of 32.
+//     Keys: tiles of 32, the context's first; the tree's own start on a tile of their
+//     own, so that a row's mask word is the tile's.
+//   * Scores as there: one fp4 product per 64 channels leaves the score's table offset in
+//     the accumulator's bits, and the weight is a look-up.
+//   * Values: f16 products over two keys a register.  fp32 and fp16 outputs take the
+//     weights' two halves, exact to 2^-23, in two products.  bf16
+//     outputs take the 11-bit high halves alone (each off by at most 2^-11, and the
+//     denominator sums the same halves, where the output's own rounding is 2^-8): half the
+//     products.  There a v bit becomes an operand in place, as one of f16's exponent bits
+//     (2^-14, 2^-13, 2^-11 or 2^-7 by the key's number % 4), and four tables of weights
+//     hold what makes the products equal again: one `and` a register instead of a
+//     multiplication more.
+//   * Four waves a workgroup share the key tiles' operands through LDS: each prepares one of
+//     four tiles, two buffers of them so that one barrier a step does.  A sequence of more
+//     than 64 rows has a wave a row tile and all keys; of 33 to 64 rows two waves a row tile,
+//     the even and the odd tiles; below, four.
+//   * The context is cut into parts of kPartTiles tiles (more beyond kMaxParts parts), the
+//     tree's tiles belonging to the last.  A wave adds a part's tiles in their order, then the
+//     parts, then come the waves of a row tile.  Where workgroups are many each takes all
+//     parts (SEQ), else a workgroup a part leaves its waves' sums in the workspace and a
+//     second launch adds them: the same additions.  So the sums depend on the sequence alone,
+//     its length and its rows, not on the batch around it.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -31,11 +38,11 @@ namespace tree {
 using namespace tiles;
 
 constexpr int kWaves = 4;
-constexpr int kKeys = 32;              // keys per tile
-constexpr int kPart = 4096;            // tokens per part
-constexpr int kPartTiles = kPart / kKeys;
+constexpr int kKeys = 32;          // keys per tile
+constexpr int kPartTiles = 32;     // tiles per part, up to kMaxParts of them
+constexpr int kMaxParts = 16;
 constexpr int kMaxNodes = 1024;
-static_assert(kPartTiles % kWaves == 0, "a wave's tiles go on across parts");
+constexpr int kTabStride = kTab + 3;
 
 struct Params {
   const uint32_t *q;        // words of (t, row, query head)
@@ -56,16 +63,17 @@ struct Params {
   int64_t rows;
   uint32_t rep_mul;         // floor(r / nrep) = r * rep_mul >> 32 for every row
   int units, Hkv, nrep, D, W, bs_log2, max_blocks, max_nodes;
-  int groups;               // row groups of a sequence (grid.x = groups * parts * units)
-  int parts;                // workgroups along the context: 1, or a part each
-  char *ws;                 // with parts > 1: sums of (sequence, group, part, unit)
+  int groups;               // workgroups along the rows of a sequence
+  int parts;                // along its context: 1, or its most parts
+  float *ws;                // with parts > 1: sums of (sequence, unit, group, part, wave)
   uint32_t tab[kTab];
 };
 
 // A sequence as the kernels take it: its rows and cached tokens, clamped to the buffers.
 struct Seq {
   int64_t first;
-  int nodes, ctx, ctiles, parts;
+  int nodes, ctx, ctiles, end;  // end: tiles of the context and of the tree
+  int ptiles, parts;            // tiles of a part, parts
 };
 
 __device__ __forceinline__ Seq sequence(const Params &p, int n) {
@@ -75,148 +83,83 @@ __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   s.nodes = static_cast<int>(min<int64_t>(end - s.first, p.max_nodes));
   s.ctx = min(max(p.lens[n], 0), p.max_blocks << p.bs_log2);
   s.ctiles = (s.ctx + kKeys - 1) / kKeys;
-  s.parts = max(1, (s.ctiles + kPartTiles - 1) / kPartTiles);
+  s.end = s.ctiles + (s.nodes + kKeys - 1) / kKeys;
+  s.ptiles = kPartTiles;
+  while (s.ptiles * kMaxParts < s.ctiles) s.ptiles <<= 1;
+  s.parts = max(1, (s.ctiles + s.ptiles - 1) / s.ptiles);
   return s;
 }
 
-// What a workgroup's threads finish: kTiles of its QT x NC output tiles a round, a wave a
-// tile, or, of a tile in two parts (fp32), a wave a half.
-template <int QT, int NC, bool F32>
-struct Shape {
-  static constexpr int kUnits = QT * NC;
-  static constexpr int kParts = F32 ? 2 : 1;
-  static constexpr int kTiles = kWaves / kParts;
-  static constexpr int kRounds = (kUnits + kTiles - 1) / kTiles;
-  static constexpr int kVals = 16 / kParts;  // values a lane and round
-  typedef std::conditional_t<F32, double, float> Sum;
-  // one (sequence, group, part, unit) of the workspace: values as the lanes hold them,
-  // then the rows' denominators
-  static constexpr int kSums = kRounds * kVals * kWaves * 64;
-  static constexpr size_t kBytes = sizeof(Sum) * (kSums + 32 * QT);
-};
+// The same for a table of `tokens` (host): most parts of a sequence.
+inline int most_parts(int64_t tokens) {
+  const int64_t tiles = (tokens + kKeys - 1) / kKeys;
+  return tiles <= kPartTiles ? 1 : static_cast<int>(tiles < kPartTiles * kMaxParts ? (tiles + kPartTiles - 1) / kPartTiles : kMaxParts);
+}
 
-// Rows r0.. of a sequence from their sums: tot as Shape has them, dens in LDS.
-template <int QT, int NC, bool F32>
-__device__ __forceinline__ void store_rows(const Params &p, const Seq &s, int unit, int r0,
-                                           const typename Shape<QT, NC, F32>::Sum (
-                                               &tot)[Shape<QT, NC, F32>::kRounds][Shape<QT, NC, F32>::kVals],
-                                           const typename Shape<QT, NC, F32>::Sum *dens) {
-  typedef Shape<QT, NC, F32> S;
-  typedef typename S::Sum Sum;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int kvh = unit % p.Hkv, t = unit / p.Hkv, rows = s.nodes * p.nrep;
+__device__ __forceinline__ int node_of(const Params &p, int r) {
+  return p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
+}
+
+// Weight tables in LDS at offset 0: one of (hi, lo) pairs, or four of high halves whose
+// entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's.
+template <bool F32> constexpr int kTables = F32 ? 1 : 4;
+template <bool F32>
+__device__ __forceinline__ void fill_tables(const Params &p, uint32_t *tab, int tid) {
+  if (tid > p.D) return;
+  const uint32_t w = p.tab[tid];
+  tab[tid] = w;
+  if constexpr (!F32) {
+    const _Float16 h = __builtin_bit_cast(_Float16, static_cast<uint16_t>(w));
 #pragma unroll
-  for (int rd = 0; rd < S::kRounds; ++rd) {
-    const int x = rd * S::kTiles + wave / S::kParts;
-    const int i = x / NC, c = x - i * NC, r = r0 + 32 * i + col;
-    if (x >= S::kUnits || r >= rows) continue;
-    const Sum den = dens[32 * i + col];
-    const Sum inv = den > 0 ? Sum(1) / den : Sum(0);  // (a row that sees nothing: zeros)
-    const int node = p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
-    const int64_t row = t * p.os0 + (s.first + node) * p.os1 + (kvh * p.nrep + r - node * p.nrep) * p.os2;
-    const int g0 = F32 ? wave % S::kParts * 2 : 0;  // first of the wave's 4-channel groups
-    constexpr int kGroups = S::kVals / 4;
-    if (p.out_vec) {  // D % 4 == 0: four channels lie in or out together
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        const int ch = 32 * c + 8 * (g0 + k) + 4 * half;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(tot[rd][4 * k + e] * inv);
-        if (ch >= p.D) continue;
-        if (p.out_dtype == SPK_F32) {
-          *reinterpret_cast<v4f *>(static_cast<float *>(p.out) + row + ch) = v4f{o[0], o[1], o[2], o[3]};
-          continue;
-        }
-        uint32_t w2[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint16_t x0, x1;
-          if (p.out_dtype == SPK_BF16) {
-            x0 = f32_to_bf16_bits(o[2 * e]);
-            x1 = f32_to_bf16_bits(o[2 * e + 1]);
-          } else {
-            x0 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(o[2 * e]));
-            x1 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(o[2 * e + 1]));
-          }
-          w2[e] = x0 | (static_cast<uint32_t>(x1) << 16);
-        }
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + row + ch) = make_uint2(w2[0], w2[1]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < S::kVals; ++j) {
-        const int ch = 32 * c + 8 * (g0 + (j >> 2)) + 4 * half + (j & 3);
-        if (ch < p.D) store_f32_as(p.out, row + ch, p.out_dtype, static_cast<float>(tot[rd][j] * inv));
-      }
-    }
+    for (int i = 1; i < 4; ++i)
+      tab[i * kTabStride + tid] =
+          __builtin_bit_cast(uint16_t, static_cast<_Float16>(h * static_cast<_Float16>(i == 1 ? 0.5f : i == 2 ? 0.125f : 0.0078125f)));
   }
 }
 
-// QT row tiles of 32 rows a workgroup; NC = channel tiles of 32 (ceil(D / 32)).
-// F32: weights of two halves (fp32 and fp16 outputs).
-template <int QT, int NC, bool F32>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void tree_attn_kernel(Params p) {
-  typedef Shape<QT, NC, F32> S;
-  typedef typename S::Sum Sum;
-  constexpr int NK = (NC + 1) / 2;  // 64-channel score steps
-  constexpr int kParts = S::kParts;
-  struct Smem {
-    uint32_t tab[kTab + 3];  // first: a score's accumulator is its entry's LDS address
-    Sum dens[32 * QT];
-    float lsum[QT][kParts][kWaves][64];
-    float red[S::kUnits * kParts < kWaves ? S::kUnits * kParts : kWaves][kWaves][16][64];
-  };
-  __shared__ Smem sm;
-  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int half = lane >> 5, col = lane & 31;
-  const int n = blockIdx.y;
-  const int unit = blockIdx.x % p.units, rest = blockIdx.x / p.units;
-  const int part = rest % p.parts, group = rest / p.parts;
-  const int kvh = unit % p.Hkv, t = unit / p.Hkv;
-  const Seq s = sequence(p, n);
-  const int rows = s.nodes * p.nrep, r0 = group * 32 * QT;
-  if (r0 >= rows || part >= s.parts) return;
-  const int nq = min(QT, (rows - r0 + 31) >> 5);
-
-  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
-
-  // Each lane's rows (clamped to the last): query words as score operands, mask words.
-  v8i qop[QT][NK];
-  const uint32_t *mrow[QT];
+// Query words of row `r` (score operands of its tile).
+template <int NK>
+__device__ __forceinline__ void load_query(const Params &p, const Seq &s, int t, int kvh, int r, int half,
+                                           v8i (&qop)[NK]) {
+  const int node = node_of(p, r), h = r - node * p.nrep;
+  const uint32_t *qp = p.q + t * p.qs0 + (s.first + node) * p.qs1 + (kvh * p.nrep + h) * p.qs2;
 #pragma unroll
-  for (int i = 0; i < QT; ++i) {
-    const int r = min(r0 + 32 * i + col, rows - 1);
-    const int node = p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
-    const int h = r - node * p.nrep;
-    mrow[i] = p.masks + (s.first + node) * p.mask_words;
-    const uint32_t *qp = p.q + t * p.qs0 + (s.first + node) * p.qs1 + (kvh * p.nrep + h) * p.qs2;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) {
-      const int w = 2 * k + half;
-      qop[i][k] = fp4_bits(w < p.W ? qp[w] : 0u);
-    }
+  for (int k = 0; k < NK; ++k) {
+    const int w = 2 * k + half;
+    qop[k] = fp4_bits(w < p.W ? qp[w] : 0u);
   }
+}
 
-  const int32_t *table = p.bt + n * p.bts0;
-  const int bs_mask = (1 << p.bs_log2) - 1;
-  const uint32_t nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
-  const uint32_t *kbase = p.k + t * p.ks0 + kvh * p.ks1, *vbase = p.v + t * p.ks0 + kvh * p.ks1;
-  const uint32_t *ktree = p.kt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
-  const uint32_t *vtree = p.vt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
-  const int last_block = max(s.ctx - 1, 0) >> p.bs_log2;
-  // Loads are unconditional (indices clamped into range, the value dropped where a key
-  // is none: zero spikes), so that the wave waits for none of them before its use.
-  auto block_of = [&](int kt) -> uint32_t {
+// A lane's key words of tile kt (lane l: key l % 32, words 2k + l / 32).  Loads are
+// unconditional (indices clamped into range, the value dropped where a key is none:
+// zero spikes), so that the wave waits for none of them before its use.
+template <int NK>
+struct Keys {
+  const Params &p;
+  const Seq &s;
+  const int32_t *table;
+  const uint32_t *kbase, *vbase, *ktree, *vtree;
+  uint32_t nblocks;
+  int last_block, half, col;
+
+  __device__ __forceinline__ Keys(const Params &p, const Seq &s, int n, int t, int kvh, int half, int col)
+      : p(p), s(s), half(half), col(col) {
+    table = p.bt + n * p.bts0;
+    kbase = p.k + t * p.ks0 + kvh * p.ks1;
+    vbase = p.v + t * p.ks0 + kvh * p.ks1;
+    ktree = p.kt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
+    vtree = p.vt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
+    nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
+    last_block = max(s.ctx - 1, 0) >> p.bs_log2;
+  }
+  __device__ __forceinline__ uint32_t block_of(int kt) const {
     return static_cast<uint32_t>(table[min((kt * kKeys + col) >> p.bs_log2, last_block) * p.bts1]);
-  };
-  auto load = [&](int kt, uint32_t phys, uint32_t (&kw)[NK], uint32_t (&vw)[NK], bool &ok) {
+  }
+  __device__ __forceinline__ void load(int kt, uint32_t phys, uint32_t (&kw)[NK], uint32_t (&vw)[NK], bool &ok) const {
     const bool own = kt >= s.ctiles;
     const int j = (own ? kt - s.ctiles : kt) * kKeys + col;
     ok = own ? j < s.nodes : j < s.ctx && phys < nblocks;
-    const int64_t slot = (static_cast<int64_t>(phys) << p.bs_log2) | (j & bs_mask);
+    const int64_t slot = (static_cast<int64_t>(phys) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1));
     const int64_t at = ok ? (own ? j * p.ts1 : slot * p.ks2) : 0;
     const uint32_t *kp = (own ? ktree : kbase) + at, *vp = (own ? vtree : vbase) + at;
 #pragma unroll
@@ -225,285 +168,432 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2))
       kw[k] = kp[w];
       vw[k] = vp[w];
     }
-  };
-  auto keep = [&](uint32_t x, int k, bool ok) { return ok && 2 * k + half < p.W ? x : 0u; };
-
-  Sum tot[S::kRounds][S::kVals], dtot = 0;
+  }
+  // Loaded words as a tile's shared operands: keys as fp4, and per channel tile a lane's
+  // channel l % 32 as bits of its keys: bit 8 * (e >> 2) + (e & 3) for its e-th key,
+  // e < 16, which is key 8 * (e >> 2) + 4 * (l / 32) + (e & 3) of the tile.
+  __device__ __forceinline__ void operands(const uint32_t (&kw)[NK], const uint32_t (&vw)[NK], bool ok, int lane,
+                                           v8i (&kop)[NK], uint32_t (&vt)[2 * NK]) const {
 #pragma unroll
-  for (int rd = 0; rd < S::kRounds; ++rd)
-#pragma unroll
-    for (int j = 0; j < S::kVals; ++j) tot[rd][j] = 0;
-  __syncthreads();
-
-  const int p0 = part, p1 = p.parts > 1 ? part + 1 : s.parts;
-  const int end = s.ctiles + (s.nodes + kKeys - 1) / kKeys;  // all tiles of the sequence
-  uint32_t kw[NK], vw[NK];
-  bool ok;
-  int kt = p0 * kPartTiles + wave;
-  load(kt, block_of(kt), kw, vw, ok);
-  uint32_t pnext = block_of(kt + kWaves);
-  for (int pt = p0; pt < p1; ++pt) {
-    v16f acc[QT][NC * kParts];
-    float l[QT][kParts];
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-#pragma unroll
-      for (int q = 0; q < kParts; ++q) l[i][q] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC * kParts; ++c) acc[i][c] = v16f{};
+    for (int k = 0; k < NK; ++k) {
+      const bool in = ok && 2 * k + half < p.W;
+      kop[k] = fp4_bits(in ? kw[k] : 0u);
+      const uint32_t x = transpose32(in ? vw[k] : 0u, lane);
+      const auto sw = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+      vt[2 * k] = sw[0] >> (4 * half);
+      vt[2 * k + 1] = sw[1] >> (4 * half);
     }
-    const int stop = pt + 1 < s.parts ? (pt + 1) * kPartTiles : end;
-    for (; kt < stop; kt += kWaves) {
-      // Operands of this tile; the next tile's words and the block of the one
-      // after are requested before they are used.
-      v8i kop[NK];
-      uint32_t vt[2 * NK];
+  }
+};
+
+// Keys of tile kt that a row sees, as bits of the tile (`word`: the row's mask words).
+__device__ __forceinline__ uint32_t seen(const Seq &s, int kt, const uint32_t *word, int half) {
+  const int nt = kt - s.ctiles, left = nt < 0 ? s.ctx - kt * kKeys : s.nodes - nt * kKeys;
+  uint32_t see = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
+  if (nt >= 0 && left > 0) see &= word[nt];
+  return see >> (4 * half);
+}
+
+// Products' value operands of a channel tile: register i of operand g pairs the lane's keys
+// 4g + i and 4g + i + 8, sixteen bits apart in vt.
+template <bool F32>
+__device__ __forceinline__ void expand(uint32_t vt, v8h (&vop)[2]) {
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        kop[k] = fp4_bits(keep(kw[k], k, ok));
-        const uint32_t x = transpose32(keep(vw[k], k, ok), lane);
-        // Both halves of the wave need every channel tile: lanes l and l + 32 take
-        // keys 4 * (l / 32) + 0..3 of each eight.
-        const auto sw = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        vt[2 * k] = sw[0] >> (4 * half);
-        vt[2 * k + 1] = sw[1] >> (4 * half);
+  for (int g = 0; g < 2; ++g) {
+    v4u x;
+    // fp32: bit b at place i <= 3 becomes 1.0 by a 24-bit product with 0x3c00 >> i; else it
+    // moves to bit 10 + i
+    const uint32_t b = F32 ? (g ? vt >> 8 : vt) : (g ? vt << 2 : vt << 10);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = F32 ? __umul24(b & (0x00010001u << i), 0x3c00u >> i) : b & (0x04000400u << i);
+    vop[g] = __builtin_bit_cast(v8h, x);
+  }
+}
+
+template <int NK>
+__device__ __forceinline__ v16f scores(const v8i (&kop)[NK], const v8i (&qop)[NK]) {
+  v16f a = {};
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+    a = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kop[k], qop[k], a, 4, 4, 0, 55, 0, 54);
+  return a;
+}
+
+template <bool F32>
+__device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint32_t at = tab0 + (F32 ? 0 : 4 * kTabStride * (e & 3)) + __float_as_uint(a[e]);
+    w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
+  }
+}
+
+// Adds a tile's weighted values to acc and its weights to l.
+template <int NC, bool F32, bool MASKED>
+__device__ __forceinline__ void products(const uint32_t (&w)[16], uint32_t see, const v8h (&vop)[NC][2],
+                                         v16f (&acc)[NC], float (&l)[4]) {
+  constexpr int kParts = F32 ? 2 : 1;
+  auto weight = [&](int e) {  // the e-th of the lane's sixteen
+    if constexpr (MASKED)
+      return w[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
+    else return w[e];
+  };
+  // fp32: the sixteen weights first, then added (a long dot2 chain loses bits that count)
+  float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    v4u x[kParts];  // the weights' halves, two keys a register
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t y0 = weight(4 * g + e), y1 = weight(4 * g + e + 8);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) {
+        const uint32_t y = __builtin_amdgcn_perm(y1, y0, q ? 0x07060302u : 0x05040100u);
+        if constexpr (F32) {
+          float &dq = d[2 * (e & 1) + q];
+          dq = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, y), v2h{1, 1}, dq, false);
+        } else {
+          const _Float16 one = static_cast<_Float16>(e == 0 ? 0x1p-14f : e == 1 ? 0x1p-13f : e == 2 ? 0x1p-11f : 0x1p-7f);
+          l[e] = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, y), v2h{one, one}, l[e], false);
+        }
+        x[q][e] = y;
       }
-      load(kt + kWaves, pnext, kw, vw, ok);
-      pnext = block_of(kt + 2 * kWaves);
-      // The lane's n-th key of the tile is 8 * (n >> 2) + 4 * half + (n & 3), n < 16.
-      // Register e of the operands pairs keys e and e + 8, sixteen bits apart in vt; a
-      // bit b at place s <= 3 becomes f16 1.0 by a 24-bit product with 0x3c00 >> s.
-      v8h vop[NC][2];
+    }
+#pragma unroll
+    for (int q = 0; q < kParts; ++q)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint32_t b = g ? vt[c] >> 8 : vt[c];
-          v4u x;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = __umul24(b & (0x00010001u << i), 0x3c00u >> i);
-          vop[c][g] = __builtin_bit_cast(v8h, x);
-        }
-      auto scores = [&](int i) {
-        v16f a = {};
-#pragma unroll
-        for (int k = 0; k < NK; ++k)
-          a = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kop[k], qop[i][k], a, 4, 4, 0, 55, 0, 54);
-        return a;
-      };
-      auto lookup = [&](const v16f &a, uint32_t (&w)[16]) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t at = tab0 + __float_as_uint(a[e]);
-          w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
-        }
-      };
-      auto products = [&](int i, const uint32_t (&w)[16], uint32_t see, auto masked) {
-        auto weight = [&](int e) {  // the e-th of the lane's sixteen
-          if constexpr (decltype(masked)::value)
-            return w[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
-          else return w[e];
-        };
-        float d[4] = {0.f, 0.f, 0.f, 0.f};  // (a chain of dot2 on one register waits for itself)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          v4u x[kParts];  // the weights' halves, two keys a register
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t y0 = weight(4 * g + e), y1 = weight(4 * g + e + 8);
-#pragma unroll
-            for (int q = 0; q < kParts; ++q) {
-              const uint32_t y = __builtin_amdgcn_perm(y1, y0, q ? 0x07060302u : 0x05040100u);
-              float &dq = d[kParts == 2 ? 2 * (e & 1) + q : e];
-              dq = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, y), v2h{1, 1}, dq, false);
-              x[q][e] = y;
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int q = 0; q < kParts; ++q) {
-              v16f &a = acc[i][kParts * c + q];
-              a = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, x[q]), a, 0, 0, 0);
-            }
-        }
-        if constexpr (kParts == 2) {
-          l[i][0] += d[0] + d[2];
-          l[i][1] += d[1] + d[3];
-        } else {
-          l[i][0] += (d[0] + d[1]) + (d[2] + d[3]);
-        }
-      };
-      if (kt * kKeys + kKeys <= s.ctx && nq == QT) {
-        // The next row tile's scores are computed and looked up under this one's
-        // products.
-        uint32_t w[2][16];
-        lookup(scores(0), w[0]);
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-          if (i + 1 < QT) lookup(scores(i + 1), w[(i + 1) & 1]);
-          products(i, w[i & 1], 0u, std::false_type{});
-          __builtin_amdgcn_sched_barrier(0);  // row tile by row tile (several at a time spill)
-        }
-      } else {
-        const int nt = kt - s.ctiles;  // the tree's tile, or the context's last
-#pragma unroll
-        for (int i = 0; i < QT; ++i) {
-          if (i >= nq) continue;
-          const int left = (nt < 0 ? s.ctx - kt * kKeys : s.nodes - nt * kKeys);
-          uint32_t see = left >= 32 ? ~0u : (1u << left) - 1;
-          if (nt >= 0) see &= mrow[i][nt];
-          uint32_t w[16];
-          lookup(scores(i), w);
-          products(i, w, see >> (4 * half), std::true_type{});
-        }
-      }
-    }
+        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, x[q]), acc[c], 0, 0, 0);
+  }
+  if constexpr (F32) {
+    l[0] += d[0] + d[2];
+    l[1] += d[1] + d[3];
+  }
+}
 
-    // The part's sums over the waves, in wave order, added to those of the parts before.
+// A lane's denominator, of its own keys.
+__device__ __forceinline__ float lane_sum(const float (&l)[4]) { return (l[0] + l[1]) + (l[2] + l[3]); }
+
+// Rows of a tile from their sums: kVals of the lane's values of channel tile c (four
+// channels 8 * (g0 + k) + 4 * half .. for each k), divided by the row's denominator.
+template <bool F32, int kVals>
+__device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, int kvh, int r, int c, int g0, int half,
+                                          const float (&val)[kVals], float den) {
+  const float inv = den > 0.f ? 1.f / den : 0.f;  // (a row that sees nothing: zeros)
+  const int node = node_of(p, r);
+  const int64_t row = t * p.os0 + (s.first + node) * p.os1 + (kvh * p.nrep + r - node * p.nrep) * p.os2;
+  if (p.out_vec) {  // D % 4 == 0: four channels lie in or out together
 #pragma unroll
-    for (int i = 0; i < QT; ++i)
+    for (int k = 0; k < kVals / 4; ++k) {
+      const int ch = 32 * c + 8 * (g0 + k) + 4 * half;
+      float o[4];
 #pragma unroll
-      for (int q = 0; q < kParts; ++q) sm.lsum[i][q][wave][lane] = l[i][q];
+      for (int e = 0; e < 4; ++e) o[e] = val[4 * k + e] * inv;
+      if (ch >= p.D) continue;
+      if (F32 && p.out_dtype == SPK_F32) {
+        *reinterpret_cast<v4f *>(static_cast<float *>(p.out) + row + ch) = v4f{o[0], o[1], o[2], o[3]};
+        continue;
+      }
+      uint32_t w2[2];
 #pragma unroll
-    for (int rd = 0; rd < S::kRounds; ++rd) {
-      if (rd) __syncthreads();
-#pragma unroll
-      for (int u = 0; u < kWaves; ++u) {
-        const int x = rd * S::kTiles + u / kParts;
-        if (x < S::kUnits) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sm.red[u][wave][j][lane] = acc[x / NC][x % NC * kParts + u % kParts][j];
+      for (int e = 0; e < 2; ++e) {
+        uint16_t x0, x1;
+        if constexpr (!F32) {
+          x0 = f32_to_bf16_bits(o[2 * e]);
+          x1 = f32_to_bf16_bits(o[2 * e + 1]);
+        } else {
+          x0 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(o[2 * e]));
+          x1 = __builtin_bit_cast(uint16_t, static_cast<_Float16>(o[2 * e + 1]));
         }
+        w2[e] = x0 | (static_cast<uint32_t>(x1) << 16);
       }
-      __syncthreads();
-      if (rd == 0 && tid < 32 * QT) {
-        Sum d = 0;
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + row + ch) = make_uint2(w2[0], w2[1]);
+    }
+  } else {
 #pragma unroll
-        for (int q = 0; q < kParts; ++q)
+    for (int j = 0; j < kVals; ++j) {
+      const int ch = 32 * c + 8 * (g0 + (j >> 2)) + 4 * half + (j & 3);
+      if (ch < p.D) store_f32_as(p.out, row + ch, F32 ? p.out_dtype : SPK_BF16, val[j] * inv);
+    }
+  }
+}
+
+// Waves that share a row tile, each a quarter or half of the tiles.
+__device__ __forceinline__ int key_waves(int rows) { return rows <= 32 ? 4 : (rows <= 64 ? 2 : 1); }
+
+// A wave's sums in the workspace: [NC][16][64] values, [64] denominators.
+constexpr int wave_sums(int NC) { return NC * 1024 + 64; }
+__device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int group, int part, int wave, int NC) {
+  return p.ws + ((((static_cast<int64_t>(n) * p.units + unit) * p.groups + group) * p.parts + part) * kWaves + wave) *
+                    wave_sums(NC);
+}
+
+// NC = channel tiles of 32.  KW: waves that share a row tile.
+template <int NC, bool F32, bool SEQ, int KW, typename Smem>
+__device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, int n, int unit, int group, int part,
+                                       int wave) {
+  constexpr int NK = (NC + 1) / 2;  // 64-channel score steps
+  constexpr int kEach = kWaves / KW;  // tiles of a step that a wave takes
+  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int kvh = unit % p.Hkv, t = unit / p.Hkv, rows = s.nodes * p.nrep;
+  const int rw = wave / KW, kw_ = wave % KW;
+  const int rt = group * kWaves + rw, r = rt * 32 + col;
+  const bool live = rt * 32 < rows;  // (without rows of its own a wave prepares tiles)
+
+  fill_tables<F32>(p, sm.tab[0], tid);
+  v8i qop[NK];
+  load_query<NK>(p, s, t, kvh, min(r, rows - 1), half, qop);
+  const uint32_t *mrow = p.masks + (s.first + node_of(p, min(r, rows - 1))) * p.mask_words;
+  const Keys<NK> keys(p, s, n, t, kvh, half, col);
+
+  const int p0 = part, p1 = SEQ ? s.parts : part + 1;
+  const int t0 = p0 * s.ptiles, stop = p1 < s.parts ? p1 * s.ptiles : s.end;
+  v16f acc[NC];
+  float l[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int w = 0; w < kWaves; ++w)
-            d += static_cast<Sum>(sm.lsum[tid >> 5][q][w][tid & 31]) + static_cast<Sum>(sm.lsum[tid >> 5][q][w][(tid & 31) + 32]);
-        dtot += d;
-      }
-      if (rd * S::kTiles + wave / kParts < S::kUnits) {
-        const int slot = wave / kParts * kParts, j0 = F32 ? wave % kParts * 8 : 0;
+  for (int c = 0; c < NC; ++c) acc[c] = v16f{};
+  float tot[SEQ ? NC : 1][16], den = 0.f;
+  if constexpr (SEQ) {
 #pragma unroll
-        for (int j = 0; j < S::kVals; ++j) {
-          Sum a = 0;
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int q = 0; q < kParts; ++q)
+      for (int j = 0; j < 16; ++j) tot[c][j] = 0.f;
+  }
+
+  uint32_t kw[NK], vw[NK];
+  bool ok;
+  keys.load(t0 + wave, keys.block_of(t0 + wave), kw, vw, ok);
+  uint32_t pnext = keys.block_of(t0 + wave + kWaves);
+  int buf = 0;
+  for (int first = t0; first < stop; first += kWaves, buf ^= 1) {
+    {
+      // This wave's tile of the four; the next one's words and the block of the one after
+      // are requested before they are used.
+      v8i kop[NK];
+      uint32_t vt[2 * NK];
+      keys.operands(kw, vw, ok, lane, kop, vt);
+      keys.load(first + wave + kWaves, pnext, kw, vw, ok);
+      pnext = keys.block_of(first + wave + 2 * kWaves);
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) a += sm.red[slot + q][w][j0 + j][lane];
-          tot[rd][j] += a;
-        }
-      }
+      for (int k = 0; k < NK; ++k)
+        sm.k[buf][wave][k][lane] = v4u{static_cast<uint32_t>(kop[k][0]), static_cast<uint32_t>(kop[k][1]),
+                                       static_cast<uint32_t>(kop[k][2]), static_cast<uint32_t>(kop[k][3])};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = vt[c];
     }
     __syncthreads();
+    if (live) {
+      auto operand = [&](int u, v8i (&kop)[NK]) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+          const v4u x = sm.k[buf][u][k][lane];
+          kop[k] = v8i{static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3])};
+        }
+      };
+      auto values = [&](int u, v8h (&vop)[NC][2]) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) expand<F32>(sm.v[buf][u][c][lane], vop[c]);
+      };
+      if ((first + kWaves) * kKeys <= s.ctx) {
+        // Every key counts: the next tile's scores are computed and looked up under this
+        // one's products.
+        uint32_t w[2][16];
+        {
+          v8i kop[NK];
+          operand(kw_, kop);
+          lookup<F32>(tab0, scores<NK>(kop, qop), w[0]);
+        }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          if (u + 1 < kEach) {
+            v8i kop[NK];
+            operand(kw_ + (u + 1) * KW, kop);
+            lookup<F32>(tab0, scores<NK>(kop, qop), w[(u + 1) & 1]);
+          }
+          v8h vop[NC][2];
+          values(kw_ + u * KW, vop);
+          products<NC, F32, false>(w[u & 1], 0u, vop, acc, l);
+          __builtin_amdgcn_sched_barrier(0);  // tile by tile (several at a time spill)
+        }
+      } else {
+#pragma unroll 1
+        for (int u = kw_; u < kWaves && first + u < stop; u += KW) {
+          uint32_t w[16];
+          v8i kop[NK];
+          v8h vop[NC][2];
+          operand(u, kop);
+          values(u, vop);
+          lookup<F32>(tab0, scores<NK>(kop, qop), w);
+          products<NC, F32, true>(w, seen(s, first + u, mrow, half), vop, acc, l);
+        }
+      }
+    }
+    if constexpr (SEQ) {
+      // (a part is a power of two of tiles, so its last step ends on it)
+      if (((first + kWaves) & (s.ptiles - 1)) == 0 && first + kWaves <= (s.parts - 1) * s.ptiles) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) tot[c][j] += acc[c][j];
+          acc[c] = v16f{};
+        }
+        den += lane_sum(l);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) l[q] = 0.f;
+      }
+    }
   }
+  if constexpr (SEQ) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[c][j] = tot[c][j] + acc[c][j];
+  }
+  den += lane_sum(l);
 
-  if (p.parts > 1 && s.parts > 1) {
-    Sum *to = reinterpret_cast<Sum *>(
-        p.ws + (((static_cast<int64_t>(n) * p.groups + group) * p.parts + part) * p.units + unit) * S::kBytes);
+  if (!SEQ && s.parts > 1) {
+    if (!live) return;
+    float *to = sums_at(p, n, unit, group, part, wave, NC);
 #pragma unroll
-    for (int rd = 0; rd < S::kRounds; ++rd)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int j = 0; j < S::kVals; ++j) to[(rd * S::kVals + j) * (kWaves * 64) + tid] = tot[rd][j];
-    if (tid < 32 * QT) to[S::kSums + tid] = dtot;
+      for (int j = 0; j < 16; ++j) to[(c * 16 + j) * 64 + lane] = acc[c][j];
+    to[NC * 1024 + lane] = den;
     return;
   }
-  if (tid < 32 * QT) sm.dens[tid] = dtot;
-  __syncthreads();
-  store_rows<QT, NC, F32>(p, s, unit, r0, tot, sm.dens);
-}
-
-// Sums of the parts, in their order.
-template <int QT, int NC, bool F32>
-__global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p) {
-  typedef Shape<QT, NC, F32> S;
-  typedef typename S::Sum Sum;
-  __shared__ Sum dens[32 * QT];
-  const int tid = threadIdx.x, n = blockIdx.y, unit = blockIdx.x % p.units, group = blockIdx.x / p.units;
-  const Seq s = sequence(p, n);
-  if (group * 32 * QT >= s.nodes * p.nrep || s.parts <= 1) return;
-  Sum tot[S::kRounds][S::kVals], dtot = 0;
+  if constexpr (KW == 1) {
+    den += __shfl_xor(den, 32);
+    if (r < rows) {
 #pragma unroll
-  for (int rd = 0; rd < S::kRounds; ++rd)
+      for (int c = 0; c < NC; ++c) {
+        float val[16];
 #pragma unroll
-    for (int j = 0; j < S::kVals; ++j) tot[rd][j] = 0;
-  for (int part = 0; part < s.parts; ++part) {
-    const Sum *from = reinterpret_cast<const Sum *>(
-        p.ws + (((static_cast<int64_t>(n) * p.groups + group) * p.parts + part) * p.units + unit) * S::kBytes);
+        for (int j = 0; j < 16; ++j) val[j] = acc[c][j];
+        store_row<F32, 16>(p, s, t, kvh, r, c, 0, half, val, den);
+      }
+    }
+  } else {
+    // The row tile's waves, in their order: wave kw_ finishes a KW-th of each channel tile.
+    constexpr int kVals = 16 / KW;
+    sm.den[wave][lane] = den;
 #pragma unroll
-    for (int rd = 0; rd < S::kRounds; ++rd)
+    for (int c = 0; c < NC; ++c) {
+      __syncthreads();  // (the staged tiles, and the channel tile before, are read)
 #pragma unroll
-      for (int j = 0; j < S::kVals; ++j) tot[rd][j] += from[(rd * S::kVals + j) * (kWaves * 64) + tid];
-    if (tid < 32 * QT) dtot += from[S::kSums + tid];
+      for (int j = 0; j < 16; ++j) sm.red[wave][j][lane] = acc[c][j];
+      __syncthreads();
+      float val[kVals], d = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) d += sm.den[rw * KW + w][col] + sm.den[rw * KW + w][col + 32];
+#pragma unroll
+      for (int j = 0; j < kVals; ++j) {
+        val[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) val[j] += sm.red[rw * KW + w][kw_ * kVals + j][lane];
+      }
+      if (r < rows) store_row<F32, kVals>(p, s, t, kvh, r, c, kw_ * kVals / 4, half, val, d);
+    }
   }
-  if (tid < 32 * QT) dens[tid] = dtot;
-  __syncthreads();
-  store_rows<QT, NC, F32>(p, s, unit, group * 32 * QT, tot, dens);
 }
 
-// Row tiles a workgroup takes of the `qt` asked for: as many as its sums leave
-// registers for.
-constexpr int row_tiles(int qt, int NC, bool f32) {
-  const int most = NC > 3 ? (f32 ? 1 : 2) : (NC > 2 ? (f32 ? 1 : 2) : (f32 ? 2 : 4));
-  return qt < most ? qt : most;
+template <int NC, bool F32, bool SEQ>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 || SEQ ? 2 : 3))) void tree_attn_kernel(
+    Params p) {
+  constexpr int NK = (NC + 1) / 2;
+  struct Smem {
+    uint32_t tab[kTables<F32>][kTabStride];  // first: a score's accumulator is its entry's LDS address
+    float den[kWaves][64];
+    union {
+      struct {
+        v4u k[2][kWaves][NK][64];
+        uint32_t v[2][kWaves][NC][64];
+      };
+      float red[kWaves][16][64];
+    };
+  };
+  __shared__ Smem sm;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (uniform: its branches are scalar)
+  const int n = blockIdx.y;
+  const int unit = blockIdx.x % p.units, rest = blockIdx.x / p.units;
+  const int part = rest % p.parts, group = rest / p.parts;
+  const Seq s = sequence(p, n);
+  const int rows = s.nodes * p.nrep;
+  if (group * kWaves * 32 >= rows || (!SEQ && part >= s.parts)) return;
+  switch (key_waves(rows)) {
+    case 4: attend<NC, F32, SEQ, 4>(p, s, sm, n, unit, group, part, wave); break;
+    case 2: attend<NC, F32, SEQ, 2>(p, s, sm, n, unit, group, part, wave); break;
+    default: attend<NC, F32, SEQ, 1>(p, s, sm, n, unit, group, part, wave);
+  }
+}
+
+// Sums of the parts, in their order, wave by wave: a wave an output tile.
+template <bool F32>
+__global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p, int NC) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, n = blockIdx.y;
+  const int id = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int c = id % NC, tile = id / NC % (p.groups * kWaves), unit = id / NC / (p.groups * kWaves);
+  if (unit >= p.units) return;
+  const Seq s = sequence(p, n);
+  const int rows = s.nodes * p.nrep, r = tile * 32 + col;
+  if (tile * 32 >= rows || s.parts <= 1) return;
+  const int kw = key_waves(rows);
+  float val[16], den = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) val[j] = 0.f;
+  for (int w = 0; w < kw; ++w) {
+    float a[16], d = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) a[j] = 0.f;
+    for (int part = 0; part < s.parts; ++part) {
+      const float *from = sums_at(p, n, unit, tile / kWaves, part, tile % kWaves * kw + w, NC);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) a[j] += from[(c * 16 + j) * 64 + lane];
+      d += from[NC * 1024 + lane];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) val[j] += a[j];
+    den += d + __shfl_xor(d, 32);
+  }
+  if (r < rows) store_row<F32, 16>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, 0, half, val, den);
 }
 
 struct Plan {
-  int qt, groups, parts;  // as asked of row_tiles; of a sequence; along the context
-  size_t bytes;           // workspace
+  int groups, parts;
+  size_t bytes;  // workspace
 };
 
-// The launch of a shape.  Row tiles share a key tile's operands, so four to a workgroup
-// while that leaves two workgroups a CU; a workgroup a part of the context where there
-// would be fewer than two a CU without.
-inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_size, int max_blocks, bool f32) {
+// The launch of a shape: a workgroup a part of the context where there would be fewer than
+// three a CU without.
+inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_size, int max_blocks) {
   Plan r;
-  const int NC = (D + 31) / 32;
-  const int64_t units = static_cast<int64_t>(T) * Hkv * N;
-  const int64_t rtiles = (static_cast<int64_t>(max_nodes) * (Hq / Hkv) + 31) / 32;
-  const int64_t parts = (static_cast<int64_t>(max_blocks) * block_size + kPart - 1) / kPart;
-  r.qt = 1;
-  for (int qt = 4; qt > 1; qt >>= 1) {
-    const int used = row_tiles(qt, NC, f32);
-    if (used == qt && rtiles > qt / 2 && units * ((rtiles + qt - 1) / qt) * (parts > 1 ? parts : 1) >= 512) {
-      r.qt = qt;
-      break;
-    }
-  }
-  r.groups = static_cast<int>((rtiles + r.qt - 1) / r.qt);
-  r.parts = parts > 1 && units * r.groups < 1024 ? static_cast<int>(parts) : 1;
-  r.bytes = 0;
-  if (r.parts > 1) {
-    const int kParts = f32 ? 2 : 1, tiles = kWaves / kParts, rounds = (r.qt * NC + tiles - 1) / tiles;
-    r.bytes = static_cast<size_t>(units) * r.groups * r.parts * (f32 ? 8 : 4) *
-              (rounds * (16 / kParts) * kWaves * 64 + 32 * r.qt);
-  }
+  const size_t units = static_cast<size_t>(T) * Hkv * N;
+  r.groups = static_cast<int>((static_cast<int64_t>(max_nodes) * (Hq / Hkv) + 32 * kWaves - 1) / (32 * kWaves));
+  r.parts = units * r.groups < 768 ? most_parts(static_cast<int64_t>(max_blocks) * block_size) : 1;
+  r.bytes = r.parts > 1 ? units * r.groups * r.parts * kWaves * wave_sums((D + 31) / 32) * sizeof(float) : 0;
   return r;
 }
 
-template <int QT, int NC, bool F32>
-static int launch_one(const Params &p, int N, hipStream_t s) {
-  if constexpr (row_tiles(QT, NC, F32) == QT) {
-    tree_attn_kernel<QT, NC, F32><<<dim3(p.groups * p.parts * p.units, N), kWaves * 64, 0, s>>>(p);
-    int rc = check_launch("tree_attn");
-    if (rc || p.parts == 1) return rc;
-    tree_join_kernel<QT, NC, F32><<<dim3(p.groups * p.units, N), kWaves * 64, 0, s>>>(p);
-    return check_launch("tree_attn");
-  }
-  return fail(SPK_EINVAL, "tree_attn: no kernel of %d row tiles", QT);
+template <int NC, bool F32>
+static int launch(const Params &p, bool one_part, int N, hipStream_t s) {
+  const dim3 grid(p.groups * p.parts * p.units, N);
+  if (p.parts == 1 && !one_part) tree_attn_kernel<NC, F32, true><<<grid, kWaves * 64, 0, s>>>(p);
+  else tree_attn_kernel<NC, F32, false><<<grid, kWaves * 64, 0, s>>>(p);
+  const int rc = check_launch("tree_attn");
+  if (rc || p.parts == 1) return rc;
+  const int waves = p.units * p.groups * kWaves * NC;
+  tree_join_kernel<F32><<<dim3((waves + kWaves - 1) / kWaves, N), kWaves * 64, 0, s>>>(p, NC);
+  return check_launch("tree_attn");
 }
 
-template <int QT, bool F32>
-static int launch(const Params &p, int N, hipStream_t s) {
-  switch ((p.D + 31) / 32) {
-    case 1: return launch_one<QT, 1, F32>(p, N, s);
-    case 2: return launch_one<QT, 2, F32>(p, N, s);
-    case 3: return launch_one<QT, 3, F32>(p, N, s);
-    default: return launch_one<QT, 4, F32>(p, N, s);
+template <bool F32>
+static int launch_type(const Params &p, bool one_part, int N, hipStream_t s) {
+  switch (p.W) {
+    case 1: return launch<1, F32>(p, one_part, N, s);
+    case 2: return launch<2, F32>(p, one_part, N, s);
+    case 3: return launch<3, F32>(p, one_part, N, s);
+    default: return launch<4, F32>(p, one_part, N, s);
   }
 }
 
@@ -517,9 +607,7 @@ extern "C" size_t spk_tree_attn_workspace_bytes(int T, int N, int Hq, int Hkv, i
   if (T <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || head_dim > 128 || max_nodes <= 0 ||
       max_nodes > tree::kMaxNodes || block_size <= 0 || max_blocks < 0)
     return 0;
-  const size_t a = tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks, false).bytes;
-  const size_t b = tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks, true).bytes;
-  return a > b ? a : b;  // (whatever the outputs' type)
+  return tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks).bytes;
 }
 
 extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const int32_t *k_tree,
@@ -551,12 +639,11 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   if (!q || !k_tree || !v_tree || !context_lens || !row_starts || !masks || !out ||
       (max_blocks > 0 && !block_tables) || (num_slots > 0 && (!k_cache || !v_cache)))
     return fail(SPK_EINVAL, "tree_attn: null pointer");
-  const bool f32 = out_dtype != SPK_BF16;
-  const tree::Plan plan = tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks, f32);
+  const tree::Plan plan = tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return fail(SPK_EINVAL, "tree_attn: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);
   const int64_t units = static_cast<int64_t>(T) * Hkv;
-  if (units * plan.groups * plan.parts > 0x7fffffffll || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
+  if (units * plan.groups * plan.parts > (1 << 26) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
     return fail(SPK_EUNSUPPORTED, "tree_attn: T=%d Hq=%d Hkv=%d with %d nodes", T, Hq, Hkv, max_nodes);
   tree::Params p{};
   p.q = reinterpret_cast<const uint32_t *>(q);
@@ -587,10 +674,10 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   p.W = (head_dim + 31) / 32; p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks; p.max_nodes = max_nodes;
   // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
   p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
-  p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<char *>(workspace);
+  p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
   tiles::build_table(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (f32) return plan.qt >= 2 ? tree::launch<2, true>(p, N, s) : tree::launch<1, true>(p, N, s);
-  return plan.qt == 4 ? tree::launch<4, false>(p, N, s)
-                      : (plan.qt == 2 ? tree::launch<2, false>(p, N, s) : tree::launch<1, false>(p, N, s));
+  const bool one_part = tree::most_parts(static_cast<int64_t>(max_blocks) * block_size) == 1;
+  return out_dtype != SPK_BF16 ? tree::launch_type<true>(p, one_part, N, s)
+                               : tree::launch_type<false>(p, one_part, N, s);
 }
