@@ -40,7 +40,7 @@ using namespace tiles;
 constexpr int kWaves = 4;
 constexpr int kKeys = 32;          // keys per tile
 constexpr int kPartTiles = 32;     // tiles per part, up to kMaxParts of them
-constexpr int kMaxParts = 16;
+constexpr int kMaxParts = 32;
 constexpr int kMaxNodes = 1024;
 constexpr int kTabStride = kTab + 3;
 
@@ -528,35 +528,44 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
   }
 }
 
-// Sums of the parts, in their order, wave by wave: a wave an output tile.
+// Sums of the parts, in their order, wave by wave.  A wave takes four channels of a lane's
+// sixteen of an output tile; four parts' sums are on their way at once.
 template <bool F32>
 __global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p, int NC) {
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, n = blockIdx.y;
-  const int id = blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int c = id % NC, tile = id / NC % (p.groups * kWaves), unit = id / NC / (p.groups * kWaves);
-  if (unit >= p.units) return;
+  const int lane = threadIdx.x & 63, quad = threadIdx.x >> 6, half = lane >> 5, col = lane & 31, n = blockIdx.y;
+  const int c = blockIdx.x % NC, tile = blockIdx.x / NC % (p.groups * kWaves), unit = blockIdx.x / NC / (p.groups * kWaves);
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep, r = tile * 32 + col;
   if (tile * 32 >= rows || s.parts <= 1) return;
   const int kw = key_waves(rows);
-  float val[16], den = 0.f;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) val[j] = 0.f;
+  const int64_t stride = kWaves * wave_sums(NC);  // from part to part
+  float val[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
   for (int w = 0; w < kw; ++w) {
-    float a[16], d = 0.f;
+    const float *from = sums_at(p, n, unit, tile / kWaves, 0, tile % kWaves * kw + w, NC) + lane;
+    const float *at = from + (c * 16 + quad * 4) * 64;
+    float a[4] = {0.f, 0.f, 0.f, 0.f}, d = 0.f;
+    for (int part = 0; part < s.parts; part += 4) {
+      float x[4][5];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) a[j] = 0.f;
-    for (int part = 0; part < s.parts; ++part) {
-      const float *from = sums_at(p, n, unit, tile / kWaves, part, tile % kWaves * kw + w, NC);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t to = min(part + u, s.parts - 1) * stride;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) a[j] += from[(c * 16 + j) * 64 + lane];
-      d += from[NC * 1024 + lane];
+        for (int j = 0; j < 4; ++j) x[u][j] = at[to + j * 64];
+        x[u][4] = from[to + NC * 1024];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (part + u >= s.parts) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] += x[u][j];
+        d += x[u][4];
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) val[j] += a[j];
+    for (int j = 0; j < 4; ++j) val[j] += a[j];
     den += d + __shfl_xor(d, 32);
   }
-  if (r < rows) store_row<F32, 16>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, 0, half, val, den);
+  if (r < rows) store_row<F32, 4>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, quad, half, val, den);
 }
 
 struct Plan {
@@ -582,8 +591,7 @@ static int launch(const Params &p, bool one_part, int N, hipStream_t s) {
   else tree_attn_kernel<NC, F32, false><<<grid, kWaves * 64, 0, s>>>(p);
   const int rc = check_launch("tree_attn");
   if (rc || p.parts == 1) return rc;
-  const int waves = p.units * p.groups * kWaves * NC;
-  tree_join_kernel<F32><<<dim3((waves + kWaves - 1) / kWaves, N), kWaves * 64, 0, s>>>(p, NC);
+  tree_join_kernel<F32><<<dim3(p.units * p.groups * kWaves * NC, N), kWaves * 64, 0, s>>>(p, NC);
   return check_launch("tree_attn");
 }
 
