@@ -39,7 +39,7 @@ using namespace tiles;
 
 constexpr int kWaves = 4;
 constexpr int kKeys = 32;          // keys per tile
-constexpr int kPartTiles = 32;     // tiles per part, up to kMaxParts of them
+constexpr int kPartTiles = 64;     // tiles per part, up to kMaxParts of them
 constexpr int kMaxParts = 32;
 constexpr int kMaxNodes = 1024;
 constexpr int kTabStride = kTab + 3;
@@ -322,7 +322,7 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
 // Waves that share a row tile, each a quarter or half of the tiles.
 __device__ __forceinline__ int key_waves(int rows) { return rows <= 32 ? 4 : (rows <= 64 ? 2 : 1); }
 
-// A wave's sums in the workspace: [NC][16][64] values, [64] denominators.
+// A wave's sums in the workspace: [NC][4][64] vectors of four channels, [64] denominators.
 constexpr int wave_sums(int NC) { return NC * 1024 + 64; }
 __device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int group, int part, int wave, int NC) {
   return p.ws + ((((static_cast<int64_t>(n) * p.units + unit) * p.groups + group) * p.parts + part) * kWaves + wave) *
@@ -459,7 +459,9 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) to[(c * 16 + j) * 64 + lane] = acc[c][j];
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<v4f *>(to + ((c * 4 + j) * 64 + lane) * 4) =
+            v4f{acc[c][4 * j], acc[c][4 * j + 1], acc[c][4 * j + 2], acc[c][4 * j + 3]};
     to[NC * 1024 + lane] = den;
     return;
   }
@@ -529,11 +531,14 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
 }
 
 // Sums of the parts, in their order, wave by wave.  A wave takes four channels of a lane's
-// sixteen of an output tile; four parts' sums are on their way at once.
+// sixteen of an output tile, with kAhead parts' sums on their way at once.  Workgroups of a
+// unit are numbered as the attention's are: with 8 units (or a multiple) they run on the XCD
+// whose L2 has the sums.
 template <bool F32>
 __global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p, int NC) {
+  constexpr int kAhead = 8;
   const int lane = threadIdx.x & 63, quad = threadIdx.x >> 6, half = lane >> 5, col = lane & 31, n = blockIdx.y;
-  const int c = blockIdx.x % NC, tile = blockIdx.x / NC % (p.groups * kWaves), unit = blockIdx.x / NC / (p.groups * kWaves);
+  const int unit = blockIdx.x % p.units, rest = blockIdx.x / p.units, c = rest % NC, tile = rest / NC;
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep, r = tile * 32 + col;
   if (tile * 32 >= rows || s.parts <= 1) return;
@@ -541,24 +546,24 @@ __global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p, int NC
   const int64_t stride = kWaves * wave_sums(NC);  // from part to part
   float val[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
   for (int w = 0; w < kw; ++w) {
-    const float *from = sums_at(p, n, unit, tile / kWaves, 0, tile % kWaves * kw + w, NC) + lane;
-    const float *at = from + (c * 16 + quad * 4) * 64;
-    float a[4] = {0.f, 0.f, 0.f, 0.f}, d = 0.f;
-    for (int part = 0; part < s.parts; part += 4) {
-      float x[4][5];
+    const float *from = sums_at(p, n, unit, tile / kWaves, 0, tile % kWaves * kw + w, NC);
+    const float *at = from + ((c * 4 + quad) * 64 + lane) * 4;
+    v4f a = {0.f, 0.f, 0.f, 0.f};
+    float d = 0.f;
+    for (int part = 0; part < s.parts; part += kAhead) {
+      v4f x[kAhead];
+      float y[kAhead];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kAhead; ++u) {
         const int64_t to = min(part + u, s.parts - 1) * stride;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[u][j] = at[to + j * 64];
-        x[u][4] = from[to + NC * 1024];
+        x[u] = *reinterpret_cast<const v4f *>(at + to);
+        y[u] = from[to + NC * 1024 + lane];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kAhead; ++u) {
         if (part + u >= s.parts) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] += x[u][j];
-        d += x[u][4];
+        a += x[u];
+        d += y[u];
       }
     }
 #pragma unroll
