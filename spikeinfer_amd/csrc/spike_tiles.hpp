@@ -22,7 +22,8 @@ typedef unsigned v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kTab = 129;  // weights of scores 0..head_dim (<= 128)
 
-// The value of x in the lane whose number differs by J (1, 2, 4, 8 or 16).
+// The value of x in the lane whose number differs by J (1, 2, 4 or 8), by data-parallel
+// moves: no LDS latency.
 template <int J>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
   const int v = static_cast<int>(x);
@@ -30,7 +31,10 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
   else if constexpr (J == 2) return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
   else if constexpr (J == 8)  // rotation by 8 within a row of 16
     return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false));
-  else return static_cast<uint32_t>(__builtin_amdgcn_ds_swizzle(v, (J << 10) | 0x1f));
+  else {  // four lanes up for banks 0 and 2 of a row, down for 1 and 3
+    const int up = __builtin_amdgcn_update_dpp(0, v, 0x104, 0xF, 0x5, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(up, v, 0x114, 0xF, 0xA, false));
+  }
 }
 
 // One step of the 32 x 32 bit transpose within each 32-lane half (lane = row,
@@ -38,13 +42,17 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
 // others.
 template <int J>
 __device__ __forceinline__ uint32_t transpose_step(uint32_t x, int lane) {
-  constexpr uint32_t m = J == 16 ? 0x0000ffffu : J == 8 ? 0x00ff00ffu : J == 4 ? 0x0f0f0f0fu
-                         : J == 2 ? 0x33333333u : 0x55555555u;
-  const uint32_t y = lane_xor<J>(x);
-  const bool up = lane & J;
-  const uint32_t keep = up ? ~m : m;
-  const uint32_t r = __builtin_amdgcn_alignbit(y, y, up ? J : 32 - J);  // rotate right
-  return (x & keep) | (r & ~keep);
+  if constexpr (J == 16) {  // rows of 16 lanes: (even, even) and (odd, odd), a half of each
+    const auto sw = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __builtin_amdgcn_perm(sw[1], sw[0], lane & 16 ? 0x07060302u : 0x05040100u);
+  } else {
+    constexpr uint32_t m = J == 8 ? 0x00ff00ffu : J == 4 ? 0x0f0f0f0fu : J == 2 ? 0x33333333u : 0x55555555u;
+    const uint32_t y = lane_xor<J>(x);
+    const bool up = lane & J;
+    const uint32_t keep = up ? ~m : m;
+    const uint32_t r = __builtin_amdgcn_alignbit(y, y, up ? J : 32 - J);  // rotate right
+    return (x & keep) | (r & ~keep);
+  }
 }
 
 __device__ __forceinline__ uint32_t transpose32(uint32_t x, int lane) {

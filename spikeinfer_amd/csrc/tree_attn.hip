@@ -100,20 +100,23 @@ __device__ __forceinline__ int node_of(const Params &p, int r) {
   return p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
 }
 
-// Weight tables in LDS at offset 0: one of (hi, lo) pairs, or four of high halves whose
-// entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's.
-template <bool F32> constexpr int kTables = F32 ? 1 : 4;
+// Weight tables in LDS at offset 0.  bf16 outputs: four of the weights' high halves as fp32,
+// whose entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's (all of them f16 numbers).  Else
+// one of (hi, lo) pairs, and kTabStride words on, their sums as fp32.
+template <bool F32> constexpr int kTables = F32 ? 2 : 4;
 template <bool F32>
-__device__ __forceinline__ void fill_tables(const Params &p, uint32_t *tab, int tid) {
+__device__ __forceinline__ void fill_tables(const Params &p, float *tab, int tid) {
   if (tid > p.D) return;
   const uint32_t w = p.tab[tid];
-  tab[tid] = w;
-  if constexpr (!F32) {
-    const _Float16 h = __builtin_bit_cast(_Float16, static_cast<uint16_t>(w));
-#pragma unroll
-    for (int i = 1; i < 4; ++i)
-      tab[i * kTabStride + tid] =
-          __builtin_bit_cast(uint16_t, static_cast<_Float16>(h * static_cast<_Float16>(i == 1 ? 0.5f : i == 2 ? 0.125f : 0.0078125f)));
+  const float hi = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
+  if constexpr (F32) {
+    tab[tid] = __uint_as_float(w);
+    tab[kTabStride + tid] = hi + static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16)));
+  } else {
+    tab[tid] = hi;
+    tab[kTabStride + tid] = hi * 0.5f;
+    tab[2 * kTabStride + tid] = hi * 0.125f;
+    tab[3 * kTabStride + tid] = hi * 0.0078125f;
   }
 }
 
@@ -220,60 +223,65 @@ __device__ __forceinline__ v16f scores(const v8i (&kop)[NK], const v8i (&qop)[NK
   return a;
 }
 
+// A tile's weights: the lane's sixteen as operand entries, and for fp32 outputs as fp32.
 template <bool F32>
-__device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&w)[16]) {
+struct Weights {
+  uint32_t w[16];
+  float f[F32 ? 16 : 1];
+};
+template <bool F32>
+__device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, Weights<F32> &x) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint32_t at = tab0 + (F32 ? 0 : 4 * kTabStride * (e & 3)) + __float_as_uint(a[e]);
-    w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
+    const uint32_t at = tab0 + __float_as_uint(a[e]);
+    const SPK_LDS uint32_t *w = reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
+    x.w[e] = w[F32 ? 0 : kTabStride * (e & 3)];
+    if constexpr (F32) x.f[e] = __uint_as_float(w[kTabStride]);
   }
 }
 
-// Adds a tile's weighted values to acc and its weights to l.
+// Adds a tile's weighted values to acc and its weights to l.  (The weights are added as fp32:
+// dot products of f16 pairs would be half as many instructions, but they take the matrix
+// cores' time: 8 behind each product 78 cycles where 8 additions take 52.)
 template <int NC, bool F32, bool MASKED>
-__device__ __forceinline__ void products(const uint32_t (&w)[16], uint32_t see, const v8h (&vop)[NC][2],
-                                         v16f (&acc)[NC], float (&l)[4]) {
+__device__ __forceinline__ void products(const Weights<F32> &x, uint32_t see, const v8h (&vop)[NC][2], v16f (&acc)[NC],
+                                         float (&l)[4]) {
   constexpr int kParts = F32 ? 2 : 1;
-  auto weight = [&](int e) {  // the e-th of the lane's sixteen
+  auto keep = [&](uint32_t w, int e) {  // the e-th of the lane's sixteen
     if constexpr (MASKED)
-      return w[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
-    else return w[e];
+      return w & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
+    else return w;
   };
-  // fp32: the sixteen weights first, then added (a long dot2 chain loses bits that count)
-  float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    v4u x[kParts];  // the weights' halves, two keys a register
+    v4u y[kParts];  // the weights' halves, two keys a register
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t y0 = weight(4 * g + e), y1 = weight(4 * g + e + 8);
-#pragma unroll
-      for (int q = 0; q < kParts; ++q) {
-        const uint32_t y = __builtin_amdgcn_perm(y1, y0, q ? 0x07060302u : 0x05040100u);
-        if constexpr (F32) {
-          float &dq = d[2 * (e & 1) + q];
-          dq = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, y), v2h{1, 1}, dq, false);
-        } else {
-          const _Float16 one = static_cast<_Float16>(e == 0 ? 0x1p-14f : e == 1 ? 0x1p-13f : e == 2 ? 0x1p-11f : 0x1p-7f);
-          l[e] = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, y), v2h{one, one}, l[e], false);
-        }
-        x[q][e] = y;
+    for (int i = 0; i < 4; ++i) {
+      const int e0 = 4 * g + i, e1 = e0 + 8;
+      const uint32_t w0 = keep(x.w[e0], e0), w1 = keep(x.w[e1], e1);
+      if constexpr (F32) {
+        l[i] += __uint_as_float(keep(__float_as_uint(x.f[e0]), e0)) + __uint_as_float(keep(__float_as_uint(x.f[e1]), e1));
+        y[0][i] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+        y[1][i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+      } else {
+        l[i] += __uint_as_float(w0) + __uint_as_float(w1);
+        y[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w0), __uint_as_float(w1)));
       }
     }
 #pragma unroll
     for (int q = 0; q < kParts; ++q)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, x[q]), acc[c], 0, 0, 0);
-  }
-  if constexpr (F32) {
-    l[0] += d[0] + d[2];
-    l[1] += d[1] + d[3];
+        acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, y[q]), acc[c], 0, 0, 0);
   }
 }
 
-// A lane's denominator, of its own keys.
-__device__ __forceinline__ float lane_sum(const float (&l)[4]) { return (l[0] + l[1]) + (l[2] + l[3]); }
+// A lane's denominator, of its own keys, in the numerators' units.
+template <bool F32>
+__device__ __forceinline__ float lane_sum(const float (&l)[4]) {
+  if constexpr (F32) return (l[0] + l[1]) + (l[2] + l[3]);
+  else return ((l[0] + 2.f * l[1]) + (8.f * l[2] + 128.f * l[3])) * 0x1p-14f;
+}
 
 // Rows of a tile from their sums: kVals of the lane's values of channel tile c (four
 // channels 8 * (g0 + k) + 4 * half .. for each k), divided by the row's denominator.
@@ -399,7 +407,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       if ((first + kWaves) * kKeys <= s.ctx) {
         // Every key counts: the next tile's scores are computed and looked up under this
         // one's products.
-        uint32_t w[2][16];
+        Weights<F32> w[2];
         {
           v8i kop[NK];
           operand(kw_, kop);
@@ -420,7 +428,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       } else {
 #pragma unroll 1
         for (int u = kw_; u < kWaves && first + u < stop; u += KW) {
-          uint32_t w[16];
+          Weights<F32> w;
           v8i kop[NK];
           v8h vop[NC][2];
           operand(u, kop);
@@ -439,7 +447,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
           for (int j = 0; j < 16; ++j) tot[c][j] += acc[c][j];
           acc[c] = v16f{};
         }
-        den += lane_sum(l);
+        den += lane_sum<F32>(l);
 #pragma unroll
         for (int q = 0; q < 4; ++q) l[q] = 0.f;
       }
@@ -451,7 +459,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[c][j] = tot[c][j] + acc[c][j];
   }
-  den += lane_sum(l);
+  den += lane_sum<F32>(l);
 
   if (!SEQ && s.parts > 1) {
     if (!live) return;
@@ -505,7 +513,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
     Params p) {
   constexpr int NK = (NC + 1) / 2;
   struct Smem {
-    uint32_t tab[kTables<F32>][kTabStride];  // first: a score's accumulator is its entry's LDS address
+    float tab[kTables<F32>][kTabStride];  // first: a score's accumulator is its entry's LDS address
     float den[kWaves][64];
     union {
       struct {
