@@ -693,7 +693,8 @@ int spk_accept_tree(const int64_t *tokens, const int32_t *parents, const int64_t
  * the rest is left as it was.  Keys as spk_tree_attn reads them.  The sums' order
  * depends on the sequence alone.  mass float at mass_strides {sequence, kv head}.
  */
-size_t spk_key_mass_workspace_bytes(int T, int64_t rows, int Hq, int block_size, int max_blocks);
+size_t spk_key_mass_workspace_bytes(int T, int N, int Hq, int Hkv, int head_dim, int max_rows,
+                                    int block_size, int max_blocks);
 int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const int32_t *k_cache,
                  const int64_t cache_strides[3], int64_t num_slots, const int32_t *block_tables,
                  int64_t bt_stride0, int64_t bt_stride1, const int32_t *seq_lens,

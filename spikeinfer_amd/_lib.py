@@ -145,7 +145,7 @@ _SIGNATURES = {
     "spk_accept_tree": (_i32, [
         _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, ctypes.c_char_p, _i32, _i64p, _i64p, _i64,
         _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
-    "spk_key_mass_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
+    "spk_key_mass_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "spk_key_mass": (_i32, [
         _vp, _i64p, _vp, _i64p, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64p, _i64, _i32, _i64, _i32,
         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _vp]),

@@ -4,16 +4,34 @@
 // positions up to its own:
 //   mass[n, g, j] (+)= sum over t, query heads h of kv head g, rows i of
 //                      exp(popc(q & k_j) * scale) / sum_j' exp(popc(q & k_j') * scale).
-// Two launches: the rows' denominators (a wave a row), then a thread a key.
-#include "common.hpp"
+//
+// MI355X design: scores of 16 rows and 16 keys are one fp4 product over 128 channels
+// (v_mfma_scale_f32_16x16x128_f8f6f4, bits as 0.5 in place, block scales that leave the
+// score's table offset in the accumulator's bits, as spike_tiles.hpp has it), a weight is a
+// look-up in LDS.  128 channels are 4 / WP timesteps of a head (WP: words of a head, a power
+// of two): a product's 16 rows are 4 * WP of each of these timesteps, whose words stand in
+// their own quarter or half of the channels beside zeros, so that decoding (7 rows of 4
+// timesteps at 64 channels) fills 14 of 16 rows and every lane loads one word of a key.
+//   den_kernel   sums the weights of a part of kPart keys for kRows or fewer such row tiles
+//                (keys as the product's rows: a lane adds its own row's weights);
+//   mass_kernel  adds the parts' sums in their order, then for a part's keys the weights
+//                over the denominators (keys as its columns: a lane adds its own key's).
+// A part's sums are taken by the same waves in the same order whatever the batch.
+#include "spike_tiles.hpp"
 
 namespace spk {
 namespace mass {
 
+using namespace tiles;
+
+constexpr int kWaves = 4;
+constexpr int kStep = 64;      // keys a wave takes at once: four products' columns
+constexpr int kPart = 1024;    // keys a workgroup
+
 struct Params {
-  const uint32_t *q;
+  const uint32_t *q;           // words of (t, row, query head)
   int64_t qs0, qs1, qs2;
-  const uint32_t *k;
+  const uint32_t *k;           // cache (t, kv head, slot)
   int64_t ks0, ks1, ks2;
   int64_t num_slots;
   const int32_t *bt;
@@ -23,74 +41,317 @@ struct Params {
   int64_t ms0, ms1, cap;
   int accumulate;
   int64_t rows;
-  int N, max_rows, T, Hq, Hkv, nrep, W, bs_log2, max_blocks;
-  float scale;
-  float *den;  // [T, rows, Hq]
+  uint32_t rep_mul;            // floor(r / nrep) = r * rep_mul >> 32 for every row
+  int N, max_rows, T, Hkv, nrep, W, D, bs_log2, max_blocks;
+  int rtiles;                  // row tiles of a timestep group, for max_rows rows
+  int tiles;                   // all row tiles: rtiles * timestep groups
+  int parts;                   // most parts of a sequence
+  float *den;                  // [N, Hkv, parts, tiles, 16]
+  float tab[kTab];             // exp((s - D) * scale)
 };
 
 struct Seq {
-  int64_t s0;
-  int m, len;
+  int64_t first;
+  int m, len, parts;
 };
 
 __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   Seq s;
-  s.s0 = p.starts ? min<int64_t>(max(p.starts[n], 0), p.rows) : min<int64_t>(n, p.rows);
-  const int64_t e = p.starts ? p.starts[n + 1] : n + 1;
-  s.m = static_cast<int>(min(min(max(e, s.s0), s.s0 + p.max_rows), p.rows) - s.s0);
+  const int64_t a = p.starts ? p.starts[n] : n, e = p.starts ? p.starts[n + 1] : n + 1;
+  s.first = min(max<int64_t>(a, 0), p.rows);
+  s.m = static_cast<int>(min(min(max(e, s.first), s.first + p.max_rows), p.rows) - s.first);
   s.len = min(max(p.lens[n], 0), p.max_blocks << p.bs_log2);
+  s.parts = (s.len + kPart - 1) / kPart;
   return s;
 }
 
-__device__ __forceinline__ int64_t slot_of(const Params &p, int n, int j, uint32_t nblocks) {
-  const uint32_t blk = static_cast<uint32_t>(p.bt[n * p.bts0 + (j >> p.bs_log2) * p.bts1]);
-  return blk < nblocks ? (static_cast<int64_t>(blk) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1)) : -1;
+__device__ __forceinline__ int row_of(const Params &p, int r) {  // r / nrep
+  return p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
 }
 
-__global__ __launch_bounds__(256) void den_kernel(Params p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.y;
-  const int unit = blockIdx.x * 4 + wave;
-  const int h = unit % p.Hq, t = unit / p.Hq % p.T, i = unit / p.Hq / p.T;
-  const Seq s = sequence(p, n);
-  if (i >= s.m) return;
-  const uint32_t nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
-  const int see = s.len - s.m + i + 1;
-  float l = 0.f;
-  for (int j = lane; j < see; j += 64) {
-    const int64_t slot = slot_of(p, n, j, nblocks);
-    int c = 0;
-    for (int w = 0; w < p.W; ++w)
-      c += __popc(p.q[t * p.qs0 + (s.s0 + i) * p.qs1 + h * p.qs2 + w] &
-                  (slot < 0 ? 0u : p.k[t * p.ks0 + h / p.nrep * p.ks1 + slot * p.ks2 + w]));
-    l += expf(c * p.scale);
+// Row tiles of a workgroup: tile x is rows 4 * WP * (x % rtiles) .. of timestep group x / rtiles.
+// A product's row y: timestep y / (4 * WP) of the group, row y % (4 * WP) of the tile.
+template <int WP, int RT>
+struct Rows {
+  v8i q[RT];
+  int tg[RT];   // timestep group (uniform; -1: no tile)
+  int lim[RT];  // last key that row l % 16 of the tile sees (-1: none)
+
+  __device__ __forceinline__ void load(const Params &p, const Seq &s, int kvh, int tile0, int lane) {
+    const int y = lane & 15, b = lane >> 4;  // row, 32-channel block of the product
+    const int dt = y / (4 * WP);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int x = tile0 + i;
+      tg[i] = x < p.tiles ? x / p.rtiles : -1;
+      const int r = (x - tg[i] * p.rtiles) * 4 * WP + y % (4 * WP);
+      const int row = row_of(p, r), t = tg[i] * (4 / WP) + dt;
+      const bool in = tg[i] >= 0 && row < s.m && t < p.T;
+      lim[i] = in ? s.len - s.m + row : -1;
+      if (tg[i] >= 0 && (x - tg[i] * p.rtiles) * 4 * WP >= s.m * p.nrep) tg[i] = -1;
+      const int w = b - dt * WP;  // this lane's word of the row's head
+      q[i] = fp4_bits(in && w >= 0 && w < WP && w < p.W
+                          ? p.q[t * p.qs0 + (s.first + row) * p.qs1 + (kvh * p.nrep + r - row * p.nrep) * p.qs2 + w]
+                          : 0u);
+    }
   }
-  for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
-  if (lane == 0) p.den[(t * p.rows + s.s0 + i) * p.Hq + h] = l;
+};
+
+// A lane's words of a step's four key tiles for one timestep group (lane l: key l % 16 of a
+// tile, block l / 16 of the product's channels), as operands.
+template <int WP>
+struct Keys {
+  const Params &p;
+  const int32_t *table;
+  const uint32_t *base;
+  uint32_t nblocks;
+  int last_block, len, y, dt, w;
+  __device__ __forceinline__ Keys(const Params &p, const Seq &s, int n, int kvh, int lane) : p(p), len(s.len) {
+    table = p.bt + n * p.bts0;
+    base = p.k + kvh * p.ks1;
+    nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
+    last_block = max(s.len - 1, 0) >> p.bs_log2;
+    y = lane & 15;
+    dt = (lane >> 4) / WP;
+    w = (lane >> 4) % WP;
+  }
+  // Slots of the lane's four keys, -1 where there is none.
+  __device__ __forceinline__ void slots(int j0, int64_t (&at)[4]) const {
+    uint32_t phys[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      phys[u] = static_cast<uint32_t>(table[min((j0 + 16 * u + y) >> p.bs_log2, last_block) * p.bts1]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + 16 * u + y;
+      at[u] = j < len && phys[u] < nblocks
+                  ? ((static_cast<int64_t>(phys[u]) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1))) * p.ks2
+                  : -1;
+    }
+  }
+  __device__ __forceinline__ void load(int tg, const int64_t (&at)[4], uint32_t (&x)[4]) const {
+    const int t = tg * (4 / WP) + dt;
+    const bool in = t < p.T && w < p.W;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = in && at[u] >= 0 ? base[t * p.ks0 + at[u] + w] : 0u;
+  }
+};
+
+__device__ __forceinline__ v4f score(const v8i &a, const v8i &b) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{}, 4, 4, 0, 55, 0, 54);
 }
 
-__global__ __launch_bounds__(256) void mass_kernel(Params p) {
-  const int g = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
-  const int64_t j = blockIdx.x * 256ll + threadIdx.x;
-  if (j >= p.cap) return;
+__device__ __forceinline__ float weight(uint32_t tab0, float score) {
+  return *reinterpret_cast<const SPK_LDS float *>(static_cast<uintptr_t>(tab0 + __float_as_uint(score)));
+}
+
+template <int WP, int RT>
+__global__ __launch_bounds__(kWaves * 64) void den_kernel(Params p) {
+  struct Smem {
+    float tab[kTab + 3];  // first: a score's accumulator is its entry's LDS address
+    float sum[kWaves][RT][16];
+  };
+  __shared__ Smem sm;
+  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = blockIdx.x % p.parts, chunk = blockIdx.x / p.parts;
+  const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
   const Seq s = sequence(p, n);
-  float *to = p.mass + n * p.ms0 + g * p.ms1 + j;
-  if (j >= s.len) {
-    if (!p.accumulate) *to = 0.f;
-    return;
-  }
-  const uint32_t nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
-  const int64_t slot = slot_of(p, n, static_cast<int>(j), nblocks);
-  float sum = 0.f;
-  for (int t = 0; t < p.T; ++t)
-    for (int i = max(0, static_cast<int>(j) - (s.len - s.m)); i < s.m; ++i)
-      for (int h = g * p.nrep; h < (g + 1) * p.nrep; ++h) {
-        int c = 0;
-        for (int w = 0; w < p.W; ++w)
-          c += __popc(p.q[t * p.qs0 + (s.s0 + i) * p.qs1 + h * p.qs2 + w] &
-                      (slot < 0 ? 0u : p.k[t * p.ks0 + g * p.ks1 + slot * p.ks2 + w]));
-        sum += expf(c * p.scale) / p.den[(t * p.rows + s.s0 + i) * p.Hq + h];
+  if (part >= s.parts || s.m == 0) return;
+  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
+  Rows<WP, RT> rows;
+  rows.load(p, s, kvh, chunk * RT, lane);
+  const Keys<WP> keys(p, s, n, kvh, lane);
+  float l[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) l[i] = 0.f;
+  __syncthreads();
+  const int end = min(s.len, (part + 1) * kPart), open = s.len - s.m;  // keys up to `open` are seen by all rows
+  for (int j0 = part * kPart + wave * kStep; j0 < end; j0 += kWaves * kStep) {
+    int64_t at[4];
+    keys.slots(j0, at);
+    v8i k[4];
+    int have = -1;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      if (rows.tg[i] < 0) continue;
+      if (rows.tg[i] != have) {
+        uint32_t x[4];
+        keys.load(rows.tg[i], at, x);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
+        have = rows.tg[i];
       }
-  *to = p.accumulate ? *to + sum : sum;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const v4f a = score(k[u], rows.q[i]);  // lane: row l % 16, keys 4 * (l / 16) + 0..3
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
+        if (j0 + 16 * u + 15 > open) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = j0 + 16 * u + 4 * (lane >> 4) + e <= rows.lim[i] ? w[e] : 0.f;
+        }
+        l[i] += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    l[i] += __shfl_xor(l[i], 16);
+    l[i] += __shfl_xor(l[i], 32);
+    if (lane < 16) sm.sum[wave][i][lane] = l[i];
+  }
+  __syncthreads();
+  float *to = p.den + ((static_cast<int64_t>(blockIdx.y) * p.parts + part) * p.tiles + chunk * RT) * 16;
+  for (int x = tid; x < RT * 16; x += kWaves * 64)
+    if (chunk * RT + x / 16 < p.tiles)
+      to[x] = (sm.sum[0][x / 16][x % 16] + sm.sum[1][x / 16][x % 16]) + (sm.sum[2][x / 16][x % 16] + sm.sum[3][x / 16][x % 16]);
+}
+
+template <int WP, int RT>
+__global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
+  constexpr int kSteps = kPart / (kWaves * kStep);  // of a wave
+  struct Smem {
+    float tab[kTab + 3];
+    float inv[RT][16];
+    int lim[RT][16];
+  };
+  __shared__ Smem sm;
+  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = blockIdx.x, kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
+  const Seq s = sequence(p, n);
+  float *mass = p.mass + n * p.ms0 + kvh * p.ms1;
+  const int64_t from = static_cast<int64_t>(part) * kPart, stop = min(p.cap, from + kPart);
+  if (!p.accumulate)
+    for (int64_t j = max<int64_t>(from, s.len) + tid; j < stop; j += kWaves * 64) mass[j] = 0.f;
+  if (part >= s.parts || from >= p.cap) return;
+  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
+  const Keys<WP> keys(p, s, n, kvh, lane);
+  const int end = min(s.len, (part + 1) * kPart), open = s.len - s.m;
+  float sum[kSteps][4];
+#pragma unroll
+  for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum[st][u] = 0.f;
+  const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tiles * 16;
+  for (int tile0 = 0; tile0 < p.tiles && s.m > 0; tile0 += RT) {
+    Rows<WP, RT> rows;
+    rows.load(p, s, kvh, tile0, lane);
+    if (tile0) __syncthreads();  // (the rows before are read)
+    if (wave == 0 && lane < 16) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) sm.lim[i][lane] = rows.lim[i];
+    }
+    for (int x = tid; x < RT * 16; x += kWaves * 64) {
+      float d = 0.f;
+      if (tile0 + x / 16 < p.tiles)
+        for (int pt = 0; pt < s.parts; ++pt) d += den[(static_cast<int64_t>(pt) * p.tiles + tile0) * 16 + x];
+      sm.inv[x / 16][x % 16] = d > 0.f ? 1.f / d : 0.f;
+    }
+    __syncthreads();
+    float inv[RT][4];  // of the product's rows 4 * (l / 16) + 0..3; no row: 0
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int y = 4 * (lane >> 4) + e;
+        inv[i][e] = sm.lim[i][y] >= 0 ? sm.inv[i][y] : 0.f;
+      }
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int j0 = part * kPart + (st * kWaves + wave) * kStep;
+      if (j0 >= end) break;
+      int64_t at[4];
+      keys.slots(j0, at);
+      v8i k[4];
+      int have = -1;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (rows.tg[i] < 0) continue;
+        if (rows.tg[i] != have) {
+          uint32_t x[4];
+          keys.load(rows.tg[i], at, x);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
+          have = rows.tg[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const v4f a = score(rows.q[i], k[u]);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
+          if (j0 + 16 * u + 15 > open) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[i][4 * (lane >> 4) + e] ? w[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[st][u] = __builtin_fmaf(w[e], inv[i][e], sum[st][u]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float x = sum[st][u];
+      x += __shfl_xor(x, 16);
+      x += __shfl_xor(x, 32);
+      const int j = part * kPart + (st * kWaves + wave) * kStep + 16 * u + (lane & 15);
+      if (lane < 16 && j < end && j < p.cap) mass[j] = p.accumulate ? mass[j] + x : x;
+    }
+}
+
+// exp((s - D) * scale), s = 0..D.
+inline void build_weights(float scale, int D, float *tab) {
+  static thread_local float last_scale = -1.f, last[kTab];
+  static thread_local int last_d = 0;
+  if (scale != last_scale || D != last_d) {
+    for (int i = 0; i <= D; ++i) last[i] = static_cast<float>(std::exp((i - D) * static_cast<double>(scale)));
+    last_scale = scale;
+    last_d = D;
+  }
+  std::memcpy(tab, last, sizeof(float) * (D + 1));
+}
+
+// Rows of a product's timestep, timestep groups, row tiles.
+struct Plan {
+  int wp, rtiles, tiles, parts;
+  size_t bytes;
+};
+inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_size, int max_blocks) {
+  Plan r;
+  const int W = (D + 31) / 32;
+  r.wp = W == 3 ? 4 : W;
+  const int64_t rows = static_cast<int64_t>(max_rows) * (Hq / Hkv);
+  r.rtiles = static_cast<int>((rows + 4 * r.wp - 1) / (4 * r.wp));
+  r.tiles = r.rtiles * ((T + 4 / r.wp - 1) / (4 / r.wp));
+  r.parts = static_cast<int>((static_cast<int64_t>(max_blocks) * block_size + kPart - 1) / kPart);
+  r.bytes = static_cast<size_t>(N) * Hkv * r.parts * r.tiles * 16 * sizeof(float);
+  return r;
+}
+
+template <int WP, int RT>
+static int launch(const Params &p, hipStream_t s) {
+  const int chunks = (p.tiles + RT - 1) / RT, zero = static_cast<int>((p.cap + kPart - 1) / kPart);
+  const int wide = p.accumulate || zero < p.parts ? p.parts : zero;  // (entries behind the table become 0)
+  if (p.parts > 0 && p.rows > 0) den_kernel<WP, RT><<<dim3(p.parts * chunks, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
+  if (wide > 0) mass_kernel<WP, RT><<<dim3(wide, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
+  return check_launch("key_mass");
+}
+
+template <int WP>
+static int launch_rows(const Params &p, hipStream_t s) {
+  // row tiles a workgroup holds in registers: those of a decode step, or eight
+  if (p.tiles <= 2) return launch<WP, 2>(p, s);
+  if (p.tiles <= 4) return launch<WP, 4>(p, s);
+  return launch<WP, 8>(p, s);
 }
 
 }  // namespace mass
@@ -98,8 +359,12 @@ __global__ __launch_bounds__(256) void mass_kernel(Params p) {
 
 using namespace spk;
 
-extern "C" size_t spk_key_mass_workspace_bytes(int T, int64_t rows, int Hq, int block_size, int max_blocks) {
-  return static_cast<size_t>(T) * rows * Hq * 4;
+extern "C" size_t spk_key_mass_workspace_bytes(int T, int N, int Hq, int Hkv, int head_dim, int max_rows,
+                                               int block_size, int max_blocks) {
+  if (T <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || head_dim <= 0 || head_dim > 128 || max_rows <= 0 ||
+      block_size <= 0 || max_blocks < 0)
+    return 0;
+  return mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks).bytes;
 }
 
 extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const int32_t *k_cache,
@@ -123,9 +388,13 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   if (static_cast<int64_t>(N) * Hkv > 65535) return fail(SPK_EUNSUPPORTED, "key_mass: %d sequences of %d heads", N, Hkv);
   if ((rows > 0 && !q) || !seq_lens || !mass || (max_blocks > 0 && !block_tables) || (num_slots > 0 && !k_cache))
     return fail(SPK_EINVAL, "key_mass: null pointer");
-  const size_t need = spk_key_mass_workspace_bytes(T, rows, Hq, block_size, max_blocks);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(SPK_EINVAL, "key_mass: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const mass::Plan plan = mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks);
+  if (static_cast<int64_t>(max_rows) * (Hq / Hkv) > (1 << 24) ||
+      static_cast<int64_t>(plan.tiles) * plan.parts > (1 << 30))
+    return fail(SPK_EUNSUPPORTED, "key_mass: %d rows of %d heads over %d x %d tokens", max_rows, Hq / Hkv, max_blocks,
+                block_size);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
+    return fail(SPK_EINVAL, "key_mass: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);
   mass::Params p{};
   p.q = reinterpret_cast<const uint32_t *>(q);
   p.qs0 = q_strides[0]; p.qs1 = q_strides[1]; p.qs2 = q_strides[2];
@@ -136,14 +405,17 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   p.lens = seq_lens; p.starts = row_starts;
   p.mass = mass; p.ms0 = mass_strides[0]; p.ms1 = mass_strides[1]; p.cap = cap;
   p.accumulate = accumulate; p.rows = rows; p.N = N; p.max_rows = max_rows;
-  p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.nrep = Hq / Hkv; p.W = (head_dim + 31) / 32;
-  p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks; p.scale = scale;
+  p.T = T; p.Hkv = Hkv; p.nrep = Hq / Hkv; p.D = head_dim; p.W = (head_dim + 31) / 32;
+  // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
+  p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
+  p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks;
+  p.rtiles = plan.rtiles; p.tiles = plan.tiles; p.parts = plan.parts;
   p.den = static_cast<float *>(workspace);
+  mass::build_weights(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (rows > 0) {
-    const int64_t units = static_cast<int64_t>(max_rows) * T * Hq;
-    mass::den_kernel<<<dim3((units + 3) / 4, N), 256, 0, s>>>(p);
+  switch (plan.wp) {
+    case 1: return mass::launch_rows<1>(p, s);
+    case 2: return mass::launch_rows<2>(p, s);
+    default: return mass::launch_rows<4>(p, s);
   }
-  mass::mass_kernel<<<dim3((cap + 255) / 256, N * Hkv), 256, 0, s>>>(p);
-  return check_launch("key_mass");
 }

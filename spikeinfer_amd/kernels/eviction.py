@@ -11,6 +11,7 @@ no counterpart there.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -21,9 +22,12 @@ from .packing import packed_width
 from .spike_attention import _as_int32, _check_packed
 
 
-def key_mass_workspace_bytes(T: int, rows: int, num_q_heads: int, block_size: int, max_blocks: int) -> int:
+@functools.lru_cache(maxsize=256)
+def key_mass_workspace_bytes(T: int, n_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, max_rows: int,
+                             block_size: int, max_blocks: int) -> int:
     """Scratch bytes :func:`paged_spike_attn_key_mass` needs for this shape."""
-    return int(_lib.load().spk_key_mass_workspace_bytes(T, rows, num_q_heads, block_size, max_blocks))
+    return int(_lib.load().spk_key_mass_workspace_bytes(T, n_seqs, num_q_heads, num_kv_heads, head_dim, max_rows,
+                                                        block_size, max_blocks))
 
 
 def paged_spike_attn_key_mass(
@@ -72,6 +76,8 @@ def paged_spike_attn_key_mass(
         row_starts = _vector("row_starts", row_starts, n_seqs + 1, torch.int32)
     elif R < n_seqs:
         raise ValueError(f"q has {R} rows for {n_seqs} sequences")
+    else:
+        max_rows = 1
     if max_rows <= 0:
         raise ValueError(f"max_rows={max_rows} must be positive")
     if out is None:
@@ -80,7 +86,7 @@ def paged_spike_attn_key_mass(
         out = torch.empty((n_seqs, hkv, max_blocks * block_size), dtype=torch.float32, device=dev)
     elif out.ndim != 3 or tuple(out.shape[:2]) != (n_seqs, hkv) or out.dtype != torch.float32 or out.stride(-1) != 1:
         raise ValueError(f"out must be float32 [{n_seqs}, {hkv}, cap] with contiguous entries")
-    need = key_mass_workspace_bytes(T, R, n_heads, block_size, max_blocks)
+    need = key_mass_workspace_bytes(T, n_seqs, n_heads, hkv, head_dim, max_rows, block_size, max_blocks)
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -91,7 +97,7 @@ def paged_spike_attn_key_mass(
             "spk_key_mass", dev, q_packed.data_ptr(), _lib.strides(q_packed), k_cache.data_ptr(), _lib.strides(k_cache),
             k_cache.shape[2], block_tables.data_ptr(), block_tables.stride(0), block_tables.stride(1),
             seq_lens.data_ptr(), _lib.ptr(row_starts), out.data_ptr(), _lib.strides(out), out.shape[2], int(accumulate),
-            R, n_seqs, max_rows if row_starts is not None else 1, T, n_heads, hkv, head_dim, block_size, max_blocks,
+            R, n_seqs, max_rows, T, n_heads, hkv, head_dim, block_size, max_blocks,
             1.0 / math.sqrt(head_dim), workspace.data_ptr() if need else None, need),
         "paged_spike_attn_key_mass",
     )
