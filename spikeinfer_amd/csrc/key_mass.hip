@@ -12,11 +12,14 @@
 // of two): a product's 16 rows are 4 * WP of each of these timesteps, whose words stand in
 // their own quarter or half of the channels beside zeros, so that decoding (7 rows of 4
 // timesteps at 64 channels) fills 14 of 16 rows and every lane loads one word of a key.
-//   den_kernel   sums the weights of a part of kPart keys for kRows or fewer such row tiles
+//   den_kernel   sums the weights of a part of kPart keys for RT or fewer such row tiles
 //                (keys as the product's rows: a lane adds its own row's weights);
-//   mass_kernel  adds the parts' sums in their order, then for a part's keys the weights
-//                over the denominators (keys as its columns: a lane adds its own key's).
-// A part's sums are taken by the same waves in the same order whatever the batch.
+//   mass_kernel  adds the parts' sums in their order, then the weights over the
+//                denominators (keys as its columns: a lane adds its own key's).  With RT row
+//                tiles or fewer (a decode step) a wave holds them and goes through its keys;
+//                with more the four waves of a workgroup have the same keys and share the row
+//                tiles, RT at a time, and their sums are added in wave order.
+// The order of all sums is the sequence's own, whatever the batch.
 #include "spike_tiles.hpp"
 
 namespace spk {
@@ -43,8 +46,8 @@ struct Params {
   int64_t rows;
   uint32_t rep_mul;            // floor(r / nrep) = r * rep_mul >> 32 for every row
   int N, max_rows, T, Hkv, nrep, W, D, bs_log2, max_blocks;
-  int rtiles;                  // row tiles of a timestep group, for max_rows rows
-  int tiles;                   // all row tiles: rtiles * timestep groups
+  int tgroups;                 // timestep groups
+  int tiles;                   // most row tiles of a sequence
   int parts;                   // most parts of a sequence
   float *den;                  // [N, Hkv, parts, tiles, 16]
   float tab[kTab];             // exp((s - D) * scale)
@@ -53,8 +56,10 @@ struct Params {
 struct Seq {
   int64_t first;
   int m, len, parts;
+  int rtiles, tiles;  // row tiles of a timestep group, of all
 };
 
+template <int WP>
 __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   Seq s;
   const int64_t a = p.starts ? p.starts[n] : n, e = p.starts ? p.starts[n + 1] : n + 1;
@@ -62,6 +67,8 @@ __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   s.m = static_cast<int>(min(min(max(e, s.first), s.first + p.max_rows), p.rows) - s.first);
   s.len = min(max(p.lens[n], 0), p.max_blocks << p.bs_log2);
   s.parts = (s.len + kPart - 1) / kPart;
+  s.rtiles = (s.m * p.nrep + 4 * WP - 1) / (4 * WP);
+  s.tiles = s.rtiles * p.tgroups;
   return s;
 }
 
@@ -83,12 +90,11 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int x = tile0 + i;
-      tg[i] = x < p.tiles ? x / p.rtiles : -1;
-      const int r = (x - tg[i] * p.rtiles) * 4 * WP + y % (4 * WP);
+      tg[i] = x < s.tiles ? x / s.rtiles : -1;
+      const int r = (x - tg[i] * s.rtiles) * 4 * WP + y % (4 * WP);
       const int row = row_of(p, r), t = tg[i] * (4 / WP) + dt;
       const bool in = tg[i] >= 0 && row < s.m && t < p.T;
       lim[i] = in ? s.len - s.m + row : -1;
-      if (tg[i] >= 0 && (x - tg[i] * p.rtiles) * 4 * WP >= s.m * p.nrep) tg[i] = -1;
       const int w = b - dt * WP;  // this lane's word of the row's head
       q[i] = fp4_bits(in && w >= 0 && w < WP && w < p.W
                           ? p.q[t * p.qs0 + (s.first + row) * p.qs1 + (kvh * p.nrep + r - row * p.nrep) * p.qs2 + w]
@@ -157,8 +163,8 @@ __global__ __launch_bounds__(kWaves * 64) void den_kernel(Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = blockIdx.x % p.parts, chunk = blockIdx.x / p.parts;
   const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
-  const Seq s = sequence(p, n);
-  if (part >= s.parts || s.m == 0) return;
+  const Seq s = sequence<WP>(p, n);
+  if (part >= s.parts || chunk * RT >= s.tiles) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
   Rows<WP, RT> rows;
   rows.load(p, s, kvh, chunk * RT, lane);
@@ -206,106 +212,142 @@ __global__ __launch_bounds__(kWaves * 64) void den_kernel(Params p) {
   __syncthreads();
   float *to = p.den + ((static_cast<int64_t>(blockIdx.y) * p.parts + part) * p.tiles + chunk * RT) * 16;
   for (int x = tid; x < RT * 16; x += kWaves * 64)
-    if (chunk * RT + x / 16 < p.tiles)
+    if (chunk * RT + x / 16 < s.tiles)
       to[x] = (sm.sum[0][x / 16][x % 16] + sm.sum[1][x / 16][x % 16]) + (sm.sum[2][x / 16][x % 16] + sm.sum[3][x / 16][x % 16]);
 }
 
-template <int WP, int RT>
+// SHARED: the waves have the same kStep * STEPS keys and share the row tiles; else each has
+// STEPS steps of its own.
+template <int WP, int RT, int STEPS, bool SHARED>
 __global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
-  constexpr int kSteps = kPart / (kWaves * kStep);  // of a wave
+  constexpr int kKeys = STEPS * kStep * (SHARED ? 1 : kWaves);  // of a workgroup
   struct Smem {
     float tab[kTab + 3];
-    float inv[RT][16];
-    int lim[RT][16];
+    float inv[kWaves][RT][16];
+    int lim[kWaves][RT][16];
+    float sum[SHARED ? kWaves : 1][kKeys];
   };
   __shared__ Smem sm;
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = blockIdx.x, kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
-  const Seq s = sequence(p, n);
+  const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
+  const Seq s = sequence<WP>(p, n);
   float *mass = p.mass + n * p.ms0 + kvh * p.ms1;
-  const int64_t from = static_cast<int64_t>(part) * kPart, stop = min(p.cap, from + kPart);
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * kKeys, stop = min(p.cap, from + kKeys);
   if (!p.accumulate)
     for (int64_t j = max<int64_t>(from, s.len) + tid; j < stop; j += kWaves * 64) mass[j] = 0.f;
-  if (part >= s.parts || from >= p.cap) return;
+  if (from >= s.len || from >= p.cap) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
+  __syncthreads();
   const Keys<WP> keys(p, s, n, kvh, lane);
-  const int end = min(s.len, (part + 1) * kPart), open = s.len - s.m;
-  float sum[kSteps][4];
-#pragma unroll
-  for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) sum[st][u] = 0.f;
+  const int end = min(s.len, static_cast<int>(stop)), open = s.len - s.m;  // keys up to `open` are seen by all rows
   const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tiles * 16;
-  for (int tile0 = 0; tile0 < p.tiles && s.m > 0; tile0 += RT) {
-    Rows<WP, RT> rows;
+
+  Rows<WP, RT> rows;
+  float inv[RT][4];  // of the products' rows 4 * (l / 16) + 0..3; no row: 0
+  auto take = [&](int tile0) {  // row tiles tile0 .. and their denominators, a wave by itself
     rows.load(p, s, kvh, tile0, lane);
-    if (tile0) __syncthreads();  // (the rows before are read)
-    if (wave == 0 && lane < 16) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) sm.lim[i][lane] = rows.lim[i];
-    }
-    for (int x = tid; x < RT * 16; x += kWaves * 64) {
+    for (int i = 0; i < RT; i += 4) {  // lane: row l % 16 of tile i + l / 16
+      const int x = i + (lane >> 4);
       float d = 0.f;
-      if (tile0 + x / 16 < p.tiles)
-        for (int pt = 0; pt < s.parts; ++pt) d += den[(static_cast<int64_t>(pt) * p.tiles + tile0) * 16 + x];
-      sm.inv[x / 16][x % 16] = d > 0.f ? 1.f / d : 0.f;
+      if (x < RT && tile0 + x < s.tiles) {
+        const float *at = den + (tile0 + x) * 16 + (lane & 15);
+        for (int pt = 0; pt < s.parts; pt += 8) {  // eight parts' sums on their way at once
+          float y[8];
+#pragma unroll
+          for (int v = 0; v < 8; ++v) y[v] = at[static_cast<int64_t>(min(pt + v, s.parts - 1)) * p.tiles * 16];
+#pragma unroll
+          for (int v = 0; v < 8; ++v) d += pt + v < s.parts ? y[v] : 0.f;
+        }
+      }
+      if (x < RT) sm.inv[wave][x][lane & 15] = d > 0.f ? 1.f / d : 0.f;
     }
-    __syncthreads();
-    float inv[RT][4];  // of the product's rows 4 * (l / 16) + 0..3; no row: 0
+    if (lane < 16) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) sm.lim[wave][i][lane] = rows.lim[i];
+    }
+    wave_lds_sync();
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int y = 4 * (lane >> 4) + e;
-        inv[i][e] = sm.lim[i][y] >= 0 ? sm.inv[i][y] : 0.f;
+        inv[i][e] = sm.lim[wave][i][y] >= 0 ? sm.inv[wave][i][y] : 0.f;
+      }
+  };
+  auto add = [&](int j0, float (&sum)[4]) {  // what the rows give the 64 keys at j0
+    int64_t at[4];
+    keys.slots(j0, at);
+    v8i k[4];
+    int have = -1;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      if (rows.tg[i] < 0) continue;
+      if (rows.tg[i] != have) {
+        uint32_t x[4];
+        keys.load(rows.tg[i], at, x);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
+        have = rows.tg[i];
       }
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const int j0 = part * kPart + (st * kWaves + wave) * kStep;
-      if (j0 >= end) break;
-      int64_t at[4];
-      keys.slots(j0, at);
-      v8i k[4];
-      int have = -1;
+      for (int u = 0; u < 4; ++u) {
+        const v4f a = score(rows.q[i], k[u]);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
+        float w[4];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rows.tg[i] < 0) continue;
-        if (rows.tg[i] != have) {
-          uint32_t x[4];
-          keys.load(rows.tg[i], at, x);
+        for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
+        if (j0 + 16 * u + 15 > open) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
-          have = rows.tg[i];
+          for (int e = 0; e < 4; ++e)
+            w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[wave][i][4 * (lane >> 4) + e] ? w[e] : 0.f;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const v4f a = score(rows.q[i], k[u]);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
-          if (j0 + 16 * u + 15 > open) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[i][4 * (lane >> 4) + e] ? w[e] : 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[st][u] = __builtin_fmaf(w[e], inv[i][e], sum[st][u]);
-        }
+        for (int e = 0; e < 4; ++e) sum[u] = __builtin_fmaf(w[e], inv[i][e], sum[u]);
       }
+    }
+  };
+  auto finish = [&](int j, float x) {
+    if (j < end) mass[j] = p.accumulate ? mass[j] + x : x;
+  };
+  if constexpr (SHARED) {
+    float sum[STEPS][4] = {};
+    for (int tile0 = wave * RT; tile0 < s.tiles; tile0 += kWaves * RT) {
+      take(tile0);
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st)
+        if (from + st * kStep < end) add(static_cast<int>(from) + st * kStep, sum[st]);
+      wave_lds_sync();  // (the limits are read before the next tiles' come)
+    }
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float x = sum[st][u];
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if (lane < 16) sm.sum[wave][st * kStep + 16 * u + lane] = x;
+      }
+    __syncthreads();
+    for (int x = tid; x < kKeys; x += kWaves * 64)
+      finish(static_cast<int>(from) + x, (sm.sum[0][x] + sm.sum[1][x]) + (sm.sum[2][x] + sm.sum[3][x]));
+  } else {
+    take(0);
+#pragma unroll 1
+    for (int j0 = static_cast<int>(from) + wave * kStep; j0 < end; j0 += kWaves * kStep) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      add(j0, sum);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        sum[u] += __shfl_xor(sum[u], 16);
+        sum[u] += __shfl_xor(sum[u], 32);
+      }
+      // lane l: key l of the step
+      const float x = lane < 32 ? (lane < 16 ? sum[0] : sum[1]) : (lane < 48 ? sum[2] : sum[3]);
+      finish(j0 + lane, x);
     }
   }
-#pragma unroll
-  for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float x = sum[st][u];
-      x += __shfl_xor(x, 16);
-      x += __shfl_xor(x, 32);
-      const int j = part * kPart + (st * kWaves + wave) * kStep + 16 * u + (lane & 15);
-      if (lane < 16 && j < end && j < p.cap) mass[j] = p.accumulate ? mass[j] + x : x;
-    }
 }
 
 // exp((s - D) * scale), s = 0..D.
@@ -322,7 +364,7 @@ inline void build_weights(float scale, int D, float *tab) {
 
 // Rows of a product's timestep, timestep groups, row tiles.
 struct Plan {
-  int wp, rtiles, tiles, parts;
+  int wp, tgroups, tiles, parts;
   size_t bytes;
 };
 inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_size, int max_blocks) {
@@ -330,28 +372,30 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_s
   const int W = (D + 31) / 32;
   r.wp = W == 3 ? 4 : W;
   const int64_t rows = static_cast<int64_t>(max_rows) * (Hq / Hkv);
-  r.rtiles = static_cast<int>((rows + 4 * r.wp - 1) / (4 * r.wp));
-  r.tiles = r.rtiles * ((T + 4 / r.wp - 1) / (4 / r.wp));
+  r.tgroups = (T + 4 / r.wp - 1) / (4 / r.wp);
+  r.tiles = static_cast<int>((rows + 4 * r.wp - 1) / (4 * r.wp)) * r.tgroups;
   r.parts = static_cast<int>((static_cast<int64_t>(max_blocks) * block_size + kPart - 1) / kPart);
   r.bytes = static_cast<size_t>(N) * Hkv * r.parts * r.tiles * 16 * sizeof(float);
   return r;
 }
 
-template <int WP, int RT>
+template <int WP, int RT, int STEPS, bool SHARED>
 static int launch(const Params &p, hipStream_t s) {
-  const int chunks = (p.tiles + RT - 1) / RT, zero = static_cast<int>((p.cap + kPart - 1) / kPart);
-  const int wide = p.accumulate || zero < p.parts ? p.parts : zero;  // (entries behind the table become 0)
+  const int chunks = (p.tiles + RT - 1) / RT, keys = STEPS * kStep * (SHARED ? 1 : kWaves);
+  // (without accumulation entries behind the table become 0)
+  const int64_t tokens = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
+  const int64_t wide = p.accumulate && tokens < p.cap ? tokens : p.cap;
   if (p.parts > 0 && p.rows > 0) den_kernel<WP, RT><<<dim3(p.parts * chunks, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
-  if (wide > 0) mass_kernel<WP, RT><<<dim3(wide, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
+  mass_kernel<WP, RT, STEPS, SHARED><<<dim3((wide + keys - 1) / keys, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
   return check_launch("key_mass");
 }
 
+// Row tiles a wave holds in registers: those of a decode step, or eight.
 template <int WP>
 static int launch_rows(const Params &p, hipStream_t s) {
-  // row tiles a workgroup holds in registers: those of a decode step, or eight
-  if (p.tiles <= 2) return launch<WP, 2>(p, s);
-  if (p.tiles <= 4) return launch<WP, 4>(p, s);
-  return launch<WP, 8>(p, s);
+  if (p.tiles <= 2) return launch<WP, 2, 4, false>(p, s);
+  if (p.tiles <= 4) return launch<WP, 4, 4, false>(p, s);
+  return launch<WP, 8, 2, true>(p, s);
 }
 
 }  // namespace mass
@@ -384,13 +428,13 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
     return fail(SPK_EUNSUPPORTED, "key_mass: block tables of %d x %d tokens (at most 2^30)", max_blocks, block_size);
   if (!(scale > 0.f) || scale * head_dim > 12.f)
     return fail(SPK_EINVAL, "key_mass: scale=%g outside (0, 12/head_dim]", (double)scale);
-  if (N == 0 || cap == 0) return SPK_OK;
+  if (N == 0 || cap == 0 || (accumulate && max_blocks == 0)) return SPK_OK;
   if (static_cast<int64_t>(N) * Hkv > 65535) return fail(SPK_EUNSUPPORTED, "key_mass: %d sequences of %d heads", N, Hkv);
   if ((rows > 0 && !q) || !seq_lens || !mass || (max_blocks > 0 && !block_tables) || (num_slots > 0 && !k_cache))
     return fail(SPK_EINVAL, "key_mass: null pointer");
   const mass::Plan plan = mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks);
   if (static_cast<int64_t>(max_rows) * (Hq / Hkv) > (1 << 24) ||
-      static_cast<int64_t>(plan.tiles) * plan.parts > (1 << 30))
+      static_cast<int64_t>(plan.tiles) * plan.parts > (1 << 30) || cap > (1 << 30))
     return fail(SPK_EUNSUPPORTED, "key_mass: %d rows of %d heads over %d x %d tokens", max_rows, Hq / Hkv, max_blocks,
                 block_size);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
@@ -409,7 +453,7 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
   p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
   p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks;
-  p.rtiles = plan.rtiles; p.tiles = plan.tiles; p.parts = plan.parts;
+  p.tgroups = plan.tgroups; p.tiles = plan.tiles; p.parts = plan.parts;
   p.den = static_cast<float *>(workspace);
   mass::build_weights(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
