@@ -135,11 +135,15 @@ struct Keys {
                   : -1;
     }
   }
+  // (unconditional loads, dropped where there is no key or word: they are all on their way
+  // before the first is waited for)
   __device__ __forceinline__ void load(int tg, const int64_t (&at)[4], uint32_t (&x)[4]) const {
     const int t = tg * (4 / WP) + dt;
     const bool in = t < p.T && w < p.W;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = in && at[u] >= 0 ? base[t * p.ks0 + at[u] + w] : 0u;
+    for (int u = 0; u < 4; ++u) x[u] = base[in && at[u] >= 0 ? t * p.ks0 + at[u] + w : 0];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = in && at[u] >= 0 ? x[u] : 0u;
   }
 };
 
@@ -149,6 +153,18 @@ __device__ __forceinline__ v4f score(const v8i &a, const v8i &b) {
 
 __device__ __forceinline__ float weight(uint32_t tab0, float score) {
   return *reinterpret_cast<const SPK_LDS float *>(static_cast<uintptr_t>(tab0 + __float_as_uint(score)));
+}
+
+// Key words of all of a wave's steps for each row tile.
+template <int WP, int RT, int STEPS>
+__device__ __forceinline__ void request(const Keys<WP> &keys, const int (&tg)[RT], int j1, uint32_t (&x)[STEPS][RT][4]) {
+  int64_t at[STEPS][4];
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) keys.slots(j1 + st * kWaves * kStep, at[st]);
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) keys.load(max(tg[i], 0), at[st], x[st][i]);
 }
 
 template <int WP, int RT>
@@ -174,32 +190,51 @@ __global__ __launch_bounds__(kWaves * 64) void den_kernel(Params p) {
   for (int i = 0; i < RT; ++i) l[i] = 0.f;
   __syncthreads();
   const int end = min(s.len, (part + 1) * kPart), open = s.len - s.m;  // keys up to `open` are seen by all rows
-  for (int j0 = part * kPart + wave * kStep; j0 < end; j0 += kWaves * kStep) {
-    int64_t at[4];
-    keys.slots(j0, at);
-    v8i k[4];
-    int have = -1;
+  auto add = [&](int i, int u, int j0, const v8i &k) {
+    const v4f a = score(k, rows.q[i]);  // lane: row l % 16, keys 4 * (l / 16) + 0..3
+    float w[4];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (rows.tg[i] < 0) continue;
-      if (rows.tg[i] != have) {
-        uint32_t x[4];
-        keys.load(rows.tg[i], at, x);
+    for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
+    if (j0 + 16 * u + 15 > open) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
-        have = rows.tg[i];
+      for (int e = 0; e < 4; ++e) w[e] = j0 + 16 * u + 4 * (lane >> 4) + e <= rows.lim[i] ? w[e] : 0.f;
+    }
+    l[i] += (w[0] + w[1]) + (w[2] + w[3]);
+  };
+  const int j1 = part * kPart + wave * kStep;
+  if constexpr (RT == 2) {  // few products a key: the words of all steps are requested first
+    constexpr int kSteps = kPart / (kWaves * kStep);
+    uint32_t x[kSteps][RT][4];
+    request<WP, RT, kSteps>(keys, rows.tg, j1, x);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int j0 = j1 + st * kWaves * kStep;
+      if (j0 >= end) break;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (rows.tg[i] < 0) continue;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) add(i, u, j0, fp4_bits(x[st][i][u]));
       }
+    }
+  } else {
+    for (int j0 = j1; j0 < end; j0 += kWaves * kStep) {
+      int64_t at[4];
+      keys.slots(j0, at);
+      v8i k[4];
+      int have = -1;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const v4f a = score(k[u], rows.q[i]);  // lane: row l % 16, keys 4 * (l / 16) + 0..3
-        float w[4];
+      for (int i = 0; i < RT; ++i) {
+        if (rows.tg[i] < 0) continue;
+        if (rows.tg[i] != have) {
+          uint32_t x[4];
+          keys.load(rows.tg[i], at, x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
-        if (j0 + 16 * u + 15 > open) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = j0 + 16 * u + 4 * (lane >> 4) + e <= rows.lim[i] ? w[e] : 0.f;
+          for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
+          have = rows.tg[i];
         }
-        l[i] += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) add(i, u, j0, k[u]);
       }
     }
   }
@@ -277,6 +312,19 @@ __global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
         inv[i][e] = sm.lim[wave][i][y] >= 0 ? sm.inv[wave][i][y] : 0.f;
       }
   };
+  auto give = [&](int i, int u, int j0, const v8i &k, float &sum) {
+    const v4f a = score(rows.q[i], k);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
+    if (j0 + 16 * u + 15 > open) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[wave][i][4 * (lane >> 4) + e] ? w[e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(w[e], inv[i][e], sum);
+  };
   auto add = [&](int j0, float (&sum)[4]) {  // what the rows give the 64 keys at j0
     int64_t at[4];
     keys.slots(j0, at);
@@ -293,19 +341,7 @@ __global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
         have = rows.tg[i];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const v4f a = score(rows.q[i], k[u]);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
-        if (j0 + 16 * u + 15 > open) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[wave][i][4 * (lane >> 4) + e] ? w[e] : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[u] = __builtin_fmaf(w[e], inv[i][e], sum[u]);
-      }
+      for (int u = 0; u < 4; ++u) give(i, u, j0, k[u], sum[u]);
     }
   };
   auto finish = [&](int j, float x) {
@@ -333,11 +369,25 @@ __global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
     for (int x = tid; x < kKeys; x += kWaves * 64)
       finish(static_cast<int>(from) + x, (sm.sum[0][x] + sm.sum[1][x]) + (sm.sum[2][x] + sm.sum[3][x]));
   } else {
+    // few products a key: the words of all steps are requested first
+    const int j1 = static_cast<int>(from) + wave * kStep;
+    int tg[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) tg[i] = i < s.tiles ? i / s.rtiles : 0;
+    uint32_t words[STEPS][RT][4];
+    request<WP, RT, STEPS>(keys, tg, j1, words);
     take(0);
-#pragma unroll 1
-    for (int j0 = static_cast<int>(from) + wave * kStep; j0 < end; j0 += kWaves * kStep) {
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      const int j0 = j1 + st * kWaves * kStep;
+      if (j0 >= end) break;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      add(j0, sum);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (rows.tg[i] < 0) continue;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) give(i, u, j0, fp4_bits(words[st][i][u]), sum[u]);
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         sum[u] += __shfl_xor(sum[u], 16);
@@ -394,7 +444,7 @@ static int launch(const Params &p, hipStream_t s) {
 template <int WP>
 static int launch_rows(const Params &p, hipStream_t s) {
   if (p.tiles <= 2) return launch<WP, 2, 4, false>(p, s);
-  if (p.tiles <= 4) return launch<WP, 4, 4, false>(p, s);
+  if (p.tiles <= 4) return launch<WP, 4, 2, false>(p, s);
   return launch<WP, 8, 2, true>(p, s);
 }
 
@@ -445,6 +495,10 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   p.k = reinterpret_cast<const uint32_t *>(k_cache);
   p.ks0 = cache_strides[0]; p.ks1 = cache_strides[1]; p.ks2 = cache_strides[2];
   p.num_slots = num_slots;
+  if (num_slots < block_size && q) {  // no block of a cache: every key is dropped, the loads read q's words
+    p.k = p.q;
+    p.ks0 = p.ks1 = p.ks2 = 0;
+  }
   p.bt = block_tables; p.bts0 = bt_stride0; p.bts1 = bt_stride1;
   p.lens = seq_lens; p.starts = row_starts;
   p.mass = mass; p.ms0 = mass_strides[0]; p.ms1 = mass_strides[1]; p.cap = cap;
