@@ -192,7 +192,9 @@ def load(path: str | None = None) -> ctypes.CDLL:
 NATIVE_FUNCTIONS = (
     "spk_decode_attn", "spk_decode_attn_workspace_bytes", "spk_lif_pack_write_sites", "spk_lif_multistep",
     "spk_prefill_attn", "spk_embed_rmsnorm", "spk_add_rmsnorm", "spk_rmsnorm_mean_t", "spk_lif_gate_mul",
-    "spk_linear_decode", "spk_mlp_gate_lif", "spk_qkv_rope_lif_pack_kv", "spk_last_error",
+    "spk_linear_decode", "spk_mlp_gate_lif", "spk_qkv_rope_lif_pack_kv", "spk_tree_attn",
+    "spk_tree_attn_workspace_bytes", "spk_accept_tree", "spk_key_mass", "spk_key_mass_workspace_bytes", "spk_evict",
+    "spk_last_error",
 )
 
 _UNBOUND = object()

@@ -19,12 +19,14 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <cmath>
 #include <cstring>
+#include <vector>
 
 #include "../../include/spikeinfer_amd.h"
 
@@ -46,6 +48,12 @@ decltype(&spk_lif_gate_mul) gate_mul_fn;
 decltype(&spk_linear_decode) linear_fn;
 decltype(&spk_mlp_gate_lif) mlp_gate_fn;
 decltype(&spk_qkv_rope_lif_pack_kv) qkv_fn;
+decltype(&spk_tree_attn) tree_fn;
+decltype(&spk_tree_attn_workspace_bytes) tree_workspace_fn;
+decltype(&spk_accept_tree) accept_fn;
+decltype(&spk_key_mass) mass_fn;
+decltype(&spk_key_mass_workspace_bytes) mass_workspace_fn;
+decltype(&spk_evict) evict_fn;
 decltype(&spk_last_error) last_error_fn;
 
 // A call this module does not take (never seen by the caller).
@@ -555,12 +563,250 @@ PyObject *qkv_rope_lif_pack(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// The current device is `t`'s (a kernel of another goes through the wrapper, which changes it).
+void here(const at::Tensor &t) { need(taken_on != at::kCUDA || c10::hip::current_device() == t.device().index()); }
+
+// An int32 vector of at least n entries on `like`'s device.
+const int32_t *ints(PyObject *o, int64_t n, const at::Tensor &like) {
+  const at::Tensor &t = tensor(o);
+  need(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.numel() >= n && t.device() == like.device());
+  return static_cast<const int32_t *>(t.data_ptr());
+}
+const int64_t *longs(PyObject *o, int64_t n, const at::Tensor &like) {
+  const at::Tensor &t = tensor(o);
+  need(t.scalar_type() == at::kLong && t.dim() == 1 && t.is_contiguous() && t.numel() == n && t.device() == like.device());
+  return static_cast<const int64_t *>(t.data_ptr());
+}
+// Block tables, int32 [N, blocks] on `like`'s device.
+const at::Tensor &block_table(PyObject *o, const at::Tensor &like) {
+  const at::Tensor &t = tensor(o);
+  need(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) < (1 << 24) && t.size(1) < (1 << 28) &&
+       t.device() == like.device());
+  return t;
+}
+// Scratch of `bytes` bytes: the caller's, or a new tensor (which has to live until the launch).
+void *scratch(PyObject *given, size_t bytes, const at::Tensor &like, at::Tensor &made) {
+  if (!bytes) return nullptr;
+  if (given == Py_None) {
+    made = empty({static_cast<int64_t>(bytes)}, at::kByte, like);
+  } else {
+    made = tensor(given);
+    need(made.is_contiguous() && static_cast<size_t>(made.nbytes()) >= bytes && made.device() == like.device());
+  }
+  return made.data_ptr();
+}
+int32_t *words(const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
+
+// Every layer's (k, v), packed tensors of one shape, layout and device: their addresses.
+const at::Tensor &layer_words(PyObject *o, std::vector<int32_t *> &to) {
+  need(PyList_CheckExact(o) || PyTuple_CheckExact(o));
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  need(n > 0 && n < (1 << 20));
+  to.reserve(2 * n);
+  const at::Tensor *first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject *pair = PySequence_Fast_GET_ITEM(o, i);
+    need(PyTuple_CheckExact(pair) && PyTuple_GET_SIZE(pair) == 2);
+    for (int j = 0; j < 2; ++j) {
+      const at::Tensor &t = tensor(PyTuple_GET_ITEM(pair, j));
+      if (!first) {
+        first = &t;
+        need(packed4(t));
+      }
+      need(t.scalar_type() == at::kInt && t.sizes() == first->sizes() && t.strides() == first->strides() &&
+           t.device() == first->device());
+      to.push_back(words(t));
+    }
+  }
+  return *first;
+}
+
+// tree_attn(q, k_words, v_words, k_cache, v_cache, tables, lens, starts, masks, max_nodes, head_dim, block_size,
+//           out|None, dtype, workspace|None) -> out
+PyObject *tree_attn(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 15, [&]() -> PyObject * {
+    const at::Tensor &q = tensor(a[0]), &kt = tensor(a[1]), &vt = tensor(a[2]), &k = tensor(a[3]), &v = tensor(a[4]);
+    here(q);
+    const int nodes = int32(a[9]), D = int32(a[10]), bs = int32(a[11]);
+    need(packed4(q) && packed4(kt) && packed4(vt) && packed4(k) && packed4(v) && D > 0 && D <= 128 && nodes > 0);
+    const int64_t T = q.size(0), R = q.size(1), Hq = q.size(2), W = q.size(3), Hkv = k.size(1);
+    need(W == (D + 31) / 32 && T < (1 << 16) && Hq < (1 << 16) && Hkv > 0 && R > 0);
+    need(k.sizes() == v.sizes() && k.strides() == v.strides() && k.size(0) == T && k.size(3) == W);
+    need(kt.sizes() == vt.sizes() && kt.strides() == vt.strides() && kt.size(0) == T && kt.size(1) == R &&
+         kt.size(2) == Hkv && kt.size(3) == W);
+    need(k.device() == q.device() && v.device() == q.device() && kt.device() == q.device() && vt.device() == q.device());
+    const at::Tensor &bt = block_table(a[5], q);
+    const int64_t N = bt.size(0);
+    need(N > 0);
+    const int32_t *lens = ints(a[6], N, q), *starts = ints(a[7], N + 1, q);
+    const at::Tensor &masks = tensor(a[8]);
+    need(masks.scalar_type() == at::kLong && masks.dim() == 2 && masks.is_contiguous() && masks.size(0) == R &&
+         masks.size(1) < (1 << 20) && masks.device() == q.device());
+    at::Tensor out;
+    if (a[12] == Py_None) {
+      out = at::zeros({T, R, Hq, D}, at::TensorOptions().dtype(dtype_of(a[13])).device(q.device()));
+    } else {
+      out = tensor(a[12]);
+      need(out.dim() == 4 && out.size(0) == T && out.size(1) == R && out.size(2) == Hq && out.size(3) == D &&
+           out.stride(3) == 1 && out.device() == q.device());
+    }
+    const int code = float_code(out.scalar_type()), mb = static_cast<int>(bt.size(1));
+    const size_t bytes = tree_workspace_fn(T, N, Hq, Hkv, D, nodes, bs, mb);
+    at::Tensor ws;
+    void *const at = scratch(a[14], bytes, q, ws);
+    const Strides qs(q), ts(kt), ks(k), os(out);
+    void *const stream = stream_of(q);
+    THPObjectPtr done = result(a[12], out);
+    launch("paged_spike_attn_tree", tree_fn, words(q), qs.s, words(kt), words(vt), ts.s, words(k), words(v), ks.s,
+           k.size(2), words(bt), bt.stride(0), bt.stride(1), lens, starts, static_cast<const int64_t *>(masks.data_ptr()),
+           static_cast<int>(masks.size(1)), out.data_ptr(), code, os.s, R, static_cast<int>(N), nodes,
+           static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), D, bs, mb,
+           static_cast<float>(1.0 / std::sqrt(static_cast<double>(D))), at, bytes, stream);
+    return done.release();
+  });
+}
+
+// accept_tree(tokens, parents, targets, starts, max_nodes, drafts, layers, tables, lens, block_size, out|None)
+// -> (path, count, next); at least one layer
+PyObject *accept_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject * {
+    const at::Tensor &tokens = tensor(a[0]);
+    here(tokens);
+    const int64_t R = tokens.numel();
+    const int64_t *tok = longs(a[0], R, tokens), *tgt = longs(a[2], R, tokens);
+    const int32_t *par = ints(a[1], R, tokens);
+    const int nodes = int32(a[4]), bs = int32(a[9]);
+    need(nodes > 0 && nodes <= 1024);
+    const at::Tensor &bt = block_table(a[7], tokens);
+    const int64_t N = bt.size(0);
+    need(tensor(a[3]).numel() == N + 1);
+    const int32_t *starts = ints(a[3], N + 1, tokens), *lens = ints(a[8], N, tokens);
+    std::vector<int32_t *> fresh, cache;
+    const at::Tensor &nw = layer_words(a[5], fresh), &ck = layer_words(a[6], cache);
+    const int64_t T = ck.size(0), Hkv = ck.size(1), W = ck.size(3);
+    need(fresh.size() == cache.size() && nw.device() == tokens.device() && ck.device() == tokens.device() &&
+         nw.size(0) == T && nw.size(1) == R && nw.size(2) == Hkv && nw.size(3) == W && T < (1 << 16) &&
+         Hkv < (1 << 16) && W < (1 << 10));
+    std::vector<SpkCommitLayer> layers(cache.size() / 2);
+    for (size_t i = 0; i < layers.size(); ++i)
+      layers[i] = SpkCommitLayer{fresh[2 * i], fresh[2 * i + 1], cache[2 * i], cache[2 * i + 1]};
+    at::Tensor out[3];
+    THPObjectPtr done;
+    if (a[10] == Py_None) {
+      out[0] = empty({N, nodes}, at::kInt, tokens);
+      out[1] = empty({N}, at::kInt, tokens);
+      out[2] = empty({N}, at::kLong, tokens);
+      done = THPObjectPtr(PyTuple_New(3));
+      need(done.get() != nullptr);
+      for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(done.get(), i, THPVariable_Wrap(out[i]));
+    } else {
+      need(PyTuple_CheckExact(a[10]) && PyTuple_GET_SIZE(a[10]) == 3);
+      for (int i = 0; i < 3; ++i) {
+        out[i] = tensor(PyTuple_GET_ITEM(a[10], i));
+        need(out[i].is_contiguous() && out[i].device() == tokens.device() && out[i].dim() == (i ? 1 : 2) &&
+             out[i].size(0) == N && out[i].scalar_type() == (i < 2 ? at::kInt : at::kLong));
+      }
+      need(out[0].size(1) == nodes);
+      done = THPObjectPtr(Py_NewRef(a[10]));
+    }
+    const Strides ns(nw), ks(ck);
+    void *const stream = stream_of(tokens);
+    launch("accept_draft_tree", accept_fn, tok, par, tgt, starts, R, static_cast<int>(N), nodes, words(out[0]),
+           words(out[1]), static_cast<int64_t *>(out[2].data_ptr()), layers.data(), static_cast<int>(layers.size()),
+           ns.s, ks.s, ck.size(2), words(bt), bt.stride(0), bt.stride(1), lens, static_cast<int>(T),
+           static_cast<int>(Hkv), static_cast<int>(32 * W), bs, static_cast<int>(bt.size(1)), stream);
+    return done.release();
+  });
+}
+
+// key_mass(q, k_cache, tables, lens, head_dim, block_size, starts|None, max_rows, out|None, accumulate,
+//          workspace|None) -> out
+PyObject *key_mass(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject * {
+    const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]);
+    here(q);
+    const int D = int32(a[4]), bs = int32(a[5]);
+    need(packed4(q) && packed4(k) && D > 0 && D <= 128 && bs > 0 && PyBool_Check(a[9]));
+    const int64_t T = q.size(0), R = q.size(1), Hq = q.size(2), W = q.size(3), Hkv = k.size(1);
+    need(W == (D + 31) / 32 && k.size(0) == T && k.size(3) == W && T < (1 << 16) && Hq < (1 << 16) && Hkv > 0 &&
+         k.device() == q.device());
+    const at::Tensor &bt = block_table(a[2], q);
+    const int64_t N = bt.size(0);
+    const int mb = static_cast<int>(bt.size(1));
+    const int32_t *lens = ints(a[3], N, q), *starts = nullptr;
+    int rows = 1;
+    if (a[6] != Py_None) {
+      starts = ints(a[6], N + 1, q);
+      rows = int32(a[7]);
+      need(rows > 0);
+    } else {
+      need(R >= N);
+    }
+    const bool accumulate = a[9] == Py_True;
+    at::Tensor out;
+    if (a[8] == Py_None) {
+      need(!accumulate);
+      out = empty({N, Hkv, static_cast<int64_t>(mb) * bs}, at::kFloat, q);
+    } else {
+      out = tensor(a[8]);
+      need(out.dim() == 3 && out.size(0) == N && out.size(1) == Hkv && out.scalar_type() == at::kFloat &&
+           out.stride(2) == 1 && out.device() == q.device());
+    }
+    const size_t bytes = mass_workspace_fn(T, N, Hq, Hkv, D, rows, bs, mb);
+    at::Tensor ws;
+    void *const at = scratch(a[10], bytes, q, ws);
+    const Strides qs(q), ks(k);
+    const int64_t os[2] = {out.stride(0), out.stride(1)};
+    void *const stream = stream_of(q);
+    THPObjectPtr done = result(a[8], out);
+    launch("paged_spike_attn_key_mass", mass_fn, words(q), qs.s, words(k), ks.s, k.size(2), words(bt), bt.stride(0),
+           bt.stride(1), lens, starts, static_cast<float *>(out.data_ptr()), os, out.size(2), accumulate ? 1 : 0, R,
+           static_cast<int>(N), rows, static_cast<int>(T), static_cast<int>(Hq), static_cast<int>(Hkv), D, bs, mb,
+           static_cast<float>(1.0 / std::sqrt(static_cast<double>(D))), at, bytes, stream);
+    return done.release();
+  });
+}
+
+// evict(layers, mass, tables, lens, budget, block_size, sinks, recent, dst_tables|None, mass_out|None)
+// -> (keep, new_lens)
+PyObject *evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject * {
+    std::vector<int32_t *> cache;
+    const at::Tensor &ck = layer_words(a[0], cache), &mass = tensor(a[1]);
+    here(ck);
+    const at::Tensor &bt = block_table(a[2], ck);
+    const int64_t N = bt.size(0), L = static_cast<int64_t>(cache.size()) / 2, Hkv = ck.size(1);
+    const int32_t *lens = ints(a[3], N, ck);
+    const int budget = int32(a[4]), bs = int32(a[5]), sinks = int32(a[6]), recent = int32(a[7]);
+    need(budget > 0 && ck.size(0) < (1 << 16) && Hkv < (1 << 16) && ck.size(3) < (1 << 10));
+    const at::Tensor *dst = a[8] == Py_None ? nullptr : &block_table(a[8], ck);
+    need(!dst || dst->size(0) == N);
+    const at::Tensor &to = a[9] == Py_None ? mass : tensor(a[9]);
+    for (const at::Tensor *t : {&mass, &to})
+      need(t->scalar_type() == at::kFloat && t->dim() == 4 && t->stride(3) == 1 && t->size(0) == L && t->size(1) == N &&
+           t->size(2) == Hkv && t->size(3) == mass.size(3) && t->device() == ck.device());
+    std::vector<SpkCacheLayer> layers(L);
+    for (int64_t i = 0; i < L; ++i) layers[i] = SpkCacheLayer{cache[2 * i], cache[2 * i + 1]};
+    const at::Tensor keep = empty({L, N, Hkv, budget}, at::kInt, ck), kept = empty({N}, at::kInt, ck);
+    const Strides ks(ck), ms(mass), os(to);
+    void *const stream = stream_of(ck);
+    THPObjectPtr done = pair(keep, kept);
+    launch("evict_cache", evict_fn, layers.data(), static_cast<int>(L), ks.s, ck.size(2),
+           static_cast<const float *>(mass.data_ptr()), ms.s, static_cast<float *>(to.data_ptr()), os.s, mass.size(3),
+           words(bt), bt.stride(0), bt.stride(1), static_cast<int>(bt.size(1)), dst ? words(*dst) : nullptr,
+           dst ? dst->stride(0) : 0, dst ? dst->stride(1) : 0, dst ? static_cast<int>(dst->size(1)) : 0, lens,
+           words(kept), words(keep), budget, sinks, recent, static_cast<int>(ck.size(0)), static_cast<int>(N),
+           static_cast<int>(Hkv), static_cast<int>(32 * ck.size(3)), bs, stream);
+    return done.release();
+  });
+}
+
 template <class F> void set(F &f, void *p) { f = reinterpret_cast<F>(p); }
 
 // bind(device, addresses): "cuda" or "cpu", and the C ABI's functions in the order of
 // the declarations above.
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  constexpr int kFns = 13;
+  constexpr int kFns = 19;
   if (n != kFns + 1 || !PyUnicode_Check(a[0])) {
     PyErr_Format(PyExc_TypeError, "bind takes a device type and %d addresses", kFns);
     return nullptr;
@@ -587,7 +833,13 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   set(linear_fn, p[9]);
   set(mlp_gate_fn, p[10]);
   set(qkv_fn, p[11]);
-  set(last_error_fn, p[12]);
+  set(tree_fn, p[12]);
+  set(tree_workspace_fn, p[13]);
+  set(accept_fn, p[14]);
+  set(mass_fn, p[15]);
+  set(mass_workspace_fn, p[16]);
+  set(evict_fn, p[17]);
+  set(last_error_fn, p[18]);
   Py_RETURN_NONE;
 }
 
@@ -597,6 +849,7 @@ PyMethodDef methods[] = {
     SPK_METHOD(bind),          SPK_METHOD(decode_attn),       SPK_METHOD(lif_sites),    SPK_METHOD(lif),
     SPK_METHOD(prefill),       SPK_METHOD(embed_rmsnorm),     SPK_METHOD(add_rmsnorm),  SPK_METHOD(rmsnorm_mean_t),
     SPK_METHOD(lif_gate_mul),  SPK_METHOD(linear_decode),     SPK_METHOD(mlp_gate_lif), SPK_METHOD(qkv_rope_lif_pack),
+    SPK_METHOD(tree_attn),     SPK_METHOD(accept_tree),       SPK_METHOD(key_mass),     SPK_METHOD(evict),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

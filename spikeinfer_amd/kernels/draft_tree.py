@@ -89,6 +89,12 @@ def paged_spike_attn_tree(
     A row that sees nothing gets zeros; rows of ``out`` that are no sequence's are left as they
     were.  A sequence's outputs do not depend on the batch.
     """
+    native = _lib.native()
+    if native is not None:  # the usual form of the arguments, checked and launched in C++
+        done = native.tree_attn(q_packed, k_words, v_words, k_cache, v_cache, block_tables, context_lens, row_starts,
+                                masks, max_nodes, head_dim, block_size, out, dtype, workspace)
+        if done is not None:
+            return done
     T, R, n_heads, words = q_packed.shape
     dev = _lib.require_gpu(q_packed, k_words, v_words, k_cache, v_cache, block_tables, context_lens, row_starts, masks,
                            out, workspace)
@@ -215,6 +221,12 @@ def accept_draft_tree(
     ``count int32 [N]`` (the path's rows, row 0 among them; 0 for a sequence without rows)
     and ``next int64 [N]``, the model's token after the path.
     """
+    native = _lib.native()
+    if native is not None and layers:
+        done = native.accept_tree(tokens, parents, targets, row_starts, max_nodes, drafts, layers, block_tables,
+                                  context_lens, block_size, out)
+        if done is not None:
+            return done
     dev = _lib.require_gpu(tokens, parents, targets, row_starts, block_tables, context_lens, *(out or ()))
     _max_nodes(max_nodes)
     R, n_seqs = tokens.numel(), row_starts.numel() - 1

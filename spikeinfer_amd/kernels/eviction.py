@@ -58,6 +58,12 @@ def paged_spike_attn_key_mass(
         accumulate: add to ``out`` instead, and leave the rest of it as it was.
         workspace: optional ``uint8`` scratch of :func:`key_mass_workspace_bytes`.
     """
+    native = _lib.native()
+    if native is not None:
+        done = native.key_mass(q_packed, k_cache, block_tables, seq_lens, head_dim, block_size, row_starts, max_rows,
+                               out, accumulate, workspace)
+        if done is not None:
+            return done
     T, R, n_heads, words = q_packed.shape
     dev = _lib.require_gpu(q_packed, k_cache, block_tables, seq_lens, row_starts, out, workspace)
     _check_packed("q_packed", q_packed)
@@ -134,6 +140,11 @@ def evict_cache(
     ``new_lens int32 [N] = min(seq_lens, budget)``.  The kept tokens stand at positions 0,
     1, ... of the destination; blocks behind them are free.
     """
+    native = _lib.native()
+    if native is not None:
+        done = native.evict(layers, mass, block_tables, seq_lens, budget, block_size, sinks, recent, dst_tables, mass_out)
+        if done is not None:
+            return done
     dev = _lib.require_gpu(mass, block_tables, seq_lens, dst_tables, mass_out)
     if block_tables.ndim != 2 or (dst_tables is not None and
                                   (dst_tables.ndim != 2 or dst_tables.shape[0] != block_tables.shape[0])):
