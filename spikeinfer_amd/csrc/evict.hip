@@ -4,11 +4,14 @@
 // `sinks` tokens, its last `recent` ones and, of the others, those of largest mass
 // (equal masses: the lowest positions) so that `budget` stay, in their order.
 //   evict_select_kernel: a workgroup a (layer, sequence, kv head) finds the smallest
-//     mass that stays with a radix selection on order-preserving 32-bit keys, then
-//     numbers the kept tokens with ballots and prefix sums, in position order.
-//   evict_move_kernel: a workgroup a (t, kv head, K or V) plane moves the kept words
-//     to positions 0, 1, ...  A kept token never moves up, so chunks in order, each
-//     read whole before it is written, move in place.
+//     mass that stays with a radix selection (11, 11 and 10 bits) on order-preserving
+//     32-bit keys, then numbers the kept tokens with ballots and one prefix sum, in position
+//     order.  The masses are read once and stay in registers, EACH to a thread, up to
+//     32,768 tokens (read five times, 12,000 tokens took 42 us, a load's latency a pass).
+//   evict_move_kernel: a workgroup a kv head and two timesteps moves the kept words of K
+//     and V to positions 0, 1, ...: slots are worked out once for the four planes.  A kept
+//     token never moves up, so chunks in order, each read whole before it is written, move
+//     in place.
 #include "common.hpp"
 
 namespace spk {
@@ -20,6 +23,7 @@ constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kMoveThreads = 256;
 constexpr int kMoveEach = 4;  // tokens a thread and chunk
+constexpr int kMoveSteps = 2; // timesteps a workgroup
 
 struct Params {
   const float *mass;
@@ -53,10 +57,32 @@ __device__ __forceinline__ uint32_t key_of(float m) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Inclusive sum of x over the workgroup's threads, in thread order; `total` by all.
+__device__ __forceinline__ uint32_t block_sum(uint32_t x, int lane, int wave, uint32_t *waves, uint32_t &total) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t y = __shfl_up(x, s);
+    if (lane >= s) x += y;
+  }
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWaves; ++w) {
+    const uint32_t y = waves[w];
+    before += w < wave ? y : 0;
+    total += y;
+  }
+  return before + x;
+}
+
+// EACH: masses a thread keeps in registers (EACH * kSelThreads tokens at most); 0: none, they
+// are read again where they are needed.
+template <int EACH>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
   __shared__ uint32_t hist[kBins];
-  __shared__ int counts[2][2][kSelWaves];
-  __shared__ uint32_t found[2];
+  __shared__ uint32_t counts[EACH ? EACH * kSelWaves : 2 * kSelWaves], waves[2][kSelWaves], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x, n = blockIdx.y, layer = p.layer0 + blockIdx.z;
   const int len = length(p, n), kept = min(len, p.budget);
@@ -73,124 +99,178 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
     return;
   }
 
+  float m[EACH ? EACH : 1];
+  if constexpr (EACH > 0) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) m[i] = mass[min(i * kSelThreads + tid, len - 1)];
+  }
   // The candidates' free-th largest key, and how many equal to it stay.
   const int lo = p.sinks, hi = len - p.recent;
   int free = p.budget - p.sinks - p.recent;
+  const bool any = free > 0;
   uint32_t prefix = 0, mask = 0;
-  if (free > 0) {
+  if (any) {
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
       for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int j = lo + tid; j < hi; j += kSelThreads) {
-        const uint32_t k = key_of(mass[j]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+      auto count = [&](int j, float x) {
+        const uint32_t k = key_of(x);
+        if (j >= lo && j < hi && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+      };
+      if constexpr (EACH > 0) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) count(i * kSelThreads + tid, m[i]);
+      } else {
+        for (int j0 = 0; j0 < len; j0 += 8 * kSelThreads) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = mass[min(j0 + i * kSelThreads + tid, len - 1)];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) count(j0 + i * kSelThreads + tid, x[i]);
+        }
       }
       __syncthreads();
-      if (wave == 0) {  // a lane holds kBins / 64 bins, the highest first
-        constexpr int kEach = kBins / 64;
-        const int top = kBins - 1 - lane * kEach;
-        uint32_t sum = 0;
-        for (int b = 0; b < kEach; ++b) sum += hist[top - b];
-        uint32_t upto = sum;
-        for (int s = 1; s < 64; s <<= 1) {
-          const uint32_t y = __shfl_up(upto, s);
-          if (lane >= s) upto += y;
-        }
-        uint32_t before = upto - sum;
-        if (before < static_cast<uint32_t>(free) && upto >= static_cast<uint32_t>(free)) {
-          int b = 0;
-          while (before + hist[top - b] < static_cast<uint32_t>(free)) before += hist[top - b++];
-          found[0] = top - b;
-          found[1] = free - before;
-        }
+      // thread t holds bins top and top - 1, the highest first
+      const int top = kBins - 1 - 2 * tid;
+      const uint32_t c0 = hist[top], c1 = hist[top - 1];
+      uint32_t total;
+      const uint32_t upto = block_sum(c0 + c1, lane, wave, waves[pass & 1], total), need = free;
+      const uint32_t before = upto - c0 - c1;
+      if (before < need && upto >= need) {  // one thread
+        const bool first = before + c0 >= need;
+        found[0] = first ? top : top - 1;
+        found[1] = need - before - (first ? 0 : c0);
       }
       __syncthreads();
       prefix |= found[0] << shift;
       mask |= static_cast<uint32_t>(bins - 1) << shift;
-      free = found[1];
+      free = static_cast<int>(found[1]);
     }
   }
-  const bool any = p.budget > p.sinks + p.recent;
 
   // Kept tokens in position order: `sure` ones, and the first `free` equal ones.
-  int sure0 = 0, equal0 = 0;
-  for (int j0 = 0, turn = 0; j0 < len; j0 += kSelThreads, turn ^= 1) {
-    const int j = j0 + tid;
-    float m = 0.f;
-    bool sure = false, equal = false;
-    if (j < len) {
-      m = mass[j];
-      const uint32_t k = key_of(m);
-      const bool edge = j < lo || j >= hi;
-      sure = edge || (any && k > prefix);
-      equal = !edge && any && k == prefix;
-    }
-    const uint64_t sb = __ballot(sure), eb = __ballot(equal);
-    if (lane == 0) {
-      counts[turn][0][wave] = __popcll(sb);
-      counts[turn][1][wave] = __popcll(eb);
+  auto look = [&](int j, float x, bool &sure, bool &equal) {
+    const uint32_t k = key_of(x);
+    const bool edge = j < len && (j < lo || j >= hi), in = j >= lo && j < hi && any;
+    sure = edge || (in && k > prefix);
+    equal = in && k == prefix;
+  };
+  const uint64_t below = (1ull << lane) - 1;
+  if constexpr (EACH > 0) {
+    // a wave's counts of each of its EACH chunks, sure ones in the low half, then one sum
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      bool sure, equal;
+      look(i * kSelThreads + tid, m[i], sure, equal);
+      const uint64_t sb = __ballot(sure), eb = __ballot(equal);
+      if (lane == 0) counts[i * kSelWaves + wave] = __popcll(sb) | __popcll(eb) << 16;
     }
     __syncthreads();
-    int s = sure0, e = equal0;
-    for (int w = 0; w < kSelWaves; ++w) {
-      const int cs = counts[turn][0][w], ce = counts[turn][1][w];
-      if (w < wave) {
-        s += cs;
-        e += ce;
+    const uint32_t mine = tid < EACH * kSelWaves ? counts[tid] : 0;
+    uint32_t total;
+    const uint32_t upto = block_sum(mine, lane, wave, waves[1], total);  // (halves stay below 2^16)
+    if (tid < EACH * kSelWaves) counts[tid] = upto - mine;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int j = i * kSelThreads + tid;
+      bool sure, equal;
+      look(j, m[i], sure, equal);
+      const uint64_t sb = __ballot(sure), eb = __ballot(equal);
+      const uint32_t base = counts[i * kSelWaves + wave];
+      const int s = (base & 0xffff) + __popcll(sb & below), e = (base >> 16) + __popcll(eb & below);
+      if (sure || (equal && e < free)) {
+        const int at = s + min(e, free);
+        keep[at] = j;
+        to[at] = m[i];
       }
-      sure0 += cs;
-      equal0 += ce;
     }
-    const uint64_t below = (1ull << lane) - 1;
-    s += __popcll(sb & below);
-    e += __popcll(eb & below);
-    if (sure || (equal && e < free)) {
-      const int at = s + min(e, free);
-      keep[at] = j;
-      to[at] = m;
+  } else {
+    int sure0 = 0, equal0 = 0;
+    for (int j0 = 0, turn = 0; j0 < len; j0 += kSelThreads, turn ^= 1) {
+      const int j = j0 + tid;
+      const float x = mass[min(j, len - 1)];
+      bool sure, equal;
+      look(j, x, sure, equal);
+      const uint64_t sb = __ballot(sure), eb = __ballot(equal);
+      if (lane == 0) counts[turn * kSelWaves + wave] = __popcll(sb) | __popcll(eb) << 16;
+      __syncthreads();  // (all of the chunk is read: what is written below lies in it or before)
+      int s = sure0, e = equal0;
+      for (int w = 0; w < kSelWaves; ++w) {
+        const int cs = counts[turn * kSelWaves + w] & 0xffff, ce = counts[turn * kSelWaves + w] >> 16;
+        if (w < wave) {
+          s += cs;
+          e += ce;
+        }
+        sure0 += cs;
+        equal0 += ce;
+      }
+      s += __popcll(sb & below);
+      e += __popcll(eb & below);
+      if (sure || (equal && e < free)) {
+        const int at = s + min(e, free);
+        keep[at] = j;
+        to[at] = x;
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
   for (int j = kept + tid; j < p.cap; j += kSelThreads) to[j] = 0.f;
 }
 
 template <int W>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(Params p) {
-  const int which = blockIdx.x & 1, h = (blockIdx.x >> 1) % p.Hkv, t = (blockIdx.x >> 1) / p.Hkv;
-  const int n = blockIdx.y;
+  const int h = blockIdx.x % p.Hkv, t0 = blockIdx.x / p.Hkv * kMoveSteps, n = blockIdx.y;
   const int len = length(p, n), kept = min(len, p.budget);
   if (p.in_place && len <= p.budget) return;
   const int32_t *keep = p.keep + ((static_cast<int64_t>(p.layer0 + blockIdx.z) * p.N + n) * p.Hkv + h) * p.budget;
-  uint32_t *base = p.kv[blockIdx.z][which] + t * p.ks0 + h * p.ks1;
+  uint32_t *plane[2 * kMoveSteps];
+#pragma unroll
+  for (int i = 0; i < 2 * kMoveSteps; ++i)
+    plane[i] = p.kv[blockIdx.z][i & 1] + min(t0 + i / 2, p.T - 1) * p.ks0 + h * p.ks1;
   const int64_t blocks = p.num_slots >> p.bs_log2;
   const int bs_mask = (1 << p.bs_log2) - 1;
-  auto slot = [&](const int32_t *table, int64_t stride, int pos) -> int64_t {
-    const int64_t phys = table[(pos >> p.bs_log2) * stride];
-    return phys < 0 || phys >= blocks ? -1 : (phys << p.bs_log2) | (pos & bs_mask);
-  };
-  for (int i0 = 0; i0 < kept; i0 += kMoveThreads * kMoveEach) {
-    uint32_t x[kMoveEach][W];
-    int64_t dst[kMoveEach];
+  const int last = min(kept, p.max_dst) - 1;
+  for (int i0 = 0; i0 <= last; i0 += kMoveThreads * kMoveEach) {
+    int64_t src[kMoveEach], dst[kMoveEach];
 #pragma unroll
     for (int e = 0; e < kMoveEach; ++e) {
-      const int i = i0 + e * kMoveThreads + threadIdx.x;
-      dst[e] = -1;
-      if (i >= kept || i >= p.max_dst) continue;
-      const int64_t src = slot(p.bt + n * p.bts0, p.bts1, keep[i]);
-      dst[e] = slot(p.dt + n * p.dts0, p.dts1, i);
-      if (src == dst[e]) dst[e] = -1;
-#pragma unroll
-      for (int w = 0; w < W; ++w) x[e][w] = src < 0 ? 0u : base[src * p.ks2 + w];
+      const int i = min(i0 + e * kMoveThreads + static_cast<int>(threadIdx.x), last);
+      const int from = keep[i];
+      const int64_t a = p.bt[n * p.bts0 + (from >> p.bs_log2) * p.bts1], b = p.dt[n * p.dts0 + (i >> p.bs_log2) * p.dts1];
+      src[e] = a < 0 || a >= blocks ? -1 : ((a << p.bs_log2) | (from & bs_mask)) * p.ks2;
+      dst[e] = b < 0 || b >= blocks || i0 + e * kMoveThreads + static_cast<int>(threadIdx.x) > last
+                   ? -1 : ((b << p.bs_log2) | (i & bs_mask)) * p.ks2;
+      if (src[e] == dst[e]) dst[e] = -1;
     }
+    uint32_t x[2 * kMoveSteps][kMoveEach][W];
+#pragma unroll
+    for (int k = 0; k < 2 * kMoveSteps; ++k)
+#pragma unroll
+      for (int e = 0; e < kMoveEach; ++e)
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[k][e][w] = src[e] < 0 || dst[e] < 0 ? 0u : plane[k][src[e] + w];
     __builtin_amdgcn_s_waitcnt(0);  // the chunk's words are here before any is overwritten
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kMoveEach; ++e)
-      if (dst[e] >= 0)
+    for (int k = 0; k < 2 * kMoveSteps; ++k) {
+      if (t0 + k / 2 >= p.T) continue;
 #pragma unroll
-        for (int w = 0; w < W; ++w) base[dst[e] * p.ks2 + w] = x[e][w];
+      for (int e = 0; e < kMoveEach; ++e)
+        if (dst[e] >= 0)
+#pragma unroll
+          for (int w = 0; w < W; ++w) plane[k][dst[e] + w] = x[k][e][w];
+    }
   }
+}
+
+static void launch_select(const Params &p, dim3 grid, hipStream_t s) {
+  const int tokens = p.cap < p.max_tokens ? p.cap : p.max_tokens;  // the longest sequence
+  if (tokens <= 2 * kSelThreads) evict_select_kernel<2><<<grid, kSelThreads, 0, s>>>(p);
+  else if (tokens <= 8 * kSelThreads) evict_select_kernel<8><<<grid, kSelThreads, 0, s>>>(p);
+  else if (tokens <= 32 * kSelThreads) evict_select_kernel<32><<<grid, kSelThreads, 0, s>>>(p);
+  else evict_select_kernel<0><<<grid, kSelThreads, 0, s>>>(p);
 }
 
 }  // namespace evict
@@ -248,10 +328,10 @@ extern "C" int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t
       p.kv[k][0] = reinterpret_cast<uint32_t *>(layers[i + k].k);
       p.kv[k][1] = reinterpret_cast<uint32_t *>(layers[i + k].v);
     }
-    evict::evict_select_kernel<<<dim3(Hkv, N, m), evict::kSelThreads, 0, s>>>(p);
+    evict::launch_select(p, dim3(Hkv, N, m), s);
     int rc = check_launch("evict");
     if (rc) return rc;
-    const dim3 grid(2 * T * Hkv, N, m);
+    const dim3 grid((T + evict::kMoveSteps - 1) / evict::kMoveSteps * Hkv, N, m);
     switch (p.W) {
       case 1: evict::evict_move_kernel<1><<<grid, evict::kMoveThreads, 0, s>>>(p); break;
       case 2: evict::evict_move_kernel<2><<<grid, evict::kMoveThreads, 0, s>>>(p); break;

@@ -167,6 +167,8 @@ def _evict_check(caches, before, mass, tables, lens, dst, keep, new, mass_out, b
     ([300, 90], 70, 1, 1, 96, 64, 80, 0, 1),           # two launches of layers
     ([40, 500], 1, 3, 2, 45, 1, 1, 1, 0),              # one token, blocks of one
     ([2049, 100], 1, 1, 1, 64, 16, 2, 0, 1),
+    ([9000, 8192, 1500], 1, 1, 2, 64, 16, 2000, 4, 32),
+    ([33000, 40], 1, 1, 1, 64, 64, 30000, 4, 32),      # masses read again, not kept in registers
 ])
 def test_eviction(gpu, lens, L, T, hkv, D, bs, budget, sinks, recent, place, ties):
     caches, mass, tables, seq, left = _evict_case(lens, L, T, hkv, D, bs, sum(lens) + budget, gpu, ties)
