@@ -102,7 +102,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
   float m[EACH ? EACH : 1];
   if constexpr (EACH > 0) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) m[i] = mass[min(i * kSelThreads + tid, len - 1)];
+    for (int i = 0; i < EACH; ++i)
+      if (i * kSelThreads < len) m[i] = mass[min(i * kSelThreads + tid, len - 1)];
   }
   // The candidates' free-th largest key, and how many equal to it stay.
   const int lo = p.sinks, hi = len - p.recent;
@@ -120,7 +121,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
       };
       if constexpr (EACH > 0) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) count(i * kSelThreads + tid, m[i]);
+        for (int i = 0; i < EACH; ++i)
+          if (i * kSelThreads < hi) count(i * kSelThreads + tid, m[i]);
       } else {
         for (int j0 = 0; j0 < len; j0 += 8 * kSelThreads) {
           float x[8];
@@ -161,6 +163,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
     // a wave's counts of each of its EACH chunks, sure ones in the low half, then one sum
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
+      if (i * kSelThreads >= len) {
+        if (lane == 0) counts[i * kSelWaves + wave] = 0;
+        continue;
+      }
       bool sure, equal;
       look(i * kSelThreads + tid, m[i], sure, equal);
       const uint64_t sb = __ballot(sure), eb = __ballot(equal);
@@ -175,6 +181,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int j = i * kSelThreads + tid;
+      if (i * kSelThreads >= len) break;
       bool sure, equal;
       look(j, m[i], sure, equal);
       const uint64_t sb = __ballot(sure), eb = __ballot(equal);
@@ -269,6 +276,7 @@ static void launch_select(const Params &p, dim3 grid, hipStream_t s) {
   const int tokens = p.cap < p.max_tokens ? p.cap : p.max_tokens;  // the longest sequence
   if (tokens <= 2 * kSelThreads) evict_select_kernel<2><<<grid, kSelThreads, 0, s>>>(p);
   else if (tokens <= 8 * kSelThreads) evict_select_kernel<8><<<grid, kSelThreads, 0, s>>>(p);
+  else if (tokens <= 16 * kSelThreads) evict_select_kernel<16><<<grid, kSelThreads, 0, s>>>(p);
   else if (tokens <= 32 * kSelThreads) evict_select_kernel<32><<<grid, kSelThreads, 0, s>>>(p);
   else evict_select_kernel<0><<<grid, kSelThreads, 0, s>>>(p);
 }
