@@ -226,8 +226,16 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
   for (int j = kept + tid; j < p.cap; j += kSelThreads) to[j] = 0.f;
 }
 
+// A token's W words, one access (they need no more than a word's alignment).
+template <int W> struct Words;
+template <> struct Words<1> { typedef uint32_t type; };
+template <> struct Words<2> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(4))); };
+template <> struct Words<3> { typedef uint32_t type __attribute__((ext_vector_type(3), aligned(4))); };
+template <> struct Words<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
+
 template <int W>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(Params p) {
+  typedef typename Words<W>::type Token;
   const int h = blockIdx.x % p.Hkv, t0 = blockIdx.x / p.Hkv * kMoveSteps, n = blockIdx.y;
   const int len = length(p, n), kept = min(len, p.budget);
   if (p.in_place && len <= p.budget) return;
@@ -251,13 +259,14 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(Params p) {
                    ? -1 : ((b << p.bs_log2) | (i & bs_mask)) * p.ks2;
       if (src[e] == dst[e]) dst[e] = -1;
     }
-    uint32_t x[2 * kMoveSteps][kMoveEach][W];
+    Token x[2 * kMoveSteps][kMoveEach];
 #pragma unroll
     for (int k = 0; k < 2 * kMoveSteps; ++k)
 #pragma unroll
-      for (int e = 0; e < kMoveEach; ++e)
-#pragma unroll
-        for (int w = 0; w < W; ++w) x[k][e][w] = src[e] < 0 || dst[e] < 0 ? 0u : plane[k][src[e] + w];
+      for (int e = 0; e < kMoveEach; ++e) {
+        x[k][e] = Token(0);
+        if (src[e] >= 0 && dst[e] >= 0) __builtin_memcpy(&x[k][e], plane[k] + src[e], 4 * W);
+      }
     __builtin_amdgcn_s_waitcnt(0);  // the chunk's words are here before any is overwritten
     __syncthreads();
 #pragma unroll
@@ -265,9 +274,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(Params p) {
       if (t0 + k / 2 >= p.T) continue;
 #pragma unroll
       for (int e = 0; e < kMoveEach; ++e)
-        if (dst[e] >= 0)
-#pragma unroll
-          for (int w = 0; w < W; ++w) plane[k][dst[e] + w] = x[k][e][w];
+        if (dst[e] >= 0) __builtin_memcpy(plane[k] + dst[e], &x[k][e], 4 * W);
     }
   }
 }
