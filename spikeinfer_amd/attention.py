@@ -27,6 +27,24 @@ from .kernels.spike_attention import (PREFILL_DTYPES, gather_kv_unpacked_pair, p
 
 
 @dataclass
+class DraftTrees:
+    """The trees of a step that verifies drafted tokens (kernels/draft_tree.py).
+
+    The step's rows are the trees' rows: ``row_starts[n] .. row_starts[n + 1]`` those of
+    sequence ``n``, row 0 its last token.  ``words`` holds each layer's ``(k, v)`` words of
+    the rows (``int32 [T, rows, H_kv, W]``), written by the step and read by
+    :func:`accept_draft_tree`; None lets the step allocate them.
+    """
+
+    row_starts: torch.Tensor  # int32 [N + 1]
+    masks: torch.Tensor  # int64 [rows, ceil(max_nodes / 64)]
+    max_nodes: int
+    context_lens: torch.Tensor  # int32 [N]: cached tokens, the trees' rows not among them
+    block_tables: torch.Tensor  # int32 [N, max_blocks]
+    words: list[tuple[torch.Tensor, torch.Tensor]] | None = None
+
+
+@dataclass
 class AttentionMetadata:
     """Per-step batch description consumed by the attention operators.
 
@@ -49,6 +67,10 @@ class AttentionMetadata:
     prefill_query_lens: list[int] = field(default_factory=list)
     prefill_context_lens: list[int] = field(default_factory=list)
     prefill_block_tables: list[torch.Tensor] = field(default_factory=list)
+    # a step of drafted trees and nothing else (slot_mapping -1: no row goes to the cache)
+    draft: DraftTrees | None = None
+    # each layer's float32 [n_dec, H_kv, cap]: the decode tokens' attention weights are added
+    key_mass: list[torch.Tensor] | None = None
 
     # device -> copy of this metadata there (see on()); not part of equality
     _copies: dict = field(default_factory=dict, repr=False, compare=False)
@@ -68,8 +90,13 @@ class AttentionMetadata:
         key = str(device)
         if key not in self._copies:
             move = lambda t: None if t is None else t.to(device, non_blocking=True)
+            draft, mass = self.draft, self.key_mass
+            if draft is not None:
+                draft = replace(draft, row_starts=move(draft.row_starts), masks=move(draft.masks),
+                                context_lens=move(draft.context_lens), block_tables=move(draft.block_tables),
+                                words=draft.words and [(move(k), move(v)) for k, v in draft.words])
             self._copies[key] = replace(
-                self, slot_mapping=move(self.slot_mapping), block_tables=move(self.block_tables),
+                self, draft=draft, key_mass=mass and [move(m) for m in mass], slot_mapping=move(self.slot_mapping), block_tables=move(self.block_tables),
                 seq_lens=move(self.seq_lens),
                 prefill_block_tables=[move(t) for t in self.prefill_block_tables], _copies={})
         return self._copies[key]

@@ -36,6 +36,8 @@ from .attention import AttentionMetadata
 from .kernels.decoder_ops import (add_rmsnorm, embed_rmsnorm, lif_gate_mul, linear_decode,
                                   mlp_gate_lif, norm_linear_decode, norm_mlp_gate_lif, pack_gate_up,
                                   pack_linear, qkv_decode_attention, qkv_rope_lif_pack, rmsnorm_mean_t)
+from .kernels.draft_tree import paged_spike_attn_tree
+from .kernels.eviction import paged_spike_attn_key_mass
 from .kernels.packing import packed_width
 from .kernels.spike_attention import (gather_kv_unpacked_pair, paged_spike_attn_decode,
                                       paged_spike_attn_prefill, prefill_supported)
@@ -233,6 +235,10 @@ class SpikingDecoder:
         """``[n_tok]`` tokens (decodes first) -> ``[n_tok, hidden]`` rate-coded
         hidden states, writing every token's K/V into ``kv_caches[i] = (k, v)``.
 
+        With ``meta.draft`` the tokens are the rows of drafted trees: each attends to its
+        sequence's cache and its tree, and its K/V go to ``meta.draft.words`` instead.  With
+        ``meta.key_mass`` the decode tokens' attention weights are added there.
+
         ``bufs`` optionally supplies preallocated ``q_packed`` ``[T, n_dec, Hq,
         W]`` and ``attn`` ``[T, n_tok, Hq, D]`` (stable addresses under graph
         capture).
@@ -241,20 +247,26 @@ class SpikingDecoder:
         T, n = self.T, input_ids.shape[0]
         H, D, Hq, Hkv = c.hidden_size, self.D, self.Hq, self.Hkv
         n_dec = meta.num_decode_tokens
+        draft = meta.draft
+        if draft is not None and (n_dec or meta.num_prefills):
+            raise ValueError("a step of drafted trees has no decode tokens and no prefill chunks")
         bufs = bufs or {}
         positions = positions.to(torch.int64).contiguous()
         h, x = embed_rmsnorm(input_ids, self.embed, self.layers[0].input_norm, c.rms_norm_eps, T)
         # Prefill chunks attend on packed words; dense spikes (SDPA) only for
         # head dims the packed kernel does not take.
         packed_prefill = bool(meta.num_prefills) and prefill_supported(D, self.dtype)
-        n_q = n if packed_prefill else n_dec
+        n_q = n if packed_prefill or draft is not None else n_dec
         q_packed = bufs.get("q_packed")
-        if n_q and (q_packed is None or packed_prefill):
+        if n_q and (q_packed is None or packed_prefill or draft is not None):
             q_packed = torch.empty((T, n_q, Hq, self.W), dtype=torch.int32, device=h.device)
         kv_packed = None
         if packed_prefill and 0 in meta.prefill_context_lens:
             kv_packed = tuple(torch.empty((T, n, Hkv, self.W), dtype=torch.int32, device=h.device)
                               for _ in range(2))
+        if draft is not None and draft.words is None:
+            draft.words = [tuple(torch.empty((T, n, Hkv, self.W), dtype=torch.int32, device=h.device)
+                                 for _ in range(2)) for _ in self.layers]
         attn = bufs.get("attn")
         if attn is None:
             attn = torch.empty((T, n, Hq, D), dtype=self.dtype, device=h.device)
@@ -279,7 +291,9 @@ class SpikingDecoder:
                 if i:
                     x = add_rmsnorm(h, delta, L.input_norm, c.rms_norm_eps, out=x)
                 qkv = self._linear(x, L.w_qkv, L.b_qkv, L.w_qkv_packed, n)
-            fused = (self.fused_attention and not meta.num_prefills and n_dec == n and
+            if draft is not None:
+                kv_packed = draft.words[i]
+            fused = (self.fused_attention and not meta.num_prefills and n_dec == n and meta.key_mass is None and
                      qkv_decode_attention(qkv, self.rope_cos, self.rope_sin, positions, L.lif_qkv_beta,
                                           L.lif_qkv_th, k_cache, v_cache, meta.slot_mapping,
                                           meta.block_tables, meta.seq_lens, Hq, Hkv, meta.block_size,
@@ -292,7 +306,13 @@ class SpikingDecoder:
                 paged_spike_attn_decode(q_packed[:, :n_dec], k_cache, v_cache, meta.block_tables, meta.seq_lens,
                                         head_dim=D, block_size=meta.block_size, num_q_heads=Hq,
                                         num_kv_heads=Hkv, out=attn[:, :n_dec])
-            if packed_prefill:
+            if n_dec and meta.key_mass is not None:
+                paged_spike_attn_key_mass(q_packed[:, :n_dec], k_cache, meta.block_tables, meta.seq_lens, D,
+                                          meta.block_size, out=meta.key_mass[i], accumulate=True)
+            if draft is not None:
+                paged_spike_attn_tree(q_packed, *kv_packed, k_cache, v_cache, draft.block_tables, draft.context_lens,
+                                      draft.row_starts, draft.masks, draft.max_nodes, D, meta.block_size, out=attn)
+            elif packed_prefill:
                 self._packed_prefill_attention(q_packed, kv_packed, k_cache, v_cache, meta, attn)
             elif meta.num_prefills:
                 self._prefill_attention(dense, k_cache, v_cache, meta, attn)

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 
+from .kernels.eviction import evict_cache
 from .kernels.packing import packed_width
 
 
@@ -72,6 +73,14 @@ class PagedSpikeCache:
     @property
     def capacity_tokens(self) -> int:
         return self.num_allocatable_blocks * self.block_size
+
+    def evict(self, mass: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, budget: int,
+              sinks: int = 4, recent: int = 32, dst_tables: torch.Tensor | None = None,
+              mass_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """:func:`evict_cache` over all layers: every sequence of more than ``budget`` tokens
+        keeps ``budget``, by the attention weights ``mass [num_layers, N, H_kv, cap]``."""
+        return evict_cache(self.layers, mass, block_tables, seq_lens, budget, self.block_size, sinks, recent,
+                           dst_tables, mass_out)
 
     def reset(self) -> None:
         for t in self.k + self.v:
