@@ -18,16 +18,15 @@
 //     (2^-14, 2^-13, 2^-11 or 2^-7 by the key's number % 4), and four tables of weights
 //     hold what makes the products equal again: one `and` a register instead of a
 //     multiplication more.
-//   * Four waves a workgroup share the key tiles' operands through LDS: each prepares one of
-//     four tiles, two buffers of them so that one barrier a step does.  A sequence of more
-//     than 64 rows has a wave a row tile and all keys; of 33 to 64 rows two waves a row tile,
-//     the even and the odd tiles; below, four.
+//   * Eight waves a workgroup share the key tiles' operands through LDS: each prepares one of
+//     a step's eight tiles, two buffers of them so that one barrier a step does.  Of a
+//     sequence of more than 128 rows a workgroup takes 256, a wave a row tile and all keys; of
+//     65 to 128 rows two waves share a row tile, of 33 to 64 four, below eight, each with its
+//     part of a step's tiles; they are added in their order.
 //   * The context is cut into parts of kPartTiles tiles (more beyond kMaxParts parts), the
-//     tree's tiles belonging to the last.  A wave adds a part's tiles in their order, then the
-//     parts, then come the waves of a row tile.  Where workgroups are many each takes all
-//     parts (SEQ), else a workgroup a part leaves its waves' sums in the workspace and a
-//     second launch adds them: the same additions.  So the sums depend on the sequence alone,
-//     its length and its rows, not on the batch around it.
+//     tree's tiles belonging to the last: a workgroup each, whose sums a second launch adds in
+//     their order.  So the sums depend on the sequence alone, its length and its rows, not on
+//     the batch around it.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -37,8 +36,9 @@ namespace tree {
 
 using namespace tiles;
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kKeys = 32;          // keys per tile
+constexpr int kStep = kWaves;      // tiles between barriers
 constexpr int kPartTiles = 64;     // tiles per part, up to kMaxParts of them
 constexpr int kMaxParts = 32;
 constexpr int kMaxNodes = 1024;
@@ -64,8 +64,9 @@ struct Params {
   uint32_t rep_mul;         // floor(r / nrep) = r * rep_mul >> 32 for every row
   int units, Hkv, nrep, D, W, bs_log2, max_blocks, max_nodes;
   int groups;               // workgroups along the rows of a sequence
-  int parts;                // along its context: 1, or its most parts
-  float *ws;                // with parts > 1: sums of (sequence, unit, group, part, wave)
+  int parts;                // along its context
+  int wide;                 // a plane of the caches passes 2^32 bytes
+  float *ws;                // with parts > 1: sums of (sequence, unit, part, row tile)
   uint32_t tab[kTab];
 };
 
@@ -102,8 +103,8 @@ __device__ __forceinline__ int node_of(const Params &p, int r) {
 
 // Weight tables in LDS at offset 0.  bf16 outputs: four of the weights' high halves as fp32,
 // whose entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's (all of them f16 numbers).  Else
-// one of (hi, lo) pairs, and kTabStride words on, their sums as fp32.
-template <bool F32> constexpr int kTables = F32 ? 2 : 4;
+// one of (hi, lo) pairs.
+template <bool F32> constexpr int kTables = F32 ? 1 : 4;
 template <bool F32>
 __device__ __forceinline__ void fill_tables(const Params &p, float *tab, int tid) {
   if (tid > p.D) return;
@@ -111,7 +112,6 @@ __device__ __forceinline__ void fill_tables(const Params &p, float *tab, int tid
   const float hi = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
   if constexpr (F32) {
     tab[tid] = __uint_as_float(w);
-    tab[kTabStride + tid] = hi + static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w >> 16)));
   } else {
     tab[tid] = hi;
     tab[kTabStride + tid] = hi * 0.5f;
@@ -142,8 +142,8 @@ struct Keys {
   const Seq &s;
   const int32_t *table;
   const uint32_t *kbase, *vbase, *ktree, *vtree;
-  uint32_t nblocks;
-  int last_block, half, col;
+  uint32_t nblocks, slot_bytes;
+  int last, half, col;
 
   __device__ __forceinline__ Keys(const Params &p, const Seq &s, int n, int t, int kvh, int half, int col)
       : p(p), s(s), half(half), col(col) {
@@ -153,23 +153,37 @@ struct Keys {
     ktree = p.kt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
     vtree = p.vt + t * p.ts0 + s.first * p.ts1 + kvh * p.ts2;
     nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
-    last_block = max(s.ctx - 1, 0) >> p.bs_log2;
+    slot_bytes = static_cast<uint32_t>(p.ks2 * 4);
+    last = max(s.ctx - 1, 0);
   }
   __device__ __forceinline__ uint32_t block_of(int kt) const {
-    return static_cast<uint32_t>(table[min((kt * kKeys + col) >> p.bs_log2, last_block) * p.bts1]);
+    return static_cast<uint32_t>(table[(min(kt * kKeys + col, last) >> p.bs_log2) * p.bts1]);
   }
-  __device__ __forceinline__ void load(int kt, uint32_t phys, uint32_t (&kw)[NK], uint32_t (&vw)[NK], bool &ok) const {
-    const bool own = kt >= s.ctiles;
-    const int j = (own ? kt - s.ctiles : kt) * kKeys + col;
-    ok = own ? j < s.nodes : j < s.ctx && phys < nblocks;
-    const int64_t slot = (static_cast<int64_t>(phys) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1));
-    const int64_t at = ok ? (own ? j * p.ts1 : slot * p.ks2) : 0;
-    const uint32_t *kp = (own ? ktree : kbase) + at, *vp = (own ? vtree : vbase) + at;
+  __device__ __forceinline__ void words(const uint32_t *kp, const uint32_t *vp, uint32_t at, uint32_t (&kw)[NK],
+                                        uint32_t (&vw)[NK]) const {
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
-      const int w = min(2 * k + half, p.W - 1);
-      kw[k] = kp[w];
-      vw[k] = vp[w];
+      const uint32_t b = at + 4 * min(2 * k + half, p.W - 1);  // (a uniform base and 32-bit bytes)
+      kw[k] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(kp) + b);
+      vw[k] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(vp) + b);
+    }
+  }
+  __device__ __forceinline__ void load(int kt, uint32_t phys, uint32_t (&kw)[NK], uint32_t (&vw)[NK], bool &ok) const {
+    if (kt < s.ctiles) {
+      const int j = kt * kKeys + col;
+      ok = j < s.ctx && phys < nblocks;
+      const uint32_t low = static_cast<uint32_t>(j & ((1 << p.bs_log2) - 1));
+      if (!p.wide) {
+        words(kbase, vbase, ok ? ((phys << p.bs_log2) | low) * slot_bytes : 0u, kw, vw);
+      } else {
+        const int64_t at = ok ? ((static_cast<int64_t>(phys) << p.bs_log2) | low) * p.ks2 : 0;
+        words(kbase + at, vbase + at, 0, kw, vw);
+      }
+    } else {
+      const int j = (kt - s.ctiles) * kKeys + col;
+      ok = j < s.nodes;
+      const int64_t at = ok ? j * p.ts1 : 0;
+      words(ktree + at, vtree + at, 0, kw, vw);
     }
   }
   // Loaded words as a tile's shared operands: keys as fp4, and per channel tile a lane's
@@ -223,56 +237,66 @@ __device__ __forceinline__ v16f scores(const v8i (&kop)[NK], const v8i (&qop)[NK
   return a;
 }
 
-// A tile's weights: the lane's sixteen as operand entries, and for fp32 outputs as fp32.
+// A tile's weights: the lane's sixteen table entries.
 template <bool F32>
-struct Weights {
-  uint32_t w[16];
-  float f[F32 ? 16 : 1];
-};
-template <bool F32>
-__device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, Weights<F32> &x) {
+__device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint32_t at = tab0 + __float_as_uint(a[e]);
-    const SPK_LDS uint32_t *w = reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
-    x.w[e] = w[F32 ? 0 : kTabStride * (e & 3)];
-    if constexpr (F32) x.f[e] = __uint_as_float(w[kTabStride]);
+    const uint32_t at = tab0 + (F32 ? 0 : 4 * kTabStride * (e & 3)) + __float_as_uint(a[e]);
+    w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
   }
 }
 
-// Adds a tile's weighted values to acc and its weights to l.  (The weights are added as fp32:
-// dot products of f16 pairs would be half as many instructions, but they take the matrix
-// cores' time: 8 behind each product 78 cycles where 8 additions take 52.)
+// Adds a tile's weighted values to acc and its weights to l.  The weights are added one by
+// one: dot products of f16 pairs would be half as many instructions, but they take the matrix
+// cores' time (8 behind each product 78 cycles where 8 additions take 52).  Of a pair's halves
+// the high ones are added in fp32.  The low ones, below 2^-11 of theirs, are first added in
+// f16, eight to a sum in three steps: off by at most 3 * 2^-11 of themselves, 2^-20 of the
+// weights at the very worst and 2^-23 in the mean, their own resolution.
 template <int NC, bool F32, bool MASKED>
-__device__ __forceinline__ void products(const Weights<F32> &x, uint32_t see, const v8h (&vop)[NC][2], v16f (&acc)[NC],
-                                         float (&l)[4]) {
+__device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, const v8h (&vop)[NC][2],
+                                         v16f (&acc)[NC], float (&l)[4]) {
   constexpr int kParts = F32 ? 2 : 1;
-  auto keep = [&](uint32_t w, int e) {  // the e-th of the lane's sixteen
+  float one = 1.f;
+  asm("" : "+v"(one));  // (kept a register: fma_mix then takes the halves as they are)
+  auto keep = [&](int e) {  // the e-th of the lane's sixteen
     if constexpr (MASKED)
-      return w & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
-    else return w;
+      return x[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
+    else return x[e];
   };
+  v2h low[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     v4u y[kParts];  // the weights' halves, two keys a register
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int e0 = 4 * g + i, e1 = e0 + 8;
-      const uint32_t w0 = keep(x.w[e0], e0), w1 = keep(x.w[e1], e1);
+      const uint32_t w0 = keep(4 * g + i), w1 = keep(4 * g + i + 8);
       if constexpr (F32) {
-        l[i] += __uint_as_float(keep(__float_as_uint(x.f[e0]), e0)) + __uint_as_float(keep(__float_as_uint(x.f[e1]), e1));
-        y[0][i] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+        const uint32_t both = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+        y[0][i] = both;
         y[1][i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+        const v2h high = __builtin_bit_cast(v2h, both);  // (of a scalar: an element would give the first)
+        l[i] = __builtin_fmaf(static_cast<float>(high[0]), one, l[i]);
+        l[i] = __builtin_fmaf(static_cast<float>(high[1]), one, l[i]);
       } else {
         l[i] += __uint_as_float(w0) + __uint_as_float(w1);
         y[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w0), __uint_as_float(w1)));
       }
+    }
+    if constexpr (F32) {
+      auto half2 = [&](int i) { return __builtin_bit_cast(v2h, static_cast<uint32_t>(y[1][i])); };
+      low[g] = (half2(0) + half2(1)) + (half2(2) + half2(3));
     }
 #pragma unroll
     for (int q = 0; q < kParts; ++q)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, y[q]), acc[c], 0, 0, 0);
+  }
+  if constexpr (F32) {
+    const v2h sum = low[0] + low[1];
+    l[0] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[0]);
+    l[1] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[1]);
   }
 }
 
@@ -327,189 +351,145 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
   }
 }
 
-// Waves that share a row tile, each a quarter or half of the tiles.
-__device__ __forceinline__ int key_waves(int rows) { return rows <= 32 ? 4 : (rows <= 64 ? 2 : 1); }
-
-// A wave's sums in the workspace: [NC][4][64] vectors of four channels, [64] denominators.
-constexpr int wave_sums(int NC) { return NC * 1024 + 64; }
-__device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int group, int part, int wave, int NC) {
-  return p.ws + ((((static_cast<int64_t>(n) * p.units + unit) * p.groups + group) * p.parts + part) * kWaves + wave) *
-                    wave_sums(NC);
+// A row tile's sums in the workspace: [NC][4][64] vectors of four channels, [32] denominators.
+constexpr int tile_sums(int NC) { return NC * 1024 + 32; }
+__device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int part, int rt, int NC) {
+  return p.ws + (((static_cast<int64_t>(n) * p.units + unit) * p.parts + part) * p.groups * kWaves + rt) * tile_sums(NC);
 }
 
-// NC = channel tiles of 32.  KW: waves that share a row tile.
-template <int NC, bool F32, bool SEQ, int KW, typename Smem>
+// KW waves a row tile; NC = channel tiles of 32.
+template <int KW, int NC, bool F32, typename Smem>
 __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, int n, int unit, int group, int part,
                                        int wave) {
-  constexpr int NK = (NC + 1) / 2;  // 64-channel score steps
-  constexpr int kEach = kWaves / KW;  // tiles of a step that a wave takes
+  constexpr int NK = (NC + 1) / 2;   // 64-channel score steps
+  constexpr int kEach = kStep / KW;  // tiles of a step that a wave takes
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int kvh = unit % p.Hkv, t = unit / p.Hkv, rows = s.nodes * p.nrep;
-  const int rw = wave / KW, kw_ = wave % KW;
-  const int rt = group * kWaves + rw, r = rt * 32 + col;
+  const int kw = wave % KW, rt = group * kWaves + wave / KW, r = rt * 32 + col;
   const bool live = rt * 32 < rows;  // (without rows of its own a wave prepares tiles)
 
+  const Keys<NK> keys(p, s, n, t, kvh, half, col);
+  const int t0 = part * s.ptiles, stop = part + 1 < s.parts ? t0 + s.ptiles : s.end;
+  // The words of this wave's tile of a step are requested a step before they are prepared,
+  // their block two.
+  uint32_t kwords[NK], vwords[NK], phys = keys.block_of(t0 + wave);
+  bool ok;
+  auto request = [&](int first) {
+    keys.load(first + wave, phys, kwords, vwords, ok);
+    phys = keys.block_of(first + kStep + wave);
+  };
+  request(t0);
   fill_tables<F32>(p, sm.tab[0], tid);
   v8i qop[NK];
   load_query<NK>(p, s, t, kvh, min(r, rows - 1), half, qop);
   const uint32_t *mrow = p.masks + (s.first + node_of(p, min(r, rows - 1))) * p.mask_words;
-  const Keys<NK> keys(p, s, n, t, kvh, half, col);
-
-  const int p0 = part, p1 = SEQ ? s.parts : part + 1;
-  const int t0 = p0 * s.ptiles, stop = p1 < s.parts ? p1 * s.ptiles : s.end;
   v16f acc[NC];
   float l[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = v16f{};
-  float tot[SEQ ? NC : 1][16], den = 0.f;
-  if constexpr (SEQ) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) tot[c][j] = 0.f;
-  }
 
-  uint32_t kw[NK], vw[NK];
-  bool ok;
-  keys.load(t0 + wave, keys.block_of(t0 + wave), kw, vw, ok);
-  uint32_t pnext = keys.block_of(t0 + wave + kWaves);
+  auto prepare = [&](int buf) {
+    v8i kop[NK];
+    uint32_t vt[2 * NK];
+    keys.operands(kwords, vwords, ok, lane, kop, vt);
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+      sm.k[buf][wave][k][lane] = v4u{static_cast<uint32_t>(kop[k][0]), static_cast<uint32_t>(kop[k][1]),
+                                     static_cast<uint32_t>(kop[k][2]), static_cast<uint32_t>(kop[k][3])};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = vt[c];
+  };
+  prepare(0);
+  request(t0 + kStep);
+  __syncthreads();
   int buf = 0;
-  for (int first = t0; first < stop; first += kWaves, buf ^= 1) {
-    {
-      // This wave's tile of the four; the next one's words and the block of the one after
-      // are requested before they are used.
-      v8i kop[NK];
-      uint32_t vt[2 * NK];
-      keys.operands(kw, vw, ok, lane, kop, vt);
-      keys.load(first + wave + kWaves, pnext, kw, vw, ok);
-      pnext = keys.block_of(first + wave + 2 * kWaves);
-#pragma unroll
-      for (int k = 0; k < NK; ++k)
-        sm.k[buf][wave][k][lane] = v4u{static_cast<uint32_t>(kop[k][0]), static_cast<uint32_t>(kop[k][1]),
-                                       static_cast<uint32_t>(kop[k][2]), static_cast<uint32_t>(kop[k][3])};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = vt[c];
+  for (int first = t0; first < stop; first += kStep, buf ^= 1) {
+    if (first + kStep < stop) {  // the next step's tile, into the other buffer
+      prepare(buf ^ 1);
+      request(first + 2 * kStep);
     }
-    __syncthreads();
+    auto tile = [&](int u, auto masked) {
+      v8i kop[NK];
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        const v4u x = sm.k[buf][u][k][lane];
+        kop[k] = v8i{static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3])};
+      }
+      uint32_t w[16];
+      lookup<F32>(tab0, scores<NK>(kop, qop), w);
+      v8h vop[NC][2];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) expand<F32>(sm.v[buf][u][c][lane], vop[c]);
+      products<NC, F32, decltype(masked)::value>(w, decltype(masked)::value ? seen(s, first + u, mrow, half) : 0u, vop,
+                                                 acc, l);
+    };
     if (live) {
-      auto operand = [&](int u, v8i (&kop)[NK]) {
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-          const v4u x = sm.k[buf][u][k][lane];
-          kop[k] = v8i{static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3])};
-        }
-      };
-      auto values = [&](int u, v8h (&vop)[NC][2]) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) expand<F32>(sm.v[buf][u][c][lane], vop[c]);
-      };
-      if ((first + kWaves) * kKeys <= s.ctx) {
-        // Every key counts: the next tile's scores are computed and looked up under this
-        // one's products.
-        Weights<F32> w[2];
-        {
-          v8i kop[NK];
-          operand(kw_, kop);
-          lookup<F32>(tab0, scores<NK>(kop, qop), w[0]);
-        }
+      if ((first + kStep) * kKeys <= s.ctx) {  // every key counts
 #pragma unroll
         for (int u = 0; u < kEach; ++u) {
-          if (u + 1 < kEach) {
-            v8i kop[NK];
-            operand(kw_ + (u + 1) * KW, kop);
-            lookup<F32>(tab0, scores<NK>(kop, qop), w[(u + 1) & 1]);
-          }
-          v8h vop[NC][2];
-          values(kw_ + u * KW, vop);
-          products<NC, F32, false>(w[u & 1], 0u, vop, acc, l);
+          tile(kw + u * KW, std::false_type{});
           __builtin_amdgcn_sched_barrier(0);  // tile by tile (several at a time spill)
         }
       } else {
 #pragma unroll 1
-        for (int u = kw_; u < kWaves && first + u < stop; u += KW) {
-          Weights<F32> w;
-          v8i kop[NK];
-          v8h vop[NC][2];
-          operand(u, kop);
-          values(u, vop);
-          lookup<F32>(tab0, scores<NK>(kop, qop), w);
-          products<NC, F32, true>(w, seen(s, first + u, mrow, half), vop, acc, l);
-        }
+        for (int u = kw; u < kStep && first + u < stop; u += KW) tile(u, std::true_type{});
       }
     }
-    if constexpr (SEQ) {
-      // (a part is a power of two of tiles, so its last step ends on it)
-      if (((first + kWaves) & (s.ptiles - 1)) == 0 && first + kWaves <= (s.parts - 1) * s.ptiles) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) tot[c][j] += acc[c][j];
-          acc[c] = v16f{};
-        }
-        den += lane_sum<F32>(l);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) l[q] = 0.f;
-      }
-    }
+    __syncthreads();
   }
-  if constexpr (SEQ) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) acc[c][j] = tot[c][j] + acc[c][j];
-  }
-  den += lane_sum<F32>(l);
 
-  if (!SEQ && s.parts > 1) {
+  auto done = [&](int c, int quad, const float (&val)[4], float den) {
+    if (s.parts > 1) {
+      float *to = sums_at(p, n, unit, part, rt, NC);
+      *reinterpret_cast<v4f *>(to + ((c * 4 + quad) * 64 + lane) * 4) = v4f{val[0], val[1], val[2], val[3]};
+      if (c == 0 && quad == 0 && half == 0) to[NC * 1024 + col] = den;
+    } else if (r < rows) {
+      store_row<F32, 4>(p, s, t, kvh, r, c, quad, half, val, den);
+    }
+  };
+  const float mine = lane_sum<F32>(l);
+  if constexpr (KW == 1) {
+    const float den = mine + __shfl_xor(mine, 32);
     if (!live) return;
-    float *to = sums_at(p, n, unit, group, part, wave, NC);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<v4f *>(to + ((c * 4 + j) * 64 + lane) * 4) =
-            v4f{acc[c][4 * j], acc[c][4 * j + 1], acc[c][4 * j + 2], acc[c][4 * j + 3]};
-    to[NC * 1024 + lane] = den;
-    return;
-  }
-  if constexpr (KW == 1) {
-    den += __shfl_xor(den, 32);
-    if (r < rows) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float val[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) val[j] = acc[c][j];
-        store_row<F32, 16>(p, s, t, kvh, r, c, 0, half, val, den);
+      for (int quad = 0; quad < 4; ++quad) {
+        const float val[4] = {acc[c][4 * quad], acc[c][4 * quad + 1], acc[c][4 * quad + 2], acc[c][4 * quad + 3]};
+        done(c, quad, val, den);
       }
-    }
   } else {
-    // The row tile's waves, in their order: wave kw_ finishes a KW-th of each channel tile.
-    constexpr int kVals = 16 / KW;
-    sm.den[wave][lane] = den;
+    // The row tile's waves in their order: wave kw finishes four channels of a lane's sixteen
+    // (two waves: eight each).
+    constexpr int kQuads = KW < 4 ? 4 / KW : 1;
+    sm.den[wave][lane] = mine;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      __syncthreads();  // (the staged tiles, and the channel tile before, are read)
+      if (c) __syncthreads();  // (the channel tile before is read)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sm.red[wave][j][lane] = acc[c][j];
       __syncthreads();
-      float val[kVals], d = 0.f;
+      if (kw >= 4 || !live) continue;
+      float den = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) d += sm.den[rw * KW + w][col] + sm.den[rw * KW + w][col + 32];
+      for (int w = 0; w < KW; ++w) den += sm.den[wave - kw + w][col] + sm.den[wave - kw + w][col + 32];
 #pragma unroll
-      for (int j = 0; j < kVals; ++j) {
-        val[j] = 0.f;
+      for (int x = 0; x < kQuads; ++x) {
+        const int quad = kw * kQuads + x;
+        float val[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < KW; ++w) val[j] += sm.red[rw * KW + w][kw_ * kVals + j][lane];
+        for (int w = 0; w < KW; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) val[j] += sm.red[wave - kw + w][quad * 4 + j][lane];
+        done(c, quad, val, den);
       }
-      if (r < rows) store_row<F32, kVals>(p, s, t, kvh, r, c, kw_ * kVals / 4, half, val, d);
     }
   }
 }
 
-template <int NC, bool F32, bool SEQ>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 || SEQ ? 2 : 3))) void tree_attn_kernel(
+template <int NC, bool F32>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void tree_attn_kernel(
     Params p) {
   constexpr int NK = (NC + 1) / 2;
   struct Smem {
@@ -517,8 +497,8 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
     float den[kWaves][64];
     union {
       struct {
-        v4u k[2][kWaves][NK][64];
-        uint32_t v[2][kWaves][NC][64];
+        v4u k[2][kStep][NK][64];
+        uint32_t v[2][kStep][NC][64];
       };
       float red[kWaves][16][64];
     };
@@ -530,54 +510,47 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
   const int part = rest % p.parts, group = rest / p.parts;
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep;
-  if (group * kWaves * 32 >= rows || (!SEQ && part >= s.parts)) return;
-  switch (key_waves(rows)) {
-    case 4: attend<NC, F32, SEQ, 4>(p, s, sm, n, unit, group, part, wave); break;
-    case 2: attend<NC, F32, SEQ, 2>(p, s, sm, n, unit, group, part, wave); break;
-    default: attend<NC, F32, SEQ, 1>(p, s, sm, n, unit, group, part, wave);
-  }
+  if (group * kWaves * 32 >= rows || part >= s.parts) return;
+  if (rows > 128) attend<1, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else if (rows > 64) attend<2, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else if (rows > 32) attend<4, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else attend<8, NC, F32>(p, s, sm, n, unit, group, part, wave);
 }
 
-// Sums of the parts, in their order, wave by wave.  A wave takes four channels of a lane's
-// sixteen of an output tile, with kAhead parts' sums on their way at once.  Workgroups of a
-// unit are numbered as the attention's are: with 8 units (or a multiple) they run on the XCD
-// whose L2 has the sums.
+// Sums of the parts, in their order.  A wave takes four channels of a lane's sixteen of an
+// output tile, with kAhead parts' sums on their way at once.  Workgroups of a unit are
+// numbered as the attention's are: with 8 units (or a multiple) they run on the XCD whose L2
+// has the sums.
 template <bool F32>
-__global__ __launch_bounds__(kWaves * 64) void tree_join_kernel(Params p, int NC) {
+__global__ __launch_bounds__(256) void tree_join_kernel(Params p, int NC) {
   constexpr int kAhead = 8;
   const int lane = threadIdx.x & 63, quad = threadIdx.x >> 6, half = lane >> 5, col = lane & 31, n = blockIdx.y;
-  const int unit = blockIdx.x % p.units, rest = blockIdx.x / p.units, c = rest % NC, tile = rest / NC;
+  const int unit = blockIdx.x % p.units, rest = blockIdx.x / p.units, c = rest % NC, rt = rest / NC;
   const Seq s = sequence(p, n);
-  const int rows = s.nodes * p.nrep, r = tile * 32 + col;
-  if (tile * 32 >= rows || s.parts <= 1) return;
-  const int kw = key_waves(rows);
-  const int64_t stride = kWaves * wave_sums(NC);  // from part to part
-  float val[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int w = 0; w < kw; ++w) {
-    const float *from = sums_at(p, n, unit, tile / kWaves, 0, tile % kWaves * kw + w, NC);
-    const float *at = from + ((c * 4 + quad) * 64 + lane) * 4;
-    v4f a = {0.f, 0.f, 0.f, 0.f};
-    float d = 0.f;
-    for (int part = 0; part < s.parts; part += kAhead) {
-      v4f x[kAhead];
-      float y[kAhead];
+  const int rows = s.nodes * p.nrep, r = rt * 32 + col;
+  if (rt * 32 >= rows || s.parts <= 1) return;
+  const int64_t stride = static_cast<int64_t>(p.groups) * kWaves * tile_sums(NC);  // from part to part
+  const float *from = sums_at(p, n, unit, 0, rt, NC);
+  const float *at = from + ((c * 4 + quad) * 64 + lane) * 4;
+  v4f a = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+  for (int part = 0; part < s.parts; part += kAhead) {
+    v4f x[kAhead];
+    float y[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int64_t to = min(part + u, s.parts - 1) * stride;
-        x[u] = *reinterpret_cast<const v4f *>(at + to);
-        y[u] = from[to + NC * 1024 + lane];
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (part + u >= s.parts) break;
-        a += x[u];
-        d += y[u];
-      }
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t to = min(part + u, s.parts - 1) * stride;
+      x[u] = *reinterpret_cast<const v4f *>(at + to);
+      y[u] = from[to + NC * 1024 + col];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) val[j] += a[j];
-    den += d + __shfl_xor(d, 32);
+    for (int u = 0; u < kAhead; ++u) {
+      if (part + u >= s.parts) break;
+      a += x[u];
+      den += y[u];
+    }
   }
+  const float val[4] = {a[0], a[1], a[2], a[3]};
   if (r < rows) store_row<F32, 4>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, quad, half, val, den);
 }
 
@@ -586,35 +559,32 @@ struct Plan {
   size_t bytes;  // workspace
 };
 
-// The launch of a shape: a workgroup a part of the context where there would be fewer than
-// three a CU without.
 inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_size, int max_blocks) {
   Plan r;
-  const size_t units = static_cast<size_t>(T) * Hkv * N;
-  r.groups = static_cast<int>((static_cast<int64_t>(max_nodes) * (Hq / Hkv) + 32 * kWaves - 1) / (32 * kWaves));
-  r.parts = units * r.groups < 768 ? most_parts(static_cast<int64_t>(max_blocks) * block_size) : 1;
-  r.bytes = r.parts > 1 ? units * r.groups * r.parts * kWaves * wave_sums((D + 31) / 32) * sizeof(float) : 0;
+  const int64_t rows = static_cast<int64_t>(max_nodes) * (Hq / Hkv);
+  r.groups = static_cast<int>((rows + 32 * kWaves - 1) / (32 * kWaves));
+  r.parts = most_parts(static_cast<int64_t>(max_blocks) * block_size);
+  r.bytes = r.parts > 1 ? static_cast<size_t>(T) * Hkv * N * r.groups * r.parts * kWaves * tile_sums((D + 31) / 32) * sizeof(float)
+                        : 0;
   return r;
 }
 
 template <int NC, bool F32>
-static int launch(const Params &p, bool one_part, int N, hipStream_t s) {
-  const dim3 grid(p.groups * p.parts * p.units, N);
-  if (p.parts == 1 && !one_part) tree_attn_kernel<NC, F32, true><<<grid, kWaves * 64, 0, s>>>(p);
-  else tree_attn_kernel<NC, F32, false><<<grid, kWaves * 64, 0, s>>>(p);
+static int launch(const Params &p, int N, hipStream_t s) {
+  tree_attn_kernel<NC, F32><<<dim3(p.groups * p.parts * p.units, N), kWaves * 64, 0, s>>>(p);
   const int rc = check_launch("tree_attn");
   if (rc || p.parts == 1) return rc;
-  tree_join_kernel<F32><<<dim3(p.units * p.groups * kWaves * NC, N), kWaves * 64, 0, s>>>(p, NC);
+  tree_join_kernel<F32><<<dim3(p.units * p.groups * kWaves * NC, N), 256, 0, s>>>(p, NC);
   return check_launch("tree_attn");
 }
 
 template <bool F32>
-static int launch_type(const Params &p, bool one_part, int N, hipStream_t s) {
+static int launch_type(const Params &p, int N, hipStream_t s) {
   switch (p.W) {
-    case 1: return launch<1, F32>(p, one_part, N, s);
-    case 2: return launch<2, F32>(p, one_part, N, s);
-    case 3: return launch<3, F32>(p, one_part, N, s);
-    default: return launch<4, F32>(p, one_part, N, s);
+    case 1: return launch<1, F32>(p, N, s);
+    case 2: return launch<2, F32>(p, N, s);
+    case 3: return launch<3, F32>(p, N, s);
+    default: return launch<4, F32>(p, N, s);
   }
 }
 
@@ -680,6 +650,7 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
     p.k = p.v = p.q;
     p.ks0 = p.ks1 = p.ks2 = 0;
   }
+  p.wide = p.num_slots * p.ks2 > (1ll << 30) || p.ks2 < 0;
   p.bt = block_tables; p.bts0 = bt_stride0; p.bts1 = bt_stride1;
   if (max_blocks == 0) {  // no context: the loads of a table entry read the lengths
     p.bt = context_lens;
@@ -698,7 +669,5 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
   tiles::build_table(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool one_part = tree::most_parts(static_cast<int64_t>(max_blocks) * block_size) == 1;
-  return out_dtype != SPK_BF16 ? tree::launch_type<true>(p, one_part, N, s)
-                               : tree::launch_type<false>(p, one_part, N, s);
+  return out_dtype != SPK_BF16 ? tree::launch_type<true>(p, N, s) : tree::launch_type<false>(p, N, s);
 }
