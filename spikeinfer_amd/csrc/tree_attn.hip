@@ -18,11 +18,11 @@
 //     (2^-14, 2^-13, 2^-11 or 2^-7 by the key's number % 4), and four tables of weights
 //     hold what makes the products equal again: one `and` a register instead of a
 //     multiplication more.
-//   * Eight waves a workgroup share the key tiles' operands through LDS: each prepares one of
-//     a step's eight tiles, two buffers of them so that one barrier a step does.  Of a
-//     sequence of more than 128 rows a workgroup takes 256, a wave a row tile and all keys; of
-//     65 to 128 rows two waves share a row tile, of 33 to 64 four, below eight, each with its
-//     part of a step's tiles; they are added in their order.
+//   * Eight waves a workgroup (four with more than 64 channels) share the key tiles' operands
+//     through LDS: each prepares one of a step's tiles, two buffers of them so that one barrier
+//     a step does.  Of a sequence of more than 128 rows a workgroup takes 256, a wave a row
+//     tile and all keys; of 65 to 128 rows two waves share a row tile, of 33 to 64 four, below
+//     eight, each with its part of a step's tiles; they are added in their order.
 //   * The context is cut into parts of kPartTiles tiles (more beyond kMaxParts parts), the
 //     tree's tiles belonging to the last: a workgroup each, whose sums a second launch adds in
 //     their order.  So the sums depend on the sequence alone, its length and its rows, not on
@@ -36,9 +36,10 @@ namespace tree {
 
 using namespace tiles;
 
-constexpr int kWaves = 8;
+// Waves a workgroup, and tiles between its barriers: eight, so that two workgroups are four
+// waves a SIMD, or with the sums of more than 64 channels, four, so that two are two.
+constexpr int waves_of(int NC) { return NC > 2 ? 4 : 8; }
 constexpr int kKeys = 32;          // keys per tile
-constexpr int kStep = kWaves;      // tiles between barriers
 constexpr int kPartTiles = 64;     // tiles per part, up to kMaxParts of them
 constexpr int kMaxParts = 32;
 constexpr int kMaxNodes = 1024;
@@ -63,7 +64,8 @@ struct Params {
   int64_t rows;
   uint32_t rep_mul;         // floor(r / nrep) = r * rep_mul >> 32 for every row
   int units, Hkv, nrep, D, W, bs_log2, max_blocks, max_nodes;
-  int groups;               // workgroups along the rows of a sequence
+  int rtiles;               // most row tiles of a sequence
+  int groups;               // workgroups along them
   int parts;                // along its context
   int wide;                 // a plane of the caches passes 2^32 bytes
   float *ws;                // with parts > 1: sums of (sequence, unit, part, row tile)
@@ -354,7 +356,7 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
 // A row tile's sums in the workspace: [NC][4][64] vectors of four channels, [32] denominators.
 constexpr int tile_sums(int NC) { return NC * 1024 + 32; }
 __device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int part, int rt, int NC) {
-  return p.ws + (((static_cast<int64_t>(n) * p.units + unit) * p.parts + part) * p.groups * kWaves + rt) * tile_sums(NC);
+  return p.ws + (((static_cast<int64_t>(n) * p.units + unit) * p.parts + part) * p.rtiles + rt) * tile_sums(NC);
 }
 
 // KW waves a row tile; NC = channel tiles of 32.
@@ -362,6 +364,7 @@ template <int KW, int NC, bool F32, typename Smem>
 __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, int n, int unit, int group, int part,
                                        int wave) {
   constexpr int NK = (NC + 1) / 2;   // 64-channel score steps
+  constexpr int kWaves = waves_of(NC), kStep = kWaves;
   constexpr int kEach = kStep / KW;  // tiles of a step that a wave takes
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
@@ -489,9 +492,9 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
 }
 
 template <int NC, bool F32>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void tree_attn_kernel(
-    Params p) {
-  constexpr int NK = (NC + 1) / 2;
+__global__ __launch_bounds__(waves_of(NC) * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void
+tree_attn_kernel(Params p) {
+  constexpr int NK = (NC + 1) / 2, kWaves = waves_of(NC), kStep = kWaves;
   struct Smem {
     float tab[kTables<F32>][kTabStride];  // first: a score's accumulator is its entry's LDS address
     float den[kWaves][64];
@@ -511,10 +514,10 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(NC 
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep;
   if (group * kWaves * 32 >= rows || part >= s.parts) return;
-  if (rows > 128) attend<1, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else if (rows > 64) attend<2, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else if (rows > 32) attend<4, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else attend<8, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  if (rows > 16 * kWaves) attend<1, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else if (rows > 8 * kWaves) attend<2, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  else attend<kWaves, NC, F32>(p, s, sm, n, unit, group, part, wave);
 }
 
 // Sums of the parts, in their order.  A wave takes four channels of a lane's sixteen of an
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int NC) {
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep, r = rt * 32 + col;
   if (rt * 32 >= rows || s.parts <= 1) return;
-  const int64_t stride = static_cast<int64_t>(p.groups) * kWaves * tile_sums(NC);  // from part to part
+  const int64_t stride = static_cast<int64_t>(p.rtiles) * tile_sums(NC);  // from part to part
   const float *from = sums_at(p, n, unit, 0, rt, NC);
   const float *at = from + ((c * 4 + quad) * 64 + lane) * 4;
   v4f a = {0.f, 0.f, 0.f, 0.f};
@@ -555,26 +558,26 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int NC) {
 }
 
 struct Plan {
-  int groups, parts;
+  int rtiles, groups, parts;
   size_t bytes;  // workspace
 };
 
 inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_size, int max_blocks) {
   Plan r;
-  const int64_t rows = static_cast<int64_t>(max_nodes) * (Hq / Hkv);
-  r.groups = static_cast<int>((rows + 32 * kWaves - 1) / (32 * kWaves));
+  const int NC = (D + 31) / 32;
+  r.rtiles = static_cast<int>((static_cast<int64_t>(max_nodes) * (Hq / Hkv) + 31) / 32);
+  r.groups = (r.rtiles + waves_of(NC) - 1) / waves_of(NC);
   r.parts = most_parts(static_cast<int64_t>(max_blocks) * block_size);
-  r.bytes = r.parts > 1 ? static_cast<size_t>(T) * Hkv * N * r.groups * r.parts * kWaves * tile_sums((D + 31) / 32) * sizeof(float)
-                        : 0;
+  r.bytes = r.parts > 1 ? static_cast<size_t>(T) * Hkv * N * r.parts * r.rtiles * tile_sums(NC) * sizeof(float) : 0;
   return r;
 }
 
 template <int NC, bool F32>
 static int launch(const Params &p, int N, hipStream_t s) {
-  tree_attn_kernel<NC, F32><<<dim3(p.groups * p.parts * p.units, N), kWaves * 64, 0, s>>>(p);
+  tree_attn_kernel<NC, F32><<<dim3(p.groups * p.parts * p.units, N), waves_of(NC) * 64, 0, s>>>(p);
   const int rc = check_launch("tree_attn");
   if (rc || p.parts == 1) return rc;
-  tree_join_kernel<F32><<<dim3(p.units * p.groups * kWaves * NC, N), 256, 0, s>>>(p, NC);
+  tree_join_kernel<F32><<<dim3(p.units * p.rtiles * NC, N), 256, 0, s>>>(p, NC);
   return check_launch("tree_attn");
 }
 
@@ -634,7 +637,7 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return fail(SPK_EINVAL, "tree_attn: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);
   const int64_t units = static_cast<int64_t>(T) * Hkv;
-  if (units * plan.groups * plan.parts > (1 << 26) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
+  if (units * plan.rtiles * plan.parts > (1 << 26) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
     return fail(SPK_EUNSUPPORTED, "tree_attn: T=%d Hq=%d Hkv=%d with %d nodes", T, Hq, Hkv, max_nodes);
   tree::Params p{};
   p.q = reinterpret_cast<const uint32_t *>(q);
@@ -666,7 +669,7 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   p.W = (head_dim + 31) / 32; p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks; p.max_nodes = max_nodes;
   // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
   p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
-  p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
+  p.rtiles = plan.rtiles; p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
   tiles::build_table(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return out_dtype != SPK_BF16 ? tree::launch_type<true>(p, N, s) : tree::launch_type<false>(p, N, s);
