@@ -12,14 +12,16 @@
 // of two): a product's 16 rows are 4 * WP of each of these timesteps, whose words stand in
 // their own quarter or half of the channels beside zeros, so that decoding (7 rows of 4
 // timesteps at 64 channels) fills 14 of 16 rows and every lane loads one word of a key.
-//   den_kernel   sums the weights of a part of kPart keys for RT or fewer such row tiles
-//                (keys as the product's rows: a lane adds its own row's weights);
-//   mass_kernel  adds the parts' sums in their order, then the weights over the
-//                denominators (keys as its columns: a lane adds its own key's).  With RT row
-//                tiles or fewer (a decode step) a wave holds them and goes through its keys;
-//                with more the four waves of a workgroup have the same keys and share the row
-//                tiles, RT at a time, and their sums are added in wave order.
+//   Few rows (a decode step): a workgroup takes kPart keys, their words requested at once and
+//     kept, and all row tiles, one a timestep group.  One launch sums the rows' weights (keys
+//     as the product's rows: a lane adds its own row's weights), another adds the parts' sums
+//     in their order, then the weights over them (keys as its columns: a lane adds its own
+//     key's); with one part a single launch does both.
+//   Many rows: den_rows_kernel goes through kPart keys with kRows row tiles in registers;
+//     mass_rows_kernel has 128 keys, in registers, and its waves share the row tiles.
 // The order of all sums is the sequence's own, whatever the batch.
+#include <type_traits>
+
 #include "spike_tiles.hpp"
 
 namespace spk {
@@ -27,9 +29,16 @@ namespace mass {
 
 using namespace tiles;
 
-constexpr int kWaves = 4;
 constexpr int kStep = 64;      // keys a wave takes at once: four products' columns
-constexpr int kPart = 1024;    // keys a workgroup
+constexpr int kPart = 1024;    // keys of a partial sum
+constexpr int kWaves = 4;      // few rows: waves, each with kSteps steps
+constexpr int kSteps = kPart / (kWaves * kStep);
+constexpr int kRows = 8;       // many rows: row tiles in registers
+constexpr int kDenWaves = 8;   // (twice kWaves: two steps a wave)
+constexpr int kDenSteps = kPart / (kDenWaves * kStep);
+constexpr int kShare = 4;      // waves that share the row tiles of their keys
+constexpr int kMassKeys = 128;
+constexpr int kChunk = 64;     // row tiles whose denominators are in LDS
 
 struct Params {
   const uint32_t *q;           // words of (t, row, query head)
@@ -47,16 +56,16 @@ struct Params {
   uint32_t rep_mul;            // floor(r / nrep) = r * rep_mul >> 32 for every row
   int N, max_rows, T, Hkv, nrep, W, D, bs_log2, max_blocks;
   int tgroups;                 // timestep groups
-  int tiles;                   // most row tiles of a sequence
+  int rtiles;                  // most row tiles of a timestep group
   int parts;                   // most parts of a sequence
-  float *den;                  // [N, Hkv, parts, tiles, 16]
+  float *den;                  // [N, Hkv, parts, tgroups, rtiles, 16]
   float tab[kTab];             // exp((s - D) * scale)
 };
 
 struct Seq {
   int64_t first;
   int m, len, parts;
-  int rtiles, tiles;  // row tiles of a timestep group, of all
+  int rtiles;  // row tiles of a timestep group
 };
 
 template <int WP>
@@ -68,7 +77,6 @@ __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   s.len = min(max(p.lens[n], 0), p.max_blocks << p.bs_log2);
   s.parts = (s.len + kPart - 1) / kPart;
   s.rtiles = (s.m * p.nrep + 4 * WP - 1) / (4 * WP);
-  s.tiles = s.rtiles * p.tgroups;
   return s;
 }
 
@@ -76,74 +84,71 @@ __device__ __forceinline__ int row_of(const Params &p, int r) {  // r / nrep
   return p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
 }
 
-// Row tiles of a workgroup: tile x is rows 4 * WP * (x % rtiles) .. of timestep group x / rtiles.
-// A product's row y: timestep y / (4 * WP) of the group, row y % (4 * WP) of the tile.
-template <int WP, int RT>
-struct Rows {
-  v8i q[RT];
-  int tg[RT];   // timestep group (uniform; -1: no tile)
-  int lim[RT];  // last key that row l % 16 of the tile sees (-1: none)
-
-  __device__ __forceinline__ void load(const Params &p, const Seq &s, int kvh, int tile0, int lane) {
-    const int y = lane & 15, b = lane >> 4;  // row, 32-channel block of the product
-    const int dt = y / (4 * WP);
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int x = tile0 + i;
-      tg[i] = x < s.tiles ? x / s.rtiles : -1;
-      const int r = (x - tg[i] * s.rtiles) * 4 * WP + y % (4 * WP);
-      const int row = row_of(p, r), t = tg[i] * (4 / WP) + dt;
-      const bool in = tg[i] >= 0 && row < s.m && t < p.T;
-      lim[i] = in ? s.len - s.m + row : -1;
-      const int w = b - dt * WP;  // this lane's word of the row's head
-      q[i] = fp4_bits(in && w >= 0 && w < WP && w < p.W
-                          ? p.q[t * p.qs0 + (s.first + row) * p.qs1 + (kvh * p.nrep + r - row * p.nrep) * p.qs2 + w]
-                          : 0u);
-    }
-  }
-};
-
-// A lane's words of a step's four key tiles for one timestep group (lane l: key l % 16 of a
-// tile, block l / 16 of the product's channels), as operands.
+// Row tile `rt` of a timestep group: its rows 4 * WP * rt .. of each timestep.  A product's row
+// y: timestep y / (4 * WP) of the group, row y % (4 * WP) of the tile.
 template <int WP>
+__device__ __forceinline__ int tile_row(const Params &p, int rt, int y) {  // of the sequence's rows
+  return row_of(p, rt * 4 * WP + y % (4 * WP));
+}
+template <int WP>
+__device__ __forceinline__ bool has_row(const Params &p, const Seq &s, int tg, int rt, int y) {
+  return tile_row<WP>(p, rt, y) < s.m && tg * (4 / WP) + y / (4 * WP) < p.T;
+}
+
+// A lane's query word of a row tile (row l % 16, block l / 16 of the product's channels).
+template <int WP>
+__device__ __forceinline__ uint32_t query_word(const Params &p, const Seq &s, int kvh, int tg, int rt, int lane) {
+  const int y = lane & 15, dt = y / (4 * WP), t = tg * (4 / WP) + dt, w = (lane >> 4) - dt * WP;
+  const int r = rt * 4 * WP + y % (4 * WP), row = row_of(p, r);
+  const bool in = row < s.m && t < p.T && w >= 0 && w < WP && w < p.W;
+  const uint32_t x =
+      p.q[in ? t * p.qs0 + (s.first + row) * p.qs1 + (kvh * p.nrep + r - row * p.nrep) * p.qs2 + w : int64_t(0)];
+  return in ? x : 0u;
+}
+
+// A lane's words of a step's four key tiles (lane l: key l % 16 of a tile, block l / 16 of
+// the product's channels).  Keys behind the sequence read its last block, what they give is
+// dropped; so is, by the queries' zeros, what a block of no timestep or word gives.
+// PAGE: blocks are of 16 slots or more, a key tile lies in one and its place is scalar.
+template <int WP, bool PAGE>
 struct Keys {
   const Params &p;
   const int32_t *table;
   const uint32_t *base;
   uint32_t nblocks;
-  int last_block, len, y, dt, w;
-  __device__ __forceinline__ Keys(const Params &p, const Seq &s, int n, int kvh, int lane) : p(p), len(s.len) {
+  int last_block, y;
+  struct Places {
+    int64_t at[4];
+    bool ok[4];
+  };
+  __device__ __forceinline__ Keys(const Params &p, const Seq &s, int n, int kvh, int lane) : p(p) {
     table = p.bt + n * p.bts0;
     base = p.k + kvh * p.ks1;
     nblocks = static_cast<uint32_t>(min<int64_t>(p.num_slots >> p.bs_log2, 0xffffffffll));
-    last_block = max(s.len - 1, 0) >> p.bs_log2;
+    last_block = (s.len - 1) >> p.bs_log2;
     y = lane & 15;
-    dt = (lane >> 4) / WP;
-    w = (lane >> 4) % WP;
   }
-  // Slots of the lane's four keys, -1 where there is none.
-  __device__ __forceinline__ void slots(int j0, int64_t (&at)[4]) const {
+  __device__ __forceinline__ const uint32_t *words(int tg, int lane) const {
+    const int t = tg * (4 / WP) + (lane >> 4) / WP, w = (lane >> 4) % WP;
+    const uint32_t *at = base + (t < p.T ? t : 0) * p.ks0 + (w < p.W ? w : 0);
+    return PAGE ? at + y * p.ks2 : at;
+  }
+  __device__ __forceinline__ Places places(int j0) const {
+    Places r;
     uint32_t phys[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      phys[u] = static_cast<uint32_t>(table[min((j0 + 16 * u + y) >> p.bs_log2, last_block) * p.bts1]);
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + 16 * u + (PAGE ? 0 : y);
+      phys[u] = static_cast<uint32_t>(table[min(j >> p.bs_log2, last_block) * p.bts1]);
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int j = j0 + 16 * u + y;
-      at[u] = j < len && phys[u] < nblocks
-                  ? ((static_cast<int64_t>(phys[u]) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1))) * p.ks2
-                  : -1;
+      const int j = j0 + 16 * u + (PAGE ? 0 : y);
+      if constexpr (PAGE) phys[u] = __builtin_amdgcn_readfirstlane(phys[u]);
+      r.ok[u] = phys[u] < nblocks;
+      r.at[u] = r.ok[u] ? ((static_cast<int64_t>(phys[u]) << p.bs_log2) | (j & ((1 << p.bs_log2) - 1))) * p.ks2 : 0;
     }
-  }
-  // (unconditional loads, dropped where there is no key or word: they are all on their way
-  // before the first is waited for)
-  __device__ __forceinline__ void load(int tg, const int64_t (&at)[4], uint32_t (&x)[4]) const {
-    const int t = tg * (4 / WP) + dt;
-    const bool in = t < p.T && w < p.W;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = base[in && at[u] >= 0 ? t * p.ks0 + at[u] + w : 0];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = in && at[u] >= 0 ? x[u] : 0u;
+    return r;
   }
 };
 
@@ -155,248 +160,359 @@ __device__ __forceinline__ float weight(uint32_t tab0, float score) {
   return *reinterpret_cast<const SPK_LDS float *>(static_cast<uintptr_t>(tab0 + __float_as_uint(score)));
 }
 
-// Key words of all of a wave's steps for each row tile.
-template <int WP, int RT, int STEPS>
-__device__ __forceinline__ void request(const Keys<WP> &keys, const int (&tg)[RT], int j1, uint32_t (&x)[STEPS][RT][4]) {
-  int64_t at[STEPS][4];
+// What 16 keys at j give a row's denominator (lane: row l % 16, keys j + 4 * (l / 16) + 0..3;
+// `lim`: the last key that the row sees).
+template <bool MASK>
+__device__ __forceinline__ float row_weights(uint32_t tab0, const v8i &q, const v8i &k, int j, int lane, int lim) {
+  const v4f a = score(k, q);
+  float w[4];
 #pragma unroll
-  for (int st = 0; st < STEPS; ++st) keys.slots(j1 + st * kWaves * kStep, at[st]);
-#pragma unroll
-  for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-    for (int i = 0; i < RT; ++i) keys.load(max(tg[i], 0), at[st], x[st][i]);
+  for (int e = 0; e < 4; ++e) {
+    w[e] = weight(tab0, a[e]);
+    if (MASK) w[e] = j + 4 * (lane >> 4) + e <= lim ? w[e] : 0.f;
+  }
+  return (w[0] + w[1]) + (w[2] + w[3]);
 }
 
-template <int WP, int RT>
-__global__ __launch_bounds__(kWaves * 64) void den_kernel(Params p) {
+// What a tile's rows 4 * (l / 16) + 0..3 give a lane's key j.
+template <bool MASK>
+__device__ __forceinline__ float key_weights(uint32_t tab0, const v8i &q, const v8i &k, int j, const v4f &inv,
+                                             const int (&lim)[4], float sum) {
+  const v4f a = score(q, k);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float w = weight(tab0, a[e]);
+    if (MASK) w = j <= lim[e] ? w : 0.f;
+    sum = __builtin_fmaf(w, inv[e], sum);
+  }
+  return sum;
+}
+
+// Sum of the parts' denominators, in their order.
+__device__ __forceinline__ float parts_sum(const Params &p, const Seq &s, const float *at) {
+  float d = 0.f;
+  for (int pt = 0; pt < s.parts; pt += 8) {  // eight on their way at once
+    float y[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+      y[v] = at[static_cast<int64_t>(min(pt + v, s.parts - 1)) * p.tgroups * p.rtiles * 16];
+#pragma unroll
+    for (int v = 0; v < 8; ++v) d += pt + v < s.parts ? y[v] : 0.f;
+  }
+  return d;
+}
+
+enum Pass { kDen, kMass, kBoth };
+
+// Few rows: one row tile for each of RT or fewer timestep groups.
+template <int WP, int RT, bool PAGE, Pass PASS>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void few_rows_kernel(Params p) {
   struct Smem {
     float tab[kTab + 3];  // first: a score's accumulator is its entry's LDS address
-    float sum[kWaves][RT][16];
+    float sum[kDenWaves][RT][16];
+    float inv[RT][16];
   };
   __shared__ Smem sm;
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = blockIdx.x % p.parts, chunk = blockIdx.x / p.parts;
   const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
   const Seq s = sequence<WP>(p, n);
-  if (part >= s.parts || chunk * RT >= s.tiles) return;
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * kPart;
+  float *mass = p.mass + n * p.ms0 + kvh * p.ms1;
+  if constexpr (PASS != kDen) {
+    if (!p.accumulate)
+      for (int64_t j = max<int64_t>(from, s.rtiles ? s.len : 0) + tid; j < min(p.cap, from + kPart); j += kWaves * 64)
+        mass[j] = 0.f;
+  }
+  if (from >= s.len || s.rtiles == 0) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
-  Rows<WP, RT> rows;
-  rows.load(p, s, kvh, chunk * RT, lane);
-  const Keys<WP> keys(p, s, n, kvh, lane);
-  float l[RT];
+
+  const Keys<WP, PAGE> keys(p, s, n, kvh, lane);
+  const int j1 = static_cast<int>(from) + wave * kStep;
+  uint32_t x[kSteps][RT][4];
+  bool ok[kSteps][4];
+  float old[kSteps];
+  {
+    const uint32_t *at[RT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) l[i] = 0.f;
-  __syncthreads();
-  const int end = min(s.len, (part + 1) * kPart), open = s.len - s.m;  // keys up to `open` are seen by all rows
-  auto add = [&](int i, int u, int j0, const v8i &k) {
-    const v4f a = score(k, rows.q[i]);  // lane: row l % 16, keys 4 * (l / 16) + 0..3
-    float w[4];
+    for (int i = 0; i < RT; ++i) at[i] = keys.words(min(i, p.tgroups - 1), lane);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
-    if (j0 + 16 * u + 15 > open) {
+    for (int st = 0; st < kSteps; ++st) {
+      const typename Keys<WP, PAGE>::Places to = keys.places(j1 + st * kWaves * kStep);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = j0 + 16 * u + 4 * (lane >> 4) + e <= rows.lim[i] ? w[e] : 0.f;
+      for (int u = 0; u < 4; ++u) {
+        ok[st][u] = to.ok[u];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) x[st][i][u] = at[i][to.at[u]];
+      }
     }
-    l[i] += (w[0] + w[1]) + (w[2] + w[3]);
-  };
-  const int j1 = part * kPart + wave * kStep;
-  if constexpr (RT == 2) {  // few products a key: the words of all steps are requested first
-    constexpr int kSteps = kPart / (kWaves * kStep);
-    uint32_t x[kSteps][RT][4];
-    request<WP, RT, kSteps>(keys, rows.tg, j1, x);
+  }
+  const int end = static_cast<int>(min<int64_t>(min<int64_t>(s.len, p.cap), from + kPart));
+  if constexpr (PASS != kDen) {
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int j = j1 + st * kWaves * kStep + lane;
+      old[st] = p.accumulate && j < end ? mass[j] : 0.f;
+    }
+  }
+  v8i q[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) q[i] = fp4_bits(i < p.tgroups ? query_word<WP>(p, s, kvh, i, 0, lane) : 0u);
+  const int open = s.len - s.m;  // keys up to `open` are seen by all rows
+  float *den = p.den + (static_cast<int64_t>(blockIdx.y) * p.parts + (PASS == kDen ? blockIdx.x : 0)) * p.tgroups * 16;
+  if constexpr (PASS == kMass) {
+    if (tid < p.tgroups * 16) {
+      const float d = parts_sum(p, s, den + tid);
+      sm.inv[tid / 16][tid % 16] = d > 0.f && has_row<WP>(p, s, tid / 16, 0, tid % 16) ? 1.f / d : 0.f;
+    }
+  }
+  __syncthreads();
+
+  if constexpr (PASS != kMass) {
+    // (two steps a sum, as den_rows_kernel's waves have them)
+    float l[2][RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) l[0][i] = l[1][i] = 0.f;
+    const int lim = open + tile_row<WP>(p, 0, lane & 15);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int j0 = j1 + st * kWaves * kStep;
+      auto add = [&](auto mask) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          if (i >= p.tgroups) continue;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            l[st & 1][i] += row_weights<decltype(mask)::value>(tab0, q[i], fp4_bits(ok[st][u] ? x[st][i][u] : 0u),
+                                                               j0 + 16 * u, lane, lim);
+        }
+      };
+      if (j0 + kStep - 1 <= open) add(std::false_type{});
+      else if (j0 < s.len) add(std::true_type{});
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = l[h][i];
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if (lane < 16) sm.sum[h * kWaves + wave][i][lane] = x;
+      }
+    }
+    __syncthreads();
+    if (tid < p.tgroups * 16) {
+      const int i = tid / 16, y = tid % 16;
+      float d = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDenWaves; ++w) d += sm.sum[w][i][y];
+      if constexpr (PASS == kDen) den[tid] = d;
+      else sm.inv[i][y] = d > 0.f && has_row<WP>(p, s, i, 0, y) ? 1.f / d : 0.f;
+    }
+    if constexpr (PASS == kBoth) __syncthreads();
+  }
+  if constexpr (PASS != kDen) {
+    v4f inv[RT];
+    int lim[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lim[e] = open + tile_row<WP>(p, 0, 4 * (lane >> 4) + e);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) inv[i] = *reinterpret_cast<const v4f *>(&sm.inv[i][4 * (lane >> 4)]);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       const int j0 = j1 + st * kWaves * kStep;
       if (j0 >= end) break;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rows.tg[i] < 0) continue;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add(i, u, j0, fp4_bits(x[st][i][u]));
-      }
-    }
-  } else {
-    for (int j0 = j1; j0 < end; j0 += kWaves * kStep) {
-      int64_t at[4];
-      keys.slots(j0, at);
-      v8i k[4];
-      int have = -1;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rows.tg[i] < 0) continue;
-        if (rows.tg[i] != have) {
-          uint32_t x[4];
-          keys.load(rows.tg[i], at, x);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
-          have = rows.tg[i];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) add(i, u, j0, k[u]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    l[i] += __shfl_xor(l[i], 16);
-    l[i] += __shfl_xor(l[i], 32);
-    if (lane < 16) sm.sum[wave][i][lane] = l[i];
-  }
-  __syncthreads();
-  float *to = p.den + ((static_cast<int64_t>(blockIdx.y) * p.parts + part) * p.tiles + chunk * RT) * 16;
-  for (int x = tid; x < RT * 16; x += kWaves * 64)
-    if (chunk * RT + x / 16 < s.tiles)
-      to[x] = (sm.sum[0][x / 16][x % 16] + sm.sum[1][x / 16][x % 16]) + (sm.sum[2][x / 16][x % 16] + sm.sum[3][x / 16][x % 16]);
-}
-
-// SHARED: the waves have the same kStep * STEPS keys and share the row tiles; else each has
-// STEPS steps of its own.
-template <int WP, int RT, int STEPS, bool SHARED>
-__global__ __launch_bounds__(kWaves * 64) void mass_kernel(Params p) {
-  constexpr int kKeys = STEPS * kStep * (SHARED ? 1 : kWaves);  // of a workgroup
-  struct Smem {
-    float tab[kTab + 3];
-    float inv[kWaves][RT][16];
-    int lim[kWaves][RT][16];
-    float sum[SHARED ? kWaves : 1][kKeys];
-  };
-  __shared__ Smem sm;
-  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
-  const Seq s = sequence<WP>(p, n);
-  float *mass = p.mass + n * p.ms0 + kvh * p.ms1;
-  const int64_t from = static_cast<int64_t>(blockIdx.x) * kKeys, stop = min(p.cap, from + kKeys);
-  if (!p.accumulate)
-    for (int64_t j = max<int64_t>(from, s.len) + tid; j < stop; j += kWaves * 64) mass[j] = 0.f;
-  if (from >= s.len || from >= p.cap) return;
-  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
-  __syncthreads();
-  const Keys<WP> keys(p, s, n, kvh, lane);
-  const int end = min(s.len, static_cast<int>(stop)), open = s.len - s.m;  // keys up to `open` are seen by all rows
-  const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tiles * 16;
-
-  Rows<WP, RT> rows;
-  float inv[RT][4];  // of the products' rows 4 * (l / 16) + 0..3; no row: 0
-  auto take = [&](int tile0) {  // row tiles tile0 .. and their denominators, a wave by itself
-    rows.load(p, s, kvh, tile0, lane);
-#pragma unroll
-    for (int i = 0; i < RT; i += 4) {  // lane: row l % 16 of tile i + l / 16
-      const int x = i + (lane >> 4);
-      float d = 0.f;
-      if (x < RT && tile0 + x < s.tiles) {
-        const float *at = den + (tile0 + x) * 16 + (lane & 15);
-        for (int pt = 0; pt < s.parts; pt += 8) {  // eight parts' sums on their way at once
-          float y[8];
-#pragma unroll
-          for (int v = 0; v < 8; ++v) y[v] = at[static_cast<int64_t>(min(pt + v, s.parts - 1)) * p.tiles * 16];
-#pragma unroll
-          for (int v = 0; v < 8; ++v) d += pt + v < s.parts ? y[v] : 0.f;
-        }
-      }
-      if (x < RT) sm.inv[wave][x][lane & 15] = d > 0.f ? 1.f / d : 0.f;
-    }
-    if (lane < 16) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i) sm.lim[wave][i][lane] = rows.lim[i];
-    }
-    wave_lds_sync();
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int y = 4 * (lane >> 4) + e;
-        inv[i][e] = sm.lim[wave][i][y] >= 0 ? sm.inv[wave][i][y] : 0.f;
-      }
-  };
-  auto give = [&](int i, int u, int j0, const v8i &k, float &sum) {
-    const v4f a = score(rows.q[i], k);  // lane: key l % 16, rows 4 * (l / 16) + 0..3
-    float w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = weight(tab0, a[e]);
-    if (j0 + 16 * u + 15 > open) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = j0 + 16 * u + (lane & 15) <= sm.lim[wave][i][4 * (lane >> 4) + e] ? w[e] : 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(w[e], inv[i][e], sum);
-  };
-  auto add = [&](int j0, float (&sum)[4]) {  // what the rows give the 64 keys at j0
-    int64_t at[4];
-    keys.slots(j0, at);
-    v8i k[4];
-    int have = -1;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (rows.tg[i] < 0) continue;
-      if (rows.tg[i] != have) {
-        uint32_t x[4];
-        keys.load(rows.tg[i], at, x);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(x[u]);
-        have = rows.tg[i];
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) give(i, u, j0, k[u], sum[u]);
-    }
-  };
-  auto finish = [&](int j, float x) {
-    if (j < end) mass[j] = p.accumulate ? mass[j] + x : x;
-  };
-  if constexpr (SHARED) {
-    float sum[STEPS][4] = {};
-    for (int tile0 = wave * RT; tile0 < s.tiles; tile0 += kWaves * RT) {
-      take(tile0);
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st)
-        if (from + st * kStep < end) add(static_cast<int>(from) + st * kStep, sum[st]);
-      wave_lds_sync();  // (the limits are read before the next tiles' come)
-    }
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float x = sum[st][u];
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        if (lane < 16) sm.sum[wave][st * kStep + 16 * u + lane] = x;
-      }
-    __syncthreads();
-    for (int x = tid; x < kKeys; x += kWaves * 64)
-      finish(static_cast<int>(from) + x, (sm.sum[0][x] + sm.sum[1][x]) + (sm.sum[2][x] + sm.sum[3][x]));
-  } else {
-    // few products a key: the words of all steps are requested first
-    const int j1 = static_cast<int>(from) + wave * kStep;
-    int tg[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) tg[i] = i < s.tiles ? i / s.rtiles : 0;
-    uint32_t words[STEPS][RT][4];
-    request<WP, RT, STEPS>(keys, tg, j1, words);
-    take(0);
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      const int j0 = j1 + st * kWaves * kStep;
-      if (j0 >= end) break;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      auto add = [&](auto mask) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rows.tg[i] < 0) continue;
+        for (int i = 0; i < RT; ++i) {
+          if (i >= p.tgroups) continue;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) give(i, u, j0, fp4_bits(words[st][i][u]), sum[u]);
-      }
+          for (int u = 0; u < 4; ++u)
+            sum[u] = key_weights<decltype(mask)::value>(tab0, q[i], fp4_bits(ok[st][u] ? x[st][i][u] : 0u),
+                                                        j0 + 16 * u + (lane & 15), inv[i], lim, sum[u]);
+        }
+      };
+      if (j0 + kStep - 1 <= open) add(std::false_type{});
+      else add(std::true_type{});
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         sum[u] += __shfl_xor(sum[u], 16);
         sum[u] += __shfl_xor(sum[u], 32);
       }
       // lane l: key l of the step
-      const float x = lane < 32 ? (lane < 16 ? sum[0] : sum[1]) : (lane < 48 ? sum[2] : sum[3]);
-      finish(j0 + lane, x);
+      const float y = lane < 32 ? (lane < 16 ? sum[0] : sum[1]) : (lane < 48 ? sum[2] : sum[3]);
+      if (j0 + lane < end) mass[j0 + lane] = old[st] + y;
     }
+  }
+}
+
+// Many rows: denominators of kRows row tiles of a timestep group over kPart keys.
+template <int WP, bool PAGE>
+__global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
+  struct Smem {
+    float tab[kTab + 3];
+    float sum[kDenWaves][kRows][16];
+  };
+  __shared__ Smem sm;
+  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunks = (p.rtiles + kRows - 1) / kRows;
+  const int part = blockIdx.x % p.parts, group = blockIdx.x / p.parts;
+  const int tg = group / chunks, rt0 = (group - tg * chunks) * kRows;
+  const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
+  const Seq s = sequence<WP>(p, n);
+  if (part >= s.parts || rt0 >= s.rtiles) return;
+  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
+  const Keys<WP, PAGE> keys(p, s, n, kvh, lane);
+  const int j1 = part * kPart + wave * kStep, tiles = min(kRows, s.rtiles - rt0);
+  uint32_t x[kDenSteps][4];
+  bool ok[kDenSteps][4];
+  const uint32_t *at = keys.words(tg, lane);
+#pragma unroll
+  for (int st = 0; st < kDenSteps; ++st) {
+    const typename Keys<WP, PAGE>::Places to = keys.places(j1 + st * kDenWaves * kStep);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      ok[st][u] = to.ok[u];
+      x[st][u] = at[to.at[u]];
+    }
+  }
+  v8i q[kRows];
+  float l[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    q[i] = fp4_bits(query_word<WP>(p, s, kvh, tg, rt0 + i, lane));  // (rows behind the sequence's: 0)
+    l[i] = 0.f;
+  }
+  __syncthreads();
+  const int open = s.len - s.m;
+#pragma unroll
+  for (int st = 0; st < kDenSteps; ++st) {
+    const int j0 = j1 + st * kDenWaves * kStep;
+    v8i k[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u] = fp4_bits(ok[st][u] ? x[st][u] : 0u);
+    auto add = [&](auto mask) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        if (i >= tiles) break;
+        const int lim = decltype(mask)::value ? open + tile_row<WP>(p, rt0 + i, lane & 15) : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          l[i] += row_weights<decltype(mask)::value>(tab0, q[i], k[u], j0 + 16 * u, lane, lim);
+      }
+    };
+    if (j0 + kStep - 1 <= open) add(std::false_type{});
+    else if (j0 < s.len) add(std::true_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    l[i] += __shfl_xor(l[i], 16);
+    l[i] += __shfl_xor(l[i], 32);
+    if (lane < 16) sm.sum[wave][i][lane] = l[i];
+  }
+  __syncthreads();
+  if (tid < tiles * 16) {
+    float d = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDenWaves; ++w) d += sm.sum[w][tid / 16][tid % 16];
+    p.den[(((static_cast<int64_t>(blockIdx.y) * p.parts + part) * p.tgroups + tg) * p.rtiles + rt0) * 16 + tid] = d;
+  }
+}
+
+// Many rows: the weights of kMassKeys keys; kShare waves go through the row tiles of 64, four
+// by four (so a sequence of few rows has the sums of few_rows_kernel, a wave's).
+template <int WP, bool PAGE>
+__global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per_eu(4))) void mass_rows_kernel(Params p) {
+  constexpr int kThreads = kMassKeys * kShare;
+  struct Smem {
+    float tab[kTab + 3];
+    union {
+      float inv[kChunk][16];
+      float sum[kShare][kMassKeys];
+    };
+  };
+  __shared__ Smem sm;
+  const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), share = wave % kShare;
+  const int kvh = blockIdx.y % p.Hkv, n = blockIdx.y / p.Hkv;
+  const Seq s = sequence<WP>(p, n);
+  float *mass = p.mass + n * p.ms0 + kvh * p.ms1;
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * kMassKeys, stop = min(p.cap, from + kMassKeys);
+  if (!p.accumulate)
+    for (int64_t j = max<int64_t>(from, s.rtiles ? s.len : 0) + tid; j < stop; j += kThreads) mass[j] = 0.f;
+  if (from >= s.len || s.rtiles == 0) return;
+  if (tid <= p.D) sm.tab[tid] = p.tab[tid];
+  const Keys<WP, PAGE> keys(p, s, n, kvh, lane);
+  const int j0 = static_cast<int>(from) + wave / kShare * kStep, open = s.len - s.m;
+  const int end = min(s.len, static_cast<int>(stop)), tiles = s.rtiles * p.tgroups;
+  const typename Keys<WP, PAGE>::Places places = keys.places(j0);
+  const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tgroups * p.rtiles * 16;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  v8i k[4];
+  // the wave's tiles: tile x is row tile x % rtiles of timestep group x / rtiles
+  int tg = 0, rt = 4 * share, have = -1;
+  auto settle = [&] {
+    while (rt >= s.rtiles) {
+      rt -= s.rtiles;
+      ++tg;
+    }
+  };
+  settle();
+  uint32_t qw = tg < p.tgroups ? query_word<WP>(p, s, kvh, tg, rt, lane) : 0u;
+  for (int c0 = 0; c0 < tiles; c0 += kChunk) {
+    if (c0) __syncthreads();
+    for (int v = tid; v < min(kChunk, tiles - c0) * 16; v += kThreads) {
+      const int x = c0 + v / 16, xg = x / s.rtiles, xr = x - xg * s.rtiles, y = v % 16;
+      const float d = parts_sum(p, s, den + (xg * p.rtiles + xr) * 16 + y);
+      sm.inv[v / 16][y] = d > 0.f && has_row<WP>(p, s, xg, xr, y) ? 1.f / d : 0.f;
+    }
+    __syncthreads();
+    for (int x = c0 + 4 * share, step; x < min(c0 + kChunk, tiles); x += step) {
+      if (tg != have) {
+        const uint32_t *at = keys.words(tg, lane);
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = at[places.at[u]];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(places.ok[u] ? w[u] : 0u);
+        have = tg;
+      }
+      const v8i q = fp4_bits(qw);
+      const int row0 = rt;
+      step = x % 4 == 3 ? 4 * kShare - 3 : 1;
+      rt += step;
+      settle();
+      qw = tg < p.tgroups ? query_word<WP>(p, s, kvh, tg, rt, lane) : 0u;  // the next tile's
+      const v4f inv = *reinterpret_cast<const v4f *>(&sm.inv[x - c0][4 * (lane >> 4)]);
+      int lim[4];
+      if (j0 + kStep - 1 <= open) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] = key_weights<false>(tab0, q, k[u], 0, inv, lim, sum[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lim[e] = open + tile_row<WP>(p, row0, 4 * (lane >> 4) + e);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          sum[u] = key_weights<true>(tab0, q, k[u], j0 + 16 * u + (lane & 15), inv, lim, sum[u]);
+      }
+    }
+  }
+  __syncthreads();  // (the denominators' place takes the sums)
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    sum[u] += __shfl_xor(sum[u], 16);
+    sum[u] += __shfl_xor(sum[u], 32);
+    if (lane < 16) sm.sum[share][j0 - static_cast<int>(from) + 16 * u + lane] = sum[u];
+  }
+  __syncthreads();
+  if (tid < kMassKeys && from + tid < end) {
+    const float x = (sm.sum[0][tid] + sm.sum[1][tid]) + (sm.sum[2][tid] + sm.sum[3][tid]);
+    mass[from + tid] = p.accumulate ? mass[from + tid] + x : x;
   }
 }
 
@@ -412,9 +528,9 @@ inline void build_weights(float scale, int D, float *tab) {
   std::memcpy(tab, last, sizeof(float) * (D + 1));
 }
 
-// Rows of a product's timestep, timestep groups, row tiles.
+// Words of a head as the products have them, timestep groups, row tiles of one, parts.
 struct Plan {
-  int wp, tgroups, tiles, parts;
+  int wp, tgroups, rtiles, parts;
   size_t bytes;
 };
 inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_size, int max_blocks) {
@@ -423,29 +539,41 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_s
   r.wp = W == 3 ? 4 : W;
   const int64_t rows = static_cast<int64_t>(max_rows) * (Hq / Hkv);
   r.tgroups = (T + 4 / r.wp - 1) / (4 / r.wp);
-  r.tiles = static_cast<int>((rows + 4 * r.wp - 1) / (4 * r.wp)) * r.tgroups;
+  r.rtiles = static_cast<int>((rows + 4 * r.wp - 1) / (4 * r.wp));
   r.parts = static_cast<int>((static_cast<int64_t>(max_blocks) * block_size + kPart - 1) / kPart);
-  r.bytes = static_cast<size_t>(N) * Hkv * r.parts * r.tiles * 16 * sizeof(float);
+  r.bytes = static_cast<size_t>(N) * Hkv * r.parts * r.tgroups * r.rtiles * 16 * sizeof(float);
   return r;
 }
 
-template <int WP, int RT, int STEPS, bool SHARED>
-static int launch(const Params &p, hipStream_t s) {
-  const int chunks = (p.tiles + RT - 1) / RT, keys = STEPS * kStep * (SHARED ? 1 : kWaves);
-  // (without accumulation entries behind the table become 0)
-  const int64_t tokens = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
-  const int64_t wide = p.accumulate && tokens < p.cap ? tokens : p.cap;
-  if (p.parts > 0 && p.rows > 0) den_kernel<WP, RT><<<dim3(p.parts * chunks, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
-  mass_kernel<WP, RT, STEPS, SHARED><<<dim3((wide + keys - 1) / keys, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
+template <int WP, int RT, bool PAGE>
+static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
+  const dim3 grid((wide + kPart - 1) / kPart, p.N * p.Hkv);
+  if (p.parts <= 1) {
+    few_rows_kernel<WP, RT, PAGE, kBoth><<<grid, kWaves * 64, 0, s>>>(p);
+  } else {
+    few_rows_kernel<WP, RT, PAGE, kDen><<<dim3(p.parts, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
+    few_rows_kernel<WP, RT, PAGE, kMass><<<grid, kWaves * 64, 0, s>>>(p);
+  }
   return check_launch("key_mass");
 }
 
-// Row tiles a wave holds in registers: those of a decode step, or eight.
+template <int WP, bool PAGE>
+static int launch(const Params &p, hipStream_t s) {
+  // (without accumulation entries behind the table become 0)
+  const int64_t tokens = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
+  const int64_t wide = p.accumulate && tokens < p.cap ? tokens : p.cap;
+  if (p.rtiles == 1 && p.tgroups <= 2) return launch_few<WP, 2, PAGE>(p, wide, s);
+  if (p.rtiles == 1 && p.tgroups <= 4) return launch_few<WP, 4, PAGE>(p, wide, s);
+  const int chunks = (p.rtiles + kRows - 1) / kRows;
+  if (p.parts > 0 && p.rows > 0)
+    den_rows_kernel<WP, PAGE><<<dim3(p.parts * p.tgroups * chunks, p.N * p.Hkv), kDenWaves * 64, 0, s>>>(p);
+  mass_rows_kernel<WP, PAGE><<<dim3((wide + kMassKeys - 1) / kMassKeys, p.N * p.Hkv), kMassKeys * kShare, 0, s>>>(p);
+  return check_launch("key_mass");
+}
+
 template <int WP>
-static int launch_rows(const Params &p, hipStream_t s) {
-  if (p.tiles <= 2) return launch<WP, 2, 4, false>(p, s);
-  if (p.tiles <= 4) return launch<WP, 4, 2, false>(p, s);
-  return launch<WP, 8, 2, true>(p, s);
+static int launch_pages(const Params &p, hipStream_t s) {
+  return p.bs_log2 >= 4 ? launch<WP, true>(p, s) : launch<WP, false>(p, s);
 }
 
 }  // namespace mass
@@ -484,7 +612,7 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
     return fail(SPK_EINVAL, "key_mass: null pointer");
   const mass::Plan plan = mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks);
   if (static_cast<int64_t>(max_rows) * (Hq / Hkv) > (1 << 24) ||
-      static_cast<int64_t>(plan.tiles) * plan.parts > (1 << 30) || cap > (1 << 30))
+      static_cast<int64_t>(plan.rtiles) * plan.tgroups * plan.parts > (1 << 30) || cap > (1 << 30))
     return fail(SPK_EUNSUPPORTED, "key_mass: %d rows of %d heads over %d x %d tokens", max_rows, Hq / Hkv, max_blocks,
                 block_size);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
@@ -507,13 +635,13 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
   p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
   p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks;
-  p.tgroups = plan.tgroups; p.tiles = plan.tiles; p.parts = plan.parts;
+  p.tgroups = plan.tgroups; p.rtiles = plan.rtiles; p.parts = plan.parts;
   p.den = static_cast<float *>(workspace);
   mass::build_weights(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (plan.wp) {
-    case 1: return mass::launch_rows<1>(p, s);
-    case 2: return mass::launch_rows<2>(p, s);
-    default: return mass::launch_rows<4>(p, s);
+    case 1: return mass::launch_pages<1>(p, s);
+    case 2: return mass::launch_pages<2>(p, s);
+    default: return mass::launch_pages<4>(p, s);
   }
 }
