@@ -80,7 +80,8 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t x, int lane, int wave, ui
 // EACH: masses a thread keeps in registers (EACH * kSelThreads tokens at most); 0: none, they
 // are read again where they are needed.
 template <int EACH>
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
+__global__ __launch_bounds__(kSelThreads) __attribute__((amdgpu_waves_per_eu(EACH <= 16 ? 8 : 4))) void
+evict_select_kernel(Params p) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t counts[EACH ? EACH * kSelWaves : 2 * kSelWaves], waves[2][kSelWaves], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -100,10 +101,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
   }
 
   float m[EACH ? EACH : 1];
+  uint32_t key[EACH ? EACH : 1];
   if constexpr (EACH > 0) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
       if (i * kSelThreads < len) m[i] = mass[min(i * kSelThreads + tid, len - 1)];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (i * kSelThreads < len) key[i] = key_of(m[i]);
   }
   // The candidates' free-th largest key, and how many equal to it stay.
   const int lo = p.sinks, hi = len - p.recent;
@@ -115,21 +120,21 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
       for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      auto count = [&](int j, float x) {
-        const uint32_t k = key_of(x);
-        if (j >= lo && j < hi && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+      auto count = [&](int j, uint32_t k, bool inside) {
+        if ((inside || (j >= lo && j < hi)) && (k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
       };
       if constexpr (EACH > 0) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
-          if (i * kSelThreads < hi) count(i * kSelThreads + tid, m[i]);
+          if (i * kSelThreads >= lo && (i + 1) * kSelThreads <= hi) count(0, key[i], true);
+          else if (i * kSelThreads < hi) count(i * kSelThreads + tid, key[i], false);
       } else {
         for (int j0 = 0; j0 < len; j0 += 8 * kSelThreads) {
           float x[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = mass[min(j0 + i * kSelThreads + tid, len - 1)];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) count(j0 + i * kSelThreads + tid, x[i]);
+          for (int i = 0; i < 8; ++i) count(j0 + i * kSelThreads + tid, key_of(x[i]), false);
         }
       }
       __syncthreads();
@@ -152,8 +157,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
   }
 
   // Kept tokens in position order: `sure` ones, and the first `free` equal ones.
-  auto look = [&](int j, float x, bool &sure, bool &equal) {
-    const uint32_t k = key_of(x);
+  auto look = [&](int j, uint32_t k, bool &sure, bool &equal) {
     const bool edge = j < len && (j < lo || j >= hi), in = j >= lo && j < hi && any;
     sure = edge || (in && k > prefix);
     equal = in && k == prefix;
@@ -168,7 +172,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
         continue;
       }
       bool sure, equal;
-      look(i * kSelThreads + tid, m[i], sure, equal);
+      look(i * kSelThreads + tid, key[i], sure, equal);
       const uint64_t sb = __ballot(sure), eb = __ballot(equal);
       if (lane == 0) counts[i * kSelWaves + wave] = __popcll(sb) | __popcll(eb) << 16;
     }
@@ -183,7 +187,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
       const int j = i * kSelThreads + tid;
       if (i * kSelThreads >= len) break;
       bool sure, equal;
-      look(j, m[i], sure, equal);
+      look(j, key[i], sure, equal);
       const uint64_t sb = __ballot(sure), eb = __ballot(equal);
       const uint32_t base = counts[i * kSelWaves + wave];
       const int s = (base & 0xffff) + __popcll(sb & below), e = (base >> 16) + __popcll(eb & below);
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(Params p) {
       const int j = j0 + tid;
       const float x = mass[min(j, len - 1)];
       bool sure, equal;
-      look(j, x, sure, equal);
+      look(j, key_of(x), sure, equal);
       const uint64_t sb = __ballot(sure), eb = __ballot(equal);
       if (lane == 0) counts[turn * kSelWaves + wave] = __popcll(sb) | __popcll(eb) << 16;
       __syncthreads();  // (all of the chunk is read: what is written below lies in it or before)
