@@ -6,7 +6,7 @@
 //                      exp(popc(q & k_j) * scale) / sum_j' exp(popc(q & k_j') * scale).
 //
 // MI355X design: scores of 16 rows and 16 keys are one fp4 product over 128 channels
-// (v_mfma_scale_f32_16x16x128_f8f6f4, bits as 0.5 in place, block scales that leave the
+// (v_mfma_scale_f32_16x16x128_f8f6f4, a spike of both as 1, block scales that leave the
 // score's table offset in the accumulator's bits, as spike_tiles.hpp has it), a weight is a
 // look-up in LDS.  128 channels are 4 / WP timesteps of a head (WP: words of a head, a power
 // of two): a product's 16 rows are 4 * WP of each of these timesteps, whose words stand in
@@ -95,6 +95,25 @@ __device__ __forceinline__ bool has_row(const Params &p, const Seq &s, int tg, i
   return tile_row<WP>(p, rt, y) < s.m && tg * (4 / WP) + y / (4 * WP) < p.T;
 }
 
+// 32 bits as 32 fp4 values, 8 of each 4th bit: a key's bits stay where they are (0.5, 1 and 2,
+// and the sign's at 2), the query's hold what makes their products 1.
+__device__ __forceinline__ v8i key_bits(uint32_t w) {
+  v8i r = {};
+  r[0] = static_cast<int>(w & 0x11111111u);
+  r[1] = static_cast<int>(w & 0x22222222u);
+  r[2] = static_cast<int>(w & 0x44444444u);
+  r[3] = static_cast<int>(w >> 1 & 0x44444444u);
+  return r;
+}
+__device__ __forceinline__ v8i query_bits(uint32_t w) {
+  v8i r = {};
+  r[0] = static_cast<int>(w << 2 & 0x44444444u);
+  r[1] = static_cast<int>(w & 0x22222222u);
+  r[2] = static_cast<int>(w >> 2 & 0x11111111u);
+  r[3] = static_cast<int>(w >> 3 & 0x11111111u);
+  return r;
+}
+
 // A lane's query word of a row tile (row l % 16, block l / 16 of the product's channels).
 template <int WP>
 __device__ __forceinline__ uint32_t query_word(const Params &p, const Seq &s, int kvh, int tg, int rt, int lane) {
@@ -153,7 +172,7 @@ struct Keys {
 };
 
 __device__ __forceinline__ v4f score(const v8i &a, const v8i &b) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{}, 4, 4, 0, 55, 0, 54);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, v4f{}, 4, 4, 0, 54, 0, 53);
 }
 
 __device__ __forceinline__ float weight(uint32_t tab0, float score) {
@@ -258,7 +277,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
   }
   v8i q[RT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) q[i] = fp4_bits(i < p.tgroups ? query_word<WP>(p, s, kvh, i, 0, lane) : 0u);
+  for (int i = 0; i < RT; ++i) q[i] = query_bits(i < p.tgroups ? query_word<WP>(p, s, kvh, i, 0, lane) : 0u);
   const int open = s.len - s.m;  // keys up to `open` are seen by all rows
   float *den = p.den + (static_cast<int64_t>(blockIdx.y) * p.parts + (PASS == kDen ? blockIdx.x : 0)) * p.tgroups * 16;
   if constexpr (PASS == kMass) {
@@ -284,7 +303,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
           if (i >= p.tgroups) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            l[st & 1][i] += row_weights<decltype(mask)::value>(tab0, q[i], fp4_bits(ok[st][u] ? x[st][i][u] : 0u),
+            l[st & 1][i] += row_weights<decltype(mask)::value>(tab0, q[i], key_bits(ok[st][u] ? x[st][i][u] : 0u),
                                                                j0 + 16 * u, lane, lim);
         }
       };
@@ -330,7 +349,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
           if (i >= p.tgroups) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            sum[u] = key_weights<decltype(mask)::value>(tab0, q[i], fp4_bits(ok[st][u] ? x[st][i][u] : 0u),
+            sum[u] = key_weights<decltype(mask)::value>(tab0, q[i], key_bits(ok[st][u] ? x[st][i][u] : 0u),
                                                         j0 + 16 * u + (lane & 15), inv[i], lim, sum[u]);
         }
       };
@@ -384,7 +403,7 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
   float l[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    q[i] = fp4_bits(query_word<WP>(p, s, kvh, tg, rt0 + i, lane));  // (rows behind the sequence's: 0)
+    q[i] = query_bits(query_word<WP>(p, s, kvh, tg, rt0 + i, lane));  // (rows behind the sequence's: 0)
     l[i] = 0.f;
   }
   __syncthreads();
@@ -394,7 +413,7 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
     const int j0 = j1 + st * kDenWaves * kStep;
     v8i k[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) k[u] = fp4_bits(ok[st][u] ? x[st][u] : 0u);
+    for (int u = 0; u < 4; ++u) k[u] = key_bits(ok[st][u] ? x[st][u] : 0u);
     auto add = [&](auto mask) {
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
@@ -479,10 +498,10 @@ __global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per
 #pragma unroll
         for (int u = 0; u < 4; ++u) w[u] = at[places.at[u]];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) k[u] = fp4_bits(places.ok[u] ? w[u] : 0u);
+        for (int u = 0; u < 4; ++u) k[u] = key_bits(places.ok[u] ? w[u] : 0u);
         have = tg;
       }
-      const v8i q = fp4_bits(qw);
+      const v8i q = query_bits(qw);
       const int row0 = rt;
       step = x % 4 == 3 ? 4 * kShare - 3 : 1;
       rt += step;
