@@ -33,7 +33,7 @@ class DraftTrees:
     The step's rows are the trees' rows: ``row_starts[n] .. row_starts[n + 1]`` those of
     sequence ``n``, row 0 its last token.  ``words`` holds each layer's ``(k, v)`` words of
     the rows (``int32 [T, rows, H_kv, W]``), written by the step and read by
-    :func:`accept_draft_tree`; None lets the step allocate them.
+    :func:`accept_draft_tree`; None (or none) lets the step allocate them.
     """
 
     row_starts: torch.Tensor  # int32 [N + 1]
@@ -91,12 +91,16 @@ class AttentionMetadata:
         if key not in self._copies:
             move = lambda t: None if t is None else t.to(device, non_blocking=True)
             draft, mass = self.draft, self.key_mass
+            for t in [t for kv in (draft and draft.words or ()) for t in kv] + list(mass or ()):
+                if (t.device.type, t.device.index or 0) != (device.type, device.index or 0):
+                    raise ValueError(f"what the step writes (draft.words, key_mass) must be on {device}, not {t.device}")
             if draft is not None:
+                if draft.words is None:
+                    draft.words = []  # (the copy's step fills the same list)
                 draft = replace(draft, row_starts=move(draft.row_starts), masks=move(draft.masks),
-                                context_lens=move(draft.context_lens), block_tables=move(draft.block_tables),
-                                words=draft.words and [(move(k), move(v)) for k, v in draft.words])
+                                context_lens=move(draft.context_lens), block_tables=move(draft.block_tables))
             self._copies[key] = replace(
-                self, draft=draft, key_mass=mass and [move(m) for m in mass], slot_mapping=move(self.slot_mapping), block_tables=move(self.block_tables),
+                self, draft=draft, slot_mapping=move(self.slot_mapping), block_tables=move(self.block_tables),
                 seq_lens=move(self.seq_lens),
                 prefill_block_tables=[move(t) for t in self.prefill_block_tables], _copies={})
         return self._copies[key]

@@ -487,7 +487,7 @@ __global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per
     if (c0) __syncthreads();
     for (int v = tid; v < min(kChunk, tiles - c0) * 16; v += kThreads) {
       const int x = c0 + v / 16, xg = x / s.rtiles, xr = x - xg * s.rtiles, y = v % 16;
-      const float d = parts_sum(p, s, den + (xg * p.rtiles + xr) * 16 + y);
+      const float d = parts_sum(p, s, den + static_cast<int64_t>(xg * p.rtiles + xr) * 16 + y);
       sm.inv[v / 16][y] = d > 0.f && has_row<WP>(p, s, xg, xr, y) ? 1.f / d : 0.f;
     }
     __syncthreads();
@@ -629,6 +629,8 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   if (static_cast<int64_t>(N) * Hkv > 65535) return fail(SPK_EUNSUPPORTED, "key_mass: %d sequences of %d heads", N, Hkv);
   if ((rows > 0 && !q) || !seq_lens || !mass || (max_blocks > 0 && !block_tables) || (num_slots > 0 && !k_cache))
     return fail(SPK_EINVAL, "key_mass: null pointer");
+  if ((N > 1 && !mass_strides[0]) || (Hkv > 1 && !mass_strides[1]))
+    return fail(SPK_EINVAL, "key_mass: rows of mass lie on one another");
   const mass::Plan plan = mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks);
   if (static_cast<int64_t>(max_rows) * (Hq / Hkv) > (1 << 24) ||
       static_cast<int64_t>(plan.rtiles) * plan.tgroups * plan.parts > (1 << 30) || cap > (1 << 30))

@@ -633,6 +633,8 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   if (!q || !k_tree || !v_tree || !context_lens || !row_starts || !masks || !out ||
       (max_blocks > 0 && !block_tables) || (num_slots > 0 && (!k_cache || !v_cache)))
     return fail(SPK_EINVAL, "tree_attn: null pointer");
+  if ((T > 1 && !out_strides[0]) || (rows > 1 && !out_strides[1]) || (Hq > 1 && !out_strides[2]))
+    return fail(SPK_EINVAL, "tree_attn: rows of out lie on one another");
   const tree::Plan plan = tree::plan(T, N, Hq, Hkv, head_dim, max_nodes, block_size, max_blocks);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return fail(SPK_EINVAL, "tree_attn: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);

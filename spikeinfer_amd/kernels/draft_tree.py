@@ -84,7 +84,8 @@ def paged_spike_attn_tree(
             ``i / 64`` lets the row see row ``i`` of its tree (:func:`draft_tree_masks`).
         out: optional ``[T, R, H_q, head_dim]``, channels contiguous (needed for graph
             capture); by default a new tensor of ``dtype``, zeros in rows of no sequence.
-        workspace: optional ``uint8`` scratch of :func:`tree_attn_workspace_bytes`.
+        workspace: optional ``uint8`` scratch of :func:`tree_attn_workspace_bytes`; calls that
+            may run at once need one each.
 
     A row that sees nothing gets zeros; rows of ``out`` that are no sequence's are left as they
     were.  A sequence's outputs do not depend on the batch.
@@ -219,7 +220,7 @@ def accept_draft_tree(
 
     Returns ``path int32 [N, max_nodes]`` (rows of the tree, -1 behind the path),
     ``count int32 [N]`` (the path's rows, row 0 among them; 0 for a sequence without rows)
-    and ``next int64 [N]``, the model's token after the path.
+    and ``next int64 [N]``, the model's token after the path (-1 without rows).
     """
     native = _lib.native()
     if native is not None and layers:

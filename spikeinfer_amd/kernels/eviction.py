@@ -54,9 +54,11 @@ def paged_spike_attn_key_mass(
         k_cache: ``int32 [T, H_kv, slots, W]``; block_tables ``int32 [N, max_blocks]``;
             seq_lens ``int32 [N]`` with the rows' own tokens.
         out: optional ``float32 [N, H_kv, cap]``, entries contiguous; by default a new one
-            of ``max_blocks * block_size`` entries.  Entries behind a sequence become 0.
+            of ``max_blocks * block_size`` entries.  Entries behind a sequence become 0;
+            tokens at ``cap`` and behind are left out.
         accumulate: add to ``out`` instead, and leave the rest of it as it was.
-        workspace: optional ``uint8`` scratch of :func:`key_mass_workspace_bytes`.
+        workspace: optional ``uint8`` scratch of :func:`key_mass_workspace_bytes`; calls that
+            may run at once need one each.
     """
     native = _lib.native()
     if native is not None:
@@ -134,7 +136,8 @@ def evict_cache(
         dst_tables: ``int32 [N, blocks]``, where the kept words go; by default the
             sequences' own blocks (which no other sequence may share).  These blocks must
             be none that the call reads.
-        mass_out: where the kept masses go (0 behind them); by default ``mass`` itself.
+        mass_out: where the kept masses go (0 behind them); by default ``mass`` itself, else a
+            tensor apart from it.
 
     Returns ``keep int32 [L, N, H_kv, budget]``, the kept positions in order (-1 behind), and
     ``new_lens int32 [N] = min(seq_lens, budget)``.  The kept tokens stand at positions 0,

@@ -264,9 +264,10 @@ class SpikingDecoder:
         if packed_prefill and 0 in meta.prefill_context_lens:
             kv_packed = tuple(torch.empty((T, n, Hkv, self.W), dtype=torch.int32, device=h.device)
                               for _ in range(2))
-        if draft is not None and draft.words is None:
-            draft.words = [tuple(torch.empty((T, n, Hkv, self.W), dtype=torch.int32, device=h.device)
-                                 for _ in range(2)) for _ in self.layers]
+        if draft is not None and not draft.words:
+            draft.words = [] if draft.words is None else draft.words
+            draft.words += [tuple(torch.empty((T, n, Hkv, self.W), dtype=torch.int32, device=h.device)
+                                  for _ in range(2)) for _ in self.layers]
         attn = bufs.get("attn")
         if attn is None:
             attn = torch.empty((T, n, Hq, D), dtype=self.dtype, device=h.device)

@@ -122,3 +122,65 @@ def test_plain_code():
     v = torch.cat([ref.bits(ref.positions(case["v_cache"], case["block_tables"][0], 2, 16), 32)[0, 0],
                    ref.bits(case["v_words"], 32)[0, :1, 0]])
     assert torch.allclose(out[0, 0, 0], w @ v)
+
+
+def test_outputs_that_lie_on_one_another_are_refused():
+    """Broadcast outputs and a cache given as two layers would be written by several
+    workgroups at once."""
+    lib = _lib.load()
+    s, flat = _i64(1, 1, 1), _i64(0, 1, 1)
+
+    def tree(out_strides, T=4, hq=14, rows=10):
+        return lib.spk_tree_attn(P, s, P, P, s, P, P, s, 100, P, 8, 1, P, P, P, 1, P, 0, out_strides, rows, 2, 8, T, hq,
+                                 2, 64, 16, 1 << 10, 0.125, None, 0, None)
+
+    for i in range(3):
+        assert tree(_i64(*(int(i != j) for j in range(3)))) == _lib.SPK_EINVAL
+        assert b"one another" in lib.spk_last_error()
+
+    def mass(strides):
+        return lib.spk_key_mass(P, s, P, s, 100, P, 8, 1, P, None, P, strides, 100, 0, 2, 2, 1, 4, 14, 2, 64, 16, 8,
+                                0.125, P, 1 << 20, None)
+
+    for strides in (_i64(0, 1), _i64(1, 0)):
+        assert mass(strides) == _lib.SPK_EINVAL and b"one another" in lib.spk_last_error()
+
+    words = lambda *p: b"".join(x.to_bytes(8, "little") for x in p)
+
+    def accept(layers, strides):
+        return lib.spk_accept_tree(P, P, P, P, 10, 2, 8, P, P, P, layers, len(layers) // 32, s, strides, 100, P, 8, 1, P,
+                                   4, 2, 64, 16, 8, None)
+
+    def evict(layers, strides=s, to=s):
+        return lib.spk_evict(layers, len(layers) // 16, strides, 100, P, s, P, to, 128, P, 8, 1, 8, None, 0, 0, 0, P, P,
+                             P, 64, 4, 32, 4, 2, 2, 64, 16, None)
+
+    four, two = words(P, P, P, 2 * P), words(P, 2 * P)
+    for i in range(3):
+        strides = _i64(*(int(i != j) for j in range(3)))
+        assert accept(four, strides) == evict(two, strides) == evict(two + words(3 * P, 4 * P), s, strides) == \
+            _lib.SPK_EINVAL
+        assert b"one another" in lib.spk_last_error()
+    for last in (words(P, 5 * P), words(5 * P, 2 * P)):
+        assert accept(four + words(P, P) + last, s) == _lib.SPK_EINVAL and b"one cache" in lib.spk_last_error()
+        assert evict(two + last) == _lib.SPK_EINVAL and b"one cache" in lib.spk_last_error()
+
+
+def test_metadata_moved_to_a_device_keeps_what_the_step_writes():
+    """A copy on another device shares the list that the step's words come into, and
+    refuses tensors that the caller would wait for in vain."""
+    from dataclasses import replace
+
+    from spikeinfer_amd.attention import AttentionMetadata, DraftTrees
+
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    trees = DraftTrees(i32(2), torch.zeros((3, 1), dtype=torch.int64), 3, i32(1), i32(1, 4))
+    meta = AttentionMetadata(slot_mapping=torch.full((3,), -1), block_size=16, draft=trees)
+    copy = meta.on("meta")
+    assert copy.draft.masks.device.type == "meta" and trees.masks.device.type == "cpu"
+    assert copy.draft.words is trees.words and trees.words == []
+    assert meta.on("cpu").draft is trees
+    for bad in (replace(meta, draft=replace(trees, words=[(i32(1), i32(1))]), _copies={}),
+                replace(meta, draft=None, key_mass=[torch.zeros(1, 1, 8)], _copies={})):
+        with pytest.raises(ValueError, match="must be on meta"):
+            bad.on("meta")
