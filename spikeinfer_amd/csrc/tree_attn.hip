@@ -10,14 +10,13 @@
 //     own, so that a row's mask word is the tile's.
 //   * Scores as there: one fp4 product per 64 channels leaves the score's table offset in
 //     the accumulator's bits, and the weight is a look-up.
-//   * Values: f16 products over two keys a register.  fp32 and fp16 outputs take the
-//     weights' two halves, exact to 2^-23, in two products.  bf16
-//     outputs take the 11-bit high halves alone (each off by at most 2^-11, and the
-//     denominator sums the same halves, where the output's own rounding is 2^-8): half the
-//     products.  There a v bit becomes an operand in place, as one of f16's exponent bits
-//     (2^-14, 2^-13, 2^-11 or 2^-7 by the key's number % 4), and four tables of weights
-//     hold what makes the products equal again: one `and` a register instead of a
-//     multiplication more.
+//   * Values: f16 products over two keys a register.  A v bit becomes an operand by one `and`,
+//     as one of f16's exponent bits, and tables of weights hold what makes the products equal
+//     again.  bf16 outputs take the weights' 11-bit high halves alone (each off by at most
+//     2^-11, and the denominator sums the same halves, where the output's own rounding is
+//     2^-8), from four tables for 2^-14, 2^-13, 2^-11 and 2^-7 by the key's number % 4.  fp32
+//     and fp16 outputs take both halves, in two products, from two tables for 2^-14 and 2^-13:
+//     the smallest weight, 2^15 / e^12, keeps 2^-21 of itself, larger ones up to 2^-23.
 //   * Eight waves a workgroup (four with more than 64 channels) share the key tiles' operands
 //     through LDS: each prepares one of a step's tiles, two buffers of them so that one barrier
 //     a step does.  Of a sequence of more than 128 rows a workgroup takes 256, a wave a row
@@ -105,15 +104,17 @@ __device__ __forceinline__ int node_of(const Params &p, int r) {
 
 // Weight tables in LDS at offset 0.  bf16 outputs: four of the weights' high halves as fp32,
 // whose entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's (all of them f16 numbers).  Else
-// one of (hi, lo) pairs.
-template <bool F32> constexpr int kTables = F32 ? 1 : 4;
+// two of (hi, lo) pairs, 2^0 and 2^-1.
+template <bool F32> constexpr int kTables = F32 ? 2 : 4;
 template <bool F32>
 __device__ __forceinline__ void fill_tables(const Params &p, float *tab, int tid) {
   if (tid > p.D) return;
   const uint32_t w = p.tab[tid];
   const float hi = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
   if constexpr (F32) {
+    const v2h half = __builtin_bit_cast(v2h, w) * v2h{static_cast<_Float16>(0.5f), static_cast<_Float16>(0.5f)};
     tab[tid] = __uint_as_float(w);
+    tab[kTabStride + tid] = __builtin_bit_cast(float, half);
   } else {
     tab[tid] = hi;
     tab[kTabStride + tid] = hi * 0.5f;
@@ -213,19 +214,28 @@ __device__ __forceinline__ uint32_t seen(const Seq &s, int kt, const uint32_t *w
   return see >> (4 * half);
 }
 
-// Products' value operands of a channel tile: register i of operand g pairs the lane's keys
-// 4g + i and 4g + i + 8, sixteen bits apart in vt.
+// A lane's v bits of a channel tile where `expand` masks them: [operand][key % 4 / kEach] with
+// kEach keys' bits from bit 10 on.
+template <bool F32> struct Bits {
+  static constexpr int kEach = F32 ? 2 : 4;
+  typedef uint32_t type __attribute__((ext_vector_type(8 / kEach)));
+};
 template <bool F32>
-__device__ __forceinline__ void expand(uint32_t vt, v8h (&vop)[2]) {
+__device__ __forceinline__ typename Bits<F32>::type place_bits(uint32_t vt) {
+  if constexpr (F32) return typename Bits<F32>::type{vt << 10, vt << 8, vt << 2, vt};
+  else return typename Bits<F32>::type{vt << 10, vt << 2};
+}
+
+// Products' value operands of a channel tile: register i of operand g pairs the lane's keys
+// 4g + i and 4g + i + 8, sixteen bits apart.
+template <bool F32>
+__device__ __forceinline__ void expand(typename Bits<F32>::type vt, v8h (&vop)[2]) {
+  constexpr int kEach = Bits<F32>::kEach, kWords = 4 / kEach;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     v4u x;
-    // fp32: bit b at place i <= 3 becomes 1.0 by a 24-bit product with 0x3c00 >> i; else it
-    // moves to bit 10 + i
-    const uint32_t b = F32 ? (g ? vt >> 8 : vt) : (g ? vt << 2 : vt << 10);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[i] = F32 ? __umul24(b & (0x00010001u << i), 0x3c00u >> i) : b & (0x04000400u << i);
+    for (int i = 0; i < 4; ++i) x[i] = vt[g * kWords + i / kEach] & (0x04000400u << i % kEach);
     vop[g] = __builtin_bit_cast(v8h, x);
   }
 }
@@ -244,7 +254,7 @@ template <bool F32>
 __device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint32_t at = tab0 + (F32 ? 0 : 4 * kTabStride * (e & 3)) + __float_as_uint(a[e]);
+    const uint32_t at = tab0 + 4 * kTabStride * (e & (kTables<F32> - 1)) + __float_as_uint(a[e]);
     w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
   }
 }
@@ -253,7 +263,7 @@ __device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&
 // one: dot products of f16 pairs would be half as many instructions, but they take the matrix
 // cores' time (8 behind each product 78 cycles where 8 additions take 52).  Of a pair's halves
 // the high ones are added in fp32.  The low ones, below 2^-11 of theirs, are first added in
-// f16, eight to a sum in three steps: off by at most 3 * 2^-11 of themselves, 2^-20 of the
+// f16, four to a sum in two steps: off by at most 2 * 2^-11 of themselves, 2^-21 of the
 // weights at the very worst and 2^-23 in the mean, their own resolution.
 template <int NC, bool F32, bool MASKED>
 __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, const v8h (&vop)[NC][2],
@@ -266,7 +276,7 @@ __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, 
       return x[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
     else return x[e];
   };
-  v2h low[2];
+  v2h low[2][2];  // by table
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     v4u y[kParts];  // the weights' halves, two keys a register
@@ -287,7 +297,8 @@ __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, 
     }
     if constexpr (F32) {
       auto half2 = [&](int i) { return __builtin_bit_cast(v2h, static_cast<uint32_t>(y[1][i])); };
-      low[g] = (half2(0) + half2(1)) + (half2(2) + half2(3));
+      low[0][g] = half2(0) + half2(2);
+      low[1][g] = half2(1) + half2(3);
     }
 #pragma unroll
     for (int q = 0; q < kParts; ++q)
@@ -296,16 +307,19 @@ __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, 
         acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, y[q]), acc[c], 0, 0, 0);
   }
   if constexpr (F32) {
-    const v2h sum = low[0] + low[1];
-    l[0] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[0]);
-    l[1] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const v2h sum = low[i][0] + low[i][1];
+      l[i] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[i]);
+      l[i] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[i]);
+    }
   }
 }
 
 // A lane's denominator, of its own keys, in the numerators' units.
 template <bool F32>
 __device__ __forceinline__ float lane_sum(const float (&l)[4]) {
-  if constexpr (F32) return (l[0] + l[1]) + (l[2] + l[3]);
+  if constexpr (F32) return ((l[0] + 2.f * l[1]) + (l[2] + 2.f * l[3])) * 0x1p-14f;
   else return ((l[0] + 2.f * l[1]) + (8.f * l[2] + 128.f * l[3])) * 0x1p-14f;
 }
 
@@ -401,7 +415,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       sm.k[buf][wave][k][lane] = v4u{static_cast<uint32_t>(kop[k][0]), static_cast<uint32_t>(kop[k][1]),
                                      static_cast<uint32_t>(kop[k][2]), static_cast<uint32_t>(kop[k][3])};
 #pragma unroll
-    for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = vt[c];
+    for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = place_bits<F32>(vt[c]);
   };
   prepare(0);
   request(t0 + kStep);
@@ -501,7 +515,7 @@ tree_attn_kernel(Params p) {
     union {
       struct {
         v4u k[2][kStep][NK][64];
-        uint32_t v[2][kStep][NC][64];
+        typename Bits<F32>::type v[2][kStep][NC][64];
       };
       float red[kWaves][16][64];
     };
