@@ -83,7 +83,8 @@ struct Params {
 // Workgroup (n, layer): its first wave walks tree n, a step a round of 64 candidate
 // children; then the threads move the path's words of the layer.  Every layer's
 // workgroup walks again: the walk takes a few hundred ns a step from LDS, a second
-// launch would take more.
+// launch would take more.  Latency only: 24 layers of one tree of 8 rows take 4.1 us, of 64
+// trees of 61 rows 7.0.
 __global__ __launch_bounds__(kThreads) void accept_kernel(Params p) {
   __shared__ int64_t tok[kMaxNodes], tgt[kMaxNodes];
   __shared__ int32_t par[kMaxNodes], path[kMaxNodes];

@@ -20,6 +20,13 @@
 //   Many rows: den_rows_kernel goes through kPart keys with kRows row tiles in registers;
 //     mass_rows_kernel has 128 keys, in registers, and its waves share the row tiles.
 // The order of all sums is the sequence's own, whatever the batch.
+//
+// Bound by instruction issue and latency, with few rows near the bytes': 4 timesteps, 14 query
+// and 2 kv heads of 64 channels, one row of each of 64 sequences of 4,096..16,384 tokens takes
+// 17 + 22 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
+// where a vector unit is busy for about half the time: a product has 24 vector instructions
+// beside it, four look-ups and their sums and the key's five.  Windows of up to 32 rows of 8
+// sequences of 2,000..8,000 tokens take 21 + 21 us.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -128,7 +135,9 @@ __device__ __forceinline__ uint32_t query_word(const Params &p, const Seq &s, in
 // A lane's words of a step's four key tiles (lane l: key l % 16 of a tile, block l / 16 of
 // the product's channels).  Keys behind the sequence read its last block, what they give is
 // dropped; so is, by the queries' zeros, what a block of no timestep or word gives.
-// PAGE: blocks are of 16 slots or more, a key tile lies in one and its place is scalar.
+// PAGE: blocks are of 16 slots or more, a key tile lies in one and its place is scalar (36.7 us
+// where lanes' own places take 40.9, 64 sequences of 4,096..16,384 tokens; with many rows there
+// is no difference).
 template <int WP, bool PAGE>
 struct Keys {
   const Params &p;
@@ -368,7 +377,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
 }
 
 // Many rows: denominators of kRows row tiles of a timestep group over kPart keys.
-template <int WP, bool PAGE>
+template <int WP>
 __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
   struct Smem {
     float tab[kTab + 3];
@@ -385,14 +394,14 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
   const Seq s = sequence<WP>(p, n);
   if (part >= s.parts || rt0 >= s.rtiles) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
-  const Keys<WP, PAGE> keys(p, s, n, kvh, lane);
+  const Keys<WP, false> keys(p, s, n, kvh, lane);
   const int j1 = part * kPart + wave * kStep, tiles = min(kRows, s.rtiles - rt0);
   uint32_t x[kDenSteps][4];
   bool ok[kDenSteps][4];
   const uint32_t *at = keys.words(tg, lane);
 #pragma unroll
   for (int st = 0; st < kDenSteps; ++st) {
-    const typename Keys<WP, PAGE>::Places to = keys.places(j1 + st * kDenWaves * kStep);
+    const typename Keys<WP, false>::Places to = keys.places(j1 + st * kDenWaves * kStep);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       ok[st][u] = to.ok[u];
@@ -444,7 +453,7 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
 
 // Many rows: the weights of kMassKeys keys; kShare waves go through the row tiles of 64, four
 // by four (so a sequence of few rows has the sums of few_rows_kernel, a wave's).
-template <int WP, bool PAGE>
+template <int WP>
 __global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per_eu(4))) void mass_rows_kernel(Params p) {
   constexpr int kThreads = kMassKeys * kShare;
   struct Smem {
@@ -466,10 +475,10 @@ __global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per
     for (int64_t j = max<int64_t>(from, s.rtiles ? s.len : 0) + tid; j < stop; j += kThreads) mass[j] = 0.f;
   if (from >= s.len || s.rtiles == 0) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
-  const Keys<WP, PAGE> keys(p, s, n, kvh, lane);
+  const Keys<WP, false> keys(p, s, n, kvh, lane);
   const int j0 = static_cast<int>(from) + wave / kShare * kStep, open = s.len - s.m;
   const int end = min(s.len, static_cast<int>(stop)), tiles = s.rtiles * p.tgroups;
-  const typename Keys<WP, PAGE>::Places places = keys.places(j0);
+  const typename Keys<WP, false>::Places places = keys.places(j0);
   const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tgroups * p.rtiles * 16;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   v8i k[4];
@@ -564,6 +573,7 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_s
   return r;
 }
 
+// With one part a launch does both passes: 8.6 us where two take 12.6 (a sequence of 700 tokens).
 template <int WP, int RT, bool PAGE>
 static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
   const dim3 grid((wide + kPart - 1) / kPart, p.N * p.Hkv);
@@ -576,23 +586,24 @@ static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
   return check_launch("key_mass");
 }
 
-template <int WP, bool PAGE>
+// Few rows: one row tile in each of four timestep groups at most (a decode step's).  The
+// kernels for many rows would take 143 us where these take 37 (64 sequences of 4,096..16,384
+// tokens, 14 query and 2 kv heads of 64 channels, 4 timesteps).
+template <int WP>
 static int launch(const Params &p, hipStream_t s) {
   // (without accumulation entries behind the table become 0)
   const int64_t tokens = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
   const int64_t wide = p.accumulate && tokens < p.cap ? tokens : p.cap;
-  if (p.rtiles == 1 && p.tgroups <= 2) return launch_few<WP, 2, PAGE>(p, wide, s);
-  if (p.rtiles == 1 && p.tgroups <= 4) return launch_few<WP, 4, PAGE>(p, wide, s);
+  if (p.rtiles == 1 && p.tgroups <= 4) {
+    const bool page = p.bs_log2 >= 4;
+    if (p.tgroups <= 2) return page ? launch_few<WP, 2, true>(p, wide, s) : launch_few<WP, 2, false>(p, wide, s);
+    return page ? launch_few<WP, 4, true>(p, wide, s) : launch_few<WP, 4, false>(p, wide, s);
+  }
   const int chunks = (p.rtiles + kRows - 1) / kRows;
   if (p.parts > 0 && p.rows > 0)
-    den_rows_kernel<WP, PAGE><<<dim3(p.parts * p.tgroups * chunks, p.N * p.Hkv), kDenWaves * 64, 0, s>>>(p);
-  mass_rows_kernel<WP, PAGE><<<dim3((wide + kMassKeys - 1) / kMassKeys, p.N * p.Hkv), kMassKeys * kShare, 0, s>>>(p);
+    den_rows_kernel<WP><<<dim3(p.parts * p.tgroups * chunks, p.N * p.Hkv), kDenWaves * 64, 0, s>>>(p);
+  mass_rows_kernel<WP><<<dim3((wide + kMassKeys - 1) / kMassKeys, p.N * p.Hkv), kMassKeys * kShare, 0, s>>>(p);
   return check_launch("key_mass");
-}
-
-template <int WP>
-static int launch_pages(const Params &p, hipStream_t s) {
-  return p.bs_log2 >= 4 ? launch<WP, true>(p, s) : launch<WP, false>(p, s);
 }
 
 }  // namespace mass
@@ -661,8 +672,8 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   mass::build_weights(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (plan.wp) {
-    case 1: return mass::launch_pages<1>(p, s);
-    case 2: return mass::launch_pages<2>(p, s);
-    default: return mass::launch_pages<4>(p, s);
+    case 1: return mass::launch<1>(p, s);
+    case 2: return mass::launch<2>(p, s);
+    default: return mass::launch<4>(p, s);
   }
 }
