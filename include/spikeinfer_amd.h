@@ -691,7 +691,8 @@ int spk_accept_tree(const int64_t *tokens, const int32_t *parents, const int64_t
  *                   weight of position j
  * for j < seq_lens[n], 0 behind (j < cap); with `accumulate` the sums are added and
  * the rest is left as it was.  Keys as spk_tree_attn reads them.  The sums' order
- * depends on the sequence alone.  mass float at mass_strides {sequence, kv head}.
+ * depends on the sequence alone.  mass float at mass_strides {sequence, kv head}, cap
+ * at most 2^29.
  */
 size_t spk_key_mass_workspace_bytes(int T, int N, int Hq, int Hkv, int head_dim, int max_rows,
                                     int block_size, int max_blocks);

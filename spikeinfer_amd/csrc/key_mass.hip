@@ -644,7 +644,10 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
     return fail(SPK_EINVAL, "key_mass: rows of mass lie on one another");
   const mass::Plan plan = mass::plan(T, N, Hq, Hkv, head_dim, max_rows, block_size, max_blocks);
   if (static_cast<int64_t>(max_rows) * (Hq / Hkv) > (1 << 24) ||
-      static_cast<int64_t>(plan.rtiles) * plan.tgroups * plan.parts > (1 << 30) || cap > (1 << 30))
+      static_cast<int64_t>(plan.rtiles) * plan.tgroups * plan.parts > (1 << 30) ||
+      // (a launch has fewer than 2^32 threads along its first axis)
+      static_cast<int64_t>((plan.rtiles + mass::kRows - 1) / mass::kRows) * plan.tgroups * plan.parts > (1 << 22) ||
+      cap > (1 << 29))
     return fail(SPK_EUNSUPPORTED, "key_mass: %d rows of %d heads over %d x %d tokens", max_rows, Hq / Hkv, max_blocks,
                 block_size);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))

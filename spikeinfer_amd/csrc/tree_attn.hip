@@ -665,7 +665,8 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return fail(SPK_EINVAL, "tree_attn: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);
   const int64_t units = static_cast<int64_t>(T) * Hkv;
-  if (units * plan.rtiles * plan.parts > (1 << 26) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
+  // (a launch has fewer than 2^32 threads along its first axis)
+  if (units * plan.rtiles * plan.parts > (1 << 22) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
     return fail(SPK_EUNSUPPORTED, "tree_attn: T=%d Hq=%d Hkv=%d with %d nodes", T, Hq, Hkv, max_nodes);
   tree::Params p{};
   p.q = reinterpret_cast<const uint32_t *>(q);

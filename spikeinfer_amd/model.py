@@ -250,6 +250,11 @@ class SpikingDecoder:
         draft = meta.draft
         if draft is not None and (n_dec or meta.num_prefills):
             raise ValueError("a step of drafted trees has no decode tokens and no prefill chunks")
+        for name, per_layer in (("key_mass", meta.key_mass), ("draft.words", draft and draft.words)):
+            if per_layer and len(per_layer) != len(self.layers):
+                raise ValueError(f"{name} has {len(per_layer)} layers, the model {len(self.layers)}")
+        if draft is not None and meta.key_mass is not None:
+            raise ValueError("key_mass takes the weights of decode tokens, a step of drafted trees has none")
         bufs = bufs or {}
         positions = positions.to(torch.int64).contiguous()
         h, x = embed_rmsnorm(input_ids, self.embed, self.layers[0].input_norm, c.rms_norm_eps, T)

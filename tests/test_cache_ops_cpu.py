@@ -184,3 +184,17 @@ def test_metadata_moved_to_a_device_keeps_what_the_step_writes():
                 replace(meta, draft=None, key_mass=[torch.zeros(1, 1, 8)], _copies={})):
         with pytest.raises(ValueError, match="must be on meta"):
             bad.on("meta")
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    lib = _lib.load()
+    assert _tree(lib, T=1 << 12, hq=1 << 12, hkv=1 << 12, max_nodes=1024, mask_words=16) == _lib.SPK_EUNSUPPORTED
+    assert _tree(lib, T=1 << 10, hq=1 << 10, hkv=1 << 10, mb=1 << 20, ws=P, wsb=1 << 60) == _lib.SPK_EUNSUPPORTED
+    s, m = _i64(1, 1, 1), _i64(1, 1)
+
+    def mass(most=1, mb=8, cap=100, T=4):
+        return lib.spk_key_mass(P, s, P, s, 100, P, 8, 1, P, P, P, m, cap, 0, 2, 2, most, T, 14, 2, 64, 16, mb, 0.125, P,
+                                1 << 60, None)
+
+    assert mass(cap=(1 << 29) + 1) == mass(most=1 << 20, mb=1 << 17) == mass(T=1 << 20, mb=1 << 10) == \
+        _lib.SPK_EUNSUPPORTED

@@ -4,6 +4,7 @@ with accumulated weights and evictions between the steps."""
 from __future__ import annotations
 
 import math
+from dataclasses import replace
 
 import pytest
 import torch
@@ -252,3 +253,18 @@ def test_a_step_of_trees_takes_no_other_tokens(gpu):
     meta = AttentionMetadata(slot_mapping=torch.full((1,), -1, device=gpu), block_size=BS, num_decode_tokens=1, draft=trees)
     with pytest.raises(ValueError, match="drafted trees"):
         model.forward_paged(z[:1].long(), z[:1].long(), cache.layers, meta)
+
+
+def test_metadata_of_another_model_is_refused(gpu):
+    model = _model(gpu, 2)
+    cache = PagedSpikeCache(2, 4, 2, 64, 3, BS, device=gpu)
+    z = torch.zeros(2, dtype=torch.int32, device=gpu)
+    word = torch.zeros((4, 1, 2, 2), dtype=torch.int32, device=gpu)
+    trees = DraftTrees(z, torch.zeros((1, 1), dtype=torch.int64, device=gpu), 1, z[:1], z[:1].view(1, 1),
+                       words=[(word, word.clone())])
+    slots, mass = torch.full((1,), -1, device=gpu), torch.zeros((1, 2, BS), device=gpu)
+    for meta, match in ((AttentionMetadata(slots, BS, draft=trees), "draft.words has 1 layers"),
+                        (AttentionMetadata(slots, BS, draft=replace(trees, words=None), key_mass=[mass] * 2), "decode tokens"),
+                        (AttentionMetadata(slots, BS, 1, z[:1].view(1, 1), z[:1], key_mass=[mass]), "key_mass has 1 layers")):
+        with pytest.raises(ValueError, match=match):
+            model.forward_paged(z[:1].long(), z[:1].long(), cache.layers, meta)
