@@ -17,8 +17,8 @@
 //     as the product's rows: a lane adds its own row's weights), another adds the parts' sums
 //     in their order, then the weights over them (keys as its columns: a lane adds its own
 //     key's); with one part a single launch does both.
-//   Many rows: den_rows_kernel goes through kPart keys with kRows row tiles in registers;
-//     mass_rows_kernel has 128 keys, in registers, and its waves share the row tiles.
+//   Many rows: den_rows_kernel has kPart keys in its waves' registers and goes through kRows row
+//     tiles; mass_rows_kernel has 128 keys, and its waves share the row tiles.
 // The order of all sums is the sequence's own, whatever the batch.
 //
 // Bound by instruction issue and latency, with few rows near the bytes': 4 timesteps, 14 query
@@ -26,7 +26,7 @@
 // 17 + 22 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
 // where a vector unit is busy for about half the time: a product has 24 vector instructions
 // beside it, four look-ups and their sums and the key's five.  Windows of up to 32 rows of 8
-// sequences of 2,000..8,000 tokens take 21 + 21 us.
+// sequences of 2,000..8,000 tokens take 17 + 20 us.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -40,7 +40,7 @@ constexpr int kStep = 64;      // keys a wave takes at once: four products' colu
 constexpr int kPart = 1024;    // keys of a partial sum
 constexpr int kWaves = 4;      // few rows: waves, each with kSteps steps
 constexpr int kSteps = kPart / (kWaves * kStep);
-constexpr int kRows = 8;       // many rows: row tiles in registers
+constexpr int kRows = 4;       // many rows: row tiles of a workgroup
 constexpr int kDenWaves = 8;   // (twice kWaves: two steps a wave)
 constexpr int kDenSteps = kPart / (kDenWaves * kStep);
 constexpr int kShare = 4;      // waves that share the row tiles of their keys
@@ -376,7 +376,10 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
   }
 }
 
-// Many rows: denominators of kRows row tiles of a timestep group over kPart keys.
+// Many rows: denominators of kRows row tiles of a timestep group over kPart keys.  A wave keeps
+// its keys and goes through the row tiles in a loop.  With four of them both kernels take 34 us
+// for windows of up to 32 rows of 8 sequences of 2,000..8,000 tokens (two 39, eight 36, eight in
+// registers and the keys in the loop 37).
 template <int WP>
 __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
   struct Smem {
@@ -396,51 +399,48 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
   const Keys<WP, false> keys(p, s, n, kvh, lane);
   const int j1 = part * kPart + wave * kStep, tiles = min(kRows, s.rtiles - rt0);
-  uint32_t x[kDenSteps][4];
-  bool ok[kDenSteps][4];
-  const uint32_t *at = keys.words(tg, lane);
+  v8i k[kDenSteps][4];
+  uint32_t qw = query_word<WP>(p, s, kvh, tg, rt0, lane);
+  {
+    uint32_t x[kDenSteps][4];
+    bool ok[kDenSteps][4];
+    const uint32_t *at = keys.words(tg, lane);
 #pragma unroll
-  for (int st = 0; st < kDenSteps; ++st) {
-    const typename Keys<WP, false>::Places to = keys.places(j1 + st * kDenWaves * kStep);
+    for (int st = 0; st < kDenSteps; ++st) {
+      const typename Keys<WP, false>::Places to = keys.places(j1 + st * kDenWaves * kStep);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      ok[st][u] = to.ok[u];
-      x[st][u] = at[to.at[u]];
+      for (int u = 0; u < 4; ++u) {
+        ok[st][u] = to.ok[u];
+        x[st][u] = at[to.at[u]];
+      }
     }
-  }
-  v8i q[kRows];
-  float l[kRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    q[i] = query_bits(query_word<WP>(p, s, kvh, tg, rt0 + i, lane));  // (rows behind the sequence's: 0)
-    l[i] = 0.f;
+    for (int st = 0; st < kDenSteps; ++st)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) k[st][u] = key_bits(ok[st][u] ? x[st][u] : 0u);
   }
   __syncthreads();
   const int open = s.len - s.m;
+#pragma unroll 1
+  for (int i = 0; i < tiles; ++i) {
+    const v8i q = query_bits(qw);
+    qw = query_word<WP>(p, s, kvh, tg, rt0 + min(i + 1, tiles - 1), lane);  // the next tile's
+    float l = 0.f;
 #pragma unroll
-  for (int st = 0; st < kDenSteps; ++st) {
-    const int j0 = j1 + st * kDenWaves * kStep;
-    v8i k[4];
+    for (int st = 0; st < kDenSteps; ++st) {
+      const int j0 = j1 + st * kDenWaves * kStep;
+      if (j0 + kStep - 1 <= open) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) k[u] = key_bits(ok[st][u] ? x[st][u] : 0u);
-    auto add = [&](auto mask) {
+        for (int u = 0; u < 4; ++u) l += row_weights<false>(tab0, q, k[st][u], j0 + 16 * u, lane, 0);
+      } else if (j0 < s.len) {
+        const int lim = open + tile_row<WP>(p, rt0 + i, lane & 15);
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        if (i >= tiles) break;
-        const int lim = decltype(mask)::value ? open + tile_row<WP>(p, rt0 + i, lane & 15) : 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          l[i] += row_weights<decltype(mask)::value>(tab0, q[i], k[u], j0 + 16 * u, lane, lim);
+        for (int u = 0; u < 4; ++u) l += row_weights<true>(tab0, q, k[st][u], j0 + 16 * u, lane, lim);
       }
-    };
-    if (j0 + kStep - 1 <= open) add(std::false_type{});
-    else if (j0 < s.len) add(std::true_type{});
-  }
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    l[i] += __shfl_xor(l[i], 16);
-    l[i] += __shfl_xor(l[i], 32);
-    if (lane < 16) sm.sum[wave][i][lane] = l[i];
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < 16) sm.sum[wave][i][lane] = l;
   }
   __syncthreads();
   if (tid < tiles * 16) {
