@@ -26,7 +26,7 @@
 // 17 + 22 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
 // where a vector unit is busy for about half the time: a product has 24 vector instructions
 // beside it, four look-ups and their sums and the key's five.  Windows of up to 32 rows of 8
-// sequences of 2,000..8,000 tokens take 17 + 20 us.
+// sequences of 2,000..8,000 tokens take 18 + 21 us.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
