@@ -38,11 +38,9 @@ using namespace tiles;
 
 constexpr int kStep = 64;      // keys a wave takes at once: four products' columns
 constexpr int kPart = 1024;    // keys of a partial sum
-constexpr int kWaves = 4;      // few rows: waves, each with kSteps steps
+constexpr int kWaves = 8;      // waves that share kPart keys, each with kSteps steps
 constexpr int kSteps = kPart / (kWaves * kStep);
 constexpr int kRows = 4;       // many rows: row tiles of a workgroup
-constexpr int kDenWaves = 8;   // (twice kWaves: two steps a wave)
-constexpr int kDenSteps = kPart / (kDenWaves * kStep);
 constexpr int kShare = 4;      // waves that share the row tiles of their keys
 constexpr int kMassKeys = 128;
 constexpr int kChunk = 64;     // row tiles whose denominators are in LDS
@@ -237,7 +235,7 @@ template <int WP, int RT, bool PAGE, Pass PASS>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void few_rows_kernel(Params p) {
   struct Smem {
     float tab[kTab + 3];  // first: a score's accumulator is its entry's LDS address
-    float sum[kDenWaves][RT][16];
+    float sum[kWaves][RT][16];
     float inv[RT][16];
   };
   __shared__ Smem sm;
@@ -298,10 +296,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
   __syncthreads();
 
   if constexpr (PASS != kMass) {
-    // (two steps a sum, as den_rows_kernel's waves have them)
-    float l[2][RT];
+    float l[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) l[0][i] = l[1][i] = 0.f;
+    for (int i = 0; i < RT; ++i) l[i] = 0.f;
     const int lim = open + tile_row<WP>(p, 0, lane & 15);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
@@ -312,8 +309,8 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
           if (i >= p.tgroups) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            l[st & 1][i] += row_weights<decltype(mask)::value>(tab0, q[i], key_bits(ok[st][u] ? x[st][i][u] : 0u),
-                                                               j0 + 16 * u, lane, lim);
+            l[i] += row_weights<decltype(mask)::value>(tab0, q[i], key_bits(ok[st][u] ? x[st][i][u] : 0u), j0 + 16 * u,
+                                                       lane, lim);
         }
       };
       if (j0 + kStep - 1 <= open) add(std::false_type{});
@@ -321,20 +318,16 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = l[h][i];
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        if (lane < 16) sm.sum[h * kWaves + wave][i][lane] = x;
-      }
+      l[i] += __shfl_xor(l[i], 16);
+      l[i] += __shfl_xor(l[i], 32);
+      if (lane < 16) sm.sum[wave][i][lane] = l[i];
     }
     __syncthreads();
     if (tid < p.tgroups * 16) {
       const int i = tid / 16, y = tid % 16;
       float d = 0.f;
 #pragma unroll
-      for (int w = 0; w < kDenWaves; ++w) d += sm.sum[w][i][y];
+      for (int w = 0; w < kWaves; ++w) d += sm.sum[w][i][y];
       if constexpr (PASS == kDen) den[tid] = d;
       else sm.inv[i][y] = d > 0.f && has_row<WP>(p, s, i, 0, y) ? 1.f / d : 0.f;
     }
@@ -381,10 +374,10 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
 // for windows of up to 32 rows of 8 sequences of 2,000..8,000 tokens (two 39, eight 36, eight in
 // registers and the keys in the loop 37).
 template <int WP>
-__global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
   struct Smem {
     float tab[kTab + 3];
-    float sum[kDenWaves][kRows][16];
+    float sum[kWaves][kRows][16];
   };
   __shared__ Smem sm;
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
@@ -399,15 +392,15 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
   const Keys<WP, false> keys(p, s, n, kvh, lane);
   const int j1 = part * kPart + wave * kStep, tiles = min(kRows, s.rtiles - rt0);
-  v8i k[kDenSteps][4];
+  v8i k[kSteps][4];
   uint32_t qw = query_word<WP>(p, s, kvh, tg, rt0, lane);
   {
-    uint32_t x[kDenSteps][4];
-    bool ok[kDenSteps][4];
+    uint32_t x[kSteps][4];
+    bool ok[kSteps][4];
     const uint32_t *at = keys.words(tg, lane);
 #pragma unroll
-    for (int st = 0; st < kDenSteps; ++st) {
-      const typename Keys<WP, false>::Places to = keys.places(j1 + st * kDenWaves * kStep);
+    for (int st = 0; st < kSteps; ++st) {
+      const typename Keys<WP, false>::Places to = keys.places(j1 + st * kWaves * kStep);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         ok[st][u] = to.ok[u];
@@ -415,7 +408,7 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
       }
     }
 #pragma unroll
-    for (int st = 0; st < kDenSteps; ++st)
+    for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int u = 0; u < 4; ++u) k[st][u] = key_bits(ok[st][u] ? x[st][u] : 0u);
   }
@@ -427,8 +420,8 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
     qw = query_word<WP>(p, s, kvh, tg, rt0 + min(i + 1, tiles - 1), lane);  // the next tile's
     float l = 0.f;
 #pragma unroll
-    for (int st = 0; st < kDenSteps; ++st) {
-      const int j0 = j1 + st * kDenWaves * kStep;
+    for (int st = 0; st < kSteps; ++st) {
+      const int j0 = j1 + st * kWaves * kStep;
       if (j0 + kStep - 1 <= open) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) l += row_weights<false>(tab0, q, k[st][u], j0 + 16 * u, lane, 0);
@@ -446,7 +439,7 @@ __global__ __launch_bounds__(kDenWaves * 64) __attribute__((amdgpu_waves_per_eu(
   if (tid < tiles * 16) {
     float d = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDenWaves; ++w) d += sm.sum[w][tid / 16][tid % 16];
+    for (int w = 0; w < kWaves; ++w) d += sm.sum[w][tid / 16][tid % 16];
     p.den[(((static_cast<int64_t>(blockIdx.y) * p.parts + part) * p.tgroups + tg) * p.rtiles + rt0) * 16 + tid] = d;
   }
 }
@@ -573,7 +566,8 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_s
   return r;
 }
 
-// With one part a launch does both passes: 8.6 us where two take 12.6 (a sequence of 700 tokens).
+// With one part a launch does both passes: 8.6 us where two took 12.6 (a sequence of 700 tokens,
+// four waves a workgroup; 7.1 with eight).
 template <int WP, int RT, bool PAGE>
 static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
   const dim3 grid((wide + kPart - 1) / kPart, p.N * p.Hkv);
@@ -601,7 +595,7 @@ static int launch(const Params &p, hipStream_t s) {
   }
   const int chunks = (p.rtiles + kRows - 1) / kRows;
   if (p.parts > 0 && p.rows > 0)
-    den_rows_kernel<WP><<<dim3(p.parts * p.tgroups * chunks, p.N * p.Hkv), kDenWaves * 64, 0, s>>>(p);
+    den_rows_kernel<WP><<<dim3(p.parts * p.tgroups * chunks, p.N * p.Hkv), kWaves * 64, 0, s>>>(p);
   mass_rows_kernel<WP><<<dim3((wide + kMassKeys - 1) / kMassKeys, p.N * p.Hkv), kMassKeys * kShare, 0, s>>>(p);
   return check_launch("key_mass");
 }
