@@ -23,7 +23,7 @@
 //
 // Bound by instruction issue and latency, with few rows near the bytes': 4 timesteps, 14 query
 // and 2 kv heads of 64 channels, one row of each of 64 sequences of 4,096..16,384 tokens takes
-// 17 + 22 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
+// 18 + 21 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
 // where a vector unit is busy for about half the time: a product has 24 vector instructions
 // beside it, four look-ups and their sums and the key's five.  Windows of up to 32 rows of 8
 // sequences of 2,000..8,000 tokens take 18 + 21 us.
@@ -38,7 +38,9 @@ using namespace tiles;
 
 constexpr int kStep = 64;      // keys a wave takes at once: four products' columns
 constexpr int kPart = 1024;    // keys of a partial sum
-constexpr int kWaves = 8;      // waves that share kPart keys, each with kSteps steps
+// Waves that share kPart keys, each with kSteps steps.  Of 4, 8 and 16: 8.6, 7.1 and 6.6 us for a
+// row of 700 tokens, 37, 37 and 51 for one of each of 64 sequences of 4,096..16,384.
+constexpr int kWaves = 8;
 constexpr int kSteps = kPart / (kWaves * kStep);
 constexpr int kRows = 4;       // many rows: row tiles of a workgroup
 constexpr int kShare = 4;      // waves that share the row tiles of their keys
