@@ -10,13 +10,11 @@
 //     own, so that a row's mask word is the tile's.
 //   * Scores as there: one fp4 product per 64 channels leaves the score's table offset in
 //     the accumulator's bits, and the weight is a look-up.
-//   * Values: f16 products over two keys a register.  A v bit becomes an operand by one `and`,
-//     as one of f16's exponent bits, and tables of weights hold what makes the products equal
-//     again.  bf16 outputs take the weights' 11-bit high halves alone (each off by at most
-//     2^-11, and the denominator sums the same halves, where the output's own rounding is
-//     2^-8), from four tables for 2^-14, 2^-13, 2^-11 and 2^-7 by the key's number % 4.  fp32
-//     and fp16 outputs take both halves, in two products, from two tables for 2^-14 and 2^-13:
-//     the smallest weight, 2^15 / e^12, keeps 2^-21 of itself, larger ones up to 2^-23.
+//   * Values: f16 products over two keys a register, one for the weights' high halves and one
+//     for their low ones, whatever the output's type: the smallest weight, 2^15 / e^12, keeps
+//     2^-21 of itself, larger ones up to 2^-23.  A v bit becomes an operand by one `and`, as
+//     one of f16's exponent bits, 2^-14 or 2^-13 by the key's number % 2, and two tables of
+//     weights hold what makes the products equal again.
 //   * Eight waves a workgroup (four with more than 64 channels) share the key tiles' operands
 //     through LDS: each prepares one of a step's tiles, two buffers of them so that one barrier
 //     a step does.  Of a sequence of more than 128 rows a workgroup takes 256, a wave a row
@@ -28,11 +26,12 @@
 //     the batch around it.
 //
 // Bound by issue: a tile of 32 rows and 32 keys is 9 matrix instructions with about 90 vector
-// ones (fp32 and fp16 outputs; bf16: 5 with 68), which hide behind one another only in part.
+// ones, which hide behind one another only in part.
 // With 14 query and 2 kv heads of 64 channels and 4 timesteps, 32 nodes on each of 16
 // contexts of 4,096..16,384 tokens, fp32, take 122 us: 617 TFLOP/s of 4 * T * Hq * nodes * keys *
 // D operations, those on values done twice.  61 nodes on 30,011 tokens, bf16,
-// take 33 us: 800 TFLOP/s, in 240 workgroups of 64 tiles, one a CU.
+// take 43 us: 609 TFLOP/s, in 240 workgroups of 64 tiles, one a CU.  (The weights' high halves
+// alone would take 33, and change bf16 outputs: up to 2^-10 of them where 2^-8 is half a step.)
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -113,25 +112,14 @@ __device__ __forceinline__ int node_of(const Params &p, int r) {
   return p.nrep == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.rep_mul));
 }
 
-// Weight tables in LDS at offset 0.  bf16 outputs: four of the weights' high halves as fp32,
-// whose entries take 2^0, 2^-1, 2^-3 and 2^-7 of the first's (all of them f16 numbers).  Else
-// two of (hi, lo) pairs, 2^0 and 2^-1.
-template <bool F32> constexpr int kTables = F32 ? 2 : 4;
-template <bool F32>
-__device__ __forceinline__ void fill_tables(const Params &p, float *tab, int tid) {
+// Two tables of (hi, lo) pairs in LDS at offset 0: the weights, and half of them.
+constexpr int kTables = 2;
+__device__ __forceinline__ void fill_tables(const Params &p, uint32_t *tab, int tid) {
   if (tid > p.D) return;
   const uint32_t w = p.tab[tid];
-  const float hi = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w)));
-  if constexpr (F32) {
-    const v2h half = __builtin_bit_cast(v2h, w) * v2h{static_cast<_Float16>(0.5f), static_cast<_Float16>(0.5f)};
-    tab[tid] = __uint_as_float(w);
-    tab[kTabStride + tid] = __builtin_bit_cast(float, half);
-  } else {
-    tab[tid] = hi;
-    tab[kTabStride + tid] = hi * 0.5f;
-    tab[2 * kTabStride + tid] = hi * 0.125f;
-    tab[3 * kTabStride + tid] = hi * 0.0078125f;
-  }
+  const v2h half = __builtin_bit_cast(v2h, w) * v2h{static_cast<_Float16>(0.5f), static_cast<_Float16>(0.5f)};
+  tab[tid] = w;
+  tab[kTabStride + tid] = __builtin_bit_cast(uint32_t, half);
 }
 
 // Query words of row `r` (score operands of its tile).
@@ -225,28 +213,18 @@ __device__ __forceinline__ uint32_t seen(const Seq &s, int kt, const uint32_t *w
   return see >> (4 * half);
 }
 
-// A lane's v bits of a channel tile where `expand` masks them: [operand][key % 4 / kEach] with
-// kEach keys' bits from bit 10 on.
-template <bool F32> struct Bits {
-  static constexpr int kEach = F32 ? 2 : 4;
-  typedef uint32_t type __attribute__((ext_vector_type(8 / kEach)));
-};
-template <bool F32>
-__device__ __forceinline__ typename Bits<F32>::type place_bits(uint32_t vt) {
-  if constexpr (F32) return typename Bits<F32>::type{vt << 10, vt << 8, vt << 2, vt};
-  else return typename Bits<F32>::type{vt << 10, vt << 2};
-}
+// A lane's v bits of a channel tile where `expand` masks them: a word for each operand and key
+// number % 4 / 2, whose two keys' bits start at bit 10.
+__device__ __forceinline__ v4u place_bits(uint32_t vt) { return v4u{vt << 10, vt << 8, vt << 2, vt}; }
 
 // Products' value operands of a channel tile: register i of operand g pairs the lane's keys
 // 4g + i and 4g + i + 8, sixteen bits apart.
-template <bool F32>
-__device__ __forceinline__ void expand(typename Bits<F32>::type vt, v8h (&vop)[2]) {
-  constexpr int kEach = Bits<F32>::kEach, kWords = 4 / kEach;
+__device__ __forceinline__ void expand(v4u vt, v8h (&vop)[2]) {
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     v4u x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = vt[g * kWords + i / kEach] & (0x04000400u << i % kEach);
+    for (int i = 0; i < 4; ++i) x[i] = vt[g * 2 + i / 2] & (0x04000400u << i % 2);
     vop[g] = __builtin_bit_cast(v8h, x);
   }
 }
@@ -261,11 +239,10 @@ __device__ __forceinline__ v16f scores(const v8i (&kop)[NK], const v8i (&qop)[NK
 }
 
 // A tile's weights: the lane's sixteen table entries.
-template <bool F32>
 __device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&w)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const uint32_t at = tab0 + 4 * kTabStride * (e & (kTables<F32> - 1)) + __float_as_uint(a[e]);
+    const uint32_t at = tab0 + 4 * kTabStride * (e & (kTables - 1)) + __float_as_uint(a[e]);
     w[e] = *reinterpret_cast<const SPK_LDS uint32_t *>(static_cast<uintptr_t>(at));
   }
 }
@@ -276,10 +253,9 @@ __device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&
 // the high ones are added in fp32.  The low ones, below 2^-11 of theirs, are first added in
 // f16, four to a sum in two steps: off by at most 2 * 2^-11 of themselves, 2^-21 of the
 // weights at the very worst and 2^-23 in the mean, their own resolution.
-template <int NC, bool F32, bool MASKED>
+template <int NC, bool MASKED>
 __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, const v8h (&vop)[NC][2],
                                          v16f (&acc)[NC], float (&l)[4]) {
-  constexpr int kParts = F32 ? 2 : 1;
   float one = 1.f;
   asm("" : "+v"(one));  // (kept a register: fma_mix then takes the halves as they are)
   auto keep = [&](int e) {  // the e-th of the lane's sixteen
@@ -290,53 +266,42 @@ __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, 
   v2h low[2][2];  // by table
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    v4u y[kParts];  // the weights' halves, two keys a register
+    v4u y[2];  // the weights' halves, two keys a register
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w0 = keep(4 * g + i), w1 = keep(4 * g + i + 8);
-      if constexpr (F32) {
-        const uint32_t both = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-        y[0][i] = both;
-        y[1][i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
-        const v2h high = __builtin_bit_cast(v2h, both);  // (of a scalar: an element would give the first)
-        l[i] = __builtin_fmaf(static_cast<float>(high[0]), one, l[i]);
-        l[i] = __builtin_fmaf(static_cast<float>(high[1]), one, l[i]);
-      } else {
-        l[i] += __uint_as_float(w0) + __uint_as_float(w1);
-        y[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w0), __uint_as_float(w1)));
-      }
+      const uint32_t both = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+      y[0][i] = both;
+      y[1][i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+      const v2h high = __builtin_bit_cast(v2h, both);  // (of a scalar: an element would give the first)
+      l[i] = __builtin_fmaf(static_cast<float>(high[0]), one, l[i]);
+      l[i] = __builtin_fmaf(static_cast<float>(high[1]), one, l[i]);
     }
-    if constexpr (F32) {
-      auto half2 = [&](int i) { return __builtin_bit_cast(v2h, static_cast<uint32_t>(y[1][i])); };
-      low[0][g] = half2(0) + half2(2);
-      low[1][g] = half2(1) + half2(3);
-    }
+    auto half2 = [&](int i) { return __builtin_bit_cast(v2h, static_cast<uint32_t>(y[1][i])); };
+    low[0][g] = half2(0) + half2(2);
+    low[1][g] = half2(1) + half2(3);
 #pragma unroll
-    for (int q = 0; q < kParts; ++q)
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, y[q]), acc[c], 0, 0, 0);
   }
-  if constexpr (F32) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const v2h sum = low[i][0] + low[i][1];
-      l[i] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[i]);
-      l[i] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[i]);
-    }
+  for (int i = 0; i < 2; ++i) {
+    const v2h sum = low[i][0] + low[i][1];
+    l[i] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[i]);
+    l[i] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[i]);
   }
 }
 
 // A lane's denominator, of its own keys, in the numerators' units.
-template <bool F32>
 __device__ __forceinline__ float lane_sum(const float (&l)[4]) {
-  if constexpr (F32) return ((l[0] + 2.f * l[1]) + (l[2] + 2.f * l[3])) * 0x1p-14f;
-  else return ((l[0] + 2.f * l[1]) + (8.f * l[2] + 128.f * l[3])) * 0x1p-14f;
+  return ((l[0] + 2.f * l[1]) + (l[2] + 2.f * l[3])) * 0x1p-14f;
 }
 
 // Rows of a tile from their sums: kVals of the lane's values of channel tile c (four
 // channels 8 * (g0 + k) + 4 * half .. for each k), divided by the row's denominator.
-template <bool F32, int kVals>
+template <int kVals>
 __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, int kvh, int r, int c, int g0, int half,
                                           const float (&val)[kVals], float den) {
   const float inv = den > 0.f ? 1.f / den : 0.f;  // (a row that sees nothing: zeros)
@@ -350,7 +315,7 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = val[4 * k + e] * inv;
       if (ch >= p.D) continue;
-      if (F32 && p.out_dtype == SPK_F32) {
+      if (p.out_dtype == SPK_F32) {
         *reinterpret_cast<v4f *>(static_cast<float *>(p.out) + row + ch) = v4f{o[0], o[1], o[2], o[3]};
         continue;
       }
@@ -358,7 +323,7 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         uint16_t x0, x1;
-        if constexpr (!F32) {
+        if (p.out_dtype == SPK_BF16) {
           x0 = f32_to_bf16_bits(o[2 * e]);
           x1 = f32_to_bf16_bits(o[2 * e + 1]);
         } else {
@@ -373,7 +338,7 @@ __device__ __forceinline__ void store_row(const Params &p, const Seq &s, int t, 
 #pragma unroll
     for (int j = 0; j < kVals; ++j) {
       const int ch = 32 * c + 8 * (g0 + (j >> 2)) + 4 * half + (j & 3);
-      if (ch < p.D) store_f32_as(p.out, row + ch, F32 ? p.out_dtype : SPK_BF16, val[j] * inv);
+      if (ch < p.D) store_f32_as(p.out, row + ch, p.out_dtype, val[j] * inv);
     }
   }
 }
@@ -385,7 +350,7 @@ __device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int 
 }
 
 // KW waves a row tile; NC = channel tiles of 32.
-template <int KW, int NC, bool F32, typename Smem>
+template <int KW, int NC, typename Smem>
 __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, int n, int unit, int group, int part,
                                        int wave) {
   constexpr int NK = (NC + 1) / 2;   // 64-channel score steps
@@ -408,7 +373,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
     phys = keys.block_of(first + kStep + wave);
   };
   request(t0);
-  fill_tables<F32>(p, sm.tab[0], tid);
+  fill_tables(p, sm.tab[0], tid);
   v8i qop[NK];
   load_query<NK>(p, s, t, kvh, min(r, rows - 1), half, qop);
   const uint32_t *mrow = p.masks + (s.first + node_of(p, min(r, rows - 1))) * p.mask_words;
@@ -426,7 +391,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       sm.k[buf][wave][k][lane] = v4u{static_cast<uint32_t>(kop[k][0]), static_cast<uint32_t>(kop[k][1]),
                                      static_cast<uint32_t>(kop[k][2]), static_cast<uint32_t>(kop[k][3])};
 #pragma unroll
-    for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = place_bits<F32>(vt[c]);
+    for (int c = 0; c < NC; ++c) sm.v[buf][wave][c][lane] = place_bits(vt[c]);
   };
   prepare(0);
   request(t0 + kStep);
@@ -445,11 +410,11 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
         kop[k] = v8i{static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3])};
       }
       uint32_t w[16];
-      lookup<F32>(tab0, scores<NK>(kop, qop), w);
+      lookup(tab0, scores<NK>(kop, qop), w);
       v8h vop[NC][2];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) expand<F32>(sm.v[buf][u][c][lane], vop[c]);
-      products<NC, F32, decltype(masked)::value>(w, decltype(masked)::value ? seen(s, first + u, mrow, half) : 0u, vop,
+      for (int c = 0; c < NC; ++c) expand(sm.v[buf][u][c][lane], vop[c]);
+      products<NC, decltype(masked)::value>(w, decltype(masked)::value ? seen(s, first + u, mrow, half) : 0u, vop,
                                                  acc, l);
     };
     if (live) {
@@ -473,10 +438,10 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       *reinterpret_cast<v4f *>(to + ((c * 4 + quad) * 64 + lane) * 4) = v4f{val[0], val[1], val[2], val[3]};
       if (c == 0 && quad == 0 && half == 0) to[NC * 1024 + col] = den;
     } else if (r < rows) {
-      store_row<F32, 4>(p, s, t, kvh, r, c, quad, half, val, den);
+      store_row<4>(p, s, t, kvh, r, c, quad, half, val, den);
     }
   };
-  const float mine = lane_sum<F32>(l);
+  const float mine = lane_sum(l);
   if constexpr (KW == 1) {
     const float den = mine + __shfl_xor(mine, 32);
     if (!live) return;
@@ -516,17 +481,17 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
   }
 }
 
-template <int NC, bool F32>
+template <int NC>
 __global__ __launch_bounds__(waves_of(NC) * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void
 tree_attn_kernel(Params p) {
   constexpr int NK = (NC + 1) / 2, kWaves = waves_of(NC), kStep = kWaves;
   struct Smem {
-    float tab[kTables<F32>][kTabStride];  // first: a score's accumulator is its entry's LDS address
+    uint32_t tab[kTables][kTabStride];  // first: a score's accumulator is its entry's LDS address
     float den[kWaves][64];
     union {
       struct {
         v4u k[2][kStep][NK][64];
-        typename Bits<F32>::type v[2][kStep][NC][64];
+        v4u v[2][kStep][NC][64];
       };
       float red[kWaves][16][64];
     };
@@ -540,17 +505,16 @@ tree_attn_kernel(Params p) {
   const int rows = s.nodes * p.nrep;
   if (group * kWaves * 32 >= rows || part >= s.parts) return;
   // (one wave a row tile throughout: 7.1 us where these take 6.2 for 8 nodes on 128 tokens)
-  if (rows > 16 * kWaves) attend<1, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else if (rows > 8 * kWaves) attend<2, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC, F32>(p, s, sm, n, unit, group, part, wave);
-  else attend<kWaves, NC, F32>(p, s, sm, n, unit, group, part, wave);
+  if (rows > 16 * kWaves) attend<1, NC>(p, s, sm, n, unit, group, part, wave);
+  else if (rows > 8 * kWaves) attend<2, NC>(p, s, sm, n, unit, group, part, wave);
+  else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC>(p, s, sm, n, unit, group, part, wave);
+  else attend<kWaves, NC>(p, s, sm, n, unit, group, part, wave);
 }
 
 // Sums of the parts, in their order.  A wave takes four channels of a lane's sixteen of an
 // output tile, with kAhead parts' sums on their way at once.  Workgroups of a unit are
 // numbered as the attention's are: with 8 units (or a multiple) they run on the XCD whose L2
 // has the sums.
-template <bool F32>
 __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int NC) {
   constexpr int kAhead = 8;
   const int lane = threadIdx.x & 63, quad = threadIdx.x >> 6, half = lane >> 5, col = lane & 31, n = blockIdx.y;
@@ -580,7 +544,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int NC) {
     }
   }
   const float val[4] = {a[0], a[1], a[2], a[3]};
-  if (r < rows) store_row<F32, 4>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, quad, half, val, den);
+  if (r < rows) store_row<4>(p, s, unit / p.Hkv, unit % p.Hkv, r, c, quad, half, val, den);
 }
 
 struct Plan {
@@ -598,23 +562,13 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_
   return r;
 }
 
-template <int NC, bool F32>
+template <int NC>
 static int launch(const Params &p, int N, hipStream_t s) {
-  tree_attn_kernel<NC, F32><<<dim3(p.groups * p.parts * p.units, N), waves_of(NC) * 64, 0, s>>>(p);
+  tree_attn_kernel<NC><<<dim3(p.groups * p.parts * p.units, N), waves_of(NC) * 64, 0, s>>>(p);
   const int rc = check_launch("tree_attn");
   if (rc || p.parts == 1) return rc;
-  tree_join_kernel<F32><<<dim3(p.units * p.rtiles * NC, N), 256, 0, s>>>(p, NC);
+  tree_join_kernel<<<dim3(p.units * p.rtiles * NC, N), 256, 0, s>>>(p, NC);
   return check_launch("tree_attn");
-}
-
-template <bool F32>
-static int launch_type(const Params &p, int N, hipStream_t s) {
-  switch (p.W) {
-    case 1: return launch<1, F32>(p, N, s);
-    case 2: return launch<2, F32>(p, N, s);
-    case 3: return launch<3, F32>(p, N, s);
-    default: return launch<4, F32>(p, N, s);
-  }
 }
 
 }  // namespace tree
@@ -701,5 +655,10 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   p.rtiles = plan.rtiles; p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
   tiles::build_table(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return out_dtype != SPK_BF16 ? tree::launch_type<true>(p, N, s) : tree::launch_type<false>(p, N, s);
+  switch (p.W) {
+    case 1: return tree::launch<1>(p, N, s);
+    case 2: return tree::launch<2>(p, N, s);
+    case 3: return tree::launch<3>(p, N, s);
+    default: return tree::launch<4>(p, N, s);
+  }
 }
