@@ -30,7 +30,7 @@
 // With 14 query and 2 kv heads of 64 channels and 4 timesteps, 32 nodes on each of 16
 // contexts of 4,096..16,384 tokens, fp32, take 122 us: 617 TFLOP/s of 4 * T * Hq * nodes * keys *
 // D operations, those on values done twice.  61 nodes on 30,011 tokens, bf16,
-// take 43 us: 609 TFLOP/s, in 240 workgroups of 64 tiles, one a CU.  (The weights' high halves
+// take 45 us: 580 TFLOP/s, in 240 workgroups of 64 tiles, one a CU.  (The weights' high halves
 // alone would take 33, and change bf16 outputs: up to 2^-10 of them where 2^-8 is half a step.)
 #include <type_traits>
 
@@ -247,15 +247,23 @@ __device__ __forceinline__ void lookup(uint32_t tab0, const v16f &a, uint32_t (&
   }
 }
 
-// Adds a tile's weighted values to acc and its weights to l.  The weights are added one by
-// one: dot products of f16 pairs would be half as many instructions, but they take the matrix
-// cores' time (8 behind each product 78 cycles where 8 additions take 52).  Of a pair's halves
-// the high ones are added in fp32.  The low ones, below 2^-11 of theirs, are first added in
-// f16, four to a sum in two steps: off by at most 2 * 2^-11 of themselves, 2^-21 of the
-// weights at the very worst and 2^-23 in the mean, their own resolution.
+// A lane's denominator: sums of high halves by the key's number % 4 and of low halves by its
+// number % 2.  Low halves among the high ones would be rounded to the large sums (1.6e-6 of the
+// outputs, in the 2-norm, where these lose 4e-7: 2,000 tokens, 140 rows, 128 channels).
+struct Sums {
+  float high[4] = {0.f, 0.f, 0.f, 0.f}, low[2] = {0.f, 0.f};
+  // in the numerators' units
+  __device__ __forceinline__ float total() const {
+    return ((high[0] + 2.f * high[1]) + (high[2] + 2.f * high[3]) + (low[0] + 2.f * low[1])) * 0x1p-14f;
+  }
+};
+
+// Adds a tile's weighted values to acc and its weights to l, one by one in fp32: dot products
+// of f16 pairs would be half as many instructions, but they take the matrix cores' time (8
+// behind each product 78 cycles where 8 additions take 52).
 template <int NC, bool MASKED>
 __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, const v8h (&vop)[NC][2],
-                                         v16f (&acc)[NC], float (&l)[4]) {
+                                         v16f (&acc)[NC], Sums &l) {
   float one = 1.f;
   asm("" : "+v"(one));  // (kept a register: fma_mix then takes the halves as they are)
   auto keep = [&](int e) {  // the e-th of the lane's sixteen
@@ -263,40 +271,28 @@ __device__ __forceinline__ void products(const uint32_t (&x)[16], uint32_t see, 
       return x[e] & static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(see), 8 * (e >> 2) + (e & 3), 1));
     else return x[e];
   };
-  v2h low[2][2];  // by table
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     v4u y[2];  // the weights' halves, two keys a register
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w0 = keep(4 * g + i), w1 = keep(4 * g + i + 8);
-      const uint32_t both = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-      y[0][i] = both;
-      y[1][i] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
-      const v2h high = __builtin_bit_cast(v2h, both);  // (of a scalar: an element would give the first)
-      l[i] = __builtin_fmaf(static_cast<float>(high[0]), one, l[i]);
-      l[i] = __builtin_fmaf(static_cast<float>(high[1]), one, l[i]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t both = __builtin_amdgcn_perm(w1, w0, q ? 0x07060302u : 0x05040100u);
+        y[q][i] = both;
+        const v2h half = __builtin_bit_cast(v2h, both);  // (of a scalar: an element would give the first)
+        float &sum = q ? l.low[i & 1] : l.high[i];
+        sum = __builtin_fmaf(static_cast<float>(half[0]), one, sum);
+        sum = __builtin_fmaf(static_cast<float>(half[1]), one, sum);
+      }
     }
-    auto half2 = [&](int i) { return __builtin_bit_cast(v2h, static_cast<uint32_t>(y[1][i])); };
-    low[0][g] = half2(0) + half2(2);
-    low[1][g] = half2(1) + half2(3);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         acc[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop[c][g], __builtin_bit_cast(v8h, y[q]), acc[c], 0, 0, 0);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const v2h sum = low[i][0] + low[i][1];
-    l[i] = __builtin_fmaf(static_cast<float>(sum[0]), one, l[i]);
-    l[i] = __builtin_fmaf(static_cast<float>(sum[1]), one, l[i]);
-  }
-}
-
-// A lane's denominator, of its own keys, in the numerators' units.
-__device__ __forceinline__ float lane_sum(const float (&l)[4]) {
-  return ((l[0] + 2.f * l[1]) + (l[2] + 2.f * l[3])) * 0x1p-14f;
 }
 
 // Rows of a tile from their sums: kVals of the lane's values of channel tile c (four
@@ -378,7 +374,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
   load_query<NK>(p, s, t, kvh, min(r, rows - 1), half, qop);
   const uint32_t *mrow = p.masks + (s.first + node_of(p, min(r, rows - 1))) * p.mask_words;
   v16f acc[NC];
-  float l[4] = {0.f, 0.f, 0.f, 0.f};
+  Sums l;
 #pragma unroll
   for (int c = 0; c < NC; ++c) acc[c] = v16f{};
 
@@ -441,7 +437,7 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
       store_row<4>(p, s, t, kvh, r, c, quad, half, val, den);
     }
   };
-  const float mine = lane_sum(l);
+  const float mine = l.total();
   if constexpr (KW == 1) {
     const float den = mine + __shfl_xor(mine, 32);
     if (!live) return;
