@@ -24,6 +24,11 @@
 //     tree's tiles belonging to the last: a workgroup each, whose sums a second launch adds in
 //     their order.  So the sums depend on the sequence alone, its length and its rows, not on
 //     the batch around it.
+//   * Sums go to the workspace every kPartTiles tiles, also within a longer part: fp32
+//     accumulators take 256 products at most (and the tree's), whatever the length.  Off from
+//     float64, fp32 outputs: random words 4e-7 in the 2-norm from 2,000 to 1 << 20 tokens; keys of
+//     equal weights with values of ones, the worst found, 2.4e-6 at 1 << 20 and 4e-6 at 1 << 22
+//     (with one accumulator a part up to 5e-5 and 2e-4).
 //
 // Bound by issue: a tile of 32 rows and 32 keys is 9 matrix instructions with about 90 vector
 // ones, which hide behind one another only in part.
@@ -345,21 +350,23 @@ __device__ __forceinline__ float *sums_at(const Params &p, int n, int unit, int 
   return p.ws + (((static_cast<int64_t>(n) * p.units + unit) * p.parts + part) * p.rtiles + rt) * tile_sums(NC);
 }
 
-// KW waves a row tile; NC = channel tiles of 32.
+// The turn-th kPartTiles tiles of a part (the last turn takes what is left).  KW waves a row
+// tile; NC = channel tiles of 32.
 template <int KW, int NC, typename Smem>
 __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, int n, int unit, int group, int part,
-                                       int wave) {
+                                       int turn, int wave, int tid) {
   constexpr int NK = (NC + 1) / 2;   // 64-channel score steps
   constexpr int kWaves = waves_of(NC), kStep = kWaves;
   constexpr int kEach = kStep / KW;  // tiles of a step that a wave takes
   const uint32_t tab0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((SPK_LDS char *)(void *)sm.tab));
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int kvh = unit % p.Hkv, t = unit / p.Hkv, rows = s.nodes * p.nrep;
   const int kw = wave % KW, rt = group * kWaves + wave / KW, r = rt * 32 + col;
   const bool live = rt * 32 < rows;  // (without rows of its own a wave prepares tiles)
 
   const Keys<NK> keys(p, s, n, t, kvh, half, col);
-  const int t0 = part * s.ptiles, stop = part + 1 < s.parts ? t0 + s.ptiles : s.end;
+  const int t0 = part * s.ptiles + turn * kPartTiles;
+  const int stop = part + 1 < s.parts || (turn + 1) * kPartTiles < s.ptiles ? min(t0 + kPartTiles, s.end) : s.end;
   // The words of this wave's tile of a step are requested a step before they are prepared,
   // their block two.
   uint32_t kwords[NK], vwords[NK], phys = keys.block_of(t0 + wave);
@@ -430,9 +437,11 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
 
   auto done = [&](int c, int quad, const float (&val)[4], float den) {
     if (s.parts > 1) {
-      float *to = sums_at(p, n, unit, part, rt, NC);
-      *reinterpret_cast<v4f *>(to + ((c * 4 + quad) * 64 + lane) * 4) = v4f{val[0], val[1], val[2], val[3]};
-      if (c == 0 && quad == 0 && half == 0) to[NC * 1024 + col] = den;
+      float *to = sums_at(p, n, unit, part, rt, NC), *to_den = to + NC * 1024 + col;
+      v4f *at = reinterpret_cast<v4f *>(to + ((c * 4 + quad) * 64 + lane) * 4);
+      const v4f sum = {val[0], val[1], val[2], val[3]};
+      *at = turn ? *at + sum : sum;  // (the turns before were this lane's too)
+      if (c == 0 && quad == 0 && half == 0) *to_den = turn ? *to_den + den : den;
     } else if (r < rows) {
       store_row<4>(p, s, t, kvh, r, c, quad, half, val, den);
     }
@@ -477,7 +486,9 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
   }
 }
 
-template <int NC>
+// LONG: parts of several turns (tables of more than 65,536 tokens); their loop costs registers,
+// 49 us where 45 do without it for 61 nodes on 30,011 tokens.
+template <int NC, bool LONG>
 __global__ __launch_bounds__(waves_of(NC) * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void
 tree_attn_kernel(Params p) {
   constexpr int NK = (NC + 1) / 2, kWaves = waves_of(NC), kStep = kWaves;
@@ -500,11 +511,25 @@ tree_attn_kernel(Params p) {
   const Seq s = sequence(p, n);
   const int rows = s.nodes * p.nrep;
   if (group * kWaves * 32 >= rows || part >= s.parts) return;
-  // (one wave a row tile throughout: 7.1 us where these take 6.2 for 8 nodes on 128 tokens)
-  if (rows > 16 * kWaves) attend<1, NC>(p, s, sm, n, unit, group, part, wave);
-  else if (rows > 8 * kWaves) attend<2, NC>(p, s, sm, n, unit, group, part, wave);
-  else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC>(p, s, sm, n, unit, group, part, wave);
-  else attend<kWaves, NC>(p, s, sm, n, unit, group, part, wave);
+  auto take = [&](int turn, int tid) {
+    // (one wave a row tile throughout: 7.1 us where these take 6.2 for 8 nodes on 128 tokens)
+    if (rows > 16 * kWaves) attend<1, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
+    else if (rows > 8 * kWaves) attend<2, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
+    else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
+    else attend<kWaves, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
+  };
+  if constexpr (LONG) {
+#pragma unroll 1
+    for (int t0 = part * s.ptiles, turn = 0; turn * kPartTiles < s.ptiles && (turn == 0 || t0 < s.end);
+         t0 += kPartTiles, ++turn) {
+      if (turn) __syncthreads();  // (the turn before has read its sums)
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));  // (nothing of a lane's is kept from turn to turn)
+      take(turn, tid);
+    }
+  } else {
+    take(0, threadIdx.x);
+  }
 }
 
 // Sums of the parts, in their order.  A wave takes four channels of a lane's sixteen of an
@@ -560,7 +585,10 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_nodes, int block_
 
 template <int NC>
 static int launch(const Params &p, int N, hipStream_t s) {
-  tree_attn_kernel<NC><<<dim3(p.groups * p.parts * p.units, N), waves_of(NC) * 64, 0, s>>>(p);
+  const dim3 grid(p.groups * p.parts * p.units, N);
+  const int64_t tokens = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
+  if (tokens <= int64_t(kPartTiles) * kMaxParts * kKeys) tree_attn_kernel<NC, false><<<grid, waves_of(NC) * 64, 0, s>>>(p);
+  else tree_attn_kernel<NC, true><<<grid, waves_of(NC) * 64, 0, s>>>(p);
   const int rc = check_launch("tree_attn");
   if (rc || p.parts == 1) return rc;
   tree_join_kernel<<<dim3(p.units * p.rtiles * NC, N), 256, 0, s>>>(p, NC);
