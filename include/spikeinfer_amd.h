@@ -685,8 +685,9 @@ int spk_accept_tree(const int64_t *tokens, const int32_t *parents, const int64_t
 
 /*
  * Attention weight of the cached tokens.  Row i of sequence n's m rows
- * ([row_starts[n], row_starts[n + 1]) of q, at most max_rows; row_starts NULL: row n)
- * is the token at position seq_lens[n] - m + i and sees positions up to its own;
+ * ([row_starts[n], row_starts[n + 1]) of q; row_starts NULL: row n) is the token at
+ * position seq_lens[n] - m + i and sees positions up to its own.  Of more than max_rows
+ * rows the last max_rows count; rows that q does not have do not.
  *   mass[n][g][j] = sum over t, query heads of kv head g, rows: the row's softmax
  *                   weight of position j
  * for j < seq_lens[n], 0 behind (j < cap); with `accumulate` the sums are added and

@@ -4,6 +4,7 @@
 // positions up to its own:
 //   mass[n, g, j] (+)= sum over t, query heads h of kv head g, rows i of
 //                      exp(popc(q & k_j) * scale) / sum_j' exp(popc(q & k_j') * scale).
+// Of more than max_rows rows the last max_rows count; rows that the buffer lacks never do.
 //
 // MI355X design: scores of 16 rows and 16 keys are one fp4 product over 128 channels
 // (v_mfma_scale_f32_16x16x128_f8f6f4, a spike of both as 1, block scales that leave the
@@ -72,16 +73,18 @@ struct Params {
 struct Seq {
   int64_t first;
   int m, len, parts;
+  int open;    // the position of the first row: keys up to it are seen by all rows
   int rtiles;  // row tiles of a timestep group
 };
 
 template <int WP>
 __device__ __forceinline__ Seq sequence(const Params &p, int n) {
   Seq s;
-  const int64_t a = p.starts ? p.starts[n] : n, e = p.starts ? p.starts[n + 1] : n + 1;
-  s.first = min(max<int64_t>(a, 0), p.rows);
-  s.m = static_cast<int>(min(min(max(e, s.first), s.first + p.max_rows), p.rows) - s.first);
+  const int64_t a = p.starts ? p.starts[n] : n, e = p.starts ? max<int64_t>(p.starts[n + 1], a) : n + 1;
+  s.first = max(max<int64_t>(a, e - p.max_rows), 0);
+  s.m = static_cast<int>(max<int64_t>(min(e, p.rows) - s.first, 0));
   s.len = min(max(p.lens[n], 0), p.max_blocks << p.bs_log2);
+  s.open = s.len - static_cast<int>(max<int64_t>(e - s.first, 0));
   s.parts = (s.len + kPart - 1) / kPart;
   s.rtiles = (s.m * p.nrep + 4 * WP - 1) / (4 * WP);
   return s;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
   v8i q[RT];
 #pragma unroll
   for (int i = 0; i < RT; ++i) q[i] = query_bits(i < p.tgroups ? query_word<WP>(p, s, kvh, i, 0, lane) : 0u);
-  const int open = s.len - s.m;  // keys up to `open` are seen by all rows
+  const int open = s.open;
   float *den = p.den + (static_cast<int64_t>(blockIdx.y) * p.parts + (PASS == kDen ? blockIdx.x : 0)) * p.tgroups * 16;
   if constexpr (PASS == kMass) {
     if (tid < p.tgroups * 16) {
@@ -415,7 +418,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
       for (int u = 0; u < 4; ++u) k[st][u] = key_bits(ok[st][u] ? x[st][u] : 0u);
   }
   __syncthreads();
-  const int open = s.len - s.m;
+  const int open = s.open;
 #pragma unroll 1
   for (int i = 0; i < tiles; ++i) {
     const v8i q = query_bits(qw);
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(kMassKeys * kShare) __attribute__((amdgpu_waves_per
   if (from >= s.len || s.rtiles == 0) return;
   if (tid <= p.D) sm.tab[tid] = p.tab[tid];
   const Keys<WP, false> keys(p, s, n, kvh, lane);
-  const int j0 = static_cast<int>(from) + wave / kShare * kStep, open = s.len - s.m;
+  const int j0 = static_cast<int>(from) + wave / kShare * kStep, open = s.open;
   const int end = min(s.len, static_cast<int>(stop)), tiles = s.rtiles * p.tgroups;
   const typename Keys<WP, false>::Places places = keys.places(j0);
   const float *den = p.den + static_cast<int64_t>(blockIdx.y) * p.parts * p.tgroups * p.rtiles * 16;

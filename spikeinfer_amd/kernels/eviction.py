@@ -49,8 +49,9 @@ def paged_spike_attn_key_mass(
     Args:
         q_packed: ``int32 [T, R, H_q, W]``: without ``row_starts`` row ``n`` is sequence
             ``n``'s last token; with ``row_starts int32 [N + 1]`` rows ``row_starts[n] ..
-            row_starts[n + 1]`` are its last ones (at most ``max_rows``; others are left
-            out), each seeing the positions up to its own.
+            row_starts[n + 1]`` are its last ones, each seeing the positions up to its own.
+            Of more than ``max_rows`` rows the last ``max_rows`` count; rows that
+            ``q_packed`` does not have do not.
         k_cache: ``int32 [T, H_kv, slots, W]``; block_tables ``int32 [N, max_blocks]``;
             seq_lens ``int32 [N]`` with the rows' own tokens.
         out: optional ``float32 [N, H_kv, cap]``, entries contiguous; by default a new one
