@@ -61,7 +61,7 @@ struct Params {
   int64_t ms0, ms1, cap;
   int accumulate;
   int64_t rows;
-  uint32_t rep_mul;            // floor(r / nrep) = r * rep_mul >> 32 for every row
+  uint32_t rep_mul;            // inverse_of(nrep)
   int N, max_rows, T, Hkv, nrep, W, D, bs_log2, max_blocks;
   int tgroups;                 // timestep groups
   int rtiles;                  // most row tiles of a timestep group
@@ -649,6 +649,8 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
       cap > (1 << 29))
     return fail(SPK_EUNSUPPORTED, "key_mass: %d rows of %d heads over %d x %d tokens", max_rows, Hq / Hkv, max_blocks,
                 block_size);
+  if (!tiles::divides_to(static_cast<int64_t>(plan.rtiles) * 4 * plan.wp, Hq / Hkv))
+    return fail(SPK_EUNSUPPORTED, "key_mass: %d heads a kv head with %d rows", Hq / Hkv, max_rows);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes))
     return fail(SPK_EINVAL, "key_mass: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes);
   mass::Params p{};
@@ -666,8 +668,7 @@ extern "C" int spk_key_mass(const int32_t *q, const int64_t q_strides[3], const 
   p.mass = mass; p.ms0 = mass_strides[0]; p.ms1 = mass_strides[1]; p.cap = cap;
   p.accumulate = accumulate; p.rows = rows; p.N = N; p.max_rows = max_rows;
   p.T = T; p.Hkv = Hkv; p.nrep = Hq / Hkv; p.D = head_dim; p.W = (head_dim + 31) / 32;
-  // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
-  p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
+  p.rep_mul = tiles::inverse_of(p.nrep);
   p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks;
   p.tgroups = plan.tgroups; p.rtiles = plan.rtiles; p.parts = plan.parts;
   p.den = static_cast<float *>(workspace);

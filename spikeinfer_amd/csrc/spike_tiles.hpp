@@ -71,6 +71,13 @@ __device__ __forceinline__ v8i fp4_bits(uint32_t w) {
   return r;
 }
 
+// Rows are divided by the n heads of a kv head with one multiplication, r * inverse >> 32.  Its
+// product is off by r * (inverse * n - 2^32) / n: right while that stays below 2^32 / n.
+inline uint32_t inverse_of(int n) { return static_cast<uint32_t>(((int64_t(1) << 32) + n - 1) / n); }  // (not of 1)
+inline bool divides_to(int64_t most, int n) {
+  return n == 1 || most * (static_cast<int64_t>(inverse_of(n)) * n - (int64_t(1) << 32)) < int64_t(1) << 32;
+}
+
 // (hi, lo) f16 pairs of exp(s * scale) * 2^15 / exp(D * scale), s = 0..D.
 inline void build_table(float scale, int D, uint32_t *tab) {
   static thread_local float last_scale = -1.f;

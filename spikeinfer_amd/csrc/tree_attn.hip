@@ -76,7 +76,7 @@ struct Params {
   int64_t os0, os1, os2;
   int out_dtype, out_vec;   // out_vec: rows take aligned 4-channel stores
   int64_t rows;
-  uint32_t rep_mul;         // floor(r / nrep) = r * rep_mul >> 32 for every row
+  uint32_t rep_mul;         // inverse_of(nrep)
   int units, Hkv, nrep, D, W, bs_log2, max_blocks, max_nodes;
   int rtiles;               // most row tiles of a sequence
   int groups;               // workgroups along them
@@ -646,6 +646,8 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
   // (a launch has fewer than 2^32 threads along its first axis)
   if (units * plan.rtiles * plan.parts > (1 << 22) || static_cast<int64_t>(max_nodes) * (Hq / Hkv) > (1 << 24))
     return fail(SPK_EUNSUPPORTED, "tree_attn: T=%d Hq=%d Hkv=%d with %d nodes", T, Hq, Hkv, max_nodes);
+  if (!tiles::divides_to(static_cast<int64_t>(max_nodes) * (Hq / Hkv), Hq / Hkv))
+    return fail(SPK_EUNSUPPORTED, "tree_attn: %d heads a kv head with %d nodes", Hq / Hkv, max_nodes);
   tree::Params p{};
   p.q = reinterpret_cast<const uint32_t *>(q);
   p.qs0 = q_strides[0]; p.qs1 = q_strides[1]; p.qs2 = q_strides[2];
@@ -674,8 +676,7 @@ extern "C" int spk_tree_attn(const int32_t *q, const int64_t q_strides[3], const
               (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   p.rows = rows; p.units = static_cast<int>(units); p.Hkv = Hkv; p.nrep = Hq / Hkv; p.D = head_dim;
   p.W = (head_dim + 31) / 32; p.bs_log2 = ilog2(block_size); p.max_blocks = max_blocks; p.max_nodes = max_nodes;
-  // ceil(2^32 / nrep): its product with r is off by less than r * nrep, below 2^32
-  p.rep_mul = static_cast<uint32_t>(((int64_t(1) << 32) + p.nrep - 1) / p.nrep);
+  p.rep_mul = tiles::inverse_of(p.nrep);
   p.rtiles = plan.rtiles; p.groups = plan.groups; p.parts = plan.parts; p.ws = static_cast<float *>(workspace);
   tiles::build_table(scale, head_dim, p.tab);
   hipStream_t s = static_cast<hipStream_t>(stream);

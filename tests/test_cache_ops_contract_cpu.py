@@ -1,0 +1,41 @@
+"""Calls of the draft-tree and eviction operators that are refused on the host: nothing is
+launched, and no pointer is read."""
+from __future__ import annotations
+
+from spikeinfer_amd import _lib
+from test_cache_ops_cpu import P, _i64, _tree
+
+
+def _mass(lib, hq=14, hkv=2, most=1, T=1, mb=8):
+    s = _i64(1, 1, 1)
+    return lib.spk_key_mass(P, s, P, s, 100, P, 8, 1, P, P, P, _i64(1, 1), 100, 0, 2, 1, most, T, hq, hkv, 64, 16, mb,
+                            0.125, P, 1 << 60, None)
+
+
+def test_head_ratios_that_the_row_division_does_not_hold():
+    """Rows are divided by the heads a kv head with one multiplication, r * ceil(2^32 / n) >> 32.
+    A ratio for which that names a wrong head for some row of the call is refused."""
+    def wrong(n, rows):  # the first row that the multiplication gets wrong
+        m = -(-2**32 // n)
+        over = m * n - 2**32
+        r = -(-2**32 // over) if over else rows
+        r += (n - 1 - r) % n  # (the last of a quotient's)
+        return r if r < rows else None
+
+    for n, rows in ((257, 65280 * 257), (4097, 1024 * 4097)):
+        r = wrong(n, rows)
+        if r is not None:
+            assert r * -(-2**32 // n) >> 32 != r // n
+    lib = _lib.load()
+    bad = [n for n in range(2049, 16384, 7) if wrong(n, 1024 * n) is not None]
+    good = [n for n in (7, 17, 256, 1024, 2048) if wrong(n, 1024 * n) is None]
+    assert len(bad) > 100 and len(good) == 5
+    for n in bad[:3] + bad[-3:]:
+        assert _tree(lib, T=1, hq=n, hkv=1, max_nodes=1024, mask_words=16, mb=1) == _lib.SPK_EUNSUPPORTED, n
+        assert b"heads" in lib.spk_last_error()
+    most = lambda n: (1 << 24) // n
+    bad = [n for n in range(257, 5000, 3) if wrong(n, most(n) * n) is not None]
+    assert len(bad) > 100
+    for n in bad[:3] + bad[-3:]:
+        assert _mass(lib, hq=n, hkv=1, most=most(n), mb=1) == _lib.SPK_EUNSUPPORTED, n
+        assert b"heads" in lib.spk_last_error()
