@@ -67,6 +67,7 @@ class AttentionMetadata:
     prefill_query_lens: list[int] = field(default_factory=list)
     prefill_context_lens: list[int] = field(default_factory=list)
     prefill_block_tables: list[torch.Tensor] = field(default_factory=list)
+    # The next two are taken by SpikingDecoder.forward_paged alone.
     # a step of drafted trees and nothing else (slot_mapping -1: no row goes to the cache)
     draft: DraftTrees | None = None
     # each layer's float32 [n_dec, H_kv, cap]: the decode tokens' attention weights are added
@@ -154,6 +155,15 @@ def _prefill(q_dense, k_cache, v_cache, meta, out, num_q_heads, num_kv_heads, he
         out[:, start:start + q_len] = o.permute(0, 2, 1, 3)
 
 
+def _no_step_of_its_own(meta: AttentionMetadata) -> None:
+    """Draft trees and key weights belong to a whole step (SpikingDecoder.forward_paged):
+    one layer's attention knows neither its layer nor where drafted words go."""
+    for name in ("draft", "key_mass"):
+        if getattr(meta, name, None) is not None:  # (a caller's own metadata may know neither)
+            raise ValueError(f"metadata with {name} is for SpikingDecoder.forward_paged; for one layer call "
+                             f"{'paged_spike_attn_tree' if name == 'draft' else 'paged_spike_attn_key_mass'}")
+
+
 def paged_attention(
     q_spk: torch.Tensor,
     k_spk: torch.Tensor,
@@ -169,7 +179,9 @@ def paged_attention(
 
     ``q_spk, k_spk, v_spk``: ``[T, 1, H, n_tok, D]`` 0/1 spikes; caches ``int32
     [T, H_kv, num_slots, W]`` of this layer.  Returns ``[T, 1, n_tok, H_q * D]``.
+    Metadata with ``draft`` or ``key_mass`` is refused.
     """
+    _no_step_of_its_own(meta)
     T, n_tok = q_spk.shape[0], q_spk.shape[3]
     dtype, device = q_spk.dtype, q_spk.device
     k_cache.index_copy_(2, meta.slot_mapping, pack_spikes(k_spk.squeeze(1)))
@@ -226,8 +238,10 @@ def paged_attention_fused(
         q_packed: optional preallocated ``int32 [T, n_dec, H_q, W]`` buffer.
         Both are needed for graph capture (stable addresses).
 
-    Returns ``[T, 1, n_tok, H_q * D]`` in ``q_cur.dtype``.
+    Returns ``[T, 1, n_tok, H_q * D]`` in ``q_cur.dtype``.  Metadata with ``draft`` or
+    ``key_mass`` is refused.
     """
+    _no_step_of_its_own(meta)
     T, n_tok = q_cur.shape[0], q_cur.shape[1]
     dtype, device = q_cur.dtype, q_cur.device
     given = out is not None

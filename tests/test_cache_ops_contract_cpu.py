@@ -2,7 +2,11 @@
 launched, and no pointer is read."""
 from __future__ import annotations
 
+import pytest
+import torch
+
 from spikeinfer_amd import _lib
+from spikeinfer_amd.attention import AttentionMetadata, DraftTrees, paged_attention, paged_attention_fused
 from test_cache_ops_cpu import P, _i64, _tree
 
 
@@ -39,3 +43,20 @@ def test_head_ratios_that_the_row_division_does_not_hold():
     for n in bad[:3] + bad[-3:]:
         assert _mass(lib, hq=n, hkv=1, most=most(n), mb=1) == _lib.SPK_EUNSUPPORTED, n
         assert b"heads" in lib.spk_last_error()
+
+
+@pytest.mark.parametrize("what", ["draft", "key_mass"])
+def test_metadata_that_one_layer_cannot_honour(what):
+    """Neither drops the weights that a step asks for, nor takes drafted rows for tokens."""
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    given = dict(draft=DraftTrees(i32(2), torch.zeros((3, 1), dtype=torch.int64), 3, i32(1), i32(1, 4)),
+                 key_mass=[torch.zeros((1, 2, 64))])[what]
+    meta = AttentionMetadata(slot_mapping=torch.full((3,), -1), block_size=16, num_decode_tokens=0 if what == "draft" else 3,
+                             block_tables=i32(3, 4), seq_lens=i32(3), **{what: given})
+    cache = i32(2, 2, 64, 2)
+    spikes = lambda h: torch.zeros((2, 1, h, 3, 64))
+    with pytest.raises(ValueError, match=f"{what} is for SpikingDecoder.forward_paged"):
+        paged_attention(spikes(4), spikes(2), spikes(2), cache, cache.clone(), meta, 4, 2, 64)
+    cur, lif = lambda h: torch.zeros((2, 3, h, 64)), (torch.full((64,), 0.9), torch.ones(64))
+    with pytest.raises(ValueError, match=f"{what} is for SpikingDecoder.forward_paged"):
+        paged_attention_fused(cur(4), cur(2), cur(2), lif, lif, lif, cache, cache.clone(), meta, 4, 2, 64)
