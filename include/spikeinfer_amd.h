@@ -663,12 +663,14 @@ int spk_tree_masks(const int32_t *parents, const int32_t *row_starts, int64_t ro
  * is none.
  *   tokens, targets int64 [rows], parents int32 [rows] as spk_tree_masks
  *   path     int32 [N, max_nodes]: the path's rows, -1 behind it
- *   count    int32 [N]: rows of the path (0 for a sequence without rows)
- *   next_tokens int64 [N]: targets of the path's last row (-1 without rows)
+ *   count    int32 [N]: rows of the path (0 for a sequence without rows, or room)
+ *   next_tokens int64 [N]: targets of the path's last row (-1 where count is 0)
  *   layers   host array: each layer's new words (t, row, kv head) at new_strides and
  *            caches (t, kv head, slot) at cache_strides; step i of the path goes to
- *            position context_lens[n] + i of the block table (dropped where the table
- *            or the cache ends); nlayers 0: the walk alone
+ *            position context_lens[n] + i of the block table.  A path ends before the
+ *            first step whose position lies past the table or in a block outside the
+ *            cache, so that count names the rows that are cached (0: not even row 0).
+ *            nlayers 0: the walk alone
  * max_nodes <= 1024.
  */
 typedef struct SpkCommitLayer {

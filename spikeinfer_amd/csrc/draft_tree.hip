@@ -81,14 +81,15 @@ struct Params {
 };
 
 // Workgroup (n, layer): its first wave walks tree n, a step a round of 64 candidate
-// children; then the threads move the path's words of the layer.  Every layer's
+// children, while the others look how many tokens behind the context have a place in the
+// cache (a path ends there); then the threads move the path's words of the layer.  Every layer's
 // workgroup walks again: the walk takes a few hundred ns a step from LDS, a second
 // launch would take more.  Latency only: 24 layers of one tree of 8 rows take 4.1 us, of 64
-// trees of 61 rows 7.0.
+// trees of 61 rows 7.3.
 __global__ __launch_bounds__(kThreads) void accept_kernel(Params p) {
   __shared__ int64_t tok[kMaxNodes], tgt[kMaxNodes];
   __shared__ int32_t par[kMaxNodes], path[kMaxNodes];
-  __shared__ int depth;
+  __shared__ int depth, room;
   const int tid = threadIdx.x, lane = tid & 63, n = blockIdx.x;
   const Rows r = rows_of(p.starts, n, p.rows, p.max_nodes);
   for (int i = tid; i < r.count; i += kThreads) {
@@ -96,8 +97,20 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(Params p) {
     tgt[i] = p.targets[r.first + i];
     par[i] = p.parents[r.first + i];
   }
+  const Layer layer = p.layer[blockIdx.y];
+  const int64_t blocks = p.num_slots >> p.bs_log2, ctx = layer.k ? max(p.lens[n], 0) : 0;
+  auto slot = [&](int step) -> int64_t {  // of a step's token, below 0: none
+    const int64_t pos = ctx + step, blk = pos >> p.bs_log2;
+    if (blk >= p.max_blocks) return -1;
+    const int64_t phys = p.bt[n * p.bts0 + blk * p.bts1];
+    return phys < 0 || phys >= blocks ? -1 : phys << p.bs_log2 | (pos & ((1 << p.bs_log2) - 1));
+  };
+  if (tid == 0) room = r.count;
   __syncthreads();
-  if (tid < 64) {
+  if (tid >= 64) {
+    for (int i = tid - 64; layer.k && i < r.count; i += kThreads - 64)
+      if (slot(i) < 0) atomicMin(&room, i);
+  } else {
     int at = 0, len = r.count > 0 ? 1 : 0;
     if (lane == 0) path[0] = 0;
     while (at < r.count) {
@@ -119,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(Params p) {
     if (lane == 0) depth = len;
   }
   __syncthreads();
-  const int len = depth;
+  const int len = min(depth, room);
   if (p.first && blockIdx.y == 0) {
     for (int i = tid; i < p.max_nodes; i += kThreads) p.path[n * static_cast<int64_t>(p.max_nodes) + i] = i < len ? path[i] : -1;
     if (tid == 0) {
@@ -127,19 +140,12 @@ __global__ __launch_bounds__(kThreads) void accept_kernel(Params p) {
       p.next[n] = len ? tgt[path[len - 1]] : -1;
     }
   }
-  const Layer layer = p.layer[blockIdx.y];
   if (!layer.k) return;
-  const int ctx = max(p.lens[n], 0);
-  const int64_t blocks = p.num_slots >> p.bs_log2;
   const int units = p.T * p.Hkv * p.W;  // words of a token
   for (int i = tid; i < len * units; i += kThreads) {
     const int step = i / units, u = i - step * units;
     const int w = u % p.W, h = u / p.W % p.Hkv, t = u / p.W / p.Hkv;
-    const int64_t pos = static_cast<int64_t>(ctx) + step, blk = pos >> p.bs_log2;
-    if (blk >= p.max_blocks) continue;
-    const int64_t phys = p.bt[n * p.bts0 + blk * p.bts1];
-    if (phys < 0 || phys >= blocks) continue;
-    const int64_t to = t * p.ks0 + h * p.ks1 + ((phys << p.bs_log2) | (pos & ((1 << p.bs_log2) - 1))) * p.ks2 + w;
+    const int64_t to = t * p.ks0 + h * p.ks1 + slot(step) * p.ks2 + w;
     const int64_t from = t * p.ns0 + (r.first + path[step]) * p.ns1 + h * p.ns2 + w;
     layer.k[to] = layer.kn[from];
     layer.v[to] = layer.vn[from];

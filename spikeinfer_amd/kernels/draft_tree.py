@@ -215,12 +215,15 @@ def accept_draft_tree(
         drafts: each layer's ``(k_words, v_words)``, ``int32 [T, R, H_kv, W]``.
         layers: each layer's ``(k_cache, v_cache)``, ``int32 [T, H_kv, slots, W]``; the
             path's words go to positions ``context_lens[n], context_lens[n] + 1, ...`` of
-            ``block_tables[n]`` (``int32 [N, max_blocks]``).  Without layers nothing moves.
+            ``block_tables[n]`` (``int32 [N, max_blocks]``).  A path ends before the first
+            row whose position lies past the table or in a block outside the cache, so that
+            ``count`` names the rows that are cached.  Without layers nothing moves.
         out: optional ``(path, count, next)`` buffers (for graph capture).
 
     Returns ``path int32 [N, max_nodes]`` (rows of the tree, -1 behind the path),
-    ``count int32 [N]`` (the path's rows, row 0 among them; 0 for a sequence without rows)
-    and ``next int64 [N]``, the model's token after the path (-1 without rows).
+    ``count int32 [N]`` (the path's rows, row 0 among them; 0 for a sequence without rows,
+    or without a place for row 0) and ``next int64 [N]``, the model's token after the path
+    (-1 where ``count`` is 0).
     """
     native = _lib.native()
     if native is not None and layers:
