@@ -180,6 +180,9 @@ def draft_tree_masks(parents: torch.Tensor, row_starts: torch.Tensor, max_nodes:
 
 def _same_layout(name: str, pairs, dev) -> tuple[torch.Size, tuple[int, ...]]:
     """Shape and strides that the packed tensors of every layer share."""
+    for pair in pairs:
+        if len(pair) != 2:
+            raise ValueError(f"{name}: every layer must be a (k, v) pair, got {len(pair)} tensors")
     first = pairs[0][0]
     _check_packed(name, first)
     for pair in pairs:
@@ -259,6 +262,8 @@ def accept_draft_tree(
         out = (torch.empty((n_seqs, max_nodes), dtype=torch.int32, device=dev),
                torch.empty(n_seqs, dtype=torch.int32, device=dev),
                torch.empty(n_seqs, dtype=torch.int64, device=dev))
+    elif len(out) != 3:
+        raise ValueError(f"out must be (path, count, next), got {len(out)} tensors")
     for t, shape, dt in zip(out, ((n_seqs, max_nodes), (n_seqs,), (n_seqs,)), (torch.int32, torch.int32, torch.int64)):
         if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
             raise ValueError(f"out needs contiguous {dt} {shape}, got {t.dtype} {tuple(t.shape)}")

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from spikeinfer_amd import _lib
+from spikeinfer_amd import _lib, kernels
 from spikeinfer_amd.attention import AttentionMetadata, DraftTrees, paged_attention, paged_attention_fused
 from test_cache_ops_cpu import P, _i64, _tree
 
@@ -60,3 +60,30 @@ def test_metadata_that_one_layer_cannot_honour(what):
     cur, lif = lambda h: torch.zeros((2, 3, h, 64)), (torch.full((64,), 0.9), torch.ones(64))
     with pytest.raises(ValueError, match=f"{what} is for SpikingDecoder.forward_paged"):
         paged_attention_fused(cur(4), cur(2), cur(2), lif, lif, lif, cache, cache.clone(), meta, 4, 2, 64)
+
+
+def test_layers_and_outputs_that_are_no_pairs_and_triples(monkeypatch):
+    """The addresses of every layer go to the host entry as pairs: one tensor less and it
+    would read behind them."""
+    def launched(*_):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "native", lambda: None)
+    monkeypatch.setattr(_lib, "launch", launched)
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    k, w, ids = i32(2, 2, 64, 2), i32(2, 3, 2, 2), torch.zeros(3, dtype=torch.int64)
+    for layer in ((k,), (k, k.clone(), k.clone()), ()):
+        for layers in ([layer], [(k, k.clone()), layer], [layer, (k, k.clone())]):
+            with pytest.raises(ValueError, match="layers: .* pair"):
+                kernels.evict_cache(layers, torch.zeros(len(layers), 1, 2, 64), i32(1, 4), i32(1), 40, 16)
+            good = [(w, w.clone())] * len(layers)
+            with pytest.raises(ValueError, match="layers: .* pair"):
+                kernels.accept_draft_tree(ids, i32(3), ids, i32(2), 3, good, layers, i32(1, 4), i32(1), 16)
+    for draft in ((w,), (w, w, w), ()):
+        with pytest.raises(ValueError, match="drafts: .* pair"):
+            kernels.accept_draft_tree(ids, i32(3), ids, i32(2), 3, [draft], [(k, k.clone())], i32(1, 4), i32(1), 16)
+    path, count, after = i32(1, 3), i32(1), torch.zeros(1, dtype=torch.int64)
+    for out in ((path, count), (path, count, after, after), ()):
+        with pytest.raises(ValueError, match="path, count, next"):
+            kernels.accept_draft_tree(ids, i32(3), ids, i32(2), 3, out=out)
