@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <string>
+#include <utility>
 
 #include "../../include/spikeinfer_amd.h"
 
@@ -39,6 +40,22 @@ inline int ilog2(int x) {
   int r = 0;
   while ((1 << r) < x) ++r;
   return r;
+}
+
+// The first layer one of whose caches, k or v, is another's too (or the layer's own other one);
+// -1: none.
+template <class KV>
+inline int shared_cache(int nlayers, KV caches) {  // caches(i): layer i's two addresses
+  for (int i = 0; i < nlayers; ++i) {
+    const auto a = caches(i);
+    bool any = a.first == a.second;
+    for (int j = 0; j < i; ++j) {
+      const auto b = caches(j);
+      any |= a.first == b.first || a.first == b.second || a.second == b.first || a.second == b.second;
+    }
+    if (any) return i;
+  }
+  return -1;
 }
 
 // ---- element access by dtype code -----------------------------------------

@@ -200,10 +200,8 @@ extern "C" int spk_accept_tree(const int64_t *tokens, const int32_t *parents, co
       return fail(SPK_EINVAL, "accept_tree: null pointer in layer %d", i);
   if (nlayers > 0 && ((T > 1 && !cache_strides[0]) || (Hkv > 1 && !cache_strides[1]) || (num_slots > 1 && !cache_strides[2])))
     return fail(SPK_EINVAL, "accept_tree: words of a cache lie on one another");
-  for (int i = 1; i < nlayers; ++i)
-    for (int j = 0; j < i; ++j)
-      if (layers[i].k_cache == layers[j].k_cache || layers[i].v_cache == layers[j].v_cache)
-        return fail(SPK_EINVAL, "accept_tree: layers %d and %d have one cache", j, i);
+  const int twice = shared_cache(nlayers, [&](int i) { return std::make_pair(layers[i].k_cache, layers[i].v_cache); });
+  if (twice >= 0) return fail(SPK_EINVAL, "accept_tree: layer %d has one cache twice, or another layer's", twice);
   draft::Params p{};
   p.tokens = tokens; p.targets = targets; p.parents = parents; p.starts = row_starts;
   p.rows = rows; p.max_nodes = max_nodes; p.path = path; p.count = count; p.next = next_tokens;

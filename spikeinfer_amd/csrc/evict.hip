@@ -336,10 +336,8 @@ extern "C" int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t
     return fail(SPK_EINVAL, "evict: words of a cache lie on one another");
   if (cap > 0 && ((nlayers > 1 && !mass_out_strides[0]) || (N > 1 && !mass_out_strides[1]) || (Hkv > 1 && !mass_out_strides[2])))
     return fail(SPK_EINVAL, "evict: rows of mass_out lie on one another");
-  for (int i = 1; i < nlayers && num_slots > 0; ++i)
-    for (int j = 0; j < i; ++j)
-      if (layers[i].k == layers[j].k || layers[i].v == layers[j].v)
-        return fail(SPK_EINVAL, "evict: layers %d and %d have one cache", j, i);
+  const int twice = shared_cache(num_slots > 0 ? nlayers : 0, [&](int i) { return std::make_pair(layers[i].k, layers[i].v); });
+  if (twice >= 0) return fail(SPK_EINVAL, "evict: layer %d has one cache twice, or another layer's", twice);
   evict::Params p{};
   p.mass = mass; p.ms0 = mass_strides[0]; p.ms1 = mass_strides[1]; p.ms2 = mass_strides[2];
   p.mass_out = mass_out; p.os0 = mass_out_strides[0]; p.os1 = mass_out_strides[1]; p.os2 = mass_out_strides[2];

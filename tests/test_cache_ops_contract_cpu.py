@@ -87,3 +87,24 @@ def test_layers_and_outputs_that_are_no_pairs_and_triples(monkeypatch):
     for out in ((path, count), (path, count, after, after), ()):
         with pytest.raises(ValueError, match="path, count, next"):
             kernels.accept_draft_tree(ids, i32(3), ids, i32(2), 3, out=out)
+
+
+def test_one_cache_as_keys_and_values():
+    """Its words would be written by several threads at once, whichever places name it."""
+    lib = _lib.load()
+    s = _i64(1, 1, 1)
+    words = lambda *p: b"".join((x * P).to_bytes(8, "little") for x in p)
+
+    def accept(layers):
+        return lib.spk_accept_tree(P, P, P, P, 10, 2, 8, P, P, P, layers, len(layers) // 32, s, s, 100, P, 8, 1, P, 4, 2,
+                                   64, 16, 8, None)
+
+    def evict(layers):
+        return lib.spk_evict(layers, len(layers) // 16, s, 100, P, s, P, s, 128, P, 8, 1, 8, None, 0, 0, 0, P, P, P, 64, 4,
+                             32, 4, 2, 2, 64, 16, None)
+
+    for pairs in ([(5, 5)], [(1, 2), (3, 1)], [(1, 2), (2, 3)], [(1, 2), (3, 4), (5, 6), (7, 3)], [(1, 2), (4, 4)]):
+        assert accept(b"".join(words(98, 99, *kv) for kv in pairs)) == _lib.SPK_EINVAL, pairs
+        assert b"one cache" in lib.spk_last_error()
+        assert evict(b"".join(words(*kv) for kv in pairs)) == _lib.SPK_EINVAL, pairs
+        assert b"one cache" in lib.spk_last_error()
