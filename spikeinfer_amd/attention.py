@@ -92,8 +92,11 @@ class AttentionMetadata:
         if key not in self._copies:
             move = lambda t: None if t is None else t.to(device, non_blocking=True)
             draft, mass = self.draft, self.key_mass
+            there = device
+            if device.type == "cuda" and device.index is None:
+                there = torch.device("cuda", torch.cuda.current_device())
             for t in [t for kv in (draft and draft.words or ()) for t in kv] + list(mass or ()):
-                if (t.device.type, t.device.index or 0) != (device.type, device.index or 0):
+                if (t.device.type, t.device.index or 0) != (there.type, there.index or 0):
                     raise ValueError(f"what the step writes (draft.words, key_mass) must be on {device}, not {t.device}")
             if draft is not None:
                 if draft.words is None:

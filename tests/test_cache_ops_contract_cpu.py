@@ -108,3 +108,18 @@ def test_one_cache_as_keys_and_values():
         assert b"one cache" in lib.spk_last_error()
         assert evict(b"".join(words(*kv) for kv in pairs)) == _lib.SPK_EINVAL, pairs
         assert b"one cache" in lib.spk_last_error()
+
+
+def test_metadata_moved_to_the_current_device(monkeypatch):
+    """A device without a number is the current one, whichever that is."""
+    from types import SimpleNamespace
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    on = lambda i: [SimpleNamespace(device=torch.device("cuda", i))]
+    slots = SimpleNamespace(device=torch.device("cpu"), to=lambda device, non_blocking: None)
+    meta = lambda mass: AttentionMetadata(slot_mapping=slots, block_size=16, key_mass=mass)
+    for device in ("cuda", torch.device("cuda"), "cuda:1"):
+        assert meta(on(1)).on(device).key_mass[0].device.index == 1
+        with pytest.raises(ValueError, match="must be on cuda"):
+            meta(on(0)).on(device)
+    assert meta(on(0)).on("cuda:0").key_mass[0].device.index == 0
