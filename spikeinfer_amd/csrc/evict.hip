@@ -13,7 +13,8 @@
 //     token never moves up, so chunks in order, each read whole before it is written, move
 //     in place.
 // Six layers of 32 sequences of 1,500..12,000 tokens cut to 2,048 (4 timesteps, 2 kv heads of
-// 64 channels) take 33 + 54 us.  The selection is bound by vector instructions and barriers.
+// 64 channels) take 32 + 54 us.  The selection is bound by vector instructions (its units are busy
+// 64 % of the time) and barriers.
 // The move touches nearly every 64-byte line of the sequences (three of ten tokens stay, eight
 // lie in a line), 166 MB, and writes 50: 4.0 TB/s of lines, and other shapes of its
 // workgroups (256..1024 threads, 1..4 timesteps) measure the same within 2 % or slower.
@@ -288,9 +289,12 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(Params p) {
   }
 }
 
-// Masses in registers as the longest sequence needs them: 16 a thread 73 us where reading them
-// five times takes 96 and 32 a thread (one workgroup a CU) 99 (the six layers above, replayed);
-// 2 a thread 11.4 us where they take 16.1 and 26.8 (one layer, 2,000 tokens to 512).
+// Masses in registers as the longest sequence needs them, against reading them five times
+// (evictions captured and replayed): 2 a thread 13.4 us, reading 18.2, 32 a thread 28.9 (one layer,
+// 2,000 tokens to 512); 8 a thread 30.4, 16 a thread 34.2, reading 40.3 (one layer of 8,000 to
+// 2,048); 16 a thread 79, reading 101, 32 a thread (one workgroup a CU) 104 (the six layers above);
+// 32 a thread 55, reading 72 (one layer of 20,000 to 4,096), and 205, reading 245 (six layers of
+// 32 sequences of 17,000..32,768 to 2,048).
 static void launch_select(const Params &p, dim3 grid, hipStream_t s) {
   const int tokens = p.cap < p.max_tokens ? p.cap : p.max_tokens;  // the longest sequence
   if (tokens <= 2 * kSelThreads) evict_select_kernel<2><<<grid, kSelThreads, 0, s>>>(p);
