@@ -631,7 +631,9 @@ int spk_sample_ws(const void *logits, int logits_dtype, int64_t row_stride, int 
  *            channel stride 1
  * Lengths, starts and masks are read on the device, so a captured call takes another
  * batch's.  head_dim <= 128, max_nodes <= 1024 (SPK_EUNSUPPORTED beyond),
- * scale * head_dim <= 12.  A sequence's rows do not depend on the batch around it.
+ * scale * head_dim <= 12.  More than 256 query heads a kv head are SPK_EUNSUPPORTED where
+ * the rows' division by them would not be exact (also for spk_key_mass).  A sequence's
+ * rows do not depend on the batch around it.
  * workspace: spk_tree_attn_workspace_bytes(...) bytes, NULL when that is 0.
  */
 size_t spk_tree_attn_workspace_bytes(int T, int N, int Hq, int Hkv, int head_dim, int max_nodes,

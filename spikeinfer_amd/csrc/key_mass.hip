@@ -22,12 +22,13 @@
 //     tiles; mass_rows_kernel has 128 keys, and its waves share the row tiles.
 // The order of all sums is the sequence's own, whatever the batch.
 //
-// Bound by instruction issue and latency, with few rows near the bytes': 4 timesteps, 14 query
-// and 2 kv heads of 64 channels, one row of each of 64 sequences of 4,096..16,384 tokens takes
-// 18 + 21 us (42 MB of keys, read twice, the second time mostly from the caches: 2.2 TB/s),
-// where a vector unit is busy for about half the time: a product has 24 vector instructions
-// beside it, four look-ups and their sums and the key's five.  Windows of up to 32 rows of 8
-// sequences of 2,000..8,000 tokens take 18 + 21 us.
+// Bound by instruction issue and latency: 4 timesteps, 14 query and 2 kv heads of 64 channels,
+// one row of each of 64 sequences of 4,096..16,384 tokens takes 17.7 + 21.6 us a dispatch (42 MB of
+// keys, read twice, the second time mostly from the caches: 2.1 TB/s), where vector units are busy
+// 52 % of the time: a product has 24 vector instructions beside it, four look-ups and their sums
+// and the key's five.  The rest is the chain lengths, table, words, LDS table, barrier, with
+// nothing under it.  Windows of up to 32 rows of 8 sequences of 2,000..8,000 tokens take 18.1 +
+// 20.9 us, vector units busy 62 and 55 %.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -39,8 +40,9 @@ using namespace tiles;
 
 constexpr int kStep = 64;      // keys a wave takes at once: four products' columns
 constexpr int kPart = 1024;    // keys of a partial sum
-// Waves that share kPart keys, each with kSteps steps.  Of 4, 8 and 16: 8.6, 7.1 and 6.6 us for a
-// row of 700 tokens, 37, 37 and 51 for one of each of 64 sequences of 4,096..16,384.
+// Waves that share kPart keys, each with kSteps steps.  Of 4, 8 and 16 (captured and replayed):
+// 10.9, 10 and 9..11 us for a row of 700 tokens, 40.6, 41.0 and 55.4 for one of each of 64 sequences
+// of 4,096..16,384.
 constexpr int kWaves = 8;
 constexpr int kSteps = kPart / (kWaves * kStep);
 constexpr int kRows = 4;       // many rows: row tiles of a workgroup
@@ -138,9 +140,9 @@ __device__ __forceinline__ uint32_t query_word(const Params &p, const Seq &s, in
 // A lane's words of a step's four key tiles (lane l: key l % 16 of a tile, block l / 16 of
 // the product's channels).  Keys behind the sequence read its last block, what they give is
 // dropped; so is, by the queries' zeros, what a block of no timestep or word gives.
-// PAGE: blocks are of 16 slots or more, a key tile lies in one and its place is scalar (36.7 us
-// where lanes' own places take 40.9, 64 sequences of 4,096..16,384 tokens; with many rows there
-// is no difference).
+// PAGE: blocks are of 16 slots or more, a key tile lies in one and its place is scalar (41.0 us
+// where lanes' own places take 43.5, 64 sequences of 4,096..16,384 tokens, captured and replayed;
+// with many rows there is no difference).
 template <int WP, bool PAGE>
 struct Keys {
   const Params &p;
@@ -375,9 +377,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))
 }
 
 // Many rows: denominators of kRows row tiles of a timestep group over kPart keys.  A wave keeps
-// its keys and goes through the row tiles in a loop.  With four of them both kernels take 34 us
-// for windows of up to 32 rows of 8 sequences of 2,000..8,000 tokens (two 39, eight 36, eight in
-// registers and the keys in the loop 37).
+// its keys and goes through the row tiles in a loop.  With four of them both kernels take 41 us
+// captured and replayed for windows of up to 32 rows of 8 sequences of 2,000..8,000 tokens (two 46,
+// eight 43).
 template <int WP>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4))) void den_rows_kernel(Params p) {
   struct Smem {
@@ -571,8 +573,8 @@ inline Plan plan(int T, int N, int Hq, int Hkv, int D, int max_rows, int block_s
   return r;
 }
 
-// With one part a launch does both passes: 8.6 us where two took 12.6 (a sequence of 700 tokens,
-// four waves a workgroup; 7.1 with eight).
+// With one part a launch does both passes: 11.0 us where two take 13.0 (a sequence of 700 tokens,
+// captured and replayed).
 template <int WP, int RT, bool PAGE>
 static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
   const dim3 grid((wide + kPart - 1) / kPart, p.N * p.Hkv);
@@ -586,8 +588,9 @@ static int launch_few(const Params &p, int64_t wide, hipStream_t s) {
 }
 
 // Few rows: one row tile in each of four timestep groups at most (a decode step's).  The
-// kernels for many rows would take 143 us where these take 37 (64 sequences of 4,096..16,384
-// tokens, 14 query and 2 kv heads of 64 channels, 4 timesteps).
+// kernels for many rows would take 133 us where these take 41 (64 sequences of 4,096..16,384
+// tokens, 14 query and 2 kv heads of 64 channels, 4 timesteps, captured and replayed).  Two rows
+// of such a step, or more than 8 heads a kv head of 64 channels, have two row tiles and go there.
 template <int WP>
 static int launch(const Params &p, hipStream_t s) {
   // (without accumulation entries behind the table become 0)

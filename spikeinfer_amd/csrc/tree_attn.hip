@@ -17,9 +17,10 @@
 //     weights hold what makes the products equal again.
 //   * Eight waves a workgroup (four with more than 64 channels) share the key tiles' operands
 //     through LDS: each prepares one of a step's tiles, two buffers of them so that one barrier
-//     a step does.  Of a sequence of more than 128 rows a workgroup takes 256, a wave a row
-//     tile and all keys; of 65 to 128 rows two waves share a row tile, of 33 to 64 four, below
-//     eight, each with its part of a step's tiles; they are added in their order.
+//     a step does.  Of a sequence of more than 16 rows a wave of the workgroup (128, 64) each
+//     wave takes a row tile of 32 and all keys; of more than 8 two waves share a row tile, of
+//     more than 4 (and with four waves of fewer) four, else all eight, each with its part of a
+//     step's tiles; they are added in their order.
 //   * The context is cut into parts of kPartTiles tiles (more beyond kMaxParts parts), the
 //     tree's tiles belonging to the last: a workgroup each, whose sums a second launch adds in
 //     their order.  So the sums depend on the sequence alone, its length and its rows, not on
@@ -30,13 +31,15 @@
 //     equal weights with values of ones, the worst found, 2.4e-6 at 1 << 20 and 4e-6 at 1 << 22
 //     (with one accumulator a part up to 5e-5 and 2e-4).
 //
-// Bound by issue: a tile of 32 rows and 32 keys is 9 matrix instructions with about 90 vector
-// ones, which hide behind one another only in part.
-// With 14 query and 2 kv heads of 64 channels and 4 timesteps, 32 nodes on each of 16
-// contexts of 4,096..16,384 tokens, fp32, take 122 us: 617 TFLOP/s of 4 * T * Hq * nodes * keys *
-// D operations, those on values done twice.  61 nodes on 30,011 tokens, bf16,
-// take 45 us: 580 TFLOP/s, in 240 workgroups of 64 tiles, one a CU.  (The weights' high halves
-// alone would take 33, and change bf16 outputs: up to 2^-10 of them where 2^-8 is half a step.)
+// Bound by issue: a tile of 32 rows and 32 keys of 64 channels is 9 matrix instructions with 64
+// vector, 19 LDS and about 11 scalar ones, which hide behind one another only in part.  With 14
+// query and 2 kv heads of 64 channels and 4 timesteps, 32 nodes on each of 16 contexts of
+// 4,096..16,384 tokens, fp32, take 115..126 us, 600..655 TFLOP/s of 4 * T * Hq * nodes * keys * D
+// operations (those on values done twice); matrix units are busy 44 % and vector units 57 % of
+// the time.  61 nodes on 30,011 tokens, bf16, take 46 us: 569 TFLOP/s, in 240 workgroups of 64
+// tiles, one a CU.  (The weights' high halves alone would take 33, and change bf16 outputs: up
+// to 2^-10 of them where 2^-8 is half a step.)  At four waves a SIMD the kernel for 64 channels
+// spills 68 registers, of which its unmasked loops reload 12 to 14 a step of eight tiles.
 #include <type_traits>
 
 #include "spike_tiles.hpp"
@@ -47,13 +50,14 @@ namespace tree {
 using namespace tiles;
 
 // Waves a workgroup, and tiles between its barriers: eight, so that two workgroups are four
-// waves a SIMD, or with the sums of more than 64 channels, four, so that two are two (67 us
-// where eight take 76: 8 sequences of 100..9,000 tokens, 25 nodes, 16 query heads of 128).
+// waves a SIMD, or with the sums of more than 64 channels, four, so that two are two (71 us
+// where eight take 78, captured and replayed: 8 sequences of 100..9,000 tokens, 25 nodes, 16
+// query heads of 128).
 constexpr int waves_of(int NC) { return NC > 2 ? 4 : 8; }
 constexpr int kKeys = 32;          // keys per tile
-// Tiles per part, up to kMaxParts of them.  Of 32, 64 and 128: 38, 32 and 51 us for 61 nodes on
-// 30,011 tokens, 40, 37 and 53 for 32 sequences of 500..5,000, 115, 123 and 117 for 32 nodes on
-// 16 of 4,096..16,384 (fp32).
+// Tiles per part, up to kMaxParts of them.  Of 32, 64 and 128 (captured and replayed): 55, 54
+// and 80 us for 61 nodes on 30,011 tokens, 53, 52 and 76 for 32 sequences of 500..5,000, 129, 136
+// and 133 for 32 nodes on 16 of 4,096..16,384, 70, 71 and 95 for the case of 128 channels above.
 constexpr int kPartTiles = 64;
 constexpr int kMaxParts = 32;
 constexpr int kMaxNodes = 1024;
@@ -486,8 +490,9 @@ __device__ __forceinline__ void attend(const Params &p, const Seq &s, Smem &sm, 
   }
 }
 
-// LONG: parts of several turns (tables of more than 65,536 tokens); their loop costs registers,
-// 49 us where 45 do without it for 61 nodes on 30,011 tokens.
+// LONG: parts of several turns (tables of more than 65,536 tokens).  Their loop costs registers:
+// 55 us where 54 do without it for 61 nodes on 30,011 tokens, 139.5 for 136 (the 16 contexts
+// above), 74.5 for 71.5 (128 channels), captured and replayed.
 template <int NC, bool LONG>
 __global__ __launch_bounds__(waves_of(NC) * 64) __attribute__((amdgpu_waves_per_eu(NC > 2 ? 2 : 4))) void
 tree_attn_kernel(Params p) {
@@ -512,7 +517,8 @@ tree_attn_kernel(Params p) {
   const int rows = s.nodes * p.nrep;
   if (group * kWaves * 32 >= rows || part >= s.parts) return;
   auto take = [&](int turn, int tid) {
-    // (one wave a row tile throughout: 7.1 us where these take 6.2 for 8 nodes on 128 tokens)
+    // (one wave a row tile throughout: 54.6 us where these take 51.6 for 32 sequences of
+    // 500..5,000 tokens, captured and replayed; 8 nodes on 128 tokens and wide trees the same)
     if (rows > 16 * kWaves) attend<1, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
     else if (rows > 8 * kWaves) attend<2, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);
     else if (kWaves == 4 || rows > 4 * kWaves) attend<4, NC>(p, s, sm, n, unit, group, part, turn, wave, tid);

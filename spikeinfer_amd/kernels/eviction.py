@@ -136,7 +136,7 @@ def evict_cache(
         block_tables: ``int32 [N, max_blocks]``; seq_lens ``int32 [N]``.
         dst_tables: ``int32 [N, blocks]``, where the kept words go; by default the
             sequences' own blocks (which no other sequence may share).  These blocks must
-            be none that the call reads.
+            be none that the call reads, and lie in the cache (words for others are dropped).
         mass_out: where the kept masses go (0 behind them); by default ``mass`` itself, else a
             tensor apart from it.
 
