@@ -52,7 +52,7 @@ const char *spk_last_error(void);
 /* ABI version, bumped on any signature change and any new entry point (2: spk_decode_advance
  * draws; 3: spk_decode_attn_combine takes the partials size, spk_norm_* GEMMs; 4: spk_prefill_attn,
  * spk_qkv_rope_lif_pack_kv; 5: spk_tree_attn, spk_tree_masks, spk_accept_tree, spk_key_mass, spk_evict). */
-#define SPK_ABI_VERSION 5
+#define SPK_ABI_VERSION 6
 int spk_abi_version(void);
 
 /*
@@ -733,6 +733,78 @@ int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_stri
               int64_t dt_stride0, int64_t dt_stride1, int max_dst_blocks, const int32_t *seq_lens,
               int32_t *new_lens, int32_t *keep, int budget, int sinks, int recent, int T, int N,
               int Hkv, int head_dim, int block_size, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Speculative decoding: products in 8-bit integers for a drafter, the distributions that
+ * tokens are drawn from, and the verification of sampled drafts.  No counterpart in the
+ * reference, which decodes one token a step with bf16 weights.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Linear layer in 8-bit integers with a scale for every row of x and of W:
+ *   s = max |x| / 127, q = rint(x / s) (both quotients rounded to fp32; s = 0: q = 0),
+ *   y[m, n] = s_x[m] s_w[n] sum_k q_x[m, k] q_w[n, k] + bias[n]
+ * The integer sum is exact; scales and bias are fp32, rounded once to y's type.  A row of x
+ * that holds an infinity or a NaN gives a row of NaN, a row of W a column.
+ *   w, x, bias, y  F32, F16 or BF16 each, channel stride 1, rows at their strides; rows of y
+ *            must not lie on one another, nor y on x
+ *   packed   spk_linear_int8_packed_bytes(N, K) bytes, 16-byte aligned, and scales float
+ *            [N rounded up to 16]: written by spk_linear_int8_pack, once per weight
+ *   workspace spk_linear_int8_workspace_bytes(M, N, K) bytes, 16-byte aligned
+ * K <= 131072 (the sums are 32 bits), M <= 2^30 (SPK_EUNSUPPORTED beyond).
+ */
+size_t spk_linear_int8_packed_bytes(int N, int K);
+int spk_linear_int8_pack(const void *w, int w_dtype, int64_t w_stride, int N, int K, void *packed,
+                         float *scales, void *stream);
+size_t spk_linear_int8_workspace_bytes(int64_t M, int N, int K);
+int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, const void *packed,
+                    const float *scales, const void *bias, int bias_dtype, void *y, int y_dtype,
+                    int64_t y_stride, int64_t M, int N, int K, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/*
+ * The distribution that spk_sample draws a row's token from, without penalties: x = logits /
+ * temperature (rounded to fp32, finite where the logit is), tokens ordered by x descending, then index ascending; of
+ * them stay those with exp(x - max) >= min_p, of these the first top_k, of these the ones
+ * before which less than top_p of their sum stands.  A greedy row (temperature < 1e-5) is 1 at
+ * its first largest logit.  A row without a logit above -infinity (all masked, NaN) is all
+ * zeros; a NaN has probability 0; of infinite logits all count the same, others nothing.
+ *   logits   [rows, vocab] at row_stride, vocab stride 1, vocab <= 262144
+ *   temperature float [rows]; top_k int32, top_p and min_p float [rows], or NULL: off
+ *   probs    float [rows, vocab] at out_stride
+ *   workspace spk_sample_probs_workspace_bytes(rows, vocab) bytes, 16-byte aligned (NULL
+ *            when that is 0)
+ */
+size_t spk_sample_probs_workspace_bytes(int rows, int vocab);
+int spk_sample_probs(const void *logits, int logits_dtype, int64_t row_stride, int rows, int vocab,
+                     const float *temperature, const int32_t *top_k, const float *top_p,
+                     const float *min_p, float *probs, int64_t out_stride, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/*
+ * Which drafted tokens stay, by given random numbers.  Rows, parents and starts as
+ * spk_accept_tree.  From row 0 the walk tests the children of its row in order: with the
+ * row's target distribution p and the drafter's q, w = max(p - A q, 0) and c the sum of w (A = 0, c
+ * = 1 at first), child i with token x stays if uniforms[i] q(x) c < w(x) (the walk goes there,
+ * with that row's p and q), and else A grows by c.  `distinct`: a row's children were drawn
+ * without replacement; c is divided by 1 minus q's sum over the children before.  Where no
+ * child stays, the token is the first whose cumulative w exceeds uniforms[first row of
+ * the tree] times the sum (w = p where nothing is left of it).
+ *   target_probs, draft_probs float [rows, V] at their strides, vocabulary stride 1; draft_probs
+ *            of rows without children are not read
+ *   uniforms float [rows] in [0, 1)
+ *   targets  int64 [rows]: for rows of the path the token after them, as spk_accept_tree
+ *            takes it, -1 for the other rows of a tree (and where p has no weight at all); rows
+ *            of no sequence are left as they were
+ *   workspace spk_verify_tree_workspace_bytes(N, V) bytes, 8-byte aligned
+ * max_nodes <= 1024, N <= 65535.
+ */
+size_t spk_verify_tree_workspace_bytes(int N, int V);
+int spk_verify_tree(const int64_t *tokens, const int32_t *parents, const float *target_probs,
+                    int64_t target_stride, const float *draft_probs, int64_t draft_stride,
+                    const float *uniforms, const int32_t *row_starts, int64_t rows, int N,
+                    int max_nodes, int V, int distinct, int64_t *targets, void *workspace,
+                    size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -29,7 +29,7 @@ _DTYPE_CODES = {
     torch.int32: SPK_I32,
 }
 
-ABI_VERSION = 5  # SPK_ABI_VERSION
+ABI_VERSION = 6  # SPK_ABI_VERSION
 DECODE_ATTN_SCRATCH_BYTES = 16 << 20  # SPK_DECODE_ATTN_SCRATCH_BYTES
 
 _i64p = ctypes.POINTER(ctypes.c_int64)
@@ -152,6 +152,17 @@ _SIGNATURES = {
     "spk_evict": (_i32, [
         ctypes.c_char_p, _i32, _i64p, _i64, _vp, _i64p, _vp, _i64p, _i64, _vp, _i64, _i64, _i32, _vp,
         _i64, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "spk_linear_int8_packed_bytes": (_sz, [_i32, _i32]),
+    "spk_linear_int8_pack": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "spk_linear_int8_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "spk_linear_int8": (_i32, [
+        _vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "spk_sample_probs_workspace_bytes": (_sz, [_i32, _i32]),
+    "spk_sample_probs": (_i32, [
+        _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
+    "spk_verify_tree_workspace_bytes": (_sz, [_i32, _i32]),
+    "spk_verify_tree": (_i32, [
+        _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -5,26 +5,13 @@
 // sequence's last token, the rest hang below it.  Both walks follow that order (a
 // parent's number is lower, a child's higher), so they end whatever the numbers are.
 #include "common.hpp"
+#include "draft_rows.hpp"
 
 namespace spk {
 namespace draft {
 
-constexpr int kMaxNodes = 1024;
 constexpr int kMaxLayers = 64;  // layers a launch (kernel arguments)
 constexpr int kThreads = 256;
-
-struct Rows {
-  int64_t first;
-  int count;
-};
-
-__device__ __forceinline__ Rows rows_of(const int32_t *starts, int n, int64_t rows, int max_nodes) {
-  Rows r;
-  r.first = min<int64_t>(max(starts[n], 0), rows);
-  const int64_t end = min(max<int64_t>(starts[n + 1], r.first), rows);
-  r.count = static_cast<int>(min<int64_t>(end - r.first, max_nodes));
-  return r;
-}
 
 // A thread a (row, mask word): it follows the row's parents and keeps the bits of its
 // word.  Latency only: depth dependent loads, from the L2 after the first.

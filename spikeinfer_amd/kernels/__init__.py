@@ -3,16 +3,20 @@
 The operators launch HIP kernels on gfx950 through the C ABI in
 include/spikeinfer_amd.h and have no CPU fallback.  The ``*_ref`` /
 ``*_cpu`` names (reference_paths.py) are the reference's eager-torch paths,
-restated; the operators never call them.  draft_tree.py and eviction.py go beyond
-the reference: drafted trees, and a cache kept within a budget.
+restated; the operators never call them.  draft_tree.py, eviction.py and int8_linear.py go
+beyond the reference: drafted trees, a cache kept within a budget, and products in 8-bit
+integers.
 """
 from .draft_tree import (
     accept_draft_tree,
     draft_tree_masks,
     paged_spike_attn_tree,
     tree_attn_workspace_bytes,
+    verify_draft_tree,
+    verify_workspace_bytes,
 )
 from .eviction import evict_cache, key_mass_workspace_bytes, paged_spike_attn_key_mass
+from .int8_linear import Int8Weight, linear_int8, linear_int8_workspace_bytes, pack_linear_int8
 from .lif import lif_multistep, lif_pack_write, lif_pack_write_sites, validate_thresholds
 from .packing import (
     BITS_PER_WORD,
@@ -67,4 +71,10 @@ __all__ = [
     "paged_spike_attn_key_mass",
     "key_mass_workspace_bytes",
     "evict_cache",
+    "verify_draft_tree",
+    "verify_workspace_bytes",
+    "Int8Weight",
+    "pack_linear_int8",
+    "linear_int8",
+    "linear_int8_workspace_bytes",
 ]

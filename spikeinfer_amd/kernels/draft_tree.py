@@ -11,6 +11,9 @@ in the step's buffers until :func:`accept_draft_tree` moves the accepted path's.
     out = paged_spike_attn_tree(q, k, v, k_cache, v_cache, tables, context_lens, row_starts, masks, ...)
     path, count, after = accept_draft_tree(tokens, parents, targets, row_starts, max_nodes, drafts, layers, ...)
 
+``targets``, the model's token after each row, are drawn from its logits row by row, or, where
+the drafts were sampled too, by :func:`verify_draft_tree`, which keeps more of them.
+
 Lengths, starts, parents and masks are device tensors that the kernels read, so a
 captured step takes other trees on replay.  The reference decodes one token a step;
 these have no counterpart there.
@@ -176,6 +179,94 @@ def draft_tree_masks(parents: torch.Tensor, row_starts: torch.Tensor, max_nodes:
     _lib.check(_lib.launch("spk_tree_masks", dev, parents.data_ptr(), row_starts.data_ptr(), R, n_seqs, max_nodes,
                            masks.data_ptr(), masks.shape[1], depths.data_ptr()), "draft_tree_masks")
     return masks, depths
+
+
+@functools.lru_cache(maxsize=256)
+def verify_workspace_bytes(n_seqs: int, vocab: int) -> int:
+    """Scratch bytes :func:`verify_draft_tree` needs for this many trees."""
+    return int(_lib.load().spk_verify_tree_workspace_bytes(n_seqs, vocab))
+
+
+def _distribution(name: str, t: torch.Tensor, rows: int) -> None:
+    if t.ndim != 2 or t.shape[0] < rows or t.dtype != torch.float32 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be float32 [{rows}, vocab] with a contiguous vocab axis, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+
+
+def verify_draft_tree(
+    tokens: torch.Tensor,
+    parents: torch.Tensor,
+    target_probs: torch.Tensor,
+    draft_probs: torch.Tensor,
+    uniforms: torch.Tensor,
+    row_starts: torch.Tensor,
+    max_nodes: int,
+    distinct: bool = False,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The tokens after the rows of every tree's accepted path, where drafts were sampled:
+    what :func:`accept_draft_tree` takes as ``targets``.  The path's tokens and the one behind it
+    are distributed as tokens drawn one by one from the target's distributions.
+
+    From row 0 a row's children are tested in order.  With p the target's distribution after the
+    row and q the one its children were drawn from, a child's token x stays with probability
+    ``min(1, w(x) / (c q(x)))``, where ``w = max(p - A q, 0)`` sums to c (A = 0, c = 1 for the first;
+    a child that does not stay adds c to A); where none stays the token is drawn from w.
+
+    Args:
+        tokens: ``int64 [R]`` the rows' tokens (row 0's: the sequence's last).
+        parents, row_starts, max_nodes: as :func:`draft_tree_masks`.
+        target_probs: ``float32 [R, V]`` the target's distribution of the token after each row
+            (:func:`sampling_probs`).
+        draft_probs: ``float32 [R, V]`` the distribution that each row's children were drawn
+            from; rows without children are not read.
+        uniforms: ``float32 [R]`` in [0, 1): a row's decides whether its token stays, row 0's draws
+            the token behind the path.
+        distinct: a row's children were drawn without replacement (otherwise one independently of
+            the other).
+        out: optional ``int64 [R]`` (needed for graph capture); rows of no sequence are left
+            as they were (-1 in a new tensor).
+        workspace: optional ``uint8`` scratch of :func:`verify_workspace_bytes`; calls that may run
+            at once need one each.
+
+    Returns ``out``: the token after each row of the path, -1 for other rows, and where the
+    target gives no token any weight.
+    """
+    dev = _lib.require_gpu(tokens, parents, target_probs, draft_probs, uniforms, row_starts, out, workspace)
+    _max_nodes(max_nodes)
+    R, n_seqs = tokens.numel(), row_starts.numel() - 1
+    if n_seqs < 0:
+        raise ValueError("row_starts must be [N + 1]")
+    tokens = _vector("tokens", tokens, R, torch.int64)
+    parents = _vector("parents", parents, R, torch.int32)
+    uniforms = _vector("uniforms", uniforms, R, torch.float32)
+    row_starts = _vector("row_starts", row_starts, n_seqs + 1, torch.int32)
+    _distribution("target_probs", target_probs, R)
+    _distribution("draft_probs", draft_probs, R)
+    V = target_probs.shape[1]
+    if draft_probs.shape[1] != V:
+        raise ValueError(f"draft_probs have {draft_probs.shape[1]} tokens, target_probs {V}")
+    if out is None:
+        out = torch.full((R,), -1, dtype=torch.int64, device=dev)
+    elif tuple(out.shape) != (R,) or out.dtype != torch.int64 or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous int64 [{R}], got {out.dtype} {tuple(out.shape)}")
+    if n_seqs == 0 or R == 0:
+        return out
+    need = verify_workspace_bytes(n_seqs, V)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+        raise ValueError(f"workspace must hold {need} contiguous bytes")
+    _lib.check(
+        _lib.launch(
+            "spk_verify_tree", dev, tokens.data_ptr(), parents.data_ptr(), target_probs.data_ptr(),
+            target_probs.stride(0), draft_probs.data_ptr(), draft_probs.stride(0), uniforms.data_ptr(),
+            row_starts.data_ptr(), R, n_seqs, max_nodes, V, int(bool(distinct)), out.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size()),
+        "verify_draft_tree",
+    )
+    return out
 
 
 def _same_layout(name: str, pairs, dev) -> tuple[torch.Size, tuple[int, ...]]:

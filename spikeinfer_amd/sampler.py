@@ -170,6 +170,63 @@ def sample_workspace_bytes(rows: int) -> int:
     return int(_lib.load().spk_sample_workspace_bytes(rows))
 
 
+def sampling_probs_workspace_bytes(rows: int, vocab: int) -> int:
+    """Scratch bytes :func:`sampling_probs` needs for this shape."""
+    return int(_lib.load().spk_sample_probs_workspace_bytes(rows, vocab))
+
+
+def sampling_probs(
+    logits: torch.Tensor,
+    temperature: torch.Tensor,
+    top_k: torch.Tensor | None = None,
+    top_p: torch.Tensor | None = None,
+    min_p: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The distribution that :func:`sample_tokens` draws each row's token from, ``float32
+    [rows, vocab]``: what :func:`~spikeinfer_amd.kernels.verify_draft_tree` takes.
+
+    ``logits [rows, vocab]`` and the per-row arrays are as :func:`sample_tokens` takes them,
+    penalties aside (they depend on the tokens before a row, which a step's drafted rows do not
+    share: apply them to the logits).  Cuts keep a prefix of the tokens ordered by value
+    descending, index ascending, decided in 64 bits (where the sampler's fp32 weights put two
+    prefixes on the other side of a border, one token differs).  A greedy row is 1 at its first
+    largest logit; a row with no logit above -infinity is all zeros; NaN has probability 0.
+
+    ``out``: optional ``float32 [rows, vocab]``, vocab contiguous; ``workspace``: optional ``uint8``
+    scratch of :func:`sampling_probs_workspace_bytes` (calls that may run at once need one each).
+    """
+    dev = _lib.require_gpu(logits, temperature, top_k, top_p, min_p, out, workspace)
+    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] with a contiguous vocab axis")
+    rows, vocab = logits.shape
+    for name, t, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None and (t.dtype != dt or t.numel() < rows or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dt} tensor of {rows} entries")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
+    elif tuple(out.shape) != (rows, vocab) or out.dtype != torch.float32 or (vocab > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be float32 {(rows, vocab)} with a contiguous vocab axis")
+    need = sampling_probs_workspace_bytes(rows, vocab)
+    have = 0
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace is not None:
+        have = workspace.numel() * workspace.element_size()
+        if have < need or not workspace.is_contiguous():
+            raise ValueError(f"workspace must hold {need} contiguous bytes")
+    _lib.check(
+        _lib.launch(
+            "spk_sample_probs", dev, logits.data_ptr(), _lib.dtype_code(logits.dtype), logits.stride(0), rows, vocab,
+            temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p), out.data_ptr(), out.stride(0),
+            _lib.ptr(workspace), have),
+        "sampling_probs",
+    )
+    return out
+
+
 class BatchSampler:
     """Device-resident sampling state for a batch of up to ``max_rows`` rows.
 
@@ -275,6 +332,16 @@ class BatchSampler:
         if record:
             self.record(n)
         return self.tokens[:n]
+
+    def probs(self, logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The distributions that :meth:`sample` draws the rows' tokens from, ``float32 [n, vocab]``
+        (:func:`sampling_probs`).  Penalties depend on the tokens before a row: rows that ask
+        for them are refused."""
+        n = logits.shape[0]
+        if any(p.repetition_penalty != 1.0 or p.presence_penalty or p.frequency_penalty for p in self.params[:n]):
+            raise ValueError("probs takes no penalties: apply them to the logits")
+        logits = self._pre_filter(logits, n)
+        return sampling_probs(logits, self.temperature[:n], self.top_k[:n], self.top_p[:n], self.min_p[:n], out)
 
     def record(self, n: int) -> None:
         """Appends ``tokens[:n]`` to the history on the device."""
