@@ -8,15 +8,19 @@
 // largest): sums do not depend on the order they are made in, and a cut falls where exact
 // arithmetic has it unless two numbers agree to 11 digits.
 //
-// A workgroup a row.  Cuts keep few tokens as a rule, so the row is read twice, once for its
-// largest and once for the candidates, those at or above a bound that the threads' maxima
-// give; the cuts are then found among the candidates in LDS, the row is filled with zeros and
-// the kept tokens are put in their places.  A cut by top_p needs the sum over the whole row:
-// candidates count with their exact weight, the rest with fp32 exponentials, whose error is
-// bounded; where the cut could fall elsewhere within that bound, or outside the candidates,
-// the row goes the long way: a histogram of the exact weights over the row, then the tokens of
-// the bin that holds the cut as candidates.  Without cuts the row is read for its largest,
-// for the sum, and for the result.
+// Two launches, both a workgroup a slice of a row.  Cuts keep few tokens as a rule, so:
+//   * the first (slice_kernel) holds its slice in registers, fills its part of the result with
+//     zeros and lists its candidates, the logits at or above a bound that so many of the
+//     threads' maxima reach, with the sum of the others' weights in fp32;
+//   * the second (row_kernel) finds the cuts among the candidates of a row's slices and puts
+//     the kept tokens in their places.  A cut by top_p needs the sum over the whole row:
+//     candidates count with their exact weight, the others with the fp32 sums, whose error is
+//     bounded; where the cut could fall elsewhere within that bound, or below a slice's bound,
+//     the row goes the long way, through histograms of the exact weights over the row.
+// A row without cuts gets its sum from the first launch and its values from the second.
+#include <algorithm>
+#include <cmath>
+
 #include "common.hpp"
 #include "lif_math.hpp"
 
@@ -25,28 +29,20 @@ namespace probs {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kSliceThreads = 512;
+constexpr int kSliceVecs = 5;     // 16-byte vectors of a slice a thread holds
+constexpr int kRowThreads = 512;
 constexpr int kIndexBits = 18;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr float kGreedyTemp = 1e-5f;
+constexpr float kMost = 3.402823466e38f;         // the largest fp32 number
 constexpr double kMassScale = 17592186044416.0;  // 2^44: 2^18 weights of at most 1 fit 64 bits
-constexpr int kCand = 4096;                      // candidates
-constexpr int kBins = 2048;                      // 11-bit digits
-constexpr int kBinsPerThread = kBins / kThreads;
-constexpr int kMostK = 640;                      // largest top_k whose bound the threads' maxima give
-constexpr int kOpenReach = 960;                  // maxima above the bound without one: about 2,800 candidates
-
-struct Shared {
-  u64 cand[kCand];  // order keys
-  u64 hist[kBins];
-  u64 wave[kWaves];
-  double dwave[kWaves];
-  u64 digit, above, in_digit;
-  uint32_t tmax[kThreads];
-  uint32_t bound;
-  int count;
-};
+constexpr int kCand = 4096;                      // candidates of a row
+constexpr int kBins = 1024;              // of a row's histogram: 10-bit digits
+constexpr int kBinsPerThread = kBins / kRowThreads;
+constexpr int kRank = 256;                       // candidates that are ranked one against the other
+constexpr int kMaxSlices = kMaxVocab / (4 * kSliceVecs * kSliceThreads) + 2;  // of a row
+constexpr int kMostK = 2048;                     // top_k beyond: the long way
 
 // Larger: earlier in the order.
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -62,10 +58,6 @@ __device__ __forceinline__ u64 order_key(float x, int i) {
 __device__ __forceinline__ float order_value(u64 k) { return key_value(static_cast<uint32_t>(k >> kIndexBits)); }
 __device__ __forceinline__ int order_index(u64 k) { return kMaxVocab - 1 - static_cast<int>(k & (kMaxVocab - 1)); }
 
-__device__ __forceinline__ u64 shfl_u64(u64 v, int lane) {
-  const uint32_t lo = __shfl(static_cast<uint32_t>(v), lane), hi = __shfl(static_cast<uint32_t>(v >> 32), lane);
-  return (static_cast<u64>(hi) << 32) | lo;
-}
 __device__ __forceinline__ u64 shfl_xor_u64(u64 v, int d) {
   const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), d), hi = __shfl_xor(static_cast<uint32_t>(v >> 32), d);
   return (static_cast<u64>(hi) << 32) | lo;
@@ -75,177 +67,140 @@ __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
   return (static_cast<u64>(hi) << 32) | lo;
 }
 
-// Over the workgroup, to every thread.
-template <class Op>
-__device__ __forceinline__ u64 block_reduce(u64 v, Shared &sh, Op op) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = op(v, shfl_xor_u64(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh.wave[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) v = op(v, sh.wave[w]);
-  return v;
-}
-__device__ __forceinline__ double block_sum(double v, Shared &sh) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.dwave[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = sh.dwave[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) v += sh.dwave[w];
-  return v;
-}
-
 // A logit over the temperature; what is finite stays finite (a mask of the type's lowest value
 // is no -infinity below a temperature of 1).  inv = 1 / temp in fp64: the quotient of two
 // fp32 numbers lies at least 2^-49 of itself from the middle between two fp32 numbers, and the
 // product is off by at most 2^-52, so its rounding is the quotient's.
 __device__ __forceinline__ float quotient(float v, double inv) {
   const float x = static_cast<float>(static_cast<double>(v) * inv);
-  return fabsf(x) == INFINITY && fabsf(v) != INFINITY ? copysignf(3.402823466e38f, v) : x;
+  return fabsf(x) == INFINITY && fabsf(v) != INFINITY ? copysignf(kMost, v) : x;
 }
 
 // A bound at or below every logit whose quotient is `x`, that of `bound`.
 __device__ __forceinline__ float same_quotient(float bound, float x, float temp) {
   if (fabsf(bound) == INFINITY) return bound;
-  if (x == 3.402823466e38f) bound = fminf(bound, x * temp);
-  if (x == -3.402823466e38f) return -INFINITY;
+  if (x == kMost) bound = fminf(bound, x * temp);
+  if (x == -kMost) return -INFINITY;
   return bound - fabsf(bound) * 0x1p-22f - temp * 0x1p-148f;
 }
 
+// exp(logit / temp - x_most) in fp32; the quotient with one correction (inv: fp32 of 1 / temp).
+__device__ __forceinline__ float power(float v, float temp, float inv, float x_most) {
+  const float q = v * inv;
+  float x = __builtin_fmaf(__builtin_fmaf(-q, temp, v), inv, q);
+  x = fabsf(q) < 1e30f ? x : quotient(v, 1.0 / static_cast<double>(temp));  // (and infinities, NaN)
+  return x == x ? expf(x == x_most ? 0.f : x - x_most) : 0.f;
+}
+
+enum Kind { kGreedy, kWhole, kCuts };
+
+// A row's parameters.
+struct Ask {
+  float temp, min_p, top_p;
+  int top_k;   // 0: none
+  double inv;  // 1 / temperature
+  double low;  // ln min_p
+  Kind kind;
+  bool open;  // a cut by top_p
+};
+
+struct Args {
+  const void *logits;
+  int64_t row_stride;
+  int V;
+  const float *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  float *out;
+  int64_t out_stride;
+  int S, cap;       // slices of a row, candidates of a slice
+  int groups;       // workgroups of a row in the second launch
+  int reach, most;  // threads whose maxima reach a slice's bound: without top_k; with the largest
+  struct Head *heads;  // [row][slice]
+  u64 *lists;          // [row][slice][cap]
+};
+
+// What a slice leaves for its row.
+struct Head {
+  int count;    // candidates; -1: more than fit
+  float most;   // the largest logit, -infinity: none
+  float whole;  // quotients from here on up are all listed
+  float rest;   // sum of exp(x - its most's x) over the others (rows without cuts: over all)
+};
+
+__device__ __forceinline__ Ask ask(const Args &a, int64_t r) {
+  Ask k;
+  k.temp = a.temperature[r];
+  k.min_p = a.min_p ? a.min_p[r] : 0.f;
+  const float tp = a.top_p ? a.top_p[r] : 1.f;
+  k.top_p = tp <= 0.f ? 0x1p-60f : tp;  // (the first token stays)
+  const int tk = a.top_k ? a.top_k[r] : -1;
+  k.top_k = tk > 0 && tk < a.V ? tk : 0;
+  k.inv = 1.0 / static_cast<double>(k.temp);
+  k.low = k.min_p > 0.f ? fmin(log(static_cast<double>(k.min_p)), 0.0) : -INFINITY;  // (the largest stays)
+  k.open = k.top_p < 1.f;
+  k.kind = !(k.temp >= kGreedyTemp) ? kGreedy : k.top_k || k.open || k.min_p > 0.f ? kCuts : kWhole;
+  return k;
+}
+
+// ---- slices --------------------------------------------------------------------------
+// A row's elements as 16-byte vectors of aligned memory: the first may begin before the row,
+// the last end behind it.
 template <int DT>
-struct Row {
+struct RowMem {
   typedef typename Elem<DT>::T E;
   static constexpr int W = Elem<DT>::kVec;
   typedef E Vec __attribute__((ext_vector_type(W)));
   const E *p;
-  int V;
-  double inv;     // 1 / temperature
-  double m, low;  // the largest x; ln min_p
+  int V, before;  // elements of the first vector that are not the row's
 
-  // f(index, logit) for every token, in no particular order; 16-byte loads, four in flight,
-  // between a head and a tail that are not aligned.
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    const int tid = threadIdx.x;
-    const int head = min(V, static_cast<int>((-(reinterpret_cast<uintptr_t>(p) / sizeof(E))) & (W - 1)));
-    if (tid < head) f(tid, elem_to_f32<DT>(p[tid]));
-    const int nv = (V - head) / W;
-    const Vec *pv = reinterpret_cast<const Vec *>(p + head);
-    auto one = [&](int v, const Vec &a) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const E e = a[j];
-        f(head + v * W + j, elem_to_f32<DT>(e));
-      }
-    };
-    int v = tid;
-    for (; v + 3 * kThreads < nv; v += 4 * kThreads) {
-      Vec a[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) a[u] = pv[v + u * kThreads];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) one(v + u * kThreads, a[u]);
-    }
-    for (; v < nv; v += kThreads) one(v, pv[v]);
-    const int t = head + nv * W + tid;
-    if (t < V) f(t, elem_to_f32<DT>(p[t]));
+  __device__ __forceinline__ RowMem(const Args &a, int64_t r) {
+    p = static_cast<const E *>(a.logits) + r * a.row_stride;
+    V = a.V;
+    before = static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(E)) & (W - 1);
   }
-  // The same with one copy of f, for passes that compute much (a workgroup waits for the
-  // instructions that it runs through once).
-  template <class F>
-  __device__ __forceinline__ void each_short(F f) const {
-#pragma unroll 1
-    for (int i0 = threadIdx.x; i0 < V; i0 += 4 * kThreads) {
-      E a[4];
+  static __device__ __forceinline__ E none() {  // a NaN
+    if constexpr (DT == SPK_F32) return __uint_as_float(0x7fc00000u);
+    else return static_cast<E>(0x7fff);
+  }
+  __device__ __forceinline__ int first(int v) const { return v * W - before; }  // index of a vector's first element
+  __device__ __forceinline__ Vec load(int v) const {
+    const int i = first(v);
+    if (i >= 0 && i + W <= V) return *reinterpret_cast<const Vec *>(p + i);
+    Vec a;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) a[u] = p[min(i0 + u * kThreads, V - 1)];
-#pragma unroll 1
-      for (int i = i0; i < V && i < i0 + 4 * kThreads; i += kThreads) {
-        f(i, elem_to_f32<DT>(a[0]));
-        a[0] = a[1];
-        a[1] = a[2];
-        a[2] = a[3];
-      }
-    }
-  }
-  __device__ __forceinline__ float x(float logit) const { return quotient(logit, inv); }
-  __device__ __forceinline__ double down(float x) const {
-    const double d = static_cast<double>(x) - m;
-    return static_cast<double>(x) == m ? 0.0 : d;  // (also where both are infinite)
-  }
-  __device__ __forceinline__ bool alive(float x) const { return down(x) >= low; }  // (a NaN is not)
-  __device__ __forceinline__ u64 mass(float x) const {
-    return static_cast<u64>(exp(down(x)) * kMassScale + 0.5);
+    for (int j = 0; j < W; ++j) a[j] = i + j >= 0 && i + j < V ? p[i + j] : none();
+    return a;
   }
 };
 
-// The bin of sh.hist, from the top, with above < target <= above + its content, `above` being
-// `base` and the bins over it, into sh.digit (kBins: none), sh.above and sh.in_digit.
-__device__ __forceinline__ void select_bin(Shared &sh, u64 base, double target) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int top = kBins - 1 - kBinsPerThread * tid;
-  u64 h[kBinsPerThread], sum = 0;
-#pragma unroll
-  for (int r = 0; r < kBinsPerThread; ++r) sum += h[r] = sh.hist[top - r];
-  u64 inc = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = shfl_up_u64(inc, d);
-    if (lane >= d) inc += o;
-  }
-  if (lane == 63) sh.wave[wave] = inc;
-  if (tid == 0) sh.digit = kBins;
-  __syncthreads();
-  u64 before = base + inc - sum;
-  for (int w = 0; w < wave; ++w) before += sh.wave[w];
-#pragma unroll
-  for (int r = 0; r < kBinsPerThread; ++r) {
-    if (h[r] && static_cast<double>(before) < target && target <= static_cast<double>(before + h[r])) {
-      sh.digit = top - r;
-      sh.above = before;
-      sh.in_digit = h[r];
-    }
-    before += h[r];
-  }
-  __syncthreads();
+// Places [i0, i1) of a row's result.
+__device__ __forceinline__ void fill_zeros(float *o, int i0, int i1, int threads) {
+  typedef float F4 __attribute__((ext_vector_type(4)));
+  o += i0;
+  const int n = i1 - i0, tid = threadIdx.x;
+  const int head = min(n, static_cast<int>((-(reinterpret_cast<uintptr_t>(o) / 4)) & 3));
+  if (tid < head) o[tid] = 0.f;
+  const int nv = (n - head) / 4;
+  F4 *ov = reinterpret_cast<F4 *>(o + head);
+  for (int v = tid; v < nv; v += threads) ov[v] = F4{0.f, 0.f, 0.f, 0.f};
+  const int t = head + 4 * nv + tid;
+  if (t < n) o[t] = 0.f;
 }
 
-// The smallest order key of the shortest prefix whose weights reach `target`, among the tokens
-// (order keys) that each(f) visits with a weight; 0 if they do not reach it.  Radix selection: 11-bit digits of the key, from the
-// first bit in which `lo` and `hi` (bounds of the keys) differ.
-template <class Each>
-__device__ __forceinline__ u64 prefix_cut(Shared &sh, u64 lo, u64 hi, double target, Each each) {
-  const u64 differ = lo ^ hi;
-  int bits = differ ? 64 - __clzll(static_cast<long long>(differ)) : 1;
-  u64 prefix = hi >> bits << bits, above = 0;
-  while (bits > 0) {
-    const int shift = max(bits - 11, 0);
-    const uint32_t mask = (1u << (bits - shift)) - 1u;
-    __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
-    __syncthreads();
-    each([&](u64 key, u64 w) {
-      if (w && key >> bits == prefix >> bits) atomicAdd(&sh.hist[static_cast<uint32_t>(key >> shift) & mask], w);
-    });
-    __syncthreads();
-    select_bin(sh, above, target);
-    if (sh.digit == kBins) return 0;
-    prefix |= sh.digit << shift;
-    above = sh.above;
-    bits = shift;
-  }
-  return prefix;
-}
+struct SliceShared {
+  float x[kCand];  // candidates: logit and index
+  int32_t i[kCand];
+  uint32_t tmax[kSliceThreads];
+  float wave[kSliceThreads / 64];
+  uint32_t bound;
+  int count, first;
+};
 
-// A key that at least `need` of the threads' maxima reach, and about as few as can be.
-__device__ __forceinline__ void find_bound(Shared &sh, uint32_t need) {
+// A key that at least `need` of the threads' maxima reach, and about as few as can be (0: fewer
+// threads have one).
+__device__ __forceinline__ void find_bound(SliceShared &sh, uint32_t need) {
   if (threadIdx.x < 64) {
-    constexpr int kPer = kThreads / 64;
+    constexpr int kPer = kSliceThreads / 64;
     uint32_t t[kPer], top = 0;
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
@@ -260,7 +215,7 @@ __device__ __forceinline__ void find_bound(Shared &sh, uint32_t need) {
       for (int q = 0; q < kPer; ++q) c += static_cast<uint32_t>(__popcll(__ballot(t[q] >= k)));
       return c;
     };
-    uint32_t lo = 0, hi = top;  // reach(lo) >= need; 0: every token
+    uint32_t lo = 0, hi = top;
     if (reach(1u) >= need) {
       lo = 1;
       if (reach(hi) >= need) lo = hi;
@@ -281,204 +236,636 @@ __device__ __forceinline__ void find_bound(Shared &sh, uint32_t need) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void probs_kernel(const void *logits, int64_t row_stride, int V,
-                                                         const float *temperature, const int32_t *top_k,
-                                                         const float *top_p, const float *min_p, float *out,
-                                                         int64_t out_stride) {
-  __shared__ Shared sh;
-  const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
-  Row<DT> row;
-  row.p = static_cast<const typename Elem<DT>::T *>(logits) + r * row_stride;
-  row.V = V;
-  const float temp = temperature[r];
-  row.inv = 1.0 / static_cast<double>(temp);
-  const float mp = min_p ? min_p[r] : 0.f, tp_given = top_p ? top_p[r] : 1.f;
-  const float tp = tp_given <= 0.f ? 0x1p-60f : tp_given;  // (the first token stays)
-  const int tk_given = top_k ? top_k[r] : -1, tk = tk_given > 0 && tk_given < V ? tk_given : 0;
-  const auto larger = [](u64 a, u64 b) { return a > b ? a : b; };
-  const auto plus = [](u64 a, u64 b) { return a + b; };
-  float *o = out + r * out_stride;
-  // 0 to every place; the kept tokens' places are written behind a barrier
-  auto zeros = [&] {
-    typedef float F4 __attribute__((ext_vector_type(4)));
-    const int head = min(V, static_cast<int>((-(reinterpret_cast<uintptr_t>(o) / 4)) & 3));
-    if (tid < head) o[tid] = 0.f;
-    const int nv = (V - head) / 4;
-    F4 *ov = reinterpret_cast<F4 *>(o + head);
-    for (int v = tid; v < nv; v += kThreads) ov[v] = F4{0.f, 0.f, 0.f, 0.f};
-    const int t = head + 4 * nv + tid;
-    if (t < V) o[t] = 0.f;
+__global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
+  typedef RowMem<DT> Mem;
+  typedef typename Mem::E E;
+  constexpr int W = Mem::W;
+  __shared__ SliceShared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t r = blockIdx.x / a.S;
+  const int s = static_cast<int>(blockIdx.x % a.S);
+  const Mem row(a, r);
+  const int v0 = s * kSliceVecs * kSliceThreads;
+  typename Mem::Vec reg[kSliceVecs];
+#pragma unroll
+  for (int q = 0; q < kSliceVecs; ++q) reg[q] = row.load(v0 + q * kSliceThreads + tid);
+  const Ask k = ask(a, r);
+  Head *head = a.heads + r * a.S + s;
+  if (k.kind != kWhole)
+    fill_zeros(a.out + r * a.out_stride, min(max(row.first(v0), 0), a.V),
+               min(max(row.first(v0 + kSliceVecs * kSliceThreads), 0), a.V), kSliceThreads);
+
+  // f(index, logit)
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int q = 0; q < kSliceVecs; ++q)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const E e = reg[q][j];
+        f(row.first(v0 + q * kSliceThreads + tid) + j, elem_to_f32<DT>(e));
+      }
   };
-
-  // ---- the largest logit; each thread's largest as a key (0: none, a NaN is none) ----
-  uint32_t mk = 0;
-  row.each([&](int, float v) { mk = max(mk, v == v ? value_key(v) : 0u); });
-  sh.tmax[tid] = mk;
-  const uint32_t best = static_cast<uint32_t>(block_reduce(mk, sh, larger));
-  if (best <= value_key(-INFINITY)) {  // nothing to draw from
-    zeros();
-    return;
-  }
-  const float most = key_value(best);
-  if (!(temp >= kGreedyTemp)) {  // greedy: the first of the largest
-    zeros();
-    int first = V;
-    row.each([&](int i, float v) { first = v == most ? min(first, i) : first; });
-    first = static_cast<int>(block_reduce(static_cast<u64>(first), sh, [](u64 a, u64 b) { return a < b ? a : b; }));
-    if (tid == 0) o[first] = 1.f;
-    return;
-  }
-  row.m = row.x(most);
-  row.low = mp > 0.f ? fmin(log(static_cast<double>(mp)), 0.0) : -INFINITY;  // (the largest stays)
-  const bool open = tp < 1.f;
-
-  // ---- no cut: the sum, then the result ----
-  if (!tk && !open && !(mp > 0.f)) {
-    double z = 0.0;
-    row.each([&](int, float v) {
-      const double d = row.down(row.x(v));
-      if (d >= -INFINITY) z += static_cast<double>(expf(static_cast<float>(d)));
-    });
-    z = block_sum(z, sh);
-    const float scale = static_cast<float>(1.0 / z);
-    row.each([&](int i, float v) {
-      const double d = row.down(row.x(v));
-      o[i] = d >= -INFINITY ? expf(static_cast<float>(d)) * scale : 0.f;
-    });
-    return;
-  }
-
-  // ---- candidates: logits at or above a bound ----
-  // Every token that a cut may keep is among them: of top_k's prefix as many are there as
-  // the threads' maxima say, of min_p's all.  Without either, a prefix of about 2,800.
-  u64 cut = 0, Z = 0;
-  if (tk <= kMostK) {
-    const bool rest_counts = open && !tk && !(mp > 0.f);
-    float bound = -INFINITY;
-    if (tk || rest_counts) {
-      find_bound(sh, tk ? tk : kOpenReach);
-      if (sh.bound > value_key(-INFINITY)) bound = key_value(sh.bound);
-    }
-    const float whole = row.x(bound);  // from here on up no token is missing
-    bound = same_quotient(bound, whole, temp);
-    if (mp > 0.f) {
-      const double x = row.m + row.low;
-      const float least = x <= -3.402823466e38 ? -INFINITY : static_cast<float>(x * static_cast<double>(temp));
-      bound = fmaxf(bound, fabsf(least) == INFINITY ? least : least - fabsf(least) * 0x1p-20f - temp * 0x1p-148f);
-    }
-    if (tid == 0) sh.count = 0;
+  float most = -INFINITY;
+  each([&](int, float v) { most = fmaxf(most, v); });
+  sh.tmax[tid] = most > -INFINITY ? value_key(most) : 0u;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  if (lane == 0) sh.wave[wave] = most;
+  if (tid == 0) sh.count = 0, sh.first = kMaxVocab;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSliceThreads / 64; ++w) most = fmaxf(most, sh.wave[w]);
+  auto sum = [&](float v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     __syncthreads();
-    const float c1 = static_cast<float>(row.inv * 1.4426950408889634);
-    const float c2 = static_cast<float>(row.m * 1.4426950408889634);
-    float rest = 0.f;
-    row.each([&](int i, float v) {
+    if (lane == 0) sh.wave[wave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSliceThreads / 64; ++w) v += sh.wave[w];
+    return v;
+  };
+  if (most == -INFINITY) {
+    if (tid == 0) *head = Head{0, most, -INFINITY, 0.f};
+    return;
+  }
+  if (k.kind == kGreedy) {
+    int first = kMaxVocab;
+    each([&](int i, float v) { first = v == most ? min(first, i) : first; });
+    atomicMin(&sh.first, first);
+    __syncthreads();
+    if (tid == 0) *head = Head{sh.first, most, -INFINITY, 0.f};
+    return;
+  }
+  const float x_most = quotient(most, k.inv);
+  if (k.kind == kWhole) {
+    const float inv = 1.f / k.temp;
+    float z = 0.f;
+    each([&](int, float v) { z += power(v, k.temp, inv, x_most); });
+    z = sum(z);
+    if (tid == 0) *head = Head{0, most, -INFINITY, z};
+    return;
+  }
+  // ---- candidates ----
+  if (k.top_k > kMostK) {
+    if (tid == 0) *head = Head{-1, most, INFINITY, 0.f};
+    return;
+  }
+  float bound = -INFINITY;
+  if (k.top_k || !(k.min_p > 0.f)) {
+    find_bound(sh, k.top_k ? min(k.top_k, a.most) : a.reach);
+    if (sh.bound > value_key(-INFINITY)) bound = key_value(sh.bound);
+  }
+  float whole = quotient(bound, k.inv);
+  bound = same_quotient(bound, whole, k.temp);
+  if (k.min_p > 0.f) {  // those below ln min_p under this slice's largest are none of the row's
+    const double x = static_cast<double>(x_most) + k.low;
+    const float least = x <= -static_cast<double>(kMost) ? -INFINITY : static_cast<float>(x * static_cast<double>(k.temp));
+    const float lower = fabsf(least) == INFINITY ? least : least - fabsf(least) * 0x1p-20f - k.temp * 0x1p-148f;
+    if (lower > bound || !k.top_k) {
+      bound = lower;
+      whole = -INFINITY;  // of the survivors none is missing
+    }
+  }
+  int mine = 0;
+  float rest = 0.f;
+  if (k.open && !k.top_k && !(k.min_p > 0.f)) {
+    const float c1 = static_cast<float>(k.inv * 1.4426950408889634);
+    const float c2 = static_cast<float>(static_cast<double>(x_most) * 1.4426950408889634);
+    each([&](int, float v) {
+      mine += v >= bound ? 1 : 0;
+      rest += __builtin_amdgcn_exp2f(__builtin_fmaf(v < bound ? v : -INFINITY, c1, -c2));
+    });
+  } else {
+    each([&](int, float v) { mine += v >= bound ? 1 : 0; });
+  }
+  int at = mine ? atomicAdd(&sh.count, mine) : 0;
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= a.cap) {
+    each([&](int i, float v) {
       if (v >= bound) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kCand) sh.cand[at] = order_key(row.x(v), i);
-      } else if (rest_counts && v == v) {
-        rest += __builtin_amdgcn_exp2f(v * c1 - c2);
+        sh.x[at] = v;
+        sh.i[at++] = i;
       }
+    });
+  }
+  rest = sum(rest);
+  if (n <= a.cap) {
+    u64 *list = a.lists + (r * a.S + s) * a.cap;
+    for (int j = tid; j < n; j += kSliceThreads) list[j] = order_key(quotient(sh.x[j], k.inv), sh.i[j]);
+  }
+  if (tid == 0) *head = Head{n <= a.cap ? n : -1, most, whole, rest};
+}
+
+// ---- rows ----------------------------------------------------------------------------
+struct RowShared {
+  u64 key[kCand], mass[kCand];
+  u64 hist[kBins];
+  u64 wave[kRowThreads / 64];
+  Head head[kMaxSlices];
+  u64 digit, above, pick;
+  int count;
+};
+
+// Over the workgroup, to every thread.
+template <class Op>
+__device__ __forceinline__ u64 block_reduce(u64 v, RowShared &sh, Op op) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v = op(v, shfl_xor_u64(v, d));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh.wave[0];
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 64; ++w) v = op(v, sh.wave[w]);
+  return v;
+}
+__device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 smaller(u64 a, u64 b) { return a < b ? a : b; }
+__device__ __forceinline__ u64 plus(u64 a, u64 b) { return a + b; }
+
+// The bin of sh.hist, from the top, with above < target <= above + its content, `above` being
+// `base` and the bins over it, into sh.digit (kBins: none) and sh.above.
+__device__ __forceinline__ void select_bin(RowShared &sh, u64 base, double target) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int top = kBins - 1 - kBinsPerThread * tid;
+  u64 h[kBinsPerThread], sum = 0;
+#pragma unroll
+  for (int q = 0; q < kBinsPerThread; ++q) sum += h[q] = sh.hist[top - q];
+  u64 inc = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const u64 o = shfl_up_u64(inc, d);
+    if (lane >= d) inc += o;
+  }
+  __syncthreads();  // (what sh.wave held is read)
+  if (lane == 63) sh.wave[wave] = inc;
+  if (tid == 0) sh.digit = kBins;
+  __syncthreads();
+  u64 before = base + inc - sum;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) before += w < wave ? sh.wave[w] : 0;
+#pragma unroll
+  for (int q = 0; q < kBinsPerThread; ++q) {
+    if (h[q] && static_cast<double>(before) < target && target <= static_cast<double>(before + h[q])) {
+      sh.digit = top - q;
+      sh.above = before;
+    }
+    before += h[q];
+  }
+  __syncthreads();
+}
+
+// The smallest order key of the shortest prefix whose weights reach `target`, among the tokens
+// (order keys) that each(f) visits with a weight, `base` of it before all of them; 0 if they do
+// not reach it.  Radix selection: 10-bit digits of the key, from the first bit in which `lo` and
+// `hi` (bounds of the keys) differ.
+template <class Each>
+__device__ __forceinline__ u64 radix_cut(RowShared &sh, u64 lo, u64 hi, u64 base, double target, Each each) {
+  const u64 differ = lo ^ hi;
+  int bits = differ ? 64 - __clzll(static_cast<long long>(differ)) : 1;
+  u64 prefix = hi >> bits << bits, above = base;
+  while (bits > 0) {
+    const int shift = max(bits - 10, 0);
+    const uint32_t mask = (1u << (bits - shift)) - 1u;
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kRowThreads) sh.hist[b] = 0;
+    __syncthreads();
+    each([&](u64 key, u64 w) {
+      if (w && key >> bits == prefix >> bits) atomicAdd(&sh.hist[static_cast<uint32_t>(key >> shift) & mask], w);
     });
     __syncthreads();
-    const int n = sh.count;
-    if (n <= kCand) {
-      auto weight = [&](u64 k) -> u64 { return k >= cut && row.alive(order_value(k)) ? row.mass(order_value(k)) : 0; };
-      auto cands = [&](auto f) {
-        for (int j = tid; j < n; j += kThreads) f(sh.cand[j]);
-      };
-      auto total = [&](u64 from) {
-        u64 z = 0;
-        cands([&](u64 k) { z += k >= from ? weight(k) : 0; });
-        return block_reduce(z, sh, plus);
-      };
-      u64 lo = ~0ull, hi = 0;
-      cands([&](u64 k) {
-        lo = min(lo, k);
-        hi = max(hi, k);
-      });
-      lo = block_reduce(lo, sh, [](u64 a, u64 b) { return a < b ? a : b; });
-      hi = block_reduce(hi, sh, larger);
-      if (tk)
-        cut = prefix_cut(sh, lo, hi, static_cast<double>(tk), [&](auto f) {
-          cands([&](u64 k) { f(k, row.alive(order_value(k)) ? 1ull : 0ull); });
-        });
-      Z = total(cut);
-      bool found = true;
-      if (open) {
-        double lowest = static_cast<double>(Z), highest = lowest;
-        if (rest_counts) {
-          // The exponent (at most 160 below c2, or the power is 0) is off by 2^-22 of its terms, a
-          // power by a step, a sum of 2^8 terms by 2^8 half steps.
-          const double s = block_sum(static_cast<double>(rest), sh) * kMassScale;
-          const double off = 0x1p-15 + 0x1p-22 * (fabs(static_cast<double>(c2)) + 160.0);
-          lowest += s * fmax(1.0 - off, 0.0);
-          highest += s * (1.0 + off) + 1.0;
-        }
-        const u64 c = prefix_cut(sh, lo, hi, static_cast<double>(tp) * lowest, [&](auto f) {
-          cands([&](u64 k) { f(k, weight(k)); });
-        });
-        if (rest_counts)  // the same cut for the largest sum there can be, and no token missing above it
-          found = c && order_value(c) >= whole && static_cast<double>(tp) * highest <= static_cast<double>(total(c));
-        if (found) {
-          cut = larger(cut, c);
-          Z = total(cut);
-        }
-      }
-      if (found) {
-        zeros();
-        const double scale = kMassScale / static_cast<double>(Z);
-        __syncthreads();
-        cands([&](u64 k) {
-          const float x = order_value(k);
-          if (k >= cut && row.alive(x)) o[order_index(k)] = static_cast<float>(exp(row.down(x)) * scale);
-        });
-        return;
+    select_bin(sh, above, target);
+    if (sh.digit == kBins) return 0;
+    prefix |= sh.digit << shift;
+    above = sh.above;
+    bits = shift;
+  }
+  return prefix;
+}
+
+// A candidate's place: how many stand before it, and their weight.  Two threads a candidate
+// (e = thread / 2, n <= kRank) take half of the others each.
+struct Place {
+  int rank;
+  u64 before;
+};
+__device__ __forceinline__ Place place(const u64 *key, const u64 *mass, int n) {
+  Place r{0, 0};
+  const int e = threadIdx.x >> 1;
+  if (e < n) {
+    const u64 k = key[e];
+#pragma unroll 4
+    for (int j = threadIdx.x & 1; j < n; j += 2) {
+      const bool first = key[j] > k;
+      r.rank += first ? 1 : 0;
+      r.before += first ? mass[j] : 0;
+    }
+    r.rank += __shfl_xor(r.rank, 1);
+    r.before += shfl_xor_u64(r.before, 1);
+  }
+  return r;
+}
+
+// The cut as radix_cut finds it, among the n candidates in sh.key (sh.mass: their weights; by_count:
+// 1 each), of which those below `from` have none.  Few are ranked one against the other.  Many go
+// into bins of equal width in x first, and those of the bin that holds the cut are ranked; where
+// that is too many as well (equal logits), by digits.
+__device__ __forceinline__ u64 rank_cut(RowShared &sh, const u64 *key, const u64 *mass, int n, bool by_count, u64 from,
+                                        u64 base, double target) {
+  if (threadIdx.x == 0) sh.pick = 0;
+  __syncthreads();
+  const Place at = place(key, mass, n);
+  const int e = threadIdx.x >> 1;
+  if (e < n && !(threadIdx.x & 1) && key[e] >= from) {
+    const u64 before = base + (by_count ? static_cast<u64>(at.rank) : at.before), w = by_count ? 1ull : mass[e];
+    if (w && static_cast<double>(before) < target && target <= static_cast<double>(before + w)) sh.pick = key[e];
+  }
+  __syncthreads();
+  return sh.pick;
+}
+__device__ __forceinline__ u64 cand_cut(RowShared &sh, int n, bool by_count, u64 from, u64 base, double target) {
+  if (n <= kRank) return rank_cut(sh, sh.key, sh.mass, n, by_count, from, base, target);
+  u64 lo = ~0ull, hi = 0;
+  for (int j = threadIdx.x; j < n; j += kRowThreads) {
+    lo = smaller(lo, sh.key[j]);
+    hi = larger(hi, sh.key[j]);
+  }
+  lo = block_reduce(lo, sh, smaller);
+  hi = block_reduce(hi, sh, larger);
+  auto weight = [&](int j) -> u64 { return sh.key[j] < from ? 0 : by_count ? 1ull : sh.mass[j]; };
+  const float top = order_value(hi), width = top - order_value(lo);
+  if (width > 0.f && width < INFINITY) {
+    const float scale = static_cast<float>(kBins) / width;
+    auto bin = [&](u64 k) { return kBins - 1 - min(kBins - 1, static_cast<int>((top - order_value(k)) * scale)); };
+    for (int b = threadIdx.x; b < kBins; b += kRowThreads) sh.hist[b] = 0;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += kRowThreads)
+      if (const u64 w = weight(j)) atomicAdd(&sh.hist[bin(sh.key[j])], w);
+    __syncthreads();
+    select_bin(sh, base, target);
+    if (sh.digit == kBins) return 0;
+    const int digit = static_cast<int>(sh.digit);
+    const u64 above = sh.above;
+    __syncthreads();
+    u64 *key = sh.hist, *mass = sh.hist + kRank;  // (the histogram is done with)
+    for (int j = threadIdx.x; j < n; j += kRowThreads) {
+      if (bin(sh.key[j]) != digit) continue;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kRank) {
+        key[at] = sh.key[j];
+        mass[at] = sh.mass[j];
       }
     }
+    __syncthreads();
+    if (sh.count <= kRank) return rank_cut(sh, key, mass, sh.count, by_count, from, above, target);
   }
-
-  // ---- the long way ----
-  const u64 highest_key = order_key(static_cast<float>(row.m), 0);
-  cut = 0;
-  if (tk)
-    cut = prefix_cut(sh, 0, highest_key, static_cast<double>(tk), [&](auto f) {
-      row.each_short([&](int i, float v) {
-        const float x = row.x(v);
-        f(order_key(x, i), row.alive(x) ? 1ull : 0ull);
-      });
-    });
-  auto total = [&](u64 from) {
-    u64 z = 0;
-    row.each_short([&](int i, float v) {
-      const float x = row.x(v);
-      if (row.alive(x) && order_key(x, i) >= from) z += row.mass(x);
-    });
-    return block_reduce(z, sh, plus);
-  };
-  Z = total(cut);
-  if (open) {
-    const u64 c = cut;
-    cut = larger(cut, prefix_cut(sh, 0, highest_key, static_cast<double>(tp) * static_cast<double>(Z), [&](auto f) {
-                   row.each_short([&](int i, float v) {
-                     const float x = row.x(v);
-                     const u64 key = order_key(x, i);
-                     f(key, key >= c && row.alive(x) ? row.mass(x) : 0ull);
-                   });
-                 }));
-    Z = total(cut);
-  }
-  const double scale = kMassScale / static_cast<double>(Z);
-  row.each_short([&](int i, float v) {
-    const float x = row.x(v);
-    o[i] = row.alive(x) && order_key(x, i) >= cut ? static_cast<float>(exp(row.down(x)) * scale) : 0.f;
+  return radix_cut(sh, lo, hi, base, target, [&](auto f) {
+    for (int j = threadIdx.x; j < n; j += kRowThreads) f(sh.key[j], weight(j));
   });
 }
 
 template <int DT>
-void launch(const void *logits, int64_t row_stride, int rows, int V, const float *temperature, const int32_t *top_k,
-            const float *top_p, const float *min_p, float *out, int64_t out_stride, hipStream_t s) {
-  probs_kernel<DT><<<rows, kThreads, 0, s>>>(logits, row_stride, V, temperature, top_k, top_p, min_p, out, out_stride);
+struct Row {
+  typedef RowMem<DT> Mem;
+  typedef typename Mem::E E;
+  Mem mem;
+  double inv, m, low;
+
+  __device__ __forceinline__ Row(const Args &a, int64_t r, const Ask &k, float most)
+      : mem(a, r), inv(k.inv), m(quotient(most, k.inv)), low(k.low) {}
+  // f(index, logit) for every token, in no particular order; one copy of f (a workgroup waits
+  // for the instructions that it runs through), 16-byte loads, two in flight.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int all = (mem.before + mem.V + Mem::W - 1) / Mem::W;
+    typename Mem::Vec next = mem.load(min(static_cast<int>(threadIdx.x), all - 1));
+#pragma unroll 1
+    for (int v = threadIdx.x; v < all; v += kRowThreads) {
+      typename Mem::Vec e = next;
+      next = mem.load(min(v + kRowThreads, all - 1));
+#pragma unroll 1
+      for (int j = 0; j < Mem::W; ++j) {
+        const int i = mem.first(v) + j;
+        const E ej = e[0];
+        if (i >= 0 && i < mem.V) f(i, elem_to_f32<DT>(ej));
+#pragma unroll
+        for (int q = 0; q + 1 < Mem::W; ++q) e[q] = e[q + 1];
+      }
+    }
+  }
+  __device__ __forceinline__ float x(float logit) const { return quotient(logit, inv); }
+  __device__ __forceinline__ double down(float x) const {
+    const double d = static_cast<double>(x) - m;
+    return static_cast<double>(x) == m ? 0.0 : d;  // (also where both are infinite)
+  }
+  __device__ __forceinline__ bool alive(float x) const { return down(x) >= low; }  // (a NaN is not)
+  __device__ __forceinline__ u64 mass(float x) const {
+    return alive(x) ? static_cast<u64>(exp(down(x)) * kMassScale + 0.5) : 0;
+  }
+};
+
+// A cut over the whole row: the tokens' weights (by_count: 1 each; below `from`: none) in bins of
+// 1 / 32 of x below the largest, then the tokens of the bin that holds the cut as candidates; by
+// digits of the key where they are too many, or lie too far below.  all: the weights' sum, where
+// target is a share of it.
+template <int DT>
+__device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool by_count, u64 from, double target,
+                                       bool share) {
+  constexpr float kPerX = 32.f;
+  const float top = static_cast<float>(row.m);
+  auto bin = [&](float x) {  // (the largest, infinite or not, in the first)
+    return x == top ? kBins - 1 : kBins - 1 - static_cast<int>(fminf((top - x) * kPerX, static_cast<float>(kBins - 1)));
+  };
+  auto weight = [&](float x, int i) -> u64 {
+    return order_key(x, i) < from ? 0 : by_count ? (row.alive(x) ? 1ull : 0ull) : row.mass(x);
+  };
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kRowThreads) sh.hist[b] = 0;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  row.each([&](int i, float v) {
+    const float x = row.x(v);
+    if (const u64 w = weight(x, i)) atomicAdd(&sh.hist[bin(x)], w);
+  });
+  __syncthreads();
+  if (share) {
+    u64 z = 0;
+    for (int b = threadIdx.x; b < kBins; b += kRowThreads) z += sh.hist[b];
+    target *= static_cast<double>(block_reduce(z, sh, plus));
+  }
+  select_bin(sh, 0, target);
+  const int digit = static_cast<int>(sh.digit);
+  const u64 above = sh.above;
+  if (digit == kBins) return 0;
+  __syncthreads();
+  if (digit > 0) {
+    row.each([&](int i, float v) {
+      const float x = row.x(v);
+      if (!(x == x) || bin(x) != digit) return;
+      const u64 w = weight(x, i);
+      if (!w) return;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) {
+        sh.key[at] = order_key(x, i);
+        sh.mass[at] = w;
+      }
+    });
+    __syncthreads();
+    const int n = sh.count;
+    __syncthreads();
+    if (n <= kCand) return cand_cut(sh, n, by_count, from, above, target);
+  }
+  return radix_cut(sh, 0, order_key(top, 0), 0, target, [&](auto f) {
+    row.each([&](int i, float v) {
+      const float x = row.x(v);
+      if (x == x) f(order_key(x, i), weight(x, i));
+    });
+  });
+}
+
+// A row whose candidates do not decide it.
+template <int DT>
+__device__ __forceinline__ void long_way(RowShared &sh, const Row<DT> &row, const Ask &k, float *o) {
+  u64 cut = 0;
+  if (k.top_k) cut = row_cut(sh, row, true, 0, static_cast<double>(k.top_k), false);
+  if (k.open) cut = larger(cut, row_cut(sh, row, false, cut, static_cast<double>(k.top_p), true));
+  double z = 0.0;
+  row.each([&](int i, float v) {
+    const float x = row.x(v);
+    if (row.alive(x) && order_key(x, i) >= cut) z += static_cast<double>(expf(static_cast<float>(row.down(x))));
+  });
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d);
+  double *part = reinterpret_cast<double *>(sh.wave);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = z;
+  __syncthreads();
+  z = 0.0;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) z += part[w];
+  const float scale = static_cast<float>(1.0 / z);
+  row.each([&](int i, float v) {
+    const float x = row.x(v);
+    if (row.alive(x) && order_key(x, i) >= cut) o[i] = expf(static_cast<float>(row.down(x))) * scale;
+  });
+}
+
+// A row without cuts: its values, groups [v0, v1) of four.
+template <int DT>
+__device__ __forceinline__ void whole_row(const RowMem<DT> &mem, const Ask &k, float x_most, float scale, float *o,
+                                          int part, int parts) {
+  typedef typename RowMem<DT>::E E;
+  typedef float F4 __attribute__((ext_vector_type(4)));
+  struct __attribute__((packed, aligned(sizeof(E)))) E4 {
+    E e[4];
+  };
+  const int V = mem.V, head = min(V, static_cast<int>((-(reinterpret_cast<uintptr_t>(o) / 4)) & 3)), groups = (V - head) / 4;
+  const int g0 = static_cast<int>(static_cast<int64_t>(groups) * part / parts);
+  const int g1 = static_cast<int>(static_cast<int64_t>(groups) * (part + 1) / parts);
+  const float inv = 1.f / k.temp;
+  auto value = [&](E e) { return power(elem_to_f32<DT>(e), k.temp, inv, x_most) * scale; };
+#pragma unroll 2
+  for (int g = g0 + static_cast<int>(threadIdx.x); g < g1; g += kRowThreads) {
+    const E4 a = *reinterpret_cast<const E4 *>(mem.p + head + 4 * g);
+    *reinterpret_cast<F4 *>(o + head + 4 * g) = F4{value(a.e[0]), value(a.e[1]), value(a.e[2]), value(a.e[3])};
+  }
+  if (part == 0) {  // (at most 3 at each end)
+    const int i = static_cast<int>(threadIdx.x) < head ? static_cast<int>(threadIdx.x) : -1, t = head + 4 * groups + static_cast<int>(threadIdx.x);
+    if (i >= 0) o[i] = value(mem.p[i]);
+    if (t < V) o[t] = value(mem.p[t]);
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
+  __shared__ RowShared sh;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / a.groups;
+  const int g = static_cast<int>(blockIdx.x % a.groups);
+  const Ask k = ask(a, r);
+  const Head *heads = a.heads + r * a.S;
+  if (tid < a.S) sh.head[tid] = heads[tid];
+  __syncthreads();
+  if (k.kind != kWhole && g) return;
+  float most = -INFINITY;
+  for (int q = 0; q < a.S; ++q) most = fmaxf(most, sh.head[q].most);
+  float *o = a.out + r * a.out_stride;
+  const Row<DT> row(a, r, k, most);
+
+  if (k.kind == kWhole) {
+    if (most == -INFINITY) {
+      fill_zeros(o, static_cast<int>(static_cast<int64_t>(a.V) * g / a.groups),
+                 static_cast<int>(static_cast<int64_t>(a.V) * (g + 1) / a.groups), kRowThreads);
+      return;
+    }
+    double z = 0.0;
+    for (int q = 0; q < a.S; ++q) {
+      const Head h = sh.head[q];
+      if (h.most > -INFINITY) z += static_cast<double>(h.rest) * exp(row.down(row.x(h.most)));
+    }
+    whole_row(row.mem, k, static_cast<float>(row.m), static_cast<float>(1.0 / z), o, g, a.groups);
+    return;
+  }
+  if (most == -INFINITY) return;
+  if (k.kind == kGreedy) {
+    int first = kMaxVocab;
+    for (int q = 0; q < a.S; ++q) first = sh.head[q].most == most ? min(first, sh.head[q].count) : first;
+    if (tid == 0) o[first] = 1.f;
+    return;
+  }
+
+  // ---- the slices' candidates, those from `whole` on up: no token there is missing ----
+  const bool rest_counts = k.open && !k.top_k && !(k.min_p > 0.f);
+  int listed = 0;
+  bool known = true;
+  float whole = -INFINITY;
+  double rest = 0.0, off = 0.0;
+  for (int q = 0; q < a.S; ++q) {
+    const Head h = sh.head[q];
+    known = known && h.count >= 0;
+    listed += h.count;
+    whole = fmaxf(whole, h.whole);
+    if (rest_counts && h.most > -INFINITY) {
+      // The exponent (at most 160 below c2, or the power is 0) is off by 2^-22 of its terms, a
+      // power by a step, a sum of 2^6 terms by 2^6 half steps.
+      const float x = row.x(h.most);
+      rest += static_cast<double>(h.rest) * exp(row.down(x));
+      off = fmax(off, 0x1p-16 + 0x1p-22 * (fabs(static_cast<double>(x)) * 1.4426950408889634 + 160.0));
+    }
+  }
+  u64 below = 0;  // weight of the candidates that are not kept here
+  int n = 0;
+  if (known) {
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    const u64 *lists = a.lists + r * a.S * a.cap;
+    for (int e = tid; e < listed; e += kRowThreads) {
+      int q = 0, j = e;
+      while (j >= sh.head[q].count) j -= sh.head[q++].count;
+      const u64 key = lists[static_cast<int64_t>(q) * a.cap + j];
+      const bool keep = order_value(key) >= whole;
+      const u64 w = keep || rest_counts ? row.mass(order_value(key)) : 0;
+      if (!keep) {
+        below += w;
+        continue;
+      }
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) {
+        sh.key[at] = key;
+        sh.mass[at] = w;
+      }
+    }
+    if (rest_counts) below = block_reduce(below, sh, plus);
+    __syncthreads();
+    n = sh.count;
+    // of top_k's prefix every token is there, or every survivor of min_p
+    known = n <= kCand && (rest_counts || (k.top_k && n >= k.top_k) || whole == -INFINITY ||
+                           row.m + row.low >= static_cast<double>(whole));
+  }
+  if (known && n <= kRank) {
+    // ---- few: ranked, each by two threads ----
+    const Place at = place(sh.key, sh.mass, n);
+    const int e = tid >> 1;
+    bool kept = e < n && (!k.top_k || at.rank < k.top_k);
+    const u64 w = e < n ? sh.mass[e] : 0;
+    u64 Z = block_reduce(kept && !(tid & 1) ? w : 0, sh, plus);
+    if (k.open) {
+      double lowest = static_cast<double>(Z), highest = lowest;
+      if (rest_counts) {
+        lowest += static_cast<double>(below) + rest * fmax(1.0 - off, 0.0) * kMassScale;
+        highest += static_cast<double>(below) + rest * (1.0 + off) * kMassScale + 1.0;
+        known = static_cast<double>(k.top_p) * highest <= static_cast<double>(Z);
+      }
+      const double before = static_cast<double>(at.before);
+      const bool other = kept && before < static_cast<double>(k.top_p) * highest;
+      kept = kept && before < static_cast<double>(k.top_p) * lowest;
+      known = !__syncthreads_or(kept != other || !known);
+      if (known) Z = block_reduce(kept && !(tid & 1) ? w : 0, sh, plus);
+    }
+    if (known) {
+      if (kept && !(tid & 1)) {
+        const float x = order_value(sh.key[e]);
+        // below 2^-20 of the largest the fixed point has fewer digits than the result
+        if (row.alive(x))
+          o[order_index(sh.key[e])] = static_cast<float>((w >> 24 ? static_cast<double>(w) : exp(row.down(x)) * kMassScale) /
+                                                         static_cast<double>(Z));
+      }
+      return;
+    }
+  } else if (known) {
+    auto total = [&](u64 from) {
+      u64 z = 0;
+      for (int j = tid; j < n; j += kRowThreads) z += sh.key[j] >= from ? sh.mass[j] : 0;
+      return block_reduce(z, sh, plus);
+    };
+    u64 cut = k.top_k && n >= k.top_k ? cand_cut(sh, n, true, 0, 0, static_cast<double>(k.top_k)) : 0;
+    u64 Z = total(cut);
+    if (k.open) {
+      double lowest = static_cast<double>(Z), highest = lowest;
+      if (rest_counts) {
+        lowest += static_cast<double>(below) + rest * fmax(1.0 - off, 0.0) * kMassScale;
+        highest += static_cast<double>(below) + rest * (1.0 + off) * kMassScale + 1.0;
+      }
+      const u64 c = cand_cut(sh, n, false, cut, 0, static_cast<double>(k.top_p) * lowest);
+      cut = larger(cut, c);
+      Z = total(cut);
+      if (rest_counts)  // the same cut for the largest sum there can be
+        known = c && static_cast<double>(k.top_p) * highest <= static_cast<double>(Z);
+    }
+    if (known) {
+      const double scale = 1.0 / static_cast<double>(Z);
+      for (int j = tid; j < n; j += kRowThreads) {
+        const u64 key = sh.key[j];
+        const float x = order_value(key);
+        if (key >= cut && row.alive(x))
+          o[order_index(key)] = static_cast<float>(
+              (sh.mass[j] >> 24 ? static_cast<double>(sh.mass[j]) : exp(row.down(x)) * kMassScale) * scale);
+      }
+      return;
+    }
+  }
+  __syncthreads();
+  long_way(sh, row, k, o);
+}
+
+struct Plan {
+  int S, cap, reach, most;
+  size_t heads, lists;  // bytes
+};
+inline Plan plan(int rows, int V, int vec) {
+  Plan p;
+  const int per = vec * kSliceVecs * kSliceThreads;
+  p.S = (V + vec - 1 + per - 1) / per;
+  p.cap = std::min(kCand, ((2 * kCand / p.S) + 63) & ~63);
+  // The number of threads r whose maxima reach a bound that c tokens of a slice of random order reach:
+  // r = T (1 - exp(-c / T)).  Without top_k about 2,048 candidates a row, with at most 3,000.
+  const auto threads = [&](double c) {
+    return std::max(1, static_cast<int>(kSliceThreads * (1.0 - std::exp(-c / p.S / kSliceThreads))));
+  };
+  p.reach = threads(2048.0);
+  p.most = threads(3000.0);
+  p.heads = (static_cast<size_t>(rows) * p.S * sizeof(Head) + 15) & ~static_cast<size_t>(15);
+  p.lists = static_cast<size_t>(rows) * p.S * p.cap * sizeof(u64);
+  return p;
+}
+
+template <int DT>
+void launch(Args a, int rows, void *workspace, hipStream_t s) {
+  const Plan p = plan(rows, a.V, Elem<DT>::kVec);
+  a.S = p.S;
+  a.cap = p.cap;
+  a.reach = p.reach;
+  a.most = p.most;
+  a.heads = static_cast<Head *>(workspace);
+  a.lists = reinterpret_cast<u64 *>(static_cast<char *>(workspace) + p.heads);
+  const unsigned grid = static_cast<unsigned>(rows) * p.S;
+  slice_kernel<DT><<<grid, kSliceThreads, 0, s>>>(a);
+  a.groups = std::max(1, std::min(p.S, 256 / rows));
+  row_kernel<DT><<<static_cast<unsigned>(rows) * a.groups, kRowThreads, 0, s>>>(a);
 }
 
 }  // namespace probs
@@ -486,7 +873,15 @@ void launch(const void *logits, int64_t row_stride, int rows, int V, const float
 
 using namespace spk;
 
-extern "C" size_t spk_sample_probs_workspace_bytes(int rows, int vocab) { return 0; }
+extern "C" size_t spk_sample_probs_workspace_bytes(int rows, int vocab) {
+  if (rows <= 0 || vocab <= 0 || vocab > probs::kMaxVocab) return 0;
+  size_t most = 0;
+  for (int vec : {4, 8}) {  // (the logits' type is not an argument)
+    const probs::Plan p = probs::plan(rows, vocab, vec);
+    most = std::max(most, p.heads + p.lists);
+  }
+  return most;
+}
 
 extern "C" int spk_sample_probs(const void *logits, int logits_dtype, int64_t row_stride, int rows, int vocab,
                                 const float *temperature, const int32_t *top_k, const float *top_p,
@@ -504,11 +899,10 @@ extern "C" int spk_sample_probs(const void *logits, int logits_dtype, int64_t ro
     return fail(SPK_EINVAL, "sample_probs: workspace of %zu bytes, %zu needed, aligned to 16",
                 workspace ? workspace_bytes : 0, need);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (logits_dtype == SPK_F32)
-    probs::launch<SPK_F32>(logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, probs_out, out_stride, s);
-  else if (logits_dtype == SPK_F16)
-    probs::launch<SPK_F16>(logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, probs_out, out_stride, s);
-  else
-    probs::launch<SPK_BF16>(logits, row_stride, rows, vocab, temperature, top_k, top_p, min_p, probs_out, out_stride, s);
+  const probs::Args a{logits, row_stride, vocab, temperature, top_p, min_p, top_k, probs_out, out_stride, 0, 0, 0, 0,
+                      0, nullptr, nullptr};
+  if (logits_dtype == SPK_F32) probs::launch<SPK_F32>(a, rows, workspace, s);
+  else if (logits_dtype == SPK_F16) probs::launch<SPK_F16>(a, rows, workspace, s);
+  else probs::launch<SPK_BF16>(a, rows, workspace, s);
   return check_launch("sample_probs");
 }
