@@ -11,12 +11,12 @@
 // Two launches, both a workgroup a slice of a row.  Cuts keep few tokens as a rule, so:
 //   * the first (slice_kernel) holds its slice in registers, fills its part of the result with
 //     zeros and lists its candidates, the logits at or above a bound that so many of the
-//     threads' maxima reach, with the sum of the others' weights in fp32;
+//     threads' maxima reach, with the sum of the others' weights;
 //   * the second (row_kernel) finds the cuts among the candidates of a row's slices and puts
 //     the kept tokens in their places.  A cut by top_p needs the sum over the whole row:
-//     candidates count with their exact weight, the others with the fp32 sums, whose error is
-//     bounded; where the cut could fall elsewhere within that bound, or below a slice's bound,
-//     the row goes the long way, through histograms of the exact weights over the row.
+//     candidates count in fixed point, the others with the slices' sums, whose error is bounded;
+//     where the cut could fall elsewhere within that bound, or below a slice's bound, the row
+//     goes the long way, through histograms of the weights over the row.
 // A row without cuts gets its sum from the first launch and its values from the second.
 #include <algorithm>
 #include <cmath>
@@ -92,6 +92,28 @@ __device__ __forceinline__ float power(float v, float temp, float inv, float x_m
   return x == x ? expf(x == x_most ? 0.f : x - x_most) : 0.f;
 }
 
+// exp(d) for -800 <= d <= 0, off by less than kPowerOff of itself: the Taylor polynomial of degree
+// 11 around multiples of ln 2 (the next term is 0.3466^12 / 12! = 6.3e-15, the roundings a few of
+// 1.1e-16).  Half of the library's instructions.
+constexpr double kPowerOff = 0x1p-46;
+__device__ __forceinline__ double power64(double d) {
+  const double n = __builtin_rint(d * 1.4426950408889634);
+  const double g = __builtin_fma(n, -2.3190468138462996e-17, __builtin_fma(n, -0.6931471805599453, d));
+  double p = 1.0 / 39916800.0;
+  p = __builtin_fma(p, g, 1.0 / 3628800.0);
+  p = __builtin_fma(p, g, 1.0 / 362880.0);
+  p = __builtin_fma(p, g, 1.0 / 40320.0);
+  p = __builtin_fma(p, g, 1.0 / 5040.0);
+  p = __builtin_fma(p, g, 1.0 / 720.0);
+  p = __builtin_fma(p, g, 1.0 / 120.0);
+  p = __builtin_fma(p, g, 1.0 / 24.0);
+  p = __builtin_fma(p, g, 1.0 / 6.0);
+  p = __builtin_fma(p, g, 0.5);
+  p = __builtin_fma(p, g, 1.0);
+  p = __builtin_fma(p, g, 1.0);
+  return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
+}
+
 enum Kind { kGreedy, kWhole, kCuts };
 
 // A row's parameters.
@@ -124,7 +146,7 @@ struct Head {
   int count;    // candidates; -1: more than fit
   float most;   // the largest logit, -infinity: none
   float whole;  // quotients from here on up are all listed
-  float rest;   // sum of exp(x - its most's x) over the others (rows without cuts: over all)
+  double rest;  // sum of exp(x - its most's x) over the others (rows without cuts: over all)
 };
 
 __device__ __forceinline__ Ask ask(const Args &a, int64_t r) {
@@ -192,6 +214,7 @@ struct SliceShared {
   int32_t i[kCand];
   uint32_t tmax[kSliceThreads];
   float wave[kSliceThreads / 64];
+  double part[kSliceThreads / 64];
   uint32_t bound;
   int count, first;
 };
@@ -275,19 +298,19 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSliceThreads / 64; ++w) most = fmaxf(most, sh.wave[w]);
-  auto sum = [&](float v) {
+  auto sum = [&](double v) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     __syncthreads();
-    if (lane == 0) sh.wave[wave] = v;
+    if (lane == 0) sh.part[wave] = v;
     __syncthreads();
-    v = 0.f;
+    v = 0.0;
 #pragma unroll
-    for (int w = 0; w < kSliceThreads / 64; ++w) v += sh.wave[w];
+    for (int w = 0; w < kSliceThreads / 64; ++w) v += sh.part[w];
     return v;
   };
   if (most == -INFINITY) {
-    if (tid == 0) *head = Head{0, most, -INFINITY, 0.f};
+    if (tid == 0) *head = Head{0, most, -INFINITY, 0.0};
     return;
   }
   if (k.kind == kGreedy) {
@@ -295,7 +318,7 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
     each([&](int i, float v) { first = v == most ? min(first, i) : first; });
     atomicMin(&sh.first, first);
     __syncthreads();
-    if (tid == 0) *head = Head{sh.first, most, -INFINITY, 0.f};
+    if (tid == 0) *head = Head{sh.first, most, -INFINITY, 0.0};
     return;
   }
   const float x_most = quotient(most, k.inv);
@@ -303,13 +326,13 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
     const float inv = 1.f / k.temp;
     float z = 0.f;
     each([&](int, float v) { z += power(v, k.temp, inv, x_most); });
-    z = sum(z);
-    if (tid == 0) *head = Head{0, most, -INFINITY, z};
+    const double all = sum(z);
+    if (tid == 0) *head = Head{0, most, -INFINITY, all};
     return;
   }
   // ---- candidates ----
   if (k.top_k > kMostK) {
-    if (tid == 0) *head = Head{-1, most, INFINITY, 0.f};
+    if (tid == 0) *head = Head{-1, most, INFINITY, 0.0};
     return;
   }
   float bound = -INFINITY;
@@ -329,13 +352,14 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
     }
   }
   int mine = 0;
-  float rest = 0.f;
+  double rest = 0.0;
   if (k.open && !k.top_k && !(k.min_p > 0.f)) {
-    const float c1 = static_cast<float>(k.inv * 1.4426950408889634);
-    const float c2 = static_cast<float>(static_cast<double>(x_most) * 1.4426950408889634);
+    const double m = x_most;
     each([&](int, float v) {
       mine += v >= bound ? 1 : 0;
-      rest += __builtin_amdgcn_exp2f(__builtin_fmaf(v < bound ? v : -INFINITY, c1, -c2));
+      // (what overflows weighs nothing beside the largest; fmax takes the difference for a NaN)
+      const double d = static_cast<double>(static_cast<float>(static_cast<double>(v) * k.inv)) - m;
+      rest += power64(v < bound ? fmax(d, -800.0) : -800.0);
     });
   } else {
     each([&](int, float v) { mine += v >= bound ? 1 : 0; });
@@ -537,23 +561,19 @@ struct Row {
 
   __device__ __forceinline__ Row(const Args &a, int64_t r, const Ask &k, float most)
       : mem(a, r), inv(k.inv), m(quotient(most, k.inv)), low(k.low) {}
-  // f(index, logit) for every token, in no particular order; one copy of f (a workgroup waits
-  // for the instructions that it runs through), 16-byte loads, two in flight.
+  // f(index, logit) for every token, in no particular order; 16-byte loads, two in flight.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     const int all = (mem.before + mem.V + Mem::W - 1) / Mem::W;
     typename Mem::Vec next = mem.load(min(static_cast<int>(threadIdx.x), all - 1));
 #pragma unroll 1
     for (int v = threadIdx.x; v < all; v += kRowThreads) {
-      typename Mem::Vec e = next;
+      const typename Mem::Vec e = next;
       next = mem.load(min(v + kRowThreads, all - 1));
-#pragma unroll 1
-      for (int j = 0; j < Mem::W; ++j) {
-        const int i = mem.first(v) + j;
-        const E ej = e[0];
-        if (i >= 0 && i < mem.V) f(i, elem_to_f32<DT>(ej));
 #pragma unroll
-        for (int q = 0; q + 1 < Mem::W; ++q) e[q] = e[q + 1];
+      for (int j = 0; j < Mem::W; ++j) {
+        const E ej = e[j];
+        f(mem.first(v) + j, elem_to_f32<DT>(ej));  // (a NaN where the row has no token)
       }
     }
   }
@@ -564,23 +584,26 @@ struct Row {
   }
   __device__ __forceinline__ bool alive(float x) const { return down(x) >= low; }  // (a NaN is not)
   __device__ __forceinline__ u64 mass(float x) const {
-    return alive(x) ? static_cast<u64>(exp(down(x)) * kMassScale + 0.5) : 0;
+    const double d = down(x);
+    if (!(d >= low)) return 0;
+    // (to the nearest: the sum's last bits are those of the integer)
+    return static_cast<u64>(__double_as_longlong(power64(fmax(d, -800.0)) * kMassScale + 0x1p52)) - 0x4330000000000000ull;
   }
 };
 
 // A cut over the whole row: the tokens' weights (by_count: 1 each; below `from`: none) in bins of
-// 1 / 32 of x below the largest, then the tokens of the bin that holds the cut as candidates; by
-// digits of the key where they are too many, or lie too far below.  all: the weights' sum, where
-// target is a share of it.
+// 1 / 64 of x below the largest, then the tokens of the bin that holds the cut as candidates; by
+// digits of the key where they are too many, or lie too far below.  share: target is one of the
+// weights' sum.
 template <int DT>
 __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool by_count, u64 from, double target,
                                        bool share) {
-  constexpr float kPerX = 32.f;
+  constexpr float kPerX = 64.f;
   const float top = static_cast<float>(row.m);
   auto bin = [&](float x) {  // (the largest, infinite or not, in the first)
     return x == top ? kBins - 1 : kBins - 1 - static_cast<int>(fminf((top - x) * kPerX, static_cast<float>(kBins - 1)));
   };
-  auto weight = [&](float x, int i) -> u64 {
+  auto weight = [&](float x, int i) -> u64 {  // (0 for a NaN)
     return order_key(x, i) < from ? 0 : by_count ? (row.alive(x) ? 1ull : 0ull) : row.mass(x);
   };
   __syncthreads();
@@ -605,19 +628,18 @@ __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool b
   if (digit > 0) {
     row.each([&](int i, float v) {
       const float x = row.x(v);
-      if (!(x == x) || bin(x) != digit) return;
-      const u64 w = weight(x, i);
-      if (!w) return;
+      if (!(x == x) || bin(x) != digit || order_key(x, i) < from) return;
       const int at = atomicAdd(&sh.count, 1);
-      if (at < kCand) {
-        sh.key[at] = order_key(x, i);
-        sh.mass[at] = w;
-      }
+      if (at < kCand) sh.key[at] = order_key(x, i);
     });
     __syncthreads();
     const int n = sh.count;
+    if (n <= kCand) {
+      for (int j = threadIdx.x; j < n; j += kRowThreads) sh.mass[j] = weight(order_value(sh.key[j]), order_index(sh.key[j]));
+      __syncthreads();
+      return cand_cut(sh, n, by_count, from, above, target);
+    }
     __syncthreads();
-    if (n <= kCand) return cand_cut(sh, n, by_count, from, above, target);
   }
   return radix_cut(sh, 0, order_key(top, 0), 0, target, [&](auto f) {
     row.each([&](int i, float v) {
@@ -633,11 +655,13 @@ __device__ __forceinline__ void long_way(RowShared &sh, const Row<DT> &row, cons
   u64 cut = 0;
   if (k.top_k) cut = row_cut(sh, row, true, 0, static_cast<double>(k.top_k), false);
   if (k.open) cut = larger(cut, row_cut(sh, row, false, cut, static_cast<double>(k.top_p), true));
-  double z = 0.0;
-  row.each([&](int i, float v) {
+  const float inv = 1.f / k.temp, top = static_cast<float>(row.m);
+  auto kept = [&](int i, float v) {
     const float x = row.x(v);
-    if (row.alive(x) && order_key(x, i) >= cut) z += static_cast<double>(expf(static_cast<float>(row.down(x))));
-  });
+    return row.alive(x) && order_key(x, i) >= cut;
+  };
+  double z = 0.0;
+  row.each([&](int i, float v) { z += kept(i, v) ? static_cast<double>(power(v, k.temp, inv, top)) : 0.0; });
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d);
   double *part = reinterpret_cast<double *>(sh.wave);
@@ -649,8 +673,7 @@ __device__ __forceinline__ void long_way(RowShared &sh, const Row<DT> &row, cons
   for (int w = 0; w < kRowThreads / 64; ++w) z += part[w];
   const float scale = static_cast<float>(1.0 / z);
   row.each([&](int i, float v) {
-    const float x = row.x(v);
-    if (row.alive(x) && order_key(x, i) >= cut) o[i] = expf(static_cast<float>(row.down(x))) * scale;
+    if (kept(i, v)) o[i] = power(v, k.temp, inv, top) * scale;
   });
 }
 
@@ -680,8 +703,9 @@ __device__ __forceinline__ void whole_row(const RowMem<DT> &mem, const Ask &k, f
   }
 }
 
+// (two workgroups a CU: the registers of the long way alone would leave room for one)
 template <int DT>
-__global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
+__global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))) void row_kernel(Args a) {
   __shared__ RowShared sh;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / a.groups;
@@ -705,7 +729,7 @@ __global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
     double z = 0.0;
     for (int q = 0; q < a.S; ++q) {
       const Head h = sh.head[q];
-      if (h.most > -INFINITY) z += static_cast<double>(h.rest) * exp(row.down(row.x(h.most)));
+      if (h.most > -INFINITY) z += h.rest * exp(row.down(row.x(h.most)));
     }
     whole_row(row.mem, k, static_cast<float>(row.m), static_cast<float>(1.0 / z), o, g, a.groups);
     return;
@@ -723,18 +747,14 @@ __global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
   int listed = 0;
   bool known = true;
   float whole = -INFINITY;
-  double rest = 0.0, off = 0.0;
+  double rest = 0.0;
   for (int q = 0; q < a.S; ++q) {
     const Head h = sh.head[q];
     known = known && h.count >= 0;
     listed += h.count;
     whole = fmaxf(whole, h.whole);
     if (rest_counts && h.most > -INFINITY) {
-      // The exponent (at most 160 below c2, or the power is 0) is off by 2^-22 of its terms, a
-      // power by a step, a sum of 2^6 terms by 2^6 half steps.
-      const float x = row.x(h.most);
-      rest += static_cast<double>(h.rest) * exp(row.down(x));
-      off = fmax(off, 0x1p-16 + 0x1p-22 * (fabs(static_cast<double>(x)) * 1.4426950408889634 + 160.0));
+      rest += h.rest * exp(row.down(row.x(h.most)));
     }
   }
   u64 below = 0;  // weight of the candidates that are not kept here
@@ -776,8 +796,8 @@ __global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
     if (k.open) {
       double lowest = static_cast<double>(Z), highest = lowest;
       if (rest_counts) {
-        lowest += static_cast<double>(below) + rest * fmax(1.0 - off, 0.0) * kMassScale;
-        highest += static_cast<double>(below) + rest * (1.0 + off) * kMassScale + 1.0;
+        lowest += static_cast<double>(below) + rest * (1.0 - kPowerOff) * kMassScale;
+        highest += static_cast<double>(below) + rest * (1.0 + kPowerOff) * kMassScale;
         known = static_cast<double>(k.top_p) * highest <= static_cast<double>(Z);
       }
       const double before = static_cast<double>(at.before);
@@ -807,8 +827,8 @@ __global__ __launch_bounds__(kRowThreads) void row_kernel(Args a) {
     if (k.open) {
       double lowest = static_cast<double>(Z), highest = lowest;
       if (rest_counts) {
-        lowest += static_cast<double>(below) + rest * fmax(1.0 - off, 0.0) * kMassScale;
-        highest += static_cast<double>(below) + rest * (1.0 + off) * kMassScale + 1.0;
+        lowest += static_cast<double>(below) + rest * (1.0 - kPowerOff) * kMassScale;
+        highest += static_cast<double>(below) + rest * (1.0 + kPowerOff) * kMassScale;
       }
       const u64 c = cand_cut(sh, n, false, cut, 0, static_cast<double>(k.top_p) * lowest);
       cut = larger(cut, c);
@@ -842,11 +862,11 @@ inline Plan plan(int rows, int V, int vec) {
   p.S = (V + vec - 1 + per - 1) / per;
   p.cap = std::min(kCand, ((2 * kCand / p.S) + 63) & ~63);
   // The number of threads r whose maxima reach a bound that c tokens of a slice of random order reach:
-  // r = T (1 - exp(-c / T)).  Without top_k about 2,048 candidates a row, with at most 3,000.
+  // r = T (1 - exp(-c / T)).  Without top_k about 2,800 candidates a row, with at most 3,000.
   const auto threads = [&](double c) {
     return std::max(1, static_cast<int>(kSliceThreads * (1.0 - std::exp(-c / p.S / kSliceThreads))));
   };
-  p.reach = threads(2048.0);
+  p.reach = threads(2800.0);
   p.most = threads(3000.0);
   p.heads = (static_cast<size_t>(rows) * p.S * sizeof(Head) + 15) & ~static_cast<size_t>(15);
   p.lists = static_cast<size_t>(rows) * p.S * p.cap * sizeof(u64);
