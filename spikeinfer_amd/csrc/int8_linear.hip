@@ -158,6 +158,124 @@ __global__ __launch_bounds__(256) void product_kernel(const v4i *xq, const float
   }
 }
 
+// ---- many rows ----------------------------------------------------------------------
+// A workgroup kBM rows by kBN columns, four waves side by side along the columns, 128 x 64
+// each (128 accumulator registers); two workgroups a CU, so that one's epilogue runs beside
+// the other's products.  The waves share x through LDS (a step's 8 KB, double-buffered, through
+// registers so that its loads are two steps ahead); each wave's part of W is its own and
+// goes from memory to registers, two steps ahead.  LDS then moves 40 KB a step of 512 cycles
+// of products, where both operands through it would take 72.
+constexpr int kBM = 128, kBN = 256;
+constexpr int kTM = kBM / 16, kTN = 4;
+
+template <int OT, bool BIAS>
+__device__ __forceinline__ void store_tile(const v4i &acc, float sx, const float *ws, const void *bias, int bias_dtype,
+                                           typename Elem<OT>::T *out, int col, int N, bool vec) {
+  typedef typename Elem<OT>::T E;
+  typedef E E4 __attribute__((ext_vector_type(4)));
+  typedef float F4 __attribute__((ext_vector_type(4)));
+  const F4 s = *reinterpret_cast<const F4 *>(ws + col);  // (padded to 16)
+  E4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float f = static_cast<float>(acc[e]) * (sx * s[e]);
+    if (BIAS) f += col + e < N ? load_as_f32(bias, col + e, bias_dtype) : 0.f;
+    v[e] = f32_to_elem<OT>(f);
+  }
+  if (vec && col + 4 <= N) {
+    *reinterpret_cast<E4 *>(out + col) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < N) out[col + e] = v[e];
+  }
+}
+
+template <int OT, bool BIAS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(
+    const v4i *xq, const float *xs, const v4i *wq, const float *ws, const void *bias, int bias_dtype, void *y,
+    int64_t ystride, int64_t M, int N, int KS, int MT, int NT, int mtiles, int ntiles, bool vec) {
+  __shared__ v4i sh[2][kTM * 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kq = lane >> 4;
+  // Tiles of one XCD (workgroup b runs on XCD b % 8): a contiguous share of the row tiles, eight
+  // of them at a time against every column tile, so that x comes into its L2 once and W
+  // once for the eight.
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
+  const int first = static_cast<int>(static_cast<int64_t>(mtiles) * xcd / 8);
+  const int mine = static_cast<int>(static_cast<int64_t>(mtiles) * (xcd + 1) / 8) - first;
+  const int group = idx / (8 * ntiles), in = idx - group * 8 * ntiles, rows = min(8, mine - 8 * group);
+  if (rows <= 0 || in >= rows * ntiles) return;
+  const int mt = first + 8 * group + in % rows, nt = in / rows;
+  const int m0 = mt * kTM, n0 = nt * (kBN / 16) + wave * kTN;
+
+  // this thread's two 16-byte pieces of a step's x, its wave's four blocks of W
+  const v4i *ax[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) ax[p] = xq + static_cast<int64_t>(min(m0 + wave + 4 * p, MT - 1)) * KS * 64 + lane;
+  const v4i *bw[kTN];
+#pragma unroll
+  for (int t = 0; t < kTN; ++t) bw[t] = wq + static_cast<int64_t>(min(n0 + t, NT - 1)) * KS * 64 + lane;
+
+  v4i acc[kTM][kTN];
+#pragma unroll
+  for (int i = 0; i < kTM; ++i)
+#pragma unroll
+    for (int j = 0; j < kTN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  v4i sa[2][2], sb[2][kTN];
+  auto load_a = [&](int k, v4i (&r)[2]) {
+    const int at = min(k, KS - 1) * 64;  // (steps behind the last are not used)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) r[p] = ax[p][at];
+  };
+  auto load_b = [&](int k, v4i (&r)[kTN]) {
+    const int at = min(k, KS - 1) * 64;
+#pragma unroll
+    for (int t = 0; t < kTN; ++t) r[t] = bw[t][at];
+  };
+  auto put = [&](v4i *to, const v4i (&r)[2]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) to[(wave + 4 * p) * 64 + lane] = r[p];
+  };
+  load_a(0, sa[0]);
+  load_b(0, sb[0]);
+  load_a(1, sa[1]);
+  load_b(1, sb[1]);
+  put(sh[0], sa[0]);
+  load_a(2, sa[0]);
+  __syncthreads();
+  auto step = [&](int k, const v4i *from, v4i *to, v4i (&a)[2], v4i (&b)[kTN]) {
+    v4i f[kTM];
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) f[i] = from[i * 64 + lane];
+    put(to, a);
+    load_a(k + 3, a);
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j], f[i], acc[i][j], 0, 0, 0);
+    load_b(k + 2, b);
+    __syncthreads();
+  };
+  int k = 0;
+  for (; k + 1 < KS; k += 2) {
+    step(k, sh[0], sh[1], sa[1], sb[0]);
+    step(k + 1, sh[1], sh[0], sa[0], sb[1]);
+  }
+  if (k < KS) step(k, sh[0], sh[1], sa[1], sb[0]);
+
+  typedef typename Elem<OT>::T E;
+#pragma unroll
+  for (int i = 0; i < kTM; ++i) {
+    const int64_t row = 16 * static_cast<int64_t>(m0 + i) + r16;
+    if (row >= M) continue;
+    const float sx = xs[row];
+    E *out = static_cast<E *>(y) + row * ystride;
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+      if (n0 + j < NT) store_tile<OT, BIAS>(acc[i][j], sx, ws, bias, bias_dtype, out, 16 * (n0 + j) + 4 * kq, N, vec);
+  }
+}
+
 template <int DT>
 void launch_rows(const void *x, int64_t stride, int64_t rows, int K, void *packed, float *scales, hipStream_t s) {
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * sizeof(typename Elem<DT>::T)) % 16 == 0;
@@ -178,6 +296,16 @@ void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, con
              int64_t ystride, int64_t M, int N, int KS, hipStream_t s) {
   const int64_t MT = row_tiles(M);
   const int NT = static_cast<int>(row_tiles(N));
+  if (M >= 512 && N >= 256) {
+    const int mtiles = static_cast<int>((M + kBM - 1) / kBM), ntiles = (N + kBN - 1) / kBN;
+    const int most = (mtiles + 7) / 8;  // row tiles of an XCD
+    const unsigned grid = 8u * ((most + 7) / 8) * 8 * ntiles;
+    typedef typename Elem<OT>::T E;
+    const bool vec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(E))) == 0 && ystride % 4 == 0;
+    if (bias) tile_kernel<OT, true><<<grid, 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y, ystride, M, N, KS, static_cast<int>(MT), NT, mtiles, ntiles, vec);
+    else tile_kernel<OT, false><<<grid, 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y, ystride, M, N, KS, static_cast<int>(MT), NT, mtiles, ntiles, vec);
+    return;
+  }
   constexpr int TM = 4, TN = 4;
   const int64_t units = (MT + TM - 1) / TM * ((NT + TN - 1) / TN);
   product_kernel<TM, TN, OT><<<static_cast<unsigned>((units + 3) / 4), 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y,
