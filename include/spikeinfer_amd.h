@@ -749,7 +749,7 @@ int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_stri
  *   w, x, bias, y  F32, F16 or BF16 each, channel stride 1, rows at their strides; rows of y
  *            must not lie on one another, nor y on x
  *   packed   spk_linear_int8_packed_bytes(N, K) bytes, 16-byte aligned, and scales float
- *            [N rounded up to 16]: written by spk_linear_int8_pack, once per weight
+ *            [N rounded up to 64]: written by spk_linear_int8_pack, once per weight
  *   workspace spk_linear_int8_workspace_bytes(M, N, K) bytes, 16-byte aligned
  * K <= 131072 (the sums are 32 bits), M <= 2^30 (SPK_EUNSUPPORTED beyond).
  */

@@ -8,7 +8,13 @@
 // Operands lie in the order of the matrix instruction (v_mfma_i32_16x16x64_i8): 16 rows by
 // 64 k are one block of 1 KB, lane l's 16 bytes row l % 16, k 16 (l / 16) .. + 15, blocks of
 // a row tile one behind the other.  W is laid out once (spk_linear_int8_pack), x by the
-// call's first kernel, with the same code.
+// call's first kernel, with the same code.  W is the instruction's first operand, so a lane
+// holds four columns of one row of y; a tile of W has four runs of four of a group of 64
+// output channels (tile j of a group: channels 16 q + 4 j + e in row 4 q + e), so that the
+// four tiles of a group give a lane 16 columns side by side, and a wave writes whole 128-byte
+// lines of y (8,188 x 9,728 of K = 64, nearly all stores: 67 -> 43 us).
+#include <algorithm>
+
 #include "common.hpp"
 #include "lif_math.hpp"
 
@@ -19,13 +25,14 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;      // k of a block
 constexpr int kMaxK = 131072;  // 127^2 kMaxK < 2^31
-constexpr int kRowWaves = 4;
-constexpr int kKeep = 4;       // blocks a wave keeps between the two passes
+constexpr int kRowWaves = 16;  // at most, of a tile of rows
+constexpr int kKeep = 5;       // blocks a wave keeps between the two passes
 
 inline int64_t row_tiles(int64_t rows) { return (rows + 15) / 16; }
 inline int64_t k_steps(int64_t K) { return (K + kStep - 1) / kStep; }
 inline int64_t packed_bytes(int64_t rows, int64_t K) { return row_tiles(rows) * k_steps(K) * 1024; }
 inline int64_t scale_bytes(int64_t rows) { return row_tiles(rows) * 64; }
+inline int groups_of(int N) { return (N + 63) / 64; }  // of 64 output channels
 
 // rint(x / s) with the quotient rounded to fp32, in -127..127.  x * (1 / s) is off by less
 // than two steps of fp32, so where it lies further than that from a half the rounding is
@@ -61,100 +68,305 @@ __device__ __forceinline__ void load16(const void *row, int k0, int K, float (&v
   }
 }
 
-// A workgroup 16 rows: their largest magnitudes, then the integers.  Rows that do not exist
-// become zeros.  A row that holds an infinity or a NaN has the scale NaN, so that its
-// products are NaN as those of the numbers themselves would be.
-template <int DT, bool VEC>
+// The magnitudes' scale.  A row that holds an infinity or a NaN (most: the largest magnitude's
+// bits) has the scale NaN, so that its products are NaN as those of the numbers themselves
+// would be.
+struct Scale {
+  float s, inv;
+  bool some;
+};
+__device__ __forceinline__ Scale scale_of(uint32_t most) {
+  const bool finite = most < 0x7f800000u;
+  Scale r;
+  r.s = finite ? __uint_as_float(most) / 127.f : __uint_as_float(0x7fc00000u);
+  r.some = finite && r.s > 0.f;
+  r.inv = r.s >= 0x1p-100f ? 1.f / r.s : __uint_as_float(0x7fc00000u);
+  return r;
+}
+__device__ __forceinline__ v4i quantise16(const float (&v)[16], const Scale &sc) {
+  v4i out = {0, 0, 0, 0};
+  if (sc.some) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) out[j >> 2] |= (quantise(v[j], sc.s, sc.inv) & 255) << 8 * (j & 3);
+  }
+  return out;
+}
+
+// A workgroup 16 rows: their largest magnitudes, then the integers.  The waves share the row's
+// blocks and keep them in registers between the two (kKeep each; longer rows are read again).
+// WEIGHT: rows in the order of the groups of output channels.  Rows that do not exist become
+// zeros.  Bound by reading x and by the latency of the two passes.
+template <int DT, bool VEC, bool WEIGHT>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int64_t stride, int64_t rows, int K, int KS,
                                                               v4i *packed, float *scales) {
   __shared__ uint32_t most[kRowWaves][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
-  const int64_t tile = blockIdx.x, row = 16 * tile + r16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, kq = lane >> 4;
+  const int64_t tile = blockIdx.x;
+  const int64_t row = WEIGHT ? tile / 4 * 64 + 16 * (r16 >> 2) + 4 * (tile & 3) + (r16 & 3) : 16 * tile + r16;
   const bool real = row < rows;
-  const char *p = static_cast<const char *>(x) + row * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
+  const char *p = static_cast<const char *>(x) + (real ? row : 0) * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
   uint32_t m = 0;
-  for (int ks = wave; ks < KS; ks += kRowWaves) {
-    if (!real) break;
-    float v[16];
-    load16<DT, VEC>(p, kStep * ks + 16 * kq, K, v);
+  float v[kKeep][16];
+  auto largest = [&](const float (&a)[16]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);  // (a NaN's bits are the largest)
+    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(a[j]) & 0x7fffffffu);  // (a NaN's bits are the largest)
+  };
+#pragma unroll
+  for (int q = 0; q < kKeep; ++q)
+    if (wave + q * waves < KS) load16<DT, VEC>(p, kStep * (wave + q * waves) + 16 * kq, real ? K : 0, v[q]);
+#pragma unroll
+  for (int q = 0; q < kKeep; ++q)
+    if (wave + q * waves < KS) largest(v[q]);
+  for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
+    float a[16];
+    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, a);
+    largest(a);
+  }
+  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
+  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
+  if (lane < 16) most[wave][lane] = m;
+  __syncthreads();
+  for (int w = 0; w < waves; ++w) m = max(m, most[w][r16]);
+  const Scale sc = scale_of(m);
+  if (threadIdx.x < 16) scales[row] = sc.s;
+#pragma unroll
+  for (int q = 0; q < kKeep; ++q)
+    if (wave + q * waves < KS) packed[(tile * KS + wave + q * waves) * 64 + lane] = quantise16(v[q], sc);
+  for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
+    float a[16];
+    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, a);
+    packed[(tile * KS + ks) * 64 + lane] = quantise16(a, sc);
+  }
+}
+
+// Sixteen columns of a row of y from column `col` on: a lane's sums of the four tiles of a group.
+struct Out {
+  const float *ws;
+  const void *bias;
+  int bias_dtype;
+  int N;
+  bool vec;  // 16-byte stores: y and its rows are aligned
+};
+template <int OT>
+__device__ __forceinline__ void store16(const Out &o, const v4i (&acc)[4], float sx, typename Elem<OT>::T *out, int col) {
+  typedef typename Elem<OT>::T E;
+  constexpr int W = Elem<OT>::kVec;
+  typedef E Vec __attribute__((ext_vector_type(W)));
+  typedef float F4 __attribute__((ext_vector_type(4)));
+  float f[16];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const F4 s = *reinterpret_cast<const F4 *>(o.ws + col + 4 * j);  // (padded to 64)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[4 * j + e] = static_cast<float>(acc[j][e]) * (sx * s[e]);
+  }
+  if (o.bias) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] += col + e < o.N ? load_as_f32(o.bias, col + e, o.bias_dtype) : 0.f;
+  }
+  if (o.vec && col + 16 <= o.N) {
+#pragma unroll
+    for (int h = 0; h < 16 / W; ++h) {
+      Vec v;
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = f32_to_elem<OT>(f[W * h + e]);
+      *reinterpret_cast<Vec *>(out + col + W * h) = v;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (col + e < o.N) out[col + e] = f32_to_elem<OT>(f[e]);
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------
+// A workgroup TM tiles of 16 rows by one group of 64 columns; its eight waves share the steps
+// of K, each with its own blocks of both operands from memory, two steps ahead, and their sums
+// meet in LDS.  Bound by latency: a wave has few steps (K = 896: two).
+//
+// FUSED (at most 16 rows): x is quantised here.  A wave loads the blocks of x that it
+// multiplies, the waves exchange the rows' largest magnitudes, and the integers are the
+// instruction's operand where they are made; W's first blocks are on their way meanwhile.
+constexpr int kSplit = 8;
+
+// Adds up the waves' sums; wave i < TM has row tile i's afterwards.
+template <int TM>
+__device__ __forceinline__ void join(v4i *sh, const v4i (&acc)[TM][4], v4i (&sum)[4]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sh[((wave * TM + i) * 4 + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  if (wave >= TM) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sum[j] = sh[(wave * 4 + j) * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < kSplit; ++w) sum[j] += sh[((w * TM + wave) * 4 + j) * 64 + lane];
+  }
+}
+
+template <int TM, int OT>
+__global__ __launch_bounds__(64 * kSplit) void split_kernel(const v4i *xq, const float *xs, const v4i *wq, Out o, void *y,
+                                                            int64_t ystride, int64_t M, int KS, int64_t MT, int NG) {
+  __shared__ v4i sh[kSplit * TM * 4 * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
+  const int g = static_cast<int>(blockIdx.x % NG);
+  const int64_t m0 = blockIdx.x / NG * TM;
+  const v4i *a = wq + static_cast<int64_t>(g) * 4 * KS * 64 + lane, *b[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) b[t] = xq + min(m0 + t, MT - 1) * KS * 64 + lane;
+  v4i acc[TM][4], av[2][4], bv[2][TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  auto load = [&](int ks, v4i (&av)[4], v4i (&bv)[TM]) {
+    const int64_t at = min(ks, KS - 1);  // (steps behind the last are not used)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) av[t] = a[(t * static_cast<int64_t>(KS) + at) * 64];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) bv[t] = b[t][at * 64];
+  };
+  auto products = [&](const v4i (&av)[4], const v4i (&bv)[TM]) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[j], bv[i], acc[i][j], 0, 0, 0);
+  };
+  load(wave, av[0], bv[0]);
+  load(wave + kSplit, av[1], bv[1]);
+  for (int ks = wave; ks < KS; ks += 2 * kSplit) {
+    products(av[0], bv[0]);
+    load(ks + 2 * kSplit, av[0], bv[0]);
+    if (ks + kSplit >= KS) break;
+    products(av[1], bv[1]);
+    load(ks + 3 * kSplit, av[1], bv[1]);
+  }
+  v4i sum[4];
+  join<TM>(sh, acc, sum);
+  const int64_t row = 16 * (m0 + wave) + r16;
+  if (wave < TM && row < M) store16<OT>(o, sum, xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
+}
+
+template <int DT, bool VEC, int OT>
+__global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64_t stride, const v4i *wq, Out o, void *y,
+                                                            int64_t ystride, int M, int K, int KS) {
+  constexpr int kHold = 2;  // blocks of x that a wave holds (K <= 1,024); the others are read again
+  __shared__ v4i sh[kSplit * 4 * 64];
+  __shared__ uint32_t most[kSplit][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4, g = blockIdx.x;
+  const v4i *a = wq + static_cast<int64_t>(g) * 4 * KS * 64 + lane;
+  const bool real = r16 < M;
+  const char *p = static_cast<const char *>(x) + (real ? r16 : 0) * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
+  v4i av[2][4];
+  auto load = [&](int ks, v4i (&av)[4]) {
+    const int64_t at = min(ks, KS - 1);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) av[t] = a[(t * static_cast<int64_t>(KS) + at) * 64];
+  };
+  float v[kHold][16];
+#pragma unroll
+  for (int q = 0; q < kHold; ++q) load16<DT, VEC>(p, kStep * (wave + q * kSplit) + 16 * kq, real && wave + q * kSplit < KS ? K : 0, v[q]);
+  load(wave, av[0]);
+  load(wave + kSplit, av[1]);
+  uint32_t m = 0;
+  auto largest = [&](const float (&e)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(e[j]) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int q = 0; q < kHold; ++q) largest(v[q]);
+  for (int ks = wave + kHold * kSplit; ks < KS; ks += kSplit) {
+    float e[16];
+    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, e);
+    largest(e);
   }
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
   if (lane < 16) most[wave][lane] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) m = max(m, most[w][r16]);
-  const bool finite = m < 0x7f800000u;
-  const float s = finite ? __uint_as_float(m) / 127.f : __uint_as_float(0x7fc00000u);
-  if (threadIdx.x < 16) scales[row] = s;
-  const bool some = finite && s > 0.f;
-  const float inv = s >= 0x1p-100f ? 1.f / s : __uint_as_float(0x7fc00000u);
-  for (int ks = wave; ks < KS; ks += kRowWaves) {
-    v4i out = {0, 0, 0, 0};
-    if (real && some) {
-      float v[16];
-      load16<DT, VEC>(p, kStep * ks + 16 * kq, K, v);
+  for (int w = 0; w < kSplit; ++w) m = max(m, most[w][r16]);
+  const Scale sc = scale_of(m);
+  v4i acc[1][4];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) out[j >> 2] |= (quantise(v[j], s, inv) & 255) << 8 * (j & 3);
-    }
-    packed[(tile * KS + ks) * 64 + lane] = out;
+  for (int j = 0; j < 4; ++j) acc[0][j] = v4i{0, 0, 0, 0};
+  auto products = [&](const v4i (&av)[4], const v4i &b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[0][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[j], b, acc[0][j], 0, 0, 0);
+  };
+#pragma unroll
+  for (int q = 0; q < kHold; ++q) {
+    if (wave + q * kSplit < KS) products(av[q], quantise16(v[q], sc));
+    load(wave + (q + kHold) * kSplit, av[q]);
   }
+  for (int ks = wave + kHold * kSplit; ks < KS; ks += 2 * kSplit) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (ks + q * kSplit < KS) {
+        float e[16];
+        load16<DT, VEC>(p, kStep * (ks + q * kSplit) + 16 * kq, real ? K : 0, e);
+        products(av[q], quantise16(e, sc));
+        load(ks + (q + 2) * kSplit, av[q]);
+      }
+    }
+  }
+  v4i sum[4];
+  join<1>(sh, acc, sum);
+  if (wave == 0 && real)
+    store16<OT>(o, sum, sc.s, static_cast<typename Elem<OT>::T *>(y) + r16 * ystride, 64 * g + 16 * kq);
 }
 
-// A wave TM x TN tiles of 16 rows (of x) by 16 columns (of y), both operands from memory.
-// The weight is the instruction's first operand: a lane then holds four columns side by
-// side of one row of y.
-template <int TM, int TN, int OT>
-__global__ __launch_bounds__(256) void product_kernel(const v4i *xq, const float *xs, const v4i *wq, const float *ws,
-                                                      const void *bias, int bias_dtype, void *y, int64_t ystride,
-                                                      int64_t M, int N, int KS, int64_t MT, int NT) {
+// ---- few rows, many columns (the lm_head) ----------------------------------------------
+// A workgroup's four waves share up to 64 rows of x in LDS, each takes a group of 64 columns
+// over the whole K and streams its part of W three steps ahead.  Bound by reading W.
+constexpr int kWideWaves = 4;
+constexpr int kWideLds = 64 * 1024;  // two workgroups a CU
+constexpr int kAhead = 3;
+template <int TM, int OT>
+__global__ __launch_bounds__(64 * kWideWaves) void wide_kernel(const v4i *xq, const float *xs, const v4i *wq, Out o, void *y,
+                                                               int64_t ystride, int M, int KS, int MT, int NG) {
+  extern __shared__ v4i shx[];  // [MT][KS][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int cols = (NT + TN - 1) / TN;
-  const int64_t m0 = unit / cols * TM;
-  const int n0 = static_cast<int>(unit % cols) * TN;
-  if (m0 >= MT) return;
-  const v4i *a[TN], *b[TM];
+  const int g = blockIdx.x * kWideWaves + wave;
+  const v4i *a = wq + static_cast<int64_t>(min(g, NG - 1)) * 4 * KS * 64 + lane;
+  v4i av[kAhead][4];
+  auto load = [&](int ks, v4i (&av)[4]) {
+    const int64_t at = min(ks, KS - 1);
 #pragma unroll
-  for (int t = 0; t < TN; ++t) a[t] = wq + static_cast<int64_t>(min(n0 + t, NT - 1)) * KS * 64 + lane;
+    for (int t = 0; t < 4; ++t) av[t] = __builtin_nontemporal_load(a + (t * static_cast<int64_t>(KS) + at) * 64);
+  };
 #pragma unroll
-  for (int t = 0; t < TM; ++t) b[t] = xq + min(m0 + t, MT - 1) * KS * 64 + lane;
-  v4i acc[TM][TN];
+  for (int q = 0; q < kAhead; ++q) load(q, av[q]);
+  for (int i = threadIdx.x; i < MT * KS * 64; i += 64 * kWideWaves) shx[i] = xq[i];
+  __syncthreads();
+  if (g >= NG) return;
+  v4i acc[TM][4];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-  for (int ks = 0; ks < KS; ++ks) {
-    v4i av[TN], bv[TM];
+    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  for (int k0 = 0; k0 < KS; k0 += kAhead) {
 #pragma unroll
-    for (int t = 0; t < TN; ++t) av[t] = a[t][ks * 64];
+    for (int q = 0; q < kAhead; ++q) {
+      if (k0 + q < KS) {
+        v4i b[TM];
 #pragma unroll
-    for (int t = 0; t < TM; ++t) bv[t] = b[t][ks * 64];
+        for (int i = 0; i < TM; ++i) b[i] = shx[(min(i, MT - 1) * KS + k0 + q) * 64 + lane];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[j], bv[i], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[q][j], b[i], acc[i][j], 0, 0, 0);
+        load(k0 + q + kAhead, av[q]);
+      }
+    }
   }
-  typedef typename Elem<OT>::T E;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int64_t row = 16 * (m0 + i) + r16;
-    if (row >= M) continue;
-    const float sx = xs[row];
-    E *out = static_cast<E *>(y) + row * ystride;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int col = 16 * (n0 + j) + 4 * kq;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < N) {
-          float v = static_cast<float>(acc[i][j][e]) * (sx * ws[col + e]);
-          if (bias) v += load_as_f32(bias, col + e, bias_dtype);
-          out[col + e] = f32_to_elem<OT>(v);
-        }
-    }
+    const int row = 16 * i + r16;
+    if (row < M) store16<OT>(o, acc[i], xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
   }
 }
 
@@ -168,33 +380,10 @@ __global__ __launch_bounds__(256) void product_kernel(const v4i *xq, const float
 constexpr int kBM = 128, kBN = 256;
 constexpr int kTM = kBM / 16, kTN = 4;
 
-template <int OT, bool BIAS>
-__device__ __forceinline__ void store_tile(const v4i &acc, float sx, const float *ws, const void *bias, int bias_dtype,
-                                           typename Elem<OT>::T *out, int col, int N, bool vec) {
-  typedef typename Elem<OT>::T E;
-  typedef E E4 __attribute__((ext_vector_type(4)));
-  typedef float F4 __attribute__((ext_vector_type(4)));
-  const F4 s = *reinterpret_cast<const F4 *>(ws + col);  // (padded to 16)
-  E4 v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float f = static_cast<float>(acc[e]) * (sx * s[e]);
-    if (BIAS) f += col + e < N ? load_as_f32(bias, col + e, bias_dtype) : 0.f;
-    v[e] = f32_to_elem<OT>(f);
-  }
-  if (vec && col + 4 <= N) {
-    *reinterpret_cast<E4 *>(out + col) = v;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < N) out[col + e] = v[e];
-  }
-}
-
-template <int OT, bool BIAS>
+template <int OT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(
-    const v4i *xq, const float *xs, const v4i *wq, const float *ws, const void *bias, int bias_dtype, void *y,
-    int64_t ystride, int64_t M, int N, int KS, int MT, int NT, int mtiles, int ntiles, bool vec) {
+    const v4i *xq, const float *xs, const v4i *wq, Out o, void *y, int64_t ystride, int64_t M, int KS, int MT, int NG,
+    int mtiles, int ntiles) {
   __shared__ v4i sh[2][kTM * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kq = lane >> 4;
   // Tiles of one XCD (workgroup b runs on XCD b % 8): a contiguous share of the row tiles, eight
@@ -206,7 +395,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int group = idx / (8 * ntiles), in = idx - group * 8 * ntiles, rows = min(8, mine - 8 * group);
   if (rows <= 0 || in >= rows * ntiles) return;
   const int mt = first + 8 * group + in % rows, nt = in / rows;
-  const int m0 = mt * kTM, n0 = nt * (kBN / 16) + wave * kTN;
+  const int m0 = mt * kTM, g = nt * (kBN / 64) + wave;
 
   // this thread's two 16-byte pieces of a step's x, its wave's four blocks of W
   const v4i *ax[2];
@@ -214,7 +403,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   for (int p = 0; p < 2; ++p) ax[p] = xq + static_cast<int64_t>(min(m0 + wave + 4 * p, MT - 1)) * KS * 64 + lane;
   const v4i *bw[kTN];
 #pragma unroll
-  for (int t = 0; t < kTN; ++t) bw[t] = wq + static_cast<int64_t>(min(n0 + t, NT - 1)) * KS * 64 + lane;
+  for (int t = 0; t < kTN; ++t) bw[t] = wq + (4 * static_cast<int64_t>(min(g, NG - 1)) + t) * KS * 64 + lane;
 
   v4i acc[kTM][kTN];
 #pragma unroll
@@ -254,6 +443,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int j = 0; j < kTN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j], f[i], acc[i][j], 0, 0, 0);
     load_b(k + 2, b);
+    // Half of a step's x is read ahead of its products, the rest between them (and the writes
+    // and loads behind): 8,192^3 534 -> 514 us against the compiler's order, two reads ahead.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);  // products
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);  // LDS writes
+    __builtin_amdgcn_sched_group_barrier(0x20, 2, 0);   // loads
+    __builtin_amdgcn_sched_group_barrier(0x8, 16, 0);
+    __builtin_amdgcn_sched_group_barrier(0x20, 4, 0);
     __syncthreads();
   };
   int k = 0;
@@ -263,53 +464,96 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   if (k < KS) step(k, sh[0], sh[1], sa[1], sb[0]);
 
-  typedef typename Elem<OT>::T E;
+  if (g >= NG) return;
 #pragma unroll
   for (int i = 0; i < kTM; ++i) {
     const int64_t row = 16 * static_cast<int64_t>(m0 + i) + r16;
-    if (row >= M) continue;
-    const float sx = xs[row];
-    E *out = static_cast<E *>(y) + row * ystride;
-#pragma unroll
-    for (int j = 0; j < kTN; ++j)
-      if (n0 + j < NT) store_tile<OT, BIAS>(acc[i][j], sx, ws, bias, bias_dtype, out, 16 * (n0 + j) + 4 * kq, N, vec);
+    if (row < M) store16<OT>(o, acc[i], xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
   }
 }
 
 template <int DT>
-void launch_rows(const void *x, int64_t stride, int64_t rows, int K, void *packed, float *scales, hipStream_t s) {
+void launch_rows(const void *x, int64_t stride, int64_t rows, int K, bool weight, void *packed, float *scales,
+                 hipStream_t s) {
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * sizeof(typename Elem<DT>::T)) % 16 == 0;
   const int KS = static_cast<int>(k_steps(K));
-  const unsigned grid = static_cast<unsigned>(row_tiles(rows));
-  if (vec) rows_kernel<DT, true><<<grid, 64 * kRowWaves, 0, s>>>(x, stride, rows, K, KS, static_cast<v4i *>(packed), scales);
-  else rows_kernel<DT, false><<<grid, 64 * kRowWaves, 0, s>>>(x, stride, rows, K, KS, static_cast<v4i *>(packed), scales);
+  const unsigned grid = static_cast<unsigned>(weight ? 4 * ((rows + 63) / 64) : row_tiles(rows));
+  const int waves = std::max(1, std::min(kRowWaves, (KS + kKeep - 1) / kKeep));
+  v4i *to = static_cast<v4i *>(packed);
+  if (weight) {
+    if (vec) rows_kernel<DT, true, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+    else rows_kernel<DT, false, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+  } else {
+    if (vec) rows_kernel<DT, true, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+    else rows_kernel<DT, false, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+  }
 }
 
-void rows(const void *x, int dtype, int64_t stride, int64_t n, int K, void *packed, float *scales, hipStream_t s) {
-  if (dtype == SPK_F32) launch_rows<SPK_F32>(x, stride, n, K, packed, scales, s);
-  else if (dtype == SPK_F16) launch_rows<SPK_F16>(x, stride, n, K, packed, scales, s);
-  else launch_rows<SPK_BF16>(x, stride, n, K, packed, scales, s);
+void rows(const void *x, int dtype, int64_t stride, int64_t n, int K, bool weight, void *packed, float *scales,
+          hipStream_t s) {
+  if (dtype == SPK_F32) launch_rows<SPK_F32>(x, stride, n, K, weight, packed, scales, s);
+  else if (dtype == SPK_F16) launch_rows<SPK_F16>(x, stride, n, K, weight, packed, scales, s);
+  else launch_rows<SPK_BF16>(x, stride, n, K, weight, packed, scales, s);
+}
+
+template <int OT>
+bool aligned(const void *y, int64_t ystride) {
+  return (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ystride * sizeof(typename Elem<OT>::T) % 16 == 0;
+}
+
+template <int TM, int OT>
+void split(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y, int64_t ystride, int64_t M, int KS,
+           int64_t MT, int NG, hipStream_t s) {
+  split_kernel<TM, OT><<<static_cast<unsigned>((MT + TM - 1) / TM * NG), 64 * kSplit, 0, s>>>(xq, xs, wq, o, y, ystride, M,
+                                                                                          KS, MT, NG);
+}
+template <int TM, int OT>
+void wide(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y, int64_t ystride, int M, int KS, int MT,
+          int NG, hipStream_t s) {
+  wide_kernel<TM, OT><<<(NG + kWideWaves - 1) / kWideWaves, 64 * kWideWaves, MT * KS * 1024, s>>>(xq, xs, wq, o, y, ystride,
+                                                                                             M, KS, MT, NG);
 }
 
 template <int OT>
 void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, const void *bias, int bias_dtype, void *y,
              int64_t ystride, int64_t M, int N, int KS, hipStream_t s) {
   const int64_t MT = row_tiles(M);
-  const int NT = static_cast<int>(row_tiles(N));
-  if (M >= 512 && N >= 256) {
-    const int mtiles = static_cast<int>((M + kBM - 1) / kBM), ntiles = (N + kBN - 1) / kBN;
-    const int most = (mtiles + 7) / 8;  // row tiles of an XCD
-    const unsigned grid = 8u * ((most + 7) / 8) * 8 * ntiles;
-    typedef typename Elem<OT>::T E;
-    const bool vec = (reinterpret_cast<uintptr_t>(y) % (4 * sizeof(E))) == 0 && ystride % 4 == 0;
-    if (bias) tile_kernel<OT, true><<<grid, 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y, ystride, M, N, KS, static_cast<int>(MT), NT, mtiles, ntiles, vec);
-    else tile_kernel<OT, false><<<grid, 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y, ystride, M, N, KS, static_cast<int>(MT), NT, mtiles, ntiles, vec);
-    return;
+  const int NG = groups_of(N);
+  const Out o{ws, bias, bias_dtype, N, aligned<OT>(y, ystride)};
+  const int64_t mtiles = (M + kBM - 1) / kBM;
+  const int ntiles = (N + kBN - 1) / kBN;
+  if (MT <= 4 && NG >= 512 && MT * KS * 1024 <= kWideLds) {
+    if (MT <= 1) wide<1, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
+    else if (MT <= 2) wide<2, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
+    else wide<4, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
+  } else if (mtiles * ntiles >= 160) {
+    const int64_t most = (mtiles + 7) / 8;  // row tiles of an XCD
+    const unsigned grid = static_cast<unsigned>(8 * ((most + 7) / 8) * 8 * ntiles);
+    tile_kernel<OT><<<grid, 256, 0, s>>>(xq, xs, wq, o, y, ystride, M, KS, static_cast<int>(MT), NG, static_cast<int>(mtiles),
+                                         ntiles);
+  } else {
+    const int64_t want = 192;  // workgroups
+    if ((MT + 3) / 4 * NG >= want) split<4, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
+    else if ((MT + 1) / 2 * NG >= want) split<2, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
+    else split<1, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
   }
-  constexpr int TM = 4, TN = 4;
-  const int64_t units = (MT + TM - 1) / TM * ((NT + TN - 1) / TN);
-  product_kernel<TM, TN, OT><<<static_cast<unsigned>((units + 3) / 4), 256, 0, s>>>(xq, xs, wq, ws, bias, bias_dtype, y,
-                                                                                  ystride, M, N, KS, MT, NT);
+}
+
+template <int DT, int OT>
+void launch_fused(const void *x, int64_t stride, const v4i *wq, const Out &o, void *y, int64_t ystride, int M, int K,
+                  hipStream_t s) {
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * sizeof(typename Elem<DT>::T)) % 16 == 0;
+  const int KS = static_cast<int>(k_steps(K)), NG = groups_of(o.N);
+  if (vec) fused_kernel<DT, true, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  else fused_kernel<DT, false, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+}
+template <int OT>
+void fused(const void *x, int dtype, int64_t stride, const v4i *wq, const float *ws, const void *bias, int bias_dtype,
+           void *y, int64_t ystride, int M, int N, int K, hipStream_t s) {
+  const Out o{ws, bias, bias_dtype, N, aligned<OT>(y, ystride)};
+  if (dtype == SPK_F32) launch_fused<SPK_F32, OT>(x, stride, wq, o, y, ystride, M, K, s);
+  else if (dtype == SPK_F16) launch_fused<SPK_F16, OT>(x, stride, wq, o, y, ystride, M, K, s);
+  else launch_fused<SPK_BF16, OT>(x, stride, wq, o, y, ystride, M, K, s);
 }
 
 }  // namespace i8
@@ -326,7 +570,7 @@ static int check_sizes(const char *what, int64_t rows, int K) {
 }
 
 extern "C" size_t spk_linear_int8_packed_bytes(int N, int K) {
-  return N > 0 && K > 0 ? static_cast<size_t>(i8::packed_bytes(N, K)) : 0;
+  return N > 0 && K > 0 ? static_cast<size_t>(i8::packed_bytes(64ll * i8::groups_of(N), K)) : 0;
 }
 
 extern "C" int spk_linear_int8_pack(const void *w, int w_dtype, int64_t w_stride, int N, int K, void *packed,
@@ -336,7 +580,7 @@ extern "C" int spk_linear_int8_pack(const void *w, int w_dtype, int64_t w_stride
   if (N == 0) return SPK_OK;
   if (!w || !packed || !scales) return fail(SPK_EINVAL, "linear_int8_pack: null pointer");
   if (reinterpret_cast<uintptr_t>(packed) & 15) return fail(SPK_EINVAL, "linear_int8_pack: packed must be 16-byte aligned");
-  i8::rows(w, w_dtype, w_stride, N, K, packed, scales, static_cast<hipStream_t>(stream));
+  i8::rows(w, w_dtype, w_stride, N, K, true, packed, scales, static_cast<hipStream_t>(stream));
   return check_launch("linear_int8_pack");
 }
 
@@ -363,8 +607,14 @@ extern "C" int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, con
   const int KS = static_cast<int>(i8::k_steps(K));
   i8::v4i *xq = static_cast<i8::v4i *>(workspace);
   float *xs = reinterpret_cast<float *>(static_cast<char *>(workspace) + i8::packed_bytes(M, K));
-  i8::rows(x, x_dtype, x_stride, M, K, xq, xs, s);
   const i8::v4i *wq = static_cast<const i8::v4i *>(packed);
+  if (M <= 16 && i8::groups_of(N) < 512) {
+    if (y_dtype == SPK_F32) i8::fused<SPK_F32>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
+    else if (y_dtype == SPK_F16) i8::fused<SPK_F16>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
+    else i8::fused<SPK_BF16>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
+    return check_launch("linear_int8");
+  }
+  i8::rows(x, x_dtype, x_stride, M, K, false, xq, xs, s);
   if (y_dtype == SPK_F32) i8::product<SPK_F32>(xq, xs, wq, scales, bias, bias_dtype, y, y_stride, M, N, KS, s);
   else if (y_dtype == SPK_F16) i8::product<SPK_F16>(xq, xs, wq, scales, bias, bias_dtype, y, y_stride, M, N, KS, s);
   else i8::product<SPK_BF16>(xq, xs, wq, scales, bias, bias_dtype, y, y_stride, M, N, KS, s);

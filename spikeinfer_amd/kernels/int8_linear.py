@@ -23,7 +23,7 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 @dataclass(frozen=True)
 class Int8Weight:
     """A weight ``[out_features, in_features]`` as :func:`linear_int8` reads it: the integers in
-    the matrix instruction's order, and the output channels' scales (padded to 16)."""
+    the matrix instruction's order, and the output channels' scales (padded to 64)."""
 
     words: torch.Tensor
     scales: torch.Tensor
@@ -45,7 +45,7 @@ def pack_linear_int8(w: torch.Tensor) -> Int8Weight:
         w = w.contiguous()
     N, K = w.shape
     words = torch.empty(int(_lib.load().spk_linear_int8_packed_bytes(N, K)), dtype=torch.uint8, device=dev)
-    scales = torch.empty(-(-N // 16) * 16, dtype=torch.float32, device=dev)
+    scales = torch.empty(-(-N // 64) * 64, dtype=torch.float32, device=dev)
     _lib.check(_lib.launch("spk_linear_int8_pack", dev, w.data_ptr(), _lib.dtype_code(w.dtype), w.stride(0), N, K,
                            words.data_ptr(), scales.data_ptr()), "pack_linear_int8")
     return Int8Weight(words, scales, N, K)

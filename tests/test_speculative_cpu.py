@@ -32,7 +32,7 @@ def test_linear_refusals():
                    (dict(ws=None), 1), (dict(wsb=16), 1), (dict(ws=P + 4), 1), (dict(packed=P + 1), 1)):
         assert linear(**kw) == rc, kw
     assert linear(M=0) == _lib.SPK_OK
-    assert lib.spk_linear_int8_packed_bytes(17, 65) == 2 * 2 * 1024
+    assert lib.spk_linear_int8_packed_bytes(17, 65) == 4 * 2 * 1024
     assert lib.spk_linear_int8_packed_bytes(0, 65) == lib.spk_linear_int8_packed_bytes(4, -1) == 0
     # offsets in 64 bits
     assert lib.spk_linear_int8_packed_bytes(2**31 - 1, 131072) == 2**31 * 131072
