@@ -6,8 +6,9 @@
 // and the bias are fp32, rounded once to y's type.
 //
 // Operands lie in the order of the matrix instruction (v_mfma_i32_16x16x64_i8): 16 rows by
-// 64 k are one block of 1 KB, lane l's 16 bytes row l % 16, k 16 (l / 16) .. + 15, blocks of
-// a row tile one behind the other.  W is laid out once (spk_linear_int8_pack), x by the
+// 64 k are one block of 1 KB, lane l's 16 bytes row l % 16 and the k of 8 (l / 16) .. + 7 and
+// 32 + 8 (l / 16) .. + 7 (any order will do that is both operands'; in this one four lanes load
+// 64 bytes of a row of 16-bit numbers side by side), blocks of a row tile one behind the other.  W is laid out once (spk_linear_int8_pack), x by the
 // call's first kernel, with the same code.  W is the instruction's first operand, so a lane
 // holds four columns of one row of y; a tile of W has four runs of four of a group of 64
 // output channels (tile j of a group: channels 16 q + 4 j + e in row 4 q + e), so that the
@@ -34,60 +35,94 @@ inline int64_t packed_bytes(int64_t rows, int64_t K) { return row_tiles(rows) * 
 inline int64_t scale_bytes(int64_t rows) { return row_tiles(rows) * 64; }
 inline int groups_of(int N) { return (N + 63) / 64; }  // of 64 output channels
 
-// rint(x / s) with the quotient rounded to fp32, in -127..127.  x * (1 / s) is off by less
-// than two steps of fp32, so where it lies further than that from a half the rounding is
-// the same; only near a half is the quotient itself needed (a division is ten instructions),
-// or where 1 / s has no value (inv NaN).
-__device__ __forceinline__ int quantise(float x, float s, float inv) {
-  const float t = x * inv;
-  float r = rintf(t);
-  if (!(fabsf(fabsf(t - r) - 0.5f) >= 6.2e-5f)) r = rintf(x / s);  // 4 steps at 127
-  return static_cast<int>(fminf(fmaxf(r, -127.f), 127.f));
-}
-
-// 16 values of a row from k0 on, zeros behind K.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load16(const void *row, int k0, int K, float (&v)[16]) {
+// Sixteen elements of a row, as a block has them in a lane: eight from `k0` on and eight from
+// k0 + 32.  What lies behind K is zero.
+template <int DT>
+struct Block {
   typedef typename Elem<DT>::T E;
-  constexpr int W = Elem<DT>::kVec;
-  typedef E Vec __attribute__((ext_vector_type(W)));
-  const E *p = static_cast<const E *>(row) + k0;
-  if (VEC && k0 + 16 <= K) {
+  E e[16];
+
+  __device__ __forceinline__ void load(const void *row, int k0, int K) {
+    typedef E Eight __attribute__((ext_vector_type(8), aligned(sizeof(E))));  // (rows need no alignment)
+    const E *p = static_cast<const E *>(row);
 #pragma unroll
-    for (int q = 0; q < 16 / W; ++q) {
-      const Vec a = reinterpret_cast<const Vec *>(p)[q];
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + 32 * h;
+      if (k + 8 <= K) {
+        const Eight a = *reinterpret_cast<const Eight *>(p + k);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const E e = a[j];
-        v[q * W + j] = elem_to_f32<DT>(e);
+        for (int j = 0; j < 8; ++j) {
+          const E v = a[j];
+          e[8 * h + j] = v;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[8 * h + j] = k + j < K ? p[k + j] : static_cast<E>(0);
       }
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = k0 + j < K ? elem_to_f32<DT>(p[j]) : 0.f;
   }
-}
+  // The largest magnitude's bits as fp32 (a NaN's are the largest).
+  __device__ __forceinline__ uint32_t most() const {
+    uint32_t m = 0;
+    if constexpr (DT == SPK_F32) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(e[j]) & 0x7fffffffu);
+      return m;
+    } else {  // (16-bit numbers of either type are ordered as their bits, infinities and NaN above)
+      typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+      U2 w = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) w = __builtin_elementwise_max(w, U2{static_cast<uint16_t>(e[j] & 0x7fff), static_cast<uint16_t>(e[j + 1] & 0x7fff)});
+      m = max(w[0], w[1]);
+      return __float_as_uint(elem_to_f32<DT>(static_cast<E>(m)));
+    }
+  }
+};
 
-// The magnitudes' scale.  A row that holds an infinity or a NaN (most: the largest magnitude's
-// bits) has the scale NaN, so that its products are NaN as those of the numbers themselves
-// would be.
+// A row's scale.  A row that holds an infinity or a NaN (most: the largest magnitude's bits)
+// has the scale NaN, so that its products are NaN as those of the numbers themselves would be.
 struct Scale {
   float s, inv;
-  bool some;
+  bool some, tiny;
 };
 __device__ __forceinline__ Scale scale_of(uint32_t most) {
   const bool finite = most < 0x7f800000u;
   Scale r;
   r.s = finite ? __uint_as_float(most) / 127.f : __uint_as_float(0x7fc00000u);
   r.some = finite && r.s > 0.f;
-  r.inv = r.s >= 0x1p-100f ? 1.f / r.s : __uint_as_float(0x7fc00000u);
+  r.tiny = !(r.s >= 0x1p-100f);  // 1 / s may have no value
+  r.inv = r.tiny ? 0.f : 1.f / r.s;
   return r;
 }
-__device__ __forceinline__ v4i quantise16(const float (&v)[16], const Scale &sc) {
+
+// rint(x / s) with the quotient rounded to fp32.  x inv is off by less than two steps of fp32
+// (1.5e-5 at 127), so where it lies further than that from a half its rounding is the same; only
+// where one of the sixteen is near a half are the quotients themselves needed (a division is ten
+// instructions, this is five).  Adding 1.5 2^23 rounds to an integer in the low bits.
+template <int DT>
+__device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
   v4i out = {0, 0, 0, 0};
-  if (sc.some) {
+  if (!sc.some) return out;
+  constexpr float kMagic = 12582912.f;
+  uint32_t w[16];
+  float far = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) out[j >> 2] |= (quantise(v[j], sc.s, sc.inv) & 255) << 8 * (j & 3);
+  for (int j = 0; j < 16; ++j) {
+    const float x = elem_to_f32<DT>(b.e[j]);
+    const float y = __builtin_fmaf(x, sc.inv, kMagic);
+    far = fmaxf(far, fabsf(__builtin_fmaf(x, sc.inv, -(y - kMagic))));
+    w[j] = __float_as_uint(y);
+  }
+  if (far > 0.5f - 6.2e-5f || sc.tiny) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      w[j] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(elem_to_f32<DT>(b.e[j]) / sc.s), -127.f), 127.f)));
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t lo = __builtin_amdgcn_perm(w[4 * q + 1], w[4 * q], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(w[4 * q + 3], w[4 * q + 2], 0x0c0c0400u);
+    out[q] = static_cast<int>(lo | hi << 16);
   }
   return out;
 }
@@ -96,7 +131,7 @@ __device__ __forceinline__ v4i quantise16(const float (&v)[16], const Scale &sc)
 // blocks and keep them in registers between the two (kKeep each; longer rows are read again).
 // WEIGHT: rows in the order of the groups of output channels.  Rows that do not exist become
 // zeros.  Bound by reading x and by the latency of the two passes.
-template <int DT, bool VEC, bool WEIGHT>
+template <int DT, bool WEIGHT>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int64_t stride, int64_t rows, int K, int KS,
                                                               v4i *packed, float *scales) {
   __shared__ uint32_t most[kRowWaves][16];
@@ -105,22 +140,19 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int
   const int64_t row = WEIGHT ? tile / 4 * 64 + 16 * (r16 >> 2) + 4 * (tile & 3) + (r16 & 3) : 16 * tile + r16;
   const bool real = row < rows;
   const char *p = static_cast<const char *>(x) + (real ? row : 0) * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
+  const int Kr = real ? K : 0;
+  Block<DT> v[kKeep];
+#pragma unroll
+  for (int q = 0; q < kKeep; ++q)
+    if (wave + q * waves < KS) v[q].load(p, kStep * (wave + q * waves) + 8 * kq, Kr);
   uint32_t m = 0;
-  float v[kKeep][16];
-  auto largest = [&](const float (&a)[16]) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(a[j]) & 0x7fffffffu);  // (a NaN's bits are the largest)
-  };
 #pragma unroll
   for (int q = 0; q < kKeep; ++q)
-    if (wave + q * waves < KS) load16<DT, VEC>(p, kStep * (wave + q * waves) + 16 * kq, real ? K : 0, v[q]);
-#pragma unroll
-  for (int q = 0; q < kKeep; ++q)
-    if (wave + q * waves < KS) largest(v[q]);
+    if (wave + q * waves < KS) m = max(m, v[q].most());
   for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
-    float a[16];
-    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, a);
-    largest(a);
+    Block<DT> a;
+    a.load(p, kStep * ks + 8 * kq, Kr);
+    m = max(m, a.most());
   }
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
@@ -133,51 +165,71 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int
   for (int q = 0; q < kKeep; ++q)
     if (wave + q * waves < KS) packed[(tile * KS + wave + q * waves) * 64 + lane] = quantise16(v[q], sc);
   for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
-    float a[16];
-    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, a);
+    Block<DT> a;
+    a.load(p, kStep * ks + 8 * kq, Kr);
     packed[(tile * KS + ks) * 64 + lane] = quantise16(a, sc);
   }
 }
 
-// Sixteen columns of a row of y from column `col` on: a lane's sums of the four tiles of a group.
+// Sixteen columns of y from column `col` on, as a lane has them of a group's four tiles: the
+// channels' scales and biases, and the store of a row.
 struct Out {
   const float *ws;
   const void *bias;
   int bias_dtype;
   int N;
-  bool vec;  // 16-byte stores: y and its rows are aligned
 };
-template <int OT>
-__device__ __forceinline__ void store16(const Out &o, const v4i (&acc)[4], float sx, typename Elem<OT>::T *out, int col) {
-  typedef typename Elem<OT>::T E;
-  constexpr int W = Elem<OT>::kVec;
-  typedef E Vec __attribute__((ext_vector_type(W)));
-  typedef float F4 __attribute__((ext_vector_type(4)));
-  float f[16];
+struct Columns {
+  float s[16], b[16];
+
+  __device__ __forceinline__ Columns(const Out &o, int col) {
+    typedef float F4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const F4 s = *reinterpret_cast<const F4 *>(o.ws + col + 4 * j);  // (padded to 64)
+    for (int j = 0; j < 4; ++j) {
+      const F4 v = *reinterpret_cast<const F4 *>(o.ws + col + 4 * j);  // (padded to 64)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[4 * j + e] = static_cast<float>(acc[j][e]) * (sx * s[e]);
-  }
-  if (o.bias) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] += col + e < o.N ? load_as_f32(o.bias, col + e, o.bias_dtype) : 0.f;
-  }
-  if (o.vec && col + 16 <= o.N) {
-#pragma unroll
-    for (int h = 0; h < 16 / W; ++h) {
-      Vec v;
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[e] = f32_to_elem<OT>(f[W * h + e]);
-      *reinterpret_cast<Vec *>(out + col + W * h) = v;
+      for (int e = 0; e < 4; ++e) s[4 * j + e] = v[e];
     }
-  } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (col + e < o.N) out[col + e] = f32_to_elem<OT>(f[e]);
+    for (int e = 0; e < 16; ++e) b[e] = 0.f;
+    if (o.bias) load_bias(o, col);
   }
-}
+  __device__ __forceinline__ void load_bias(const Out &o, int col) {
+    auto all = [&](auto get) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) b[e] = get(min(col + e, o.N - 1));
+    };
+    if (o.bias_dtype == SPK_F32) all([&](int c) { return static_cast<const float *>(o.bias)[c]; });
+    else if (o.bias_dtype == SPK_F16) all([&](int c) { return static_cast<float>(static_cast<const _Float16 *>(o.bias)[c]); });
+    else all([&](int c) { return bf16_bits_to_f32(static_cast<const uint16_t *>(o.bias)[c]); });
+  }
+  template <int OT>
+  __device__ __forceinline__ void store(const Out &o, const v4i (&acc)[4], float sx, void *y, int64_t at, int col) const {
+    typedef typename Elem<OT>::T E;
+    constexpr int W = Elem<OT>::kVec;
+    typedef E Some __attribute__((ext_vector_type(W), aligned(sizeof(E))));  // (rows need no alignment)
+    E v[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[4 * j + e] = f32_to_elem<OT>(static_cast<float>(acc[j][e]) * (sx * s[4 * j + e]) + b[4 * j + e]);
+    E *out = static_cast<E *>(y) + at + col;
+    if (col + 16 <= o.N) {
+#pragma unroll
+      for (int h = 0; h < 16 / W; ++h) {
+        Some w;
+#pragma unroll
+        for (int e = 0; e < W; ++e) w[e] = v[W * h + e];
+        *reinterpret_cast<Some *>(out + W * h) = w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (col + e < o.N) out[e] = v[e];
+    }
+  }
+};
 
 // ---- few rows -----------------------------------------------------------------------
 // A workgroup TM tiles of 16 rows by one group of 64 columns; its eight waves share the steps
@@ -247,41 +299,39 @@ __global__ __launch_bounds__(64 * kSplit) void split_kernel(const v4i *xq, const
   v4i sum[4];
   join<TM>(sh, acc, sum);
   const int64_t row = 16 * (m0 + wave) + r16;
-  if (wave < TM && row < M) store16<OT>(o, sum, xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
+  const int col = 64 * g + 16 * kq;
+  if (wave < TM && row < M) Columns(o, col).store<OT>(o, sum, xs[row], y, row * ystride, col);
 }
 
-template <int DT, bool VEC, int OT>
+// HOLD: blocks of x that a wave holds; those of longer rows are read again.
+template <int DT, int HOLD, int OT>
 __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64_t stride, const v4i *wq, Out o, void *y,
                                                             int64_t ystride, int M, int K, int KS) {
-  constexpr int kHold = 2;  // blocks of x that a wave holds (K <= 1,024); the others are read again
   __shared__ v4i sh[kSplit * 4 * 64];
   __shared__ uint32_t most[kSplit][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4, g = blockIdx.x;
   const v4i *a = wq + static_cast<int64_t>(g) * 4 * KS * 64 + lane;
   const bool real = r16 < M;
   const char *p = static_cast<const char *>(x) + (real ? r16 : 0) * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
+  const int Kr = real ? K : 0;
   v4i av[2][4];
   auto load = [&](int ks, v4i (&av)[4]) {
     const int64_t at = min(ks, KS - 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t) av[t] = a[(t * static_cast<int64_t>(KS) + at) * 64];
   };
-  float v[kHold][16];
+  Block<DT> v[HOLD];
 #pragma unroll
-  for (int q = 0; q < kHold; ++q) load16<DT, VEC>(p, kStep * (wave + q * kSplit) + 16 * kq, real && wave + q * kSplit < KS ? K : 0, v[q]);
+  for (int q = 0; q < HOLD; ++q) v[q].load(p, kStep * (wave + q * kSplit) + 8 * kq, Kr);
   load(wave, av[0]);
   load(wave + kSplit, av[1]);
   uint32_t m = 0;
-  auto largest = [&](const float (&e)[16]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(e[j]) & 0x7fffffffu);
-  };
-#pragma unroll
-  for (int q = 0; q < kHold; ++q) largest(v[q]);
-  for (int ks = wave + kHold * kSplit; ks < KS; ks += kSplit) {
-    float e[16];
-    load16<DT, VEC>(p, kStep * ks + 16 * kq, real ? K : 0, e);
-    largest(e);
+  for (int q = 0; q < HOLD; ++q) m = max(m, v[q].most());
+  for (int ks = wave + HOLD * kSplit; ks < KS; ks += kSplit) {
+    Block<DT> e;
+    e.load(p, kStep * ks + 8 * kq, Kr);
+    m = max(m, e.most());
   }
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
   m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
@@ -297,17 +347,18 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[0][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[j], b, acc[0][j], 0, 0, 0);
   };
+  static_assert(HOLD % 2 == 0, "two buffers of W take turns");
 #pragma unroll
-  for (int q = 0; q < kHold; ++q) {
-    if (wave + q * kSplit < KS) products(av[q], quantise16(v[q], sc));
-    load(wave + (q + kHold) * kSplit, av[q]);
+  for (int q = 0; q < HOLD; ++q) {
+    if (wave + q * kSplit < KS) products(av[q & 1], quantise16(v[q], sc));
+    load(wave + (q + 2) * kSplit, av[q & 1]);
   }
-  for (int ks = wave + kHold * kSplit; ks < KS; ks += 2 * kSplit) {
+  for (int ks = wave + HOLD * kSplit; ks < KS; ks += 2 * kSplit) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       if (ks + q * kSplit < KS) {
-        float e[16];
-        load16<DT, VEC>(p, kStep * (ks + q * kSplit) + 16 * kq, real ? K : 0, e);
+        Block<DT> e;
+        e.load(p, kStep * (ks + q * kSplit) + 8 * kq, Kr);
         products(av[q], quantise16(e, sc));
         load(ks + (q + 2) * kSplit, av[q]);
       }
@@ -315,8 +366,8 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
   }
   v4i sum[4];
   join<1>(sh, acc, sum);
-  if (wave == 0 && real)
-    store16<OT>(o, sum, sc.s, static_cast<typename Elem<OT>::T *>(y) + r16 * ystride, 64 * g + 16 * kq);
+  const int col = 64 * g + 16 * kq;
+  if (wave == 0 && real) Columns(o, col).store<OT>(o, sum, sc.s, y, r16 * ystride, col);
 }
 
 // ---- few rows, many columns (the lm_head) ----------------------------------------------
@@ -363,10 +414,12 @@ __global__ __launch_bounds__(64 * kWideWaves) void wide_kernel(const v4i *xq, co
       }
     }
   }
+  const int col = 64 * g + 16 * kq;
+  const Columns cols(o, col);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int row = 16 * i + r16;
-    if (row < M) store16<OT>(o, acc[i], xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
+    if (row < M) cols.store<OT>(o, acc[i], xs[row], y, row * ystride, col);
   }
 }
 
@@ -386,15 +439,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int mtiles, int ntiles) {
   __shared__ v4i sh[2][kTM * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kq = lane >> 4;
-  // Tiles of one XCD (workgroup b runs on XCD b % 8): a contiguous share of the row tiles, eight
-  // of them at a time against every column tile, so that x comes into its L2 once and W
-  // once for the eight.
+  // Tiles of one XCD (workgroup b runs on XCD b % 8): a contiguous share of the tiles along
+  // the longer side, eight of them at a time against every tile of the other side, so that one
+  // operand comes into the XCD's L2 once and the other once for the eight.
   const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-  const int first = static_cast<int>(static_cast<int64_t>(mtiles) * xcd / 8);
-  const int mine = static_cast<int>(static_cast<int64_t>(mtiles) * (xcd + 1) / 8) - first;
-  const int group = idx / (8 * ntiles), in = idx - group * 8 * ntiles, rows = min(8, mine - 8 * group);
-  if (rows <= 0 || in >= rows * ntiles) return;
-  const int mt = first + 8 * group + in % rows, nt = in / rows;
+  const bool by_rows = mtiles >= ntiles;
+  const int along = by_rows ? mtiles : ntiles, across = by_rows ? ntiles : mtiles;
+  const int first = static_cast<int>(static_cast<int64_t>(along) * xcd / 8);
+  const int mine = static_cast<int>(static_cast<int64_t>(along) * (xcd + 1) / 8) - first;
+  const int group = idx / (8 * across), in = idx - group * 8 * across, some = min(8, mine - 8 * group);
+  if (some <= 0 || in >= some * across) return;
+  const int u = first + 8 * group + in % some, v = in / some;
+  const int mt = by_rows ? u : v, nt = by_rows ? v : u;
   const int m0 = mt * kTM, g = nt * (kBN / 64) + wave;
 
   // this thread's two 16-byte pieces of a step's x, its wave's four blocks of W
@@ -465,28 +521,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if (k < KS) step(k, sh[0], sh[1], sa[1], sb[0]);
 
   if (g >= NG) return;
+  const int col = 64 * g + 16 * kq;
+  const Columns cols(o, col);
 #pragma unroll
   for (int i = 0; i < kTM; ++i) {
     const int64_t row = 16 * static_cast<int64_t>(m0 + i) + r16;
-    if (row < M) store16<OT>(o, acc[i], xs[row], static_cast<typename Elem<OT>::T *>(y) + row * ystride, 64 * g + 16 * kq);
+    if (row < M) cols.store<OT>(o, acc[i], xs[row], y, row * ystride, col);
   }
 }
 
 template <int DT>
 void launch_rows(const void *x, int64_t stride, int64_t rows, int K, bool weight, void *packed, float *scales,
                  hipStream_t s) {
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * sizeof(typename Elem<DT>::T)) % 16 == 0;
   const int KS = static_cast<int>(k_steps(K));
   const unsigned grid = static_cast<unsigned>(weight ? 4 * ((rows + 63) / 64) : row_tiles(rows));
-  const int waves = std::max(1, std::min(kRowWaves, (KS + kKeep - 1) / kKeep));
+  const int waves = std::min(kRowWaves, (KS + 1) / 2);
   v4i *to = static_cast<v4i *>(packed);
-  if (weight) {
-    if (vec) rows_kernel<DT, true, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
-    else rows_kernel<DT, false, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
-  } else {
-    if (vec) rows_kernel<DT, true, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
-    else rows_kernel<DT, false, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
-  }
+  if (weight) rows_kernel<DT, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+  else rows_kernel<DT, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
 }
 
 void rows(const void *x, int dtype, int64_t stride, int64_t n, int K, bool weight, void *packed, float *scales,
@@ -494,11 +546,6 @@ void rows(const void *x, int dtype, int64_t stride, int64_t n, int K, bool weigh
   if (dtype == SPK_F32) launch_rows<SPK_F32>(x, stride, n, K, weight, packed, scales, s);
   else if (dtype == SPK_F16) launch_rows<SPK_F16>(x, stride, n, K, weight, packed, scales, s);
   else launch_rows<SPK_BF16>(x, stride, n, K, weight, packed, scales, s);
-}
-
-template <int OT>
-bool aligned(const void *y, int64_t ystride) {
-  return (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ystride * sizeof(typename Elem<OT>::T) % 16 == 0;
 }
 
 template <int TM, int OT>
@@ -519,7 +566,7 @@ void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, con
              int64_t ystride, int64_t M, int N, int KS, hipStream_t s) {
   const int64_t MT = row_tiles(M);
   const int NG = groups_of(N);
-  const Out o{ws, bias, bias_dtype, N, aligned<OT>(y, ystride)};
+  const Out o{ws, bias, bias_dtype, N};
   const int64_t mtiles = (M + kBM - 1) / kBM;
   const int ntiles = (N + kBN - 1) / kBN;
   if (MT <= 4 && NG >= 512 && MT * KS * 1024 <= kWideLds) {
@@ -527,8 +574,8 @@ void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, con
     else if (MT <= 2) wide<2, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
     else wide<4, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
   } else if (mtiles * ntiles >= 160) {
-    const int64_t most = (mtiles + 7) / 8;  // row tiles of an XCD
-    const unsigned grid = static_cast<unsigned>(8 * ((most + 7) / 8) * 8 * ntiles);
+    const int64_t along = std::max<int64_t>(mtiles, ntiles), across = std::min<int64_t>(mtiles, ntiles);
+    const unsigned grid = static_cast<unsigned>(8 * (((along + 7) / 8 + 7) / 8) * 8 * across);
     tile_kernel<OT><<<grid, 256, 0, s>>>(xq, xs, wq, o, y, ystride, M, KS, static_cast<int>(MT), NG, static_cast<int>(mtiles),
                                          ntiles);
   } else {
@@ -542,15 +589,14 @@ void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, con
 template <int DT, int OT>
 void launch_fused(const void *x, int64_t stride, const v4i *wq, const Out &o, void *y, int64_t ystride, int M, int K,
                   hipStream_t s) {
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * sizeof(typename Elem<DT>::T)) % 16 == 0;
   const int KS = static_cast<int>(k_steps(K)), NG = groups_of(o.N);
-  if (vec) fused_kernel<DT, true, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
-  else fused_kernel<DT, false, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  if (KS <= 2 * kSplit) fused_kernel<DT, 2, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  else fused_kernel<DT, 10, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
 }
 template <int OT>
 void fused(const void *x, int dtype, int64_t stride, const v4i *wq, const float *ws, const void *bias, int bias_dtype,
            void *y, int64_t ystride, int M, int N, int K, hipStream_t s) {
-  const Out o{ws, bias, bias_dtype, N, aligned<OT>(y, ystride)};
+  const Out o{ws, bias, bias_dtype, N};
   if (dtype == SPK_F32) launch_fused<SPK_F32, OT>(x, stride, wq, o, y, ystride, M, K, s);
   else if (dtype == SPK_F16) launch_fused<SPK_F16, OT>(x, stride, wq, o, y, ystride, M, K, s);
   else launch_fused<SPK_BF16, OT>(x, stride, wq, o, y, ystride, M, K, s);
