@@ -15,6 +15,7 @@
 // four tiles of a group give a lane 16 columns side by side, and a wave writes whole 128-byte
 // lines of y (8,188 x 9,728 of K = 64, nearly all stores: 67 -> 43 us).
 #include <algorithm>
+#include <cmath>
 
 #include "common.hpp"
 #include "lif_math.hpp"
@@ -561,28 +562,45 @@ void wide(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y, 
                                                                                              M, KS, MT, NG);
 }
 
+// The kernel for a size: the least of the times, in us, that fits to measurements give (64 to 2,048
+// rows, 512 to 9,728 columns, K = 896 and 4,864; within a fifth, near their borders).  Measured,
+// with one, two, four row tiles a workgroup of the split kernel and with large tiles: 64 x 896 x
+// 896 3.6, 4.1, 5.1, 9.1; 256 x 9,728 x 896 16.1, 12.5, 14.0, 12.4; 1,024 x 896 x 4,864 20.5,
+// 14.9, 12.9, 32.5; 2,048 x 4,864 x 896 57, 42, 44, 21.
+enum Way { kSplit1, kSplit2, kSplit4, kTiles };
+inline Way way(int64_t M, int N, int KS, int out_bytes) {
+  const double ks = KS, ng = groups_of(N), mt = static_cast<double>(row_tiles(M));
+  const int64_t tiles = (M + kBM - 1) / kBM * ((N + kBN - 1) / kBN);
+  const double t[] = {3.0 + 0.041 * ks + mt * ng * (0.0020 + 0.00025 * ks),
+                      3.5 + 0.041 * ks + std::ceil(mt / 2) * ng * (0.0039 + 0.00031 * ks),
+                      4.5 + 0.052 * ks + std::ceil(mt / 4) * ng * (0.0108 + 0.00044 * ks),
+                      7.0 + 0.33 * ks * static_cast<double>((tiles + 255) / 256) + static_cast<double>(M) * N * out_bytes / 3.7e6};
+  return static_cast<Way>(std::min_element(t, t + 4) - t);
+}
+
 template <int OT>
 void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, const void *bias, int bias_dtype, void *y,
              int64_t ystride, int64_t M, int N, int KS, hipStream_t s) {
   const int64_t MT = row_tiles(M);
   const int NG = groups_of(N);
   const Out o{ws, bias, bias_dtype, N};
-  const int64_t mtiles = (M + kBM - 1) / kBM;
-  const int ntiles = (N + kBN - 1) / kBN;
   if (MT <= 4 && NG >= 512 && MT * KS * 1024 <= kWideLds) {
     if (MT <= 1) wide<1, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
     else if (MT <= 2) wide<2, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
     else wide<4, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
-  } else if (mtiles * ntiles >= 160) {
-    const int64_t along = std::max<int64_t>(mtiles, ntiles), across = std::min<int64_t>(mtiles, ntiles);
-    const unsigned grid = static_cast<unsigned>(8 * (((along + 7) / 8 + 7) / 8) * 8 * across);
-    tile_kernel<OT><<<grid, 256, 0, s>>>(xq, xs, wq, o, y, ystride, M, KS, static_cast<int>(MT), NG, static_cast<int>(mtiles),
-                                         ntiles);
-  } else {
-    const int64_t want = 192;  // workgroups
-    if ((MT + 3) / 4 * NG >= want) split<4, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
-    else if ((MT + 1) / 2 * NG >= want) split<2, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
-    else split<1, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s);
+    return;
+  }
+  switch (way(M, N, KS, sizeof(typename Elem<OT>::T))) {
+    case kSplit1: split<1, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
+    case kSplit2: split<2, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
+    case kSplit4: split<4, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
+    default: {
+      const int64_t mtiles = (M + kBM - 1) / kBM, ntiles = (N + kBN - 1) / kBN;
+      const int64_t along = std::max(mtiles, ntiles), across = std::min(mtiles, ntiles);
+      const unsigned grid = static_cast<unsigned>(8 * (((along + 7) / 8 + 7) / 8) * 8 * across);
+      tile_kernel<OT><<<grid, 256, 0, s>>>(xq, xs, wq, o, y, ystride, M, KS, static_cast<int>(MT), NG, static_cast<int>(mtiles),
+                                           static_cast<int>(ntiles));
+    }
   }
 }
 
