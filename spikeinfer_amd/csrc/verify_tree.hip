@@ -10,13 +10,13 @@
 // token that did not stay has w = 0 afterwards either way.  Where no child stays, the token
 // is the first whose cumulative w exceeds u (row 0's) times the sum.
 //
-// A test needs two numbers, a rejection the sum over the vocabulary (two rows of it).  The
-// sums' passes are split over workgroups: launch r of the walk follows each tree up to its
-// r-th sum (the sums before it are there, so every workgroup repeats the walk in a few
-// dependent loads), and its slices add up their share.  The last launch, one workgroup a
-// tree, follows the walk to its end, sums by itself where a tree needs more, and draws.
-// Sums and tests are fp64: a decision differs from exact arithmetic's only where the numbers
-// are equal to 15 digits.
+// A test needs two numbers, all trees' of which are loaded at once before the walk; a rejection
+// needs the sum over the vocabulary, two rows of it.  These passes are split over workgroups:
+// launch r follows each tree up to its r-th sum (the sums before it are there, so every
+// workgroup repeats the walk, in LDS), and its slices add up their share.  The last launch,
+// one workgroup a tree, follows the walk to its end, sums by itself where a tree needs more, and
+// draws.  Bound by reading the rows: 64 chains, 78 MB.  Sums and tests are fp64: a decision
+// differs from exact arithmetic's only where the numbers are equal to 15 digits.
 #include <algorithm>
 
 #include "common.hpp"
@@ -28,8 +28,14 @@ namespace verify {
 using draft::kMaxNodes;
 constexpr int kSliceThreads = 256;
 constexpr int kEndThreads = 1024;
-constexpr int kMaxSlices = 64;
-constexpr int kRounds = 1;
+constexpr int kMaxSlices = 64;  // a lane each
+constexpr int kMaxRounds = 4;
+
+// Launches of slices.  A chain needs one sum, a tree one a rejected sibling, a few as a rule;
+// those that are left to the last launch take a workgroup 10 us each at 151,936 tokens, a
+// launch that finds every tree done about 2.  (16 trees of 25 nodes with up to three siblings,
+// one launch to five: FIGURES.)
+inline int rounds_for(int max_nodes) { return std::min(kMaxRounds, 1 + (max_nodes - 1) / 8); }
 
 struct Params {
   const int64_t *tokens;
@@ -38,14 +44,15 @@ struct Params {
   int64_t ps, qs;  // row strides
   int64_t rows;
   int max_nodes, V, distinct, G, round;
-  double *part;  // [round][tree][slice]
+  double *part;   // [round][tree][slice]
+  int32_t *done;  // [tree]: the launch that found its sums complete; written before it is read
   int64_t *out;
 };
 
 struct Shared {
   int64_t tok[kMaxNodes], target[kMaxNodes];
   int32_t par[kMaxNodes];
-  float u[kMaxNodes];
+  float u[kMaxNodes], p[kMaxNodes], q[kMaxNodes];  // p and q of each row's token after its parent
   double part[kMaxSlices], wave[kEndThreads / 64];
   int found, last;
 };
@@ -54,6 +61,11 @@ __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   return v;
+}
+// The sum of the slices' sums, in one order.
+__device__ __forceinline__ double total_of(const double *part, int G) {
+  const int lane = threadIdx.x & 63;
+  return wave_sum(lane < G ? part[lane] : 0.0);
 }
 
 // A tree's walk.  Every thread of a workgroup follows it with the same numbers.
@@ -67,13 +79,26 @@ struct Walk {
   __device__ __forceinline__ const float *prow() const { return P.p + (r.first + at) * P.ps; }
   __device__ __forceinline__ const float *qrow() const { return P.q + (r.first + at) * P.qs; }
 
+  __device__ __forceinline__ void load() {
+    for (int i = threadIdx.x; i < r.count; i += blockDim.x) {
+      const int64_t x = P.tokens[r.first + i];
+      const int up = P.parents[r.first + i];
+      const bool child = up >= 0 && up < i && x >= 0 && x < P.V;
+      sh.tok[i] = x;
+      sh.par[i] = up;
+      sh.u[i] = P.u[r.first + i];
+      sh.p[i] = child ? P.p[(r.first + up) * P.ps + x] : 0.f;
+      sh.q[i] = child ? P.q[(r.first + up) * P.qs + x] : 0.f;
+      sh.target[i] = -1;
+    }
+  }
   __device__ __forceinline__ void go(int row) {
     at = row;
     next = row + 1;
     A = before = 0.0;
     mass = 1.0;
   }
-  // The lowest-numbered child of `at` from row `next` on that `ok` takes, or -1.
+  // The lowest-numbered child of `at` from row `from` on that `ok` takes, or -1.
   template <class Ok>
   __device__ __forceinline__ int child(int from, Ok ok) const {
     const int lane = threadIdx.x & 63;
@@ -90,9 +115,7 @@ struct Walk {
     for (;;) {
       const int i = child(next, [](int) { return true; });
       if (i < 0) return true;
-      const int64_t x = sh.tok[i];
-      double px = 0.0, qx = 0.0;
-      if (x >= 0 && x < P.V) px = prow()[x], qx = qrow()[x];
+      const double px = sh.p[i], qx = sh.q[i];
       const double w = fmax(px - A * qx, 0.0);
       double c = mass;
       if (P.distinct) {
@@ -100,7 +123,7 @@ struct Walk {
         if (left > 0.0) c /= left;
       }
       if (static_cast<double>(sh.u[i]) * qx * c < w) {
-        if (threadIdx.x == 0) sh.target[at] = x;
+        if (threadIdx.x == 0) sh.target[at] = sh.tok[i];
         go(i);
         continue;
       }
@@ -110,56 +133,77 @@ struct Walk {
       return false;
     }
   }
-  __device__ __forceinline__ double weight(const float *p, const float *q, int x) const {
-    const double v = p[x];
-    return fmax(A == 0.0 ? v : v - A * static_cast<double>(q[x]), 0.0);
-  }
   __device__ __forceinline__ int begin(int slice) const {
     return static_cast<int>(static_cast<int64_t>(P.V) * slice / P.G);
   }
-};
-
-__device__ __forceinline__ void load_tree(const Params &P, Shared &sh, const draft::Rows &r) {
-  for (int i = threadIdx.x; i < r.count; i += blockDim.x) {
-    sh.tok[i] = P.tokens[r.first + i];
-    sh.par[i] = P.parents[r.first + i];
-    sh.u[i] = P.u[r.first + i];
-    sh.target[i] = -1;
+  // Weights of the tokens x .. x + 3 that lie below `end`, 0 for the others.
+  __device__ __forceinline__ void weights(const float *p, const float *q, int x, int end, double (&w)[4]) const {
+    typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+    F4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    if (x + 4 <= end) {
+      a = *reinterpret_cast<const F4 *>(p + x);
+      if (A != 0.0) b = *reinterpret_cast<const F4 *>(q + x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x + j < end) {
+          a[j] = p[x + j];
+          if (A != 0.0) b[j] = q[x + j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // (a NaN has none; A may be infinite)
+      const double v = a[j];
+      w[j] = fmax(A == 0.0 ? v : v - A * static_cast<double>(b[j]), 0.0);
+    }
   }
-}
-
-// The sum of the slices' partial sums, in their order.
-__device__ __forceinline__ double total_of(const double *part, int G) {
-  double s = 0.0;
-  for (int g = 0; g < G; ++g) s += part[g];
-  return s;
-}
+  // This thread's share of a slice's sum, `threads` of them from number `me` on.
+  __device__ __forceinline__ double share(int slice, int me, int threads) const {
+    const float *p = prow(), *q = qrow();
+    const int end = begin(slice + 1);
+    double s = 0.0;
+#pragma unroll 4
+    for (int x = begin(slice) + 4 * me; x < end; x += 4 * threads) {
+      double w[4];
+      weights(p, q, x, end, w);
+      s += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    return s;
+  }
+};
 
 __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Params P) {
   __shared__ Shared sh;
   const int n = blockIdx.y, tid = threadIdx.x, N = gridDim.y;
+  if (P.round > 0 && P.done[n] < P.round) return;
   Walk w{P, sh, draft::rows_of(P.starts, n, P.rows, P.max_nodes)};
-  if (w.r.count == 0) return;
-  load_tree(P, sh, w.r);
-  __syncthreads();
-  w.go(0);
-  bool draw = w.tests();
-  for (int k = 0; k < P.round; ++k) {
-    if (draw) return;  // this tree's last sum is there
-    w.mass = total_of(P.part + (static_cast<int64_t>(k) * N + n) * P.G, P.G);
-    draw = w.tests();
-    // (after the last child the sum that was just taken is the draw's)
-    if (draw && w.A != 0.0) return;
+  bool more = w.r.count > 0;
+  if (more) {
+    w.load();
+    __syncthreads();
+    w.go(0);
+    bool draw = w.tests();
+    for (int k = 0; k < P.round && more; ++k) {
+      if (draw) {  // this tree's last sum is there
+        more = false;
+        break;
+      }
+      w.mass = total_of(P.part + (static_cast<int64_t>(k) * N + n) * P.G, P.G);
+      draw = w.tests();
+      more = !(draw && w.A != 0.0);  // (after the last child the sum that was just taken is the draw's)
+    }
   }
-  const float *p = w.prow(), *q = w.qrow();
-  double s = 0.0;
-  for (int x = w.begin(blockIdx.x) + tid; x < w.begin(blockIdx.x + 1); x += kSliceThreads) s += w.weight(p, q, x);
-  s = wave_sum(s);
+  if (!more) {  // (the launch that finds it tells the ones behind)
+    if (tid == 0 && blockIdx.x == 0) P.done[n] = P.round;
+    return;
+  }
+  double s = wave_sum(w.share(blockIdx.x, tid, kSliceThreads));
   if ((tid & 63) == 0) sh.wave[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) {
     for (int k = 1; k < kSliceThreads / 64; ++k) s += sh.wave[k];
     P.part[(static_cast<int64_t>(P.round) * N + n) * P.G + blockIdx.x] = s;
+    if (P.round == 0 && blockIdx.x == 0) P.done[n] = kMaxRounds;
   }
 }
 
@@ -168,7 +212,7 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
   const int n = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, N = gridDim.x;
   Walk w{P, sh, draft::rows_of(P.starts, n, P.rows, P.max_nodes)};
   if (w.r.count == 0) return;
-  load_tree(P, sh, w.r);
+  w.load();
   __syncthreads();
   int taken = 0;  // sums used of the launches before
   auto sum = [&] {  // the slices' sums into sh.part
@@ -177,11 +221,8 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
       const double *part = P.part + (static_cast<int64_t>(taken++) * N + n) * P.G;
       if (tid < P.G) sh.part[tid] = part[tid];
     } else {
-      const float *p = w.prow(), *q = w.qrow();
       for (int g = wave; g < P.G; g += kEndThreads / 64) {
-        double s = 0.0;
-        for (int x = w.begin(g) + lane; x < w.begin(g + 1); x += 64) s += w.weight(p, q, x);
-        s = wave_sum(s);
+        const double s = wave_sum(w.share(g, lane, 64));
         if (lane == 0) sh.part[g] = s;
       }
     }
@@ -203,52 +244,55 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
       w.mass = sum();
     }
     if (!(w.mass > 0.0)) break;  // no token
-    // the slice that holds u times the sum, then the token in it
+    // the slice that holds u times the sum, or the last with any weight, then the token in it
     const double t = static_cast<double>(sh.u[0]) * w.mass;
-    double below = 0.0, cum = 0.0;
-    int slice = 0;
-    for (int g = 0; g < P.G; ++g) {
-      const double s = sh.part[g];
-      if (s > 0.0) {
-        slice = g;
-        below = cum;
-        if (cum + s > t) break;
-      }
-      cum += s;
+    const double own = lane < P.G ? sh.part[lane] : 0.0;
+    double upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
     }
+    const uint64_t some = __ballot(own > 0.0), past = __ballot(own > 0.0 && upto > t);
+    const int slice = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some | 1);
+    double below = __shfl(upto - own, slice);
     const float *p = w.prow(), *q = w.qrow();
-    const int b = w.begin(slice), e = w.begin(slice + 1), each = (e - b + kEndThreads - 1) / kEndThreads;
-    const int x0 = min(b + tid * each, e), x1 = min(x0 + each, e);
-    double mine = 0.0;
-    for (int x = x0; x < x1; ++x) mine += w.weight(p, q, x);
+    const int b = w.begin(slice), e = w.begin(slice + 1);
+    const int each = 4 * ((e - b + 4 * kEndThreads - 1) / (4 * kEndThreads)), x0 = b + tid * each, x1 = min(x0 + each, e);
+    double v[4], mine = 0.0;
+    for (int x = x0; x < x1; x += 4) {
+      w.weights(p, q, x, x1, v);
+      mine += (v[0] + v[1]) + (v[2] + v[3]);
+    }
     double inc = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const double o = __shfl_up(inc, d);
       if (lane >= d) inc += o;
     }
+    __syncthreads();  // (the walk's and the last draw's reads are over)
     if (lane == 63) sh.wave[wave] = inc;
     if (tid == 0) sh.found = P.V, sh.last = -1;
     __syncthreads();
     for (int k = 0; k < wave; ++k) below += sh.wave[k];
-    double c = below + (inc - mine);
     if (mine > 0.0) {
-      int last = -1;
-      for (int x = x0; x < x1; ++x) {
-        const double v = w.weight(p, q, x);
-        if (!(v > 0.0)) continue;
-        last = x;
-        c += v;
-        if (c > t) {
-          atomicMin(&sh.found, x);
-          break;
-        }
+      double c = below + (inc - mine);
+      int last = -1, found = P.V;
+      for (int x = x0; x < x1 && found == P.V; x += 4) {
+        if (each > 4) w.weights(p, q, x, x1, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v[j] > 0.0 && found == P.V) {
+            last = x + j;
+            c += v[j];
+            if (c > t) found = x + j;
+          }
       }
+      if (found < P.V) atomicMin(&sh.found, found);
       atomicMax(&sh.last, last);
     }
     __syncthreads();
     const int token = sh.found < P.V ? sh.found : sh.last;  // (rounding may leave t at the slice's end)
-    __syncthreads();
     if (token < 0) break;
     if (tid == 0) sh.target[w.at] = token;
     // A drafted token that was not given its weight may be drawn after all: the walk of the
@@ -273,7 +317,7 @@ static int verify_slices(int N, int V) {
 }
 
 extern "C" size_t spk_verify_tree_workspace_bytes(int N, int V) {
-  return N > 0 && V > 0 ? static_cast<size_t>(verify::kRounds) * N * verify_slices(N, V) * 8 : 0;
+  return N > 0 && V > 0 ? static_cast<size_t>(N) * (verify::kMaxRounds * verify_slices(N, V) * 8 + 8) : 0;
 }
 
 extern "C" int spk_verify_tree(const int64_t *tokens, const int32_t *parents, const float *target_probs,
@@ -293,11 +337,14 @@ extern "C" int spk_verify_tree(const int64_t *tokens, const int32_t *parents, co
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(SPK_EINVAL, "verify_tree: workspace of %zu bytes, %zu needed, aligned to 8", workspace ? workspace_bytes : 0,
                 need);
+  const int G = verify_slices(N, V), rounds = verify::rounds_for(max_nodes);
+  double *part = static_cast<double *>(workspace);
   verify::Params P{tokens, parents, row_starts, target_probs, draft_probs, uniforms, target_stride, draft_stride, rows,
-                   max_nodes, V, distinct, verify_slices(N, V), 0, static_cast<double *>(workspace), targets};
+                   max_nodes, V, distinct, G, 0, part,
+                   reinterpret_cast<int32_t *>(part + static_cast<size_t>(verify::kMaxRounds) * N * G), targets};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  for (; P.round < verify::kRounds; ++P.round)
-    verify::slice_kernel<<<dim3(P.G, N), verify::kSliceThreads, 0, s>>>(P);
+  for (; P.round < rounds; ++P.round)
+    verify::slice_kernel<<<dim3(G, N), verify::kSliceThreads, 0, s>>>(P);
   verify::end_kernel<<<N, verify::kEndThreads, 0, s>>>(P);
   return check_launch("verify_tree");
 }
