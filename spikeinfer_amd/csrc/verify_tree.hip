@@ -45,7 +45,7 @@ struct Params {
   int64_t rows;
   int max_nodes, V, distinct, G, round;
   double *part;   // [round][tree][slice]
-  int32_t *done;  // [tree]: the launch that found its sums complete; written before it is read
+  int32_t *done;  // [tree]: the launch behind which its sums are complete (kMaxRounds: not known yet)
   int64_t *out;
 };
 
@@ -53,8 +53,11 @@ struct Shared {
   int64_t tok[kMaxNodes], target[kMaxNodes];
   int32_t par[kMaxNodes];
   float u[kMaxNodes], p[kMaxNodes], q[kMaxNodes];  // p and q of each row's token after its parent
+  uint8_t stays[kMaxNodes];  // whether it does as its parent's first child
   double part[kMaxSlices], wave[kEndThreads / 64];
-  int found, last;
+  double A;  // the walk's, for the waves that do not follow it
+  int at, draw;
+  int found, last, token;
 };
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -68,7 +71,8 @@ __device__ __forceinline__ double total_of(const double *part, int G) {
   return wave_sum(lane < G ? part[lane] : 0.0);
 }
 
-// A tree's walk.  Every thread of a workgroup follows it with the same numbers.
+// A tree's walk.  The first wave follows it (sixteen would get in each other's way: 0.35 us
+// a row against 0.1), the others get the row and A.
 struct Walk {
   const Params &P;
   Shared &sh;
@@ -79,16 +83,32 @@ struct Walk {
   __device__ __forceinline__ const float *prow() const { return P.p + (r.first + at) * P.ps; }
   __device__ __forceinline__ const float *qrow() const { return P.q + (r.first + at) * P.qs; }
 
+  // What c is, divided by what q leaves to a token with qx.
+  __device__ __forceinline__ double scaled(double c, double qx) const {
+    if (P.distinct) {
+      const double left = fmax(1.0 - before, qx);
+      if (left > 0.0) c /= left;
+    }
+    return c;
+  }
+  __device__ __forceinline__ bool test(double u, double px, double qx, double c) const {
+    return u * qx * c < fmax(px - A * qx, 0.0);
+  }
   __device__ __forceinline__ void load() {
+    go(0);
     for (int i = threadIdx.x; i < r.count; i += blockDim.x) {
       const int64_t x = P.tokens[r.first + i];
       const int up = P.parents[r.first + i];
       const bool child = up >= 0 && up < i && x >= 0 && x < P.V;
+      const float u = P.u[r.first + i];
+      const float px = child ? P.p[(r.first + up) * P.ps + x] : 0.f;
+      const float qx = child ? P.q[(r.first + up) * P.qs + x] : 0.f;
       sh.tok[i] = x;
       sh.par[i] = up;
-      sh.u[i] = P.u[r.first + i];
-      sh.p[i] = child ? P.p[(r.first + up) * P.ps + x] : 0.f;
-      sh.q[i] = child ? P.q[(r.first + up) * P.qs + x] : 0.f;
+      sh.u[i] = u;
+      sh.p[i] = px;
+      sh.q[i] = qx;
+      sh.stays[i] = test(u, px, qx, scaled(1.0, qx));
       sh.target[i] = -1;
     }
   }
@@ -109,20 +129,31 @@ struct Walk {
     }
     return -1;
   }
+  // tests() for the workgroup.
+  __device__ __forceinline__ bool follow() {
+    __syncthreads();  // (what the last one wrote is read)
+    if (threadIdx.x < 64) {
+      const bool draw = tests();
+      if (threadIdx.x == 0) sh.at = at, sh.A = A, sh.draw = draw;
+    }
+    __syncthreads();
+    at = sh.at;
+    A = sh.A;
+    return sh.draw;
+  }
   // Tests children until a sum over the vocabulary is needed, for the next test or (true) for
   // the draw.
   __device__ __forceinline__ bool tests() {
     for (;;) {
       const int i = child(next, [](int) { return true; });
       if (i < 0) return true;
-      const double px = sh.p[i], qx = sh.q[i];
-      const double w = fmax(px - A * qx, 0.0);
-      double c = mass;
-      if (P.distinct) {
-        const double left = fmax(1.0 - before, qx);
-        if (left > 0.0) c /= left;
+      if (A == 0.0 && sh.stays[i]) {  // (a path is mostly first children)
+        if (threadIdx.x == 0) sh.target[at] = sh.tok[i];
+        go(i);
+        continue;
       }
-      if (static_cast<double>(sh.u[i]) * qx * c < w) {
+      const double px = sh.p[i], qx = sh.q[i], c = scaled(mass, qx);
+      if (A != 0.0 && test(sh.u[i], px, qx, c)) {
         if (threadIdx.x == 0) sh.target[at] = sh.tok[i];
         go(i);
         continue;
@@ -177,33 +208,28 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Params P) {
   const int n = blockIdx.y, tid = threadIdx.x, N = gridDim.y;
   if (P.round > 0 && P.done[n] < P.round) return;
   Walk w{P, sh, draft::rows_of(P.starts, n, P.rows, P.max_nodes)};
-  bool more = w.r.count > 0;
-  if (more) {
-    w.load();
-    __syncthreads();
-    w.go(0);
-    bool draw = w.tests();
-    for (int k = 0; k < P.round && more; ++k) {
-      if (draw) {  // this tree's last sum is there
-        more = false;
-        break;
-      }
-      w.mass = total_of(P.part + (static_cast<int64_t>(k) * N + n) * P.G, P.G);
-      draw = w.tests();
-      more = !(draw && w.A != 0.0);  // (after the last child the sum that was just taken is the draw's)
-    }
-  }
-  if (!more) {  // (the launch that finds it tells the ones behind)
-    if (tid == 0 && blockIdx.x == 0) P.done[n] = P.round;
+  if (w.r.count == 0) {
+    if (tid == 0 && blockIdx.x == 0) P.done[n] = -1;
     return;
   }
+  w.load();
+  __syncthreads();
+  // (a tree whose sums are complete did not get here: the k sums before were not its last)
+  bool draw = w.follow();
+  for (int k = 0; k < P.round; ++k) {
+    w.mass = total_of(P.part + (static_cast<int64_t>(k) * N + n) * P.G, P.G);
+    draw = w.follow();
+  }
+  // Is this the last sum, the draw's or the one behind the last child?  (A child that stays
+  // leads on; one whose test the sum decides may.)
+  const bool last = draw || w.child(w.next, [](int) { return true; }) < 0;  // (the first wave's)
   double s = wave_sum(w.share(blockIdx.x, tid, kSliceThreads));
   if ((tid & 63) == 0) sh.wave[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) {
     for (int k = 1; k < kSliceThreads / 64; ++k) s += sh.wave[k];
     P.part[(static_cast<int64_t>(P.round) * N + n) * P.G + blockIdx.x] = s;
-    if (P.round == 0 && blockIdx.x == 0) P.done[n] = kMaxRounds;
+    if (blockIdx.x == 0) P.done[n] = last ? P.round : kMaxRounds;
   }
 }
 
@@ -212,14 +238,16 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
   const int n = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, N = gridDim.x;
   Walk w{P, sh, draft::rows_of(P.starts, n, P.rows, P.max_nodes)};
   if (w.r.count == 0) return;
+  const double first = P.round > 0 && tid < P.G ? P.part[static_cast<int64_t>(n) * P.G + tid] : 0.0;  // (asked for early)
   w.load();
   __syncthreads();
   int taken = 0;  // sums used of the launches before
   auto sum = [&] {  // the slices' sums into sh.part
     __syncthreads();
     if (taken < P.round) {
-      const double *part = P.part + (static_cast<int64_t>(taken++) * N + n) * P.G;
-      if (tid < P.G) sh.part[tid] = part[tid];
+      const double *part = P.part + (static_cast<int64_t>(taken) * N + n) * P.G;
+      if (tid < P.G) sh.part[tid] = taken ? part[tid] : first;
+      ++taken;
     } else {
       for (int g = wave; g < P.G; g += kEndThreads / 64) {
         const double s = wave_sum(w.share(g, lane, 64));
@@ -229,11 +257,10 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
     __syncthreads();
     return total_of(sh.part, P.G);
   };
-  w.go(0);
   while (true) {
     // the children, one sum a rejection; `fresh`: sh.part is of the weights as they are
     bool fresh = false;
-    while (!w.tests()) {
+    while (!w.follow()) {
       w.mass = sum();
       fresh = true;
     }
@@ -270,29 +297,39 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
       const double o = __shfl_up(inc, d);
       if (lane >= d) inc += o;
     }
-    __syncthreads();  // (the walk's and the last draw's reads are over)
+    __syncthreads();  // (the last draw's reads are over)
     if (lane == 63) sh.wave[wave] = inc;
-    if (tid == 0) sh.found = P.V, sh.last = -1;
+    if (tid == 0) sh.found = kEndThreads, sh.last = -1;
     __syncthreads();
-    for (int k = 0; k < wave; ++k) below += sh.wave[k];
-    if (mine > 0.0) {
+    double waves = lane < kEndThreads / 64 ? sh.wave[lane] : 0.0;
+#pragma unroll
+    for (int d = 1; d < kEndThreads / 64; d <<= 1) {
+      const double o = __shfl_up(waves, d);
+      if (lane >= d) waves += o;
+    }
+    waves = __shfl(waves, max(wave - 1, 0));
+    if (wave > 0) below += waves;
+    // the first thread whose tokens reach t (rounding may leave t behind them all: the last)
+    const uint64_t have = __ballot(mine > 0.0), reach = __ballot(mine > 0.0 && below + inc > t);
+    if (lane == 0 && reach) atomicMin(&sh.found, 64 * wave + __builtin_ctzll(reach));
+    if (lane == 0 && have) atomicMax(&sh.last, 64 * wave + 63 - __builtin_clzll(have));
+    __syncthreads();
+    if (tid == (sh.found < kEndThreads ? sh.found : sh.last)) {
       double c = below + (inc - mine);
-      int last = -1, found = P.V;
-      for (int x = x0; x < x1 && found == P.V; x += 4) {
+      int token = -1;
+      for (int x = x0; x < x1 && !(c > t); x += 4) {
         if (each > 4) w.weights(p, q, x, x1, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (v[j] > 0.0 && found == P.V) {
-            last = x + j;
+          if (v[j] > 0.0 && !(c > t)) {
+            token = x + j;
             c += v[j];
-            if (c > t) found = x + j;
           }
       }
-      if (found < P.V) atomicMin(&sh.found, found);
-      atomicMax(&sh.last, last);
+      sh.token = token;
     }
     __syncthreads();
-    const int token = sh.found < P.V ? sh.found : sh.last;  // (rounding may leave t at the slice's end)
+    const int token = sh.last < 0 ? -1 : sh.token;
     if (token < 0) break;
     if (tid == 0) sh.target[w.at] = token;
     // A drafted token that was not given its weight may be drawn after all: the walk of the
