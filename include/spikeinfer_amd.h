@@ -751,7 +751,7 @@ int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_stri
  *   packed   spk_linear_int8_packed_bytes(N, K) bytes, 16-byte aligned, and scales float
  *            [N rounded up to 64]: written by spk_linear_int8_pack, once per weight
  *   workspace spk_linear_int8_workspace_bytes(M, N, K) bytes, 16-byte aligned
- * K <= 131072 (the sums are 32 bits), M <= 2^30 (SPK_EUNSUPPORTED beyond).
+ * K <= 131072 (the sums are 32 bits), M and N <= 2^30 (SPK_EUNSUPPORTED beyond).
  */
 size_t spk_linear_int8_packed_bytes(int N, int K);
 int spk_linear_int8_pack(const void *w, int w_dtype, int64_t w_stride, int N, int K, void *packed,

@@ -205,7 +205,8 @@ NATIVE_FUNCTIONS = (
     "spk_prefill_attn", "spk_embed_rmsnorm", "spk_add_rmsnorm", "spk_rmsnorm_mean_t", "spk_lif_gate_mul",
     "spk_linear_decode", "spk_mlp_gate_lif", "spk_qkv_rope_lif_pack_kv", "spk_tree_attn",
     "spk_tree_attn_workspace_bytes", "spk_accept_tree", "spk_key_mass", "spk_key_mass_workspace_bytes", "spk_evict",
-    "spk_last_error",
+    "spk_linear_int8", "spk_linear_int8_workspace_bytes", "spk_sample_probs", "spk_sample_probs_workspace_bytes",
+    "spk_verify_tree", "spk_verify_tree_workspace_bytes", "spk_last_error",
 )
 
 _UNBOUND = object()

@@ -30,11 +30,12 @@ constexpr int kMaxK = 131072;  // 127^2 kMaxK < 2^31
 constexpr int kRowWaves = 16;  // at most, of a tile of rows
 constexpr int kKeep = 5;       // blocks a wave keeps between the two passes
 
+inline int row_waves(int KS) { return std::min(kRowWaves, (KS + 1) / 2); }
 inline int64_t row_tiles(int64_t rows) { return (rows + 15) / 16; }
 inline int64_t k_steps(int64_t K) { return (K + kStep - 1) / kStep; }
 inline int64_t packed_bytes(int64_t rows, int64_t K) { return row_tiles(rows) * k_steps(K) * 1024; }
 inline int64_t scale_bytes(int64_t rows) { return row_tiles(rows) * 64; }
-inline int groups_of(int N) { return (N + 63) / 64; }  // of 64 output channels
+inline int groups_of(int64_t N) { return static_cast<int>((N + 63) / 64); }  // of 64 output channels
 
 // Sixteen elements of a row, as a block has them in a lane: eight from `k0` on and eight from
 // k0 + 32.  What lies behind K is zero.
@@ -536,7 +537,7 @@ void launch_rows(const void *x, int64_t stride, int64_t rows, int K, bool weight
                  hipStream_t s) {
   const int KS = static_cast<int>(k_steps(K));
   const unsigned grid = static_cast<unsigned>(weight ? 4 * ((rows + 63) / 64) : row_tiles(rows));
-  const int waves = std::min(kRowWaves, (KS + 1) / 2);
+  const int waves = row_waves(KS);
   v4i *to = static_cast<v4i *>(packed);
   if (weight) rows_kernel<DT, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
   else rows_kernel<DT, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
@@ -568,6 +569,7 @@ void wide(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y, 
 // 896 3.6, 4.1, 5.1, 9.1; 256 x 9,728 x 896 16.1, 12.5, 14.0, 12.4; 1,024 x 896 x 4,864 20.5,
 // 14.9, 12.9, 32.5; 2,048 x 4,864 x 896 57, 42, 44, 21.
 enum Way { kSplit1, kSplit2, kSplit4, kTiles };
+constexpr double kMostThreads = 4294967295.0;  // of a launch
 inline Way way(int64_t M, int N, int KS, int out_bytes) {
   const double ks = KS, ng = groups_of(N), mt = static_cast<double>(row_tiles(M));
   const int64_t tiles = (M + kBM - 1) / kBM * ((N + kBN - 1) / kBN);
@@ -575,7 +577,12 @@ inline Way way(int64_t M, int N, int KS, int out_bytes) {
                       3.5 + 0.041 * ks + std::ceil(mt / 2) * ng * (0.0039 + 0.00031 * ks),
                       4.5 + 0.052 * ks + std::ceil(mt / 4) * ng * (0.0108 + 0.00044 * ks),
                       7.0 + 0.33 * ks * static_cast<double>((tiles + 255) / 256) + static_cast<double>(M) * N * out_bytes / 3.7e6};
-  return static_cast<Way>(std::min_element(t, t + 4) - t);
+  return mt * ng * 64 * kSplit > kMostThreads ? kTiles : static_cast<Way>(std::min_element(t, t + 4) - t);
+}
+// Whether the launches for these sizes have few enough threads.
+inline bool launchable(int64_t M, int N, int KS) {
+  return static_cast<double>(row_tiles(M)) * 64 * row_waves(KS) <= kMostThreads &&
+         (M / kBM + 64.0) * (N / kBN + 64.0) * 256 <= kMostThreads;
 }
 
 template <int OT>
@@ -642,6 +649,8 @@ extern "C" int spk_linear_int8_pack(const void *w, int w_dtype, int64_t w_stride
   if (!valid_float_dtype(w_dtype)) return fail(SPK_EINVAL, "linear_int8_pack: dtype %d is not a float type", w_dtype);
   if (const int rc = check_sizes("linear_int8_pack", N, K)) return rc;
   if (N == 0) return SPK_OK;
+  if (!i8::launchable(N, 1, static_cast<int>(i8::k_steps(K))))
+    return fail(SPK_EUNSUPPORTED, "linear_int8_pack: more threads than a launch has, N=%d K=%d", N, K);
   if (!w || !packed || !scales) return fail(SPK_EINVAL, "linear_int8_pack: null pointer");
   if (reinterpret_cast<uintptr_t>(packed) & 15) return fail(SPK_EINVAL, "linear_int8_pack: packed must be 16-byte aligned");
   i8::rows(w, w_dtype, w_stride, N, K, true, packed, scales, static_cast<hipStream_t>(stream));
@@ -659,8 +668,11 @@ extern "C" int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, con
     return fail(SPK_EINVAL, "linear_int8: x, y and bias must be of float types");
   if (N <= 0) return fail(SPK_EINVAL, "linear_int8: N=%d", N);
   if (const int rc = check_sizes("linear_int8", M, K)) return rc;
+  if (N > (1 << 30)) return fail(SPK_EUNSUPPORTED, "linear_int8: N=%d (at most 2^30)", N);
   if (M > 1 && y_stride < N) return fail(SPK_EINVAL, "linear_int8: rows of y lie on one another");
   if (M == 0) return SPK_OK;
+  if (!i8::launchable(M, N, static_cast<int>(i8::k_steps(K))))
+    return fail(SPK_EUNSUPPORTED, "linear_int8: more threads than a launch has, M=%lld N=%d K=%d", (long long)M, N, K);
   if (!x || !packed || !scales || !y) return fail(SPK_EINVAL, "linear_int8: null pointer");
   const size_t need = spk_linear_int8_workspace_bytes(M, N, K);
   if (!workspace || workspace_bytes < need)

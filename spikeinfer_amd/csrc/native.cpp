@@ -54,6 +54,12 @@ decltype(&spk_accept_tree) accept_fn;
 decltype(&spk_key_mass) mass_fn;
 decltype(&spk_key_mass_workspace_bytes) mass_workspace_fn;
 decltype(&spk_evict) evict_fn;
+decltype(&spk_linear_int8) linear8_fn;
+decltype(&spk_linear_int8_workspace_bytes) linear8_workspace_fn;
+decltype(&spk_sample_probs) probs_fn;
+decltype(&spk_sample_probs_workspace_bytes) probs_workspace_fn;
+decltype(&spk_verify_tree) verify_fn;
+decltype(&spk_verify_tree_workspace_bytes) verify_workspace_fn;
 decltype(&spk_last_error) last_error_fn;
 
 // A call this module does not take (never seen by the caller).
@@ -801,12 +807,121 @@ PyObject *evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// linear_int8(x, words, scales, N, K, bias|None, out|None, dtype|None, workspace|None) -> y
+PyObject *linear_int8(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject * {
+    const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &scales = tensor(a[2]);
+    here(x);
+    const int N = int32(a[3]), K = int32(a[4]), code = float_code(x.scalar_type());
+    need(N > 0 && K > 0 && x.is_contiguous() && x.dim() >= 1 && x.size(-1) == K && x.numel() > 0 &&
+         w.device() == x.device() && scales.device() == x.device());
+    const int64_t M = x.numel() / K;
+    const at::Tensor *bias = a[5] == Py_None ? nullptr : &vector(a[5], N, x);
+    need(!bias || bias->dim() == 1);
+    at::Tensor y;
+    c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = N;
+    if (a[6] == Py_None) {
+      const at::ScalarType dt = a[7] == Py_None ? x.scalar_type() : dtype_of(a[7]);
+      float_code(dt);
+      y = empty(shape, dt, x);
+    } else {
+      y = tensor(a[6]);
+      need(a[7] == Py_None && y.is_contiguous() && y.sizes() == at::IntArrayRef(shape) && y.device() == x.device());
+    }
+    const int out_code = float_code(y.scalar_type()), bias_code = bias ? float_code(bias->scalar_type()) : 0;
+    const size_t bytes = linear8_workspace_fn(M, N, K);
+    at::Tensor ws;
+    void *const at = scratch(a[8], bytes, x, ws);
+    void *const stream = stream_of(x);
+    THPObjectPtr done = result(a[6], y);
+    launch("linear_int8", linear8_fn, x.data_ptr(), code, static_cast<int64_t>(K), w.data_ptr(),
+           static_cast<const float *>(scales.data_ptr()), bias ? bias->data_ptr() : nullptr, bias_code, y.data_ptr(),
+           out_code, static_cast<int64_t>(N), M, N, K, at, bytes, stream);
+    return done.release();
+  });
+}
+
+// sampling_probs(logits, temperature, top_k|None, top_p|None, min_p|None, out|None, workspace|None) -> out
+PyObject *sampling_probs(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject * {
+    const at::Tensor &x = tensor(a[0]);
+    here(x);
+    const int code = float_code(x.scalar_type());
+    need(x.dim() == 2 && x.stride(1) == 1 && x.numel() > 0 && x.size(0) < (1 << 24) && x.size(1) < (1 << 28));
+    const int rows = static_cast<int>(x.size(0)), vocab = static_cast<int>(x.size(1));
+    auto each = [&](PyObject *o, at::ScalarType dt) -> void * {
+      if (o == Py_None) return nullptr;
+      const at::Tensor &t = tensor(o);
+      need(t.scalar_type() == dt && t.is_contiguous() && t.numel() >= rows && t.device() == x.device());
+      return t.data_ptr();
+    };
+    void *const temp = each(a[1], at::kFloat), *const k = each(a[2], at::kInt), *const p = each(a[3], at::kFloat),
+               *const m = each(a[4], at::kFloat);
+    need(temp);
+    at::Tensor out;
+    if (a[5] == Py_None) {
+      out = empty({rows, vocab}, at::kFloat, x);
+    } else {
+      out = tensor(a[5]);
+      need(out.dim() == 2 && out.size(0) == rows && out.size(1) == vocab && out.scalar_type() == at::kFloat &&
+           out.stride(1) == 1 && out.device() == x.device());
+    }
+    const size_t bytes = probs_workspace_fn(rows, vocab);
+    at::Tensor ws;
+    void *const at = scratch(a[6], bytes, x, ws);
+    void *const stream = stream_of(x);
+    THPObjectPtr done = result(a[5], out);
+    launch("sampling_probs", probs_fn, x.data_ptr(), code, x.stride(0), rows, vocab, static_cast<const float *>(temp),
+           static_cast<const int32_t *>(k), static_cast<const float *>(p), static_cast<const float *>(m),
+           static_cast<float *>(out.data_ptr()), out.stride(0), at, bytes, stream);
+    return done.release();
+  });
+}
+
+// verify_tree(tokens, parents, target_probs, draft_probs, uniforms, starts, max_nodes, distinct, out|None,
+//             workspace|None) -> out
+PyObject *verify_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject * {
+    const at::Tensor &tokens = tensor(a[0]), &p = tensor(a[2]), &q = tensor(a[3]), &u = tensor(a[4]);
+    here(tokens);
+    const int64_t R = tokens.numel(), N = tensor(a[5]).numel() - 1;
+    const int64_t *tok = longs(a[0], R, tokens);
+    const int32_t *par = ints(a[1], R, tokens), *starts = ints(a[5], N + 1, tokens);
+    const int nodes = int32(a[6]);
+    need(R > 0 && N > 0 && N < (1 << 20) && nodes > 0 && nodes <= 1024 && PyBool_Check(a[7]));
+    need(u.scalar_type() == at::kFloat && u.dim() == 1 && u.is_contiguous() && u.numel() >= R &&
+         u.device() == tokens.device());
+    for (const at::Tensor *t : {&p, &q})
+      need(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) >= R && t->size(1) == p.size(1) &&
+           t->size(1) > 0 && t->size(1) < (1 << 30) && t->stride(1) == 1 && t->device() == tokens.device());
+    const int V = static_cast<int>(p.size(1));
+    at::Tensor out;
+    if (a[8] == Py_None) {
+      out = at::full({R}, -1, at::TensorOptions().dtype(at::kLong).device(tokens.device()));
+    } else {
+      out = tensor(a[8]);
+      longs(a[8], R, tokens);
+    }
+    const size_t bytes = verify_workspace_fn(static_cast<int>(N), V);
+    at::Tensor ws;
+    void *const at = scratch(a[9], bytes, tokens, ws);
+    void *const stream = stream_of(tokens);
+    THPObjectPtr done = result(a[8], out);
+    launch("verify_draft_tree", verify_fn, tok, par, static_cast<const float *>(p.data_ptr()), p.stride(0),
+           static_cast<const float *>(q.data_ptr()), q.stride(0), static_cast<const float *>(u.data_ptr()), starts, R,
+           static_cast<int>(N), nodes, V, a[7] == Py_True ? 1 : 0, static_cast<int64_t *>(out.data_ptr()), at, bytes,
+           stream);
+    return done.release();
+  });
+}
+
 template <class F> void set(F &f, void *p) { f = reinterpret_cast<F>(p); }
 
 // bind(device, addresses): "cuda" or "cpu", and the C ABI's functions in the order of
 // the declarations above.
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  constexpr int kFns = 19;
+  constexpr int kFns = 25;
   if (n != kFns + 1 || !PyUnicode_Check(a[0])) {
     PyErr_Format(PyExc_TypeError, "bind takes a device type and %d addresses", kFns);
     return nullptr;
@@ -839,7 +954,13 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   set(mass_fn, p[15]);
   set(mass_workspace_fn, p[16]);
   set(evict_fn, p[17]);
-  set(last_error_fn, p[18]);
+  set(linear8_fn, p[18]);
+  set(linear8_workspace_fn, p[19]);
+  set(probs_fn, p[20]);
+  set(probs_workspace_fn, p[21]);
+  set(verify_fn, p[22]);
+  set(verify_workspace_fn, p[23]);
+  set(last_error_fn, p[24]);
   Py_RETURN_NONE;
 }
 
@@ -850,6 +971,7 @@ PyMethodDef methods[] = {
     SPK_METHOD(prefill),       SPK_METHOD(embed_rmsnorm),     SPK_METHOD(add_rmsnorm),  SPK_METHOD(rmsnorm_mean_t),
     SPK_METHOD(lif_gate_mul),  SPK_METHOD(linear_decode),     SPK_METHOD(mlp_gate_lif), SPK_METHOD(qkv_rope_lif_pack),
     SPK_METHOD(tree_attn),     SPK_METHOD(accept_tree),       SPK_METHOD(key_mass),     SPK_METHOD(evict),
+    SPK_METHOD(linear_int8),   SPK_METHOD(sampling_probs),    SPK_METHOD(verify_tree),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

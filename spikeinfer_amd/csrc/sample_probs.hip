@@ -913,6 +913,8 @@ extern "C" int spk_sample_probs(const void *logits, int logits_dtype, int64_t ro
     return fail(SPK_EINVAL, "sample_probs: rows=%d, vocab=%d must be in [1, %d]", rows, vocab, probs::kMaxVocab);
   if (rows > 1 && out_stride < vocab) return fail(SPK_EINVAL, "sample_probs: rows of the output lie on one another");
   if (rows == 0) return SPK_OK;
+  if (static_cast<double>(rows) * probs::plan(1, vocab, 4).S * probs::kSliceThreads > 4294967295.0)
+    return fail(SPK_EUNSUPPORTED, "sample_probs: more threads than a launch has, rows=%d vocab=%d", rows, vocab);
   if (!logits || !temperature || !probs_out) return fail(SPK_EINVAL, "sample_probs: null pointer");
   const size_t need = spk_sample_probs_workspace_bytes(rows, vocab);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))

@@ -233,6 +233,12 @@ def verify_draft_tree(
     Returns ``out``: the token after each row of the path, -1 for other rows, and where the
     target gives no token any weight.
     """
+    native = _lib.native()
+    if native is not None:
+        done = native.verify_tree(tokens, parents, target_probs, draft_probs, uniforms, row_starts, max_nodes, distinct,
+                                  out, workspace)
+        if done is not None:
+            return done
     dev = _lib.require_gpu(tokens, parents, target_probs, draft_probs, uniforms, row_starts, out, workspace)
     _max_nodes(max_nodes)
     R, n_seqs = tokens.numel(), row_starts.numel() - 1

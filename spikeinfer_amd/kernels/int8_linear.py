@@ -73,6 +73,11 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, bias: torch.Tensor | None = None
     A row of x with an infinity or a NaN gives a row of NaN (a row of the weight such a
     column).  Rows do not depend on the rows around them.
     """
+    native = _lib.native()
+    if native is not None:  # the usual form of the arguments, checked and launched in C++
+        done = native.linear_int8(x, w.words, w.scales, w.out_features, w.in_features, bias, out, dtype, workspace)
+        if done is not None:
+            return done
     dev = _lib.require_gpu(x, w.words, w.scales, bias, out, workspace)
     N, K = w.out_features, w.in_features
     if x.dtype not in _FLOATS or x.ndim < 1 or x.shape[-1] != K:

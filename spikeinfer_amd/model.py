@@ -26,6 +26,7 @@ Weights load from the reference's parameter names
 """
 from __future__ import annotations
 
+import copy
 import math
 from dataclasses import dataclass
 
@@ -38,6 +39,7 @@ from .kernels.decoder_ops import (add_rmsnorm, embed_rmsnorm, lif_gate_mul, line
                                   pack_linear, qkv_decode_attention, qkv_rope_lif_pack, rmsnorm_mean_t)
 from .kernels.draft_tree import paged_spike_attn_tree
 from .kernels.eviction import paged_spike_attn_key_mass
+from .kernels.int8_linear import linear_int8, pack_linear_int8
 from .kernels.packing import packed_width
 from .kernels.spike_attention import (gather_kv_unpacked_pair, paged_spike_attn_decode,
                                       paged_spike_attn_prefill, prefill_supported)
@@ -82,7 +84,10 @@ def small_down_rows(hidden: int, inter: int) -> int:
 class _Layer:
     __slots__ = ("input_norm", "post_norm", "w_qkv", "b_qkv", "lif_qkv_beta", "lif_qkv_th",
                  "w_o", "w_gu", "lif_gate_beta", "lif_gate_th", "w_down", "w_gu_packed",
-                 "w_qkv_packed", "w_o_packed", "w_down_packed")
+                 "w_qkv_packed", "w_o_packed", "w_down_packed", "int8")
+
+    def __init__(self) -> None:
+        self.int8 = None  # name -> Int8Weight of an int8_copy
 
 
 class SpikingDecoder:
@@ -148,6 +153,7 @@ class SpikingDecoder:
         # group), which costs more than the launches it saves (config 5: 2.28
         # against 1.63 ms a step).
         self.fused_norm = False
+        self.lm_head_int8 = None  # an int8_copy's
         self._pack_mlp()
         # Rotary inverse frequencies as Qwen2RotaryEmbedding builds them (fp32, host).
         exps = torch.arange(0, self.D, 2, dtype=torch.int64).float() / self.D
@@ -202,9 +208,31 @@ class SpikingDecoder:
                     setattr(L, name + "_packed", fn(getattr(L, name)))
                 except ValueError:
                     pass
+        if self.lm_head_int8 is not None:
+            self._pack_int8()
 
-    def _linear(self, x: torch.Tensor, w: torch.Tensor, b, wp, n: int) -> torch.Tensor:
-        """F.linear, or linear_decode for batches of at most fused_mlp_max_tokens."""
+    _INT8_NAMES = ("w_qkv", "w_o", "w_gu", "w_down")
+
+    def _pack_int8(self) -> None:
+        self.lm_head_int8 = pack_linear_int8(self.lm_head)
+        for L in self.layers:
+            L.int8 = {name: pack_linear_int8(getattr(L, name)) for name in self._INT8_NAMES}
+
+    def int8_copy(self) -> "SpikingDecoder":
+        """A model of the same parameters whose linear layers multiply 8-bit integers
+        (:func:`~spikeinfer_amd.kernels.linear_int8`): half of the weights' bytes a step, for
+        drafting what this model then verifies.  It shares this model's tensors, its embedding
+        among them; its keys and values differ, so it needs a cache of its own."""
+        other = copy.copy(self)
+        other.layers = [copy.copy(L) for L in self.layers]
+        other._pack_int8()
+        return other
+
+    def _linear(self, x: torch.Tensor, w: torch.Tensor, b, wp, n: int, w8=None) -> torch.Tensor:
+        """F.linear, or linear_decode for batches of at most fused_mlp_max_tokens, or
+        linear_int8 from an int8_copy's weight ``w8``."""
+        if w8 is not None:
+            return linear_int8(x, w8, b)
         if self.small_linear and wp is not None and n <= self.fused_mlp_max_tokens:
             y = linear_decode(x, wp, b)
             if y is not None:
@@ -215,12 +243,15 @@ class SpikingDecoder:
     def weight_bytes(self) -> int:
         """Bytes of weights one decode step reads (tied lm_head counted once
         as the head, the embedding gather aside)."""
-        n = self.lm_head.numel() + self.final_norm.numel()
+        n = self.final_norm.numel() + (0 if self.lm_head_int8 else self.lm_head.numel())
+        n8 = self.lm_head_int8.nbytes if self.lm_head_int8 else 0
         for L in self.layers:
+            n8 += sum(w.nbytes for w in (L.int8 or {}).values())
             for name in _Layer.__slots__:
-                if not name.endswith("_packed"):  # a step reads these instead of the originals
+                # a step reads the packed ones, or those in 8 bits, instead of the originals
+                if name != "int8" and not name.endswith("_packed") and name not in (L.int8 or ()):
                     n += getattr(L, name).numel()
-        return n * self.lm_head.element_size()
+        return n * self.lm_head.element_size() + n8
 
     # -- forward -----------------------------------------------------------
     def rope_tables(self, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -282,11 +313,13 @@ class SpikingDecoder:
                      torch.empty((T, Hkv, n, D), dtype=self.dtype, device=h.device),
                      torch.empty((T, Hkv, n, D), dtype=self.dtype, device=h.device))
         delta = None
-        fold = (self.fused_norm and self.small_linear and n <= self.fused_mlp_max_tokens
+        int8 = self.lm_head_int8 is not None
+        fold = (self.fused_norm and not int8 and self.small_linear and n <= self.fused_mlp_max_tokens
                 and self.dtype == torch.bfloat16)
         h_alt = torch.empty_like(h) if fold else None  # the other residual buffer
         for i, L in enumerate(self.layers):
             k_cache, v_cache = kv_caches[i]
+            w8 = L.int8 or {}
             qkv = None
             if i and fold and L.w_qkv_packed is not None:
                 qkv = norm_linear_decode(h, delta, L.input_norm, c.rms_norm_eps, L.w_qkv_packed, L.b_qkv,
@@ -296,7 +329,7 @@ class SpikingDecoder:
             if qkv is None:
                 if i:
                     x = add_rmsnorm(h, delta, L.input_norm, c.rms_norm_eps, out=x)
-                qkv = self._linear(x, L.w_qkv, L.b_qkv, L.w_qkv_packed, n)
+                qkv = self._linear(x, L.w_qkv, L.b_qkv, L.w_qkv_packed, n, w8.get("w_qkv"))
             if draft is not None:
                 kv_packed = draft.words[i]
             fused = (self.fused_attention and not meta.num_prefills and n_dec == n and meta.key_mass is None and
@@ -322,7 +355,7 @@ class SpikingDecoder:
                 self._packed_prefill_attention(q_packed, kv_packed, k_cache, v_cache, meta, attn)
             elif meta.num_prefills:
                 self._prefill_attention(dense, k_cache, v_cache, meta, attn)
-            o = self._linear(attn.view(T, n, Hq * D), L.w_o, None, L.w_o_packed, n)
+            o = self._linear(attn.view(T, n, Hq * D), L.w_o, None, L.w_o_packed, n, w8.get("w_o"))
             y = None
             if fold and self.fused_mlp and L.w_gu_packed is not None:
                 y = norm_mlp_gate_lif(h, o, L.post_norm, c.rms_norm_eps, L.w_gu_packed, L.lif_gate_beta,
@@ -331,13 +364,15 @@ class SpikingDecoder:
                     h, h_alt = h_alt, h
             if y is None:
                 x = add_rmsnorm(h, o, L.post_norm, c.rms_norm_eps, out=x)
-            if y is None and self.fused_mlp and L.w_gu_packed is not None and n <= self.fused_mlp_max_tokens:
+            if y is None and not int8 and self.fused_mlp and L.w_gu_packed is not None \
+                    and n <= self.fused_mlp_max_tokens:
                 y = mlp_gate_lif(x, L.w_gu_packed, L.lif_gate_beta, L.lif_gate_th)
             if y is None:
-                y = lif_gate_mul(F.linear(x, L.w_gu), L.lif_gate_beta, L.lif_gate_th)
+                gate_up = linear_int8(x, w8["w_gu"]) if int8 else F.linear(x, L.w_gu)
+                y = lif_gate_mul(gate_up, L.lif_gate_beta, L.lif_gate_th)
             delta = None
-            if T * n <= self.small_down_max_rows:
-                delta = self._linear(y, L.w_down, None, L.w_down_packed, n)
+            if int8 or T * n <= self.small_down_max_rows:
+                delta = self._linear(y, L.w_down, None, L.w_down_packed, n, w8.get("w_down"))
             if delta is None:
                 delta = F.linear(y, L.w_down)
         return rmsnorm_mean_t(h, self.final_norm, c.rms_norm_eps, delta=delta)
@@ -399,6 +434,8 @@ class SpikingDecoder:
         """lm_head on the rows that sample (modeling_fast.py:335-355)."""
         if indices is not None:
             hidden = hidden.index_select(0, indices)
+        if self.lm_head_int8 is not None:
+            return linear_int8(hidden, self.lm_head_int8, out=out)
         if self.small_linear and self.lm_head_packed is not None and hidden.shape[0] <= 64:
             y = linear_decode(hidden, self.lm_head_packed, None, out)
             if y is not None:

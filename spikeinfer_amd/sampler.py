@@ -197,6 +197,11 @@ def sampling_probs(
     ``out``: optional ``float32 [rows, vocab]``, vocab contiguous; ``workspace``: optional ``uint8``
     scratch of :func:`sampling_probs_workspace_bytes` (calls that may run at once need one each).
     """
+    native = _lib.native()
+    if native is not None:  # the usual form of the arguments, checked and launched in C++
+        done = native.sampling_probs(logits, temperature, top_k, top_p, min_p, out, workspace)
+        if done is not None:
+            return done
     dev = _lib.require_gpu(logits, temperature, top_k, top_p, min_p, out, workspace)
     if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocab] with a contiguous vocab axis")

@@ -27,11 +27,14 @@ def test_linear_refusals():
         return lib.spk_linear_int8(x, xdt, K, packed, scales, bias, bdt, y, ydt, ys, M, N, K, ws, wsb, None)
 
     for kw, rc in ((dict(x=None), 1), (dict(xdt=3), 1), (dict(ydt=9), 1), (dict(bias=P, bdt=4), 1), (dict(N=0), 1),
-                   (dict(K=0), 1), (dict(M=-1), 1), (dict(K=131073), 2), (dict(M=(1 << 30) + 1), 2), (dict(ys=47), 1),
+                   (dict(K=0), 1), (dict(M=-1), 1), (dict(K=131073), 2), (dict(M=(1 << 30) + 1), 2), (dict(N=(1 << 30) + 1, ys=1 << 31), 2), (dict(ys=47), 1),
                    (dict(ys=0), 1), (dict(packed=None), 1), (dict(scales=None), 1), (dict(y=None), 1),
                    (dict(ws=None), 1), (dict(wsb=16), 1), (dict(ws=P + 4), 1), (dict(packed=P + 1), 1)):
         assert linear(**kw) == rc, kw
     assert linear(M=0) == _lib.SPK_OK
+    # more threads than a launch has
+    assert linear(M=1 << 30, N=1 << 20, ys=1 << 20, wsb=1 << 62) == _lib.SPK_EUNSUPPORTED
+    assert linear(M=1 << 30, K=4096, wsb=1 << 62) == _lib.SPK_EUNSUPPORTED and b"launch" in lib.spk_last_error()
     assert lib.spk_linear_int8_packed_bytes(17, 65) == 4 * 2 * 1024
     assert lib.spk_linear_int8_packed_bytes(0, 65) == lib.spk_linear_int8_packed_bytes(4, -1) == 0
     # offsets in 64 bits
@@ -46,7 +49,9 @@ def test_distribution_refusals():
         return lib.spk_sample_probs(x, dt, V, rows, V, temp, None, None, None, out, os, ws, wsb, None)
 
     for kw, rc in ((dict(x=None), 1), (dict(dt=4), 1), (dict(rows=-1), 1), (dict(V=0), 1), (dict(V=262145), 1),
-                   (dict(temp=None), 1), (dict(out=None), 1), (dict(os=99), 1), (dict(os=0), 1)):
+                   (dict(temp=None), 1), (dict(out=None), 1), (dict(os=99), 1), (dict(os=0), 1),
+                   (dict(rows=1 << 23, V=10, os=10, wsb=1 << 62), 2), (dict(ws=None), 1), (dict(wsb=64), 1),
+                   (dict(ws=P + 8), 1)):
         assert probs(**kw) == rc, kw
     assert probs(rows=0) == _lib.SPK_OK
 
