@@ -210,8 +210,7 @@ __device__ __forceinline__ void fill_zeros(float *o, int i0, int i1, int threads
 }
 
 struct SliceShared {
-  float x[kCand];  // candidates: logit and index
-  int32_t i[kCand];
+  int32_t i[kCand];  // the candidates
   uint32_t tmax[kSliceThreads];
   float wave[kSliceThreads / 64];
   double part[kSliceThreads / 64];
@@ -351,34 +350,51 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
       whole = -INFINITY;  // of the survivors none is missing
     }
   }
-  int mine = 0;
+  // A thread's candidates as bits of its elements, then their indices into LDS; the values
+  // are read again (one round trip for all; a branch an element took 4.4 us against 1).
+  constexpr int kSlots = kSliceVecs * W;
+  static_assert(kSlots <= 64, "a bit each");
+  u64 hits = 0;
   double rest = 0.0;
   if (k.open && !k.top_k && !(k.min_p > 0.f)) {
     const double m = x_most;
+    int slot = 0;
     each([&](int, float v) {
-      mine += v >= bound ? 1 : 0;
+      hits |= v >= bound ? 1ull << slot : 0;
+      ++slot;
       // (what overflows weighs nothing beside the largest; fmax takes the difference for a NaN)
       const double d = static_cast<double>(static_cast<float>(static_cast<double>(v) * k.inv)) - m;
       rest += power64(v < bound ? fmax(d, -800.0) : -800.0);
     });
+    rest = sum(rest);
   } else {
-    each([&](int, float v) { mine += v >= bound ? 1 : 0; });
+    int slot = 0;
+    each([&](int, float v) {
+      hits |= v >= bound ? 1ull << slot : 0;
+      ++slot;
+    });
   }
-  int at = mine ? atomicAdd(&sh.count, mine) : 0;
+  const int own = __popcll(hits);
+  int upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  int at = 0;
+  if (lane == 63 && upto) at = atomicAdd(&sh.count, upto);
+  at = __shfl(at, 63) + upto - own;
   __syncthreads();
   const int n = sh.count;
   if (n <= a.cap) {
-    each([&](int i, float v) {
-      if (v >= bound) {
-        sh.x[at] = v;
-        sh.i[at++] = i;
-      }
-    });
-  }
-  rest = sum(rest);
-  if (n <= a.cap) {
+    for (; hits; hits &= hits - 1) {
+      const int slot = __builtin_ctzll(hits);
+      sh.i[at++] = row.first(v0 + slot / W * kSliceThreads + tid) + slot % W;
+    }
+    __syncthreads();
     u64 *list = a.lists + (r * a.S + s) * a.cap;
-    for (int j = tid; j < n; j += kSliceThreads) list[j] = order_key(quotient(sh.x[j], k.inv), sh.i[j]);
+#pragma unroll 4
+    for (int j = tid; j < n; j += kSliceThreads) list[j] = order_key(quotient(elem_to_f32<DT>(row.p[sh.i[j]]), k.inv), sh.i[j]);
   }
   if (tid == 0) *head = Head{n <= a.cap ? n : -1, most, whole, rest};
 }
@@ -494,7 +510,8 @@ __device__ __forceinline__ Place place(const u64 *key, const u64 *mass, int n) {
 }
 
 // The cut as radix_cut finds it, among the n candidates in sh.key (sh.mass: their weights; by_count:
-// 1 each), of which those below `from` have none.  Few are ranked one against the other.  Many go
+// 1 each), of which those below `from` have none, x between `bottom` and `top` (where they are no
+// finite distance apart, the candidates are looked at).  Few are ranked one against the other.  Many go
 // into bins of equal width in x first, and those of the bin that holds the cut are ranked; where
 // that is too many as well (equal logits), by digits.
 __device__ __forceinline__ u64 rank_cut(RowShared &sh, const u64 *key, const u64 *mass, int n, bool by_count, u64 from,
@@ -510,17 +527,22 @@ __device__ __forceinline__ u64 rank_cut(RowShared &sh, const u64 *key, const u64
   __syncthreads();
   return sh.pick;
 }
-__device__ __forceinline__ u64 cand_cut(RowShared &sh, int n, bool by_count, u64 from, u64 base, double target) {
+__device__ __forceinline__ u64 cand_cut(RowShared &sh, int n, bool by_count, u64 from, u64 base, double target, float top,
+                                        float bottom) {
   if (n <= kRank) return rank_cut(sh, sh.key, sh.mass, n, by_count, from, base, target);
-  u64 lo = ~0ull, hi = 0;
-  for (int j = threadIdx.x; j < n; j += kRowThreads) {
-    lo = smaller(lo, sh.key[j]);
-    hi = larger(hi, sh.key[j]);
+  u64 lo = order_key(bottom, kMaxVocab - 1), hi = order_key(top, 0);
+  if (!(top - bottom < 1e30f)) {
+    lo = ~0ull, hi = 0;
+    for (int j = threadIdx.x; j < n; j += kRowThreads) {
+      lo = smaller(lo, sh.key[j]);
+      hi = larger(hi, sh.key[j]);
+    }
+    lo = block_reduce(lo, sh, smaller);
+    hi = block_reduce(hi, sh, larger);
+    top = order_value(hi), bottom = order_value(lo);
   }
-  lo = block_reduce(lo, sh, smaller);
-  hi = block_reduce(hi, sh, larger);
   auto weight = [&](int j) -> u64 { return sh.key[j] < from ? 0 : by_count ? 1ull : sh.mass[j]; };
-  const float top = order_value(hi), width = top - order_value(lo);
+  const float width = top - bottom;
   if (width > 0.f && width < INFINITY) {
     const float scale = static_cast<float>(kBins) / width;
     auto bin = [&](u64 k) { return kBins - 1 - min(kBins - 1, static_cast<int>((top - order_value(k)) * scale)); };
@@ -637,7 +659,7 @@ __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool b
     if (n <= kCand) {
       for (int j = threadIdx.x; j < n; j += kRowThreads) sh.mass[j] = weight(order_value(sh.key[j]), order_index(sh.key[j]));
       __syncthreads();
-      return cand_cut(sh, n, by_count, from, above, target);
+      return cand_cut(sh, n, by_count, from, above, target, INFINITY, 0.f);
     }
     __syncthreads();
   }
@@ -762,21 +784,44 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
   if (known) {
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    const u64 *lists = a.lists + r * a.S * a.cap;
-    for (int e = tid; e < listed; e += kRowThreads) {
-      int q = 0, j = e;
-      while (j >= sh.head[q].count) j -= sh.head[q++].count;
-      const u64 key = lists[static_cast<int64_t>(q) * a.cap + j];
-      const bool keep = order_value(key) >= whole;
-      const u64 w = keep || rest_counts ? row.mass(order_value(key)) : 0;
-      if (!keep) {
-        below += w;
-        continue;
-      }
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCand) {
-        sh.key[at] = key;
-        sh.mass[at] = w;
+    // a wave a slice, eight of its candidates a lane at a time
+    const int lane = tid & 63;
+    for (int q = tid >> 6; q < a.S; q += kRowThreads / 64) {
+      const int count = sh.head[q].count;
+      const u64 *list = a.lists + (r * a.S + q) * a.cap;
+      for (int j0 = 0; j0 < count; j0 += 512) {
+        u64 key[8];
+        uint64_t kept[8];
+        int all = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int j = j0 + 64 * u + lane;
+          key[u] = j < count ? list[j] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          kept[u] = __ballot(j0 + 64 * u + lane < count && order_value(key[u]) >= whole);
+          all += __popcll(kept[u]);
+        }
+        int base = 0;
+        if (lane == 0 && all) base = atomicAdd(&sh.count, all);
+        base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (j0 + 64 * u >= count) break;
+          const bool keep = kept[u] >> lane & 1;
+          const u64 w = keep || (j0 + 64 * u + lane < count && rest_counts) ? row.mass(order_value(key[u])) : 0;
+          if (keep) {
+            const int at = base + __popcll(kept[u] & ((1ull << lane) - 1));
+            if (at < kCand) {
+              sh.key[at] = key[u];
+              sh.mass[at] = w;
+            }
+          } else {
+            below += w;
+          }
+          base += __popcll(kept[u]);
+        }
       }
     }
     if (rest_counts) below = block_reduce(below, sh, plus);
@@ -817,12 +862,13 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
       return;
     }
   } else if (known) {
+    const float top = static_cast<float>(row.m);
     auto total = [&](u64 from) {
       u64 z = 0;
       for (int j = tid; j < n; j += kRowThreads) z += sh.key[j] >= from ? sh.mass[j] : 0;
       return block_reduce(z, sh, plus);
     };
-    u64 cut = k.top_k && n >= k.top_k ? cand_cut(sh, n, true, 0, 0, static_cast<double>(k.top_k)) : 0;
+    u64 cut = k.top_k && n >= k.top_k ? cand_cut(sh, n, true, 0, 0, static_cast<double>(k.top_k), top, whole) : 0;
     u64 Z = total(cut);
     if (k.open) {
       double lowest = static_cast<double>(Z), highest = lowest;
@@ -830,7 +876,7 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
         lowest += static_cast<double>(below) + rest * (1.0 - kPowerOff) * kMassScale;
         highest += static_cast<double>(below) + rest * (1.0 + kPowerOff) * kMassScale;
       }
-      const u64 c = cand_cut(sh, n, false, cut, 0, static_cast<double>(k.top_p) * lowest);
+      const u64 c = cand_cut(sh, n, false, cut, 0, static_cast<double>(k.top_p) * lowest, top, whole);
       cut = larger(cut, c);
       Z = total(cut);
       if (rest_counts)  // the same cut for the largest sum there can be
