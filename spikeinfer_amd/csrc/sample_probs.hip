@@ -70,7 +70,8 @@ __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
 // A logit over the temperature; what is finite stays finite (a mask of the type's lowest value
 // is no -infinity below a temperature of 1).  inv = 1 / temp in fp64: the quotient of two
 // fp32 numbers lies at least 2^-49 of itself from the middle between two fp32 numbers, and the
-// product is off by at most 2^-52, so its rounding is the quotient's.
+// product is off by at most 2^-52, so its rounding is the quotient's (below 2^-126, where the
+// numbers have fewer bits, it may be the one beside it).
 __device__ __forceinline__ float quotient(float v, double inv) {
   const float x = static_cast<float>(static_cast<double>(v) * inv);
   return fabsf(x) == INFINITY && fabsf(v) != INFINITY ? copysignf(kMost, v) : x;

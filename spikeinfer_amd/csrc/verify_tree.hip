@@ -29,13 +29,15 @@ using draft::kMaxNodes;
 constexpr int kSliceThreads = 256;
 constexpr int kEndThreads = 1024;
 constexpr int kMaxSlices = 64;  // a lane each
-constexpr int kMaxRounds = 4;
+constexpr int kMaxRounds = 3;
 
-// Launches of slices.  A chain needs one sum, a tree one a rejected sibling, a few as a rule;
-// those that are left to the last launch take a workgroup 10 us each at 151,936 tokens, a
-// launch that finds every tree done about 2.  (16 trees of 25 nodes with up to three siblings,
-// one launch to five: FIGURES.)
-inline int rounds_for(int max_nodes) { return std::min(kMaxRounds, 1 + (max_nodes - 1) / 8); }
+// Launches of slices.  A chain needs one sum, a tree one a rejected sibling, a few as a rule.
+// Those that are left to the last launch take one workgroup: 5 to 10 us each at 151,936 tokens,
+// 2 at 32,000; a launch that finds every tree done takes 2 to 3.  One launch against three, us:
+// 16 trees of 25 nodes at 151,936 tokens 56 and 36, 14 of 8 nodes with up to 3 siblings 52 and
+// 36, 64 chains of 8 nodes 27 and 30, one chain of 5 15 and 21; 7 trees of 13 nodes at 32,003
+// 20 and 28.  (Which of them it is the host does not know: few nodes are chains as a rule.)
+inline int rounds_for(int max_nodes, int V) { return max_nodes > 8 && V >= 65536 ? kMaxRounds : 1; }
 
 struct Params {
   const int64_t *tokens;
@@ -374,7 +376,7 @@ extern "C" int spk_verify_tree(const int64_t *tokens, const int32_t *parents, co
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(SPK_EINVAL, "verify_tree: workspace of %zu bytes, %zu needed, aligned to 8", workspace ? workspace_bytes : 0,
                 need);
-  const int G = verify_slices(N, V), rounds = verify::rounds_for(max_nodes);
+  const int G = verify_slices(N, V), rounds = verify::rounds_for(max_nodes, V);
   double *part = static_cast<double *>(workspace);
   verify::Params P{tokens, parents, row_starts, target_probs, draft_probs, uniforms, target_stride, draft_stride, rows,
                    max_nodes, V, distinct, G, 0, part,
