@@ -45,6 +45,19 @@ def test_matches_64_bits(gpu, M, N, K):
     _assert_close(linear_int8(x.to(gpu), w8), x, w)
 
 
+@pytest.mark.parametrize("M,N,K", [
+    (1, 32769, 64), (17, 32770, 200), (33, 32800, 65), (64, 32769, 1024), (64, 32769, 1030), (16, 32769, 1030),  # many columns
+    (16, 70, 1025), (9, 70, 5121), (2, 8, 5120), (16, 1000, 9000),                                               # few rows
+    (4096, 1100, 64), (4100, 300, 65), (300, 9000, 192), (2049, 1025, 130), (129, 20000, 64)])                   # many of both
+def test_sizes_of_every_kernel(gpu, M, N, K):
+    """Around the sizes from which another kernel takes the call: what fits LDS or is kept in
+    registers, odd and even numbers of steps, tiles that end inside."""
+    print(f"linear {M} {N} {K}", flush=True)
+    x, w = _data(M, N, K, M + N + K)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(K))
+    _assert_close(linear_int8(x.to(gpu), pack_linear_int8(w.to(gpu)), bias.to(gpu)), x, w, bias)
+
+
 @pytest.mark.parametrize("out", [F32, F16, BF16])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_types_and_bias(gpu, dtype, out):

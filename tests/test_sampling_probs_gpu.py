@@ -54,6 +54,37 @@ def test_matches_64_bits(gpu, V, scale, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.3, 1.0, 2.7])
+def test_cuts_that_keep_many(gpu, scale, dtype):
+    """Rows whose cuts lie far down: nearly flat ones by top_p, large top_k, small min_p."""
+    V = 151936
+    combos = [(1.0, -1, 0.5, 0.0), (1.0, -1, 0.97, 0.0), (1.0, 2049, 1.0, 0.0), (0.7, 5000, 0.9, 0.0), (1.3, 100000, 1.0, 0.0),
+              (1.0, -1, 1.0, 0.01), (1.0, -1, 0.8, 1e-4), (1.0, 20000, 0.99, 1e-5), (5.0, -1, 0.3, 0.0), (1.0, 2048, 0.999, 0.0)]
+    g = torch.Generator().manual_seed(int(10 * scale))
+    logits = (torch.randn((len(combos), V), generator=g) * scale).to(DTYPES[dtype])
+    logits[::2, ::7] = -torch.inf
+    cols = list(zip(*combos))
+    args = [torch.tensor(c, dtype=torch.int32 if i == 1 else torch.float32, device=gpu) for i, c in enumerate(cols)]
+    _assert_close(sampling_probs(logits.to(gpu), *args), _rows(logits, *cols))
+
+
+def test_parameters_out_of_range(gpu):
+    """A top_p of 0 or less and a min_p above 1 leave the first token (those equal to it); a
+    temperature that is no number, or negative, is greedy; cuts that are none of a number's
+    order are off; an infinite temperature makes all equal."""
+    inf, nan = float("inf"), float("nan")
+    V = 3000
+    logits = torch.randn((9, V), generator=torch.Generator().manual_seed(11))
+    given = [(1.0, -1, 0.0, 0.0), (1.0, -1, -3.0, 0.0), (1.0, -1, 1.0, 1.5), (nan, 5, 0.5, 0.1), (-1.0, -1, 1.0, 0.0),
+             (1.0, -1, nan, nan), (1.0, 0, 2.0, -1.0), (inf, 7, 1.0, 0.0), (1.0, 2**31 - 1, inf, 0.0)]
+    same = [(1.0, 1, 1.0, 0.0), (1.0, 1, 1.0, 0.0), (1.0, 1, 1.0, 0.0), (0.0, -1, 1.0, 0.0), (0.0, -1, 1.0, 0.0),
+            (1.0, -1, 1.0, 0.0), (1.0, -1, 1.0, 0.0), (inf, 7, 1.0, 0.0), (1.0, -1, 1.0, 0.0)]
+    cols = list(zip(*given))
+    args = [torch.tensor(c, dtype=torch.int32 if i == 1 else torch.float32, device=gpu) for i, c in enumerate(cols)]
+    _assert_close(sampling_probs(logits.to(gpu), *args), _rows(logits, *zip(*same)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_equal_logits(gpu, dtype):
     """A cut within equal logits keeps the lowest indices; whole rows of one value, of two,
     values that become equal by the temperature, zeros of both signs."""

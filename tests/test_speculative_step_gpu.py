@@ -9,9 +9,9 @@ import torch
 import speculative_ref as ref
 from spikeinfer_amd import model as model_mod
 from spikeinfer_amd.attention import AttentionMetadata, DraftTrees
-from spikeinfer_amd.kernels import accept_draft_tree, draft_tree_masks, verify_draft_tree
+from spikeinfer_amd.kernels import accept_draft_tree, draft_tree_masks, verify_draft_tree, verify_workspace_bytes
 from spikeinfer_amd.runner import DecodeRunner
-from spikeinfer_amd.sampler import SamplingParams, sample_tokens, sampling_probs
+from spikeinfer_amd.sampler import SamplingParams, sample_tokens, sampling_probs, sampling_probs_workspace_bytes
 from spikeinfer_amd.spike_cache import PagedSpikeCache
 from test_verify_step_gpu import BS, _decode, _model, _prefill
 
@@ -126,3 +126,56 @@ def test_drafting_and_verifying(gpu, temperature):
         lens = lens + count
         last = after
     assert kept > 0  # (a random model's 8-bit copy agrees with it now and then)
+
+
+def test_captured_steps_share_a_workspace(gpu):
+    """Distributions of both models, verification and acceptance as one captured step; two such
+    steps of other sizes, whose graphs share their scratch, replayed in turn with eager work
+    between them."""
+    V, g = 5003, torch.Generator().manual_seed(3)
+    scratch = torch.empty(1 << 22, dtype=torch.uint8, device=gpu)
+    steps = []
+    for counts, dtype in (([5, 5, 5], torch.bfloat16), ([17, 2, 9, 1, 12], torch.float32)):
+        case = ref.draft_case(counts, V, sum(counts), 3)
+        rows, n = len(case["tokens"]), len(counts)
+        s = {k: v.to(gpu) for k, v in case.items() if isinstance(v, torch.Tensor) and not k.endswith("probs")}
+        s.update(logits=torch.zeros((2, rows, V), dtype=dtype, device=gpu), probs=torch.zeros((2, rows, V), device=gpu),
+                 temp=torch.full((rows,), 0.8, device=gpu), top_p=torch.full((rows,), 0.9, device=gpu),
+                 out=torch.full((rows,), -1, device=gpu), most=case["max_nodes"],)
+        assert max(sampling_probs_workspace_bytes(rows, V), verify_workspace_bytes(n, V)) <= scratch.numel()
+        steps.append(s)
+
+    def run(s, probs, out, workspace):
+        for i in range(2):
+            sampling_probs(s["logits"][i], s["temp"], None, s["top_p"], out=probs[i], workspace=workspace)
+        verify_draft_tree(s["tokens"], s["parents"], probs[0], probs[1], s["uniforms"], s["row_starts"], s["most"],
+                          out=out, workspace=workspace)
+        return accept_draft_tree(s["tokens"], s["parents"], out, s["row_starts"], s["most"])
+
+    graphs = []
+    for s in steps:
+        run(s, s["probs"], s["out"], scratch)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s["accepted"] = run(s, s["probs"], s["out"], scratch)
+        graphs.append(graph)
+    for turn in range(4):
+        for s in steps:
+            x = torch.randn(s["logits"].shape[1:], generator=g) * 3
+            s["logits"].copy_(torch.stack([x, x + torch.randn(x.shape, generator=g)]))
+            s["uniforms"].copy_(torch.rand(len(s["uniforms"]), generator=g))
+            starts = s["row_starts"].tolist()
+            for a, e in zip(starts[:-1], starts[1:]):  # drafts that the drafter favours
+                s["tokens"][a + 1:e] = s["logits"][1][a + s["parents"][a + 1:e].long()].argmax(1)
+        for graph in graphs[::1 if turn % 2 else -1]:
+            graph.replay()
+        for s in steps:
+            probs, out = torch.zeros_like(s["probs"]), torch.full_like(s["out"], -1)
+            path, count, after = run(s, probs, out, None)
+            assert torch.equal(probs, s["probs"]) and torch.equal(out, s["out"])
+            assert out.tolist() == ref.verify(s["tokens"].cpu(), s["parents"].cpu(), probs[0], probs[1], s["uniforms"].cpu(),
+                                              s["row_starts"].cpu(), s["most"])
+            assert torch.equal(count, s["accepted"][1]) and torch.equal(after, s["accepted"][2])
+            for i, c in enumerate(count.tolist()):
+                assert torch.equal(path[i, :c], s["accepted"][0][i, :c])
