@@ -30,7 +30,10 @@ namespace probs {
 typedef unsigned long long u64;
 
 constexpr int kSliceThreads = 512;
-constexpr int kSliceVecs = 5;     // 16-byte vectors of a slice a thread holds
+// 16-byte vectors of a slice that a thread holds, by the elements of one: 10,240 or 12,288 tokens.
+// (16-bit rows with five: one row of 151,936 29 us against 27; fp32 with three: slices of 6,144
+// miss top_k's tokens too often, 56 rows 100 us against 29.)
+constexpr int slice_vecs(int vec) { return vec == 4 ? 5 : 3; }
 constexpr int kRowThreads = 512;
 constexpr int kIndexBits = 18;
 constexpr int kMaxVocab = 1 << kIndexBits;
@@ -41,8 +44,9 @@ constexpr int kCand = 4096;                      // candidates of a row
 constexpr int kBins = 1024;              // of a row's histogram: 10-bit digits
 constexpr int kBinsPerThread = kBins / kRowThreads;
 constexpr int kRank = 256;                       // candidates that are ranked one against the other
-constexpr int kMaxSlices = kMaxVocab / (4 * kSliceVecs * kSliceThreads) + 2;  // of a row
+constexpr int kMaxSlices = kMaxVocab / (4 * slice_vecs(4) * kSliceThreads) + 2;  // of a row
 constexpr int kMostK = 2048;                     // top_k beyond: the long way
+constexpr int kChunk = 256;                     // candidates that a wave takes at a time
 
 // Larger: earlier in the order.
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -171,7 +175,7 @@ __device__ __forceinline__ Ask ask(const Args &a, int64_t r) {
 template <int DT>
 struct RowMem {
   typedef typename Elem<DT>::T E;
-  static constexpr int W = Elem<DT>::kVec;
+  static constexpr int W = Elem<DT>::kVec, kVecs = slice_vecs(W);
   typedef E Vec __attribute__((ext_vector_type(W)));
   const E *p;
   int V, before;  // elements of the first vector that are not the row's
@@ -262,26 +266,26 @@ template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
   typedef RowMem<DT> Mem;
   typedef typename Mem::E E;
-  constexpr int W = Mem::W;
+  constexpr int W = Mem::W, kVecs = Mem::kVecs;
   __shared__ SliceShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x / a.S;
   const int s = static_cast<int>(blockIdx.x % a.S);
   const Mem row(a, r);
-  const int v0 = s * kSliceVecs * kSliceThreads;
-  typename Mem::Vec reg[kSliceVecs];
+  const int v0 = s * kVecs * kSliceThreads;
+  typename Mem::Vec reg[kVecs];
 #pragma unroll
-  for (int q = 0; q < kSliceVecs; ++q) reg[q] = row.load(v0 + q * kSliceThreads + tid);
+  for (int q = 0; q < kVecs; ++q) reg[q] = row.load(v0 + q * kSliceThreads + tid);
   const Ask k = ask(a, r);
   Head *head = a.heads + r * a.S + s;
   if (k.kind != kWhole)
     fill_zeros(a.out + r * a.out_stride, min(max(row.first(v0), 0), a.V),
-               min(max(row.first(v0 + kSliceVecs * kSliceThreads), 0), a.V), kSliceThreads);
+               min(max(row.first(v0 + kVecs * kSliceThreads), 0), a.V), kSliceThreads);
 
   // f(index, logit)
   auto each = [&](auto f) {
 #pragma unroll
-    for (int q = 0; q < kSliceVecs; ++q)
+    for (int q = 0; q < kVecs; ++q)
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const E e = reg[q][j];
@@ -353,7 +357,7 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
   }
   // A thread's candidates as bits of its elements, then their indices into LDS; the values
   // are read again (one round trip for all; a branch an element took 4.4 us against 1).
-  constexpr int kSlots = kSliceVecs * W;
+  constexpr int kSlots = kVecs * W;
   static_assert(kSlots <= 64, "a bit each");
   u64 hits = 0;
   double rest = 0.0;
@@ -605,6 +609,10 @@ struct Row {
     const double d = static_cast<double>(x) - m;
     return static_cast<double>(x) == m ? 0.0 : d;  // (also where both are infinite)
   }
+  // What a slice's sum is of weights below the row's largest.
+  __device__ __forceinline__ double rest(const Head &h) const {
+    return h.most > -INFINITY ? h.rest * exp(down(x(h.most))) : 0.0;
+  }
   __device__ __forceinline__ bool alive(float x) const { return down(x) >= low; }  // (a NaN is not)
   __device__ __forceinline__ u64 mass(float x) const {
     const double d = down(x);
@@ -737,8 +745,12 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
   const Head *heads = a.heads + r * a.S;
   if (tid < a.S) sh.head[tid] = heads[tid];
   __syncthreads();
+  // (a lane a slice here and below, in every wave)
+  const int lane = tid & 63, wave = tid >> 6;
   float most = -INFINITY;
-  for (int q = 0; q < a.S; ++q) most = fmaxf(most, sh.head[q].most);
+  for (int q = lane; q < a.S; q += 64) most = fmaxf(most, sh.head[q].most);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   float *o = a.out + r * a.out_stride;
   const Row<DT> row(a, r, k, most);
 
@@ -749,79 +761,82 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
       return;
     }
     double z = 0.0;
-    for (int q = 0; q < a.S; ++q) {
-      const Head h = sh.head[q];
-      if (h.most > -INFINITY) z += h.rest * exp(row.down(row.x(h.most)));
-    }
+    for (int q = lane; q < a.S; q += 64) z += row.rest(sh.head[q]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d);
     whole_row(row.mem, k, static_cast<float>(row.m), static_cast<float>(1.0 / z), o, g, a.groups);
     return;
   }
   if (most == -INFINITY) return;
   if (k.kind == kGreedy) {
     int first = kMaxVocab;
-    for (int q = 0; q < a.S; ++q) first = sh.head[q].most == most ? min(first, sh.head[q].count) : first;
+    for (int q = lane; q < a.S; q += 64) first = sh.head[q].most == most ? min(first, sh.head[q].count) : first;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) first = min(first, __shfl_xor(first, d));
     if (tid == 0) o[first] = 1.f;
     return;
   }
 
   // ---- the slices' candidates, those from `whole` on up: no token there is missing ----
   const bool rest_counts = k.open && !k.top_k && !(k.min_p > 0.f);
-  int listed = 0;
   bool known = true;
   float whole = -INFINITY;
   double rest = 0.0;
-  for (int q = 0; q < a.S; ++q) {
+  for (int q = lane; q < a.S; q += 64) {
     const Head h = sh.head[q];
     known = known && h.count >= 0;
-    listed += h.count;
     whole = fmaxf(whole, h.whole);
-    if (rest_counts && h.most > -INFINITY) {
-      rest += h.rest * exp(row.down(row.x(h.most)));
-    }
+    if (rest_counts) rest += row.rest(h);
+  }
+  known = __all(known);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    whole = fmaxf(whole, __shfl_xor(whole, d));
+    rest += __shfl_xor(rest, d);
   }
   u64 below = 0;  // weight of the candidates that are not kept here
   int n = 0;
   if (known) {
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    // a wave a slice, eight of its candidates a lane at a time
-    const int lane = tid & 63;
-    for (int q = tid >> 6; q < a.S; q += kRowThreads / 64) {
-      const int count = sh.head[q].count;
+    // a wave kChunk of a slice's candidates at a time
+    constexpr int kEach = kChunk / 64;
+    const int chunks = (a.cap + kChunk - 1) / kChunk;
+    for (int t = wave; t < a.S * chunks; t += kRowThreads / 64) {
+      const int q = t / chunks, j0 = t % chunks * kChunk, count = sh.head[q].count;
+      if (j0 >= count) continue;
       const u64 *list = a.lists + (r * a.S + q) * a.cap;
-      for (int j0 = 0; j0 < count; j0 += 512) {
-        u64 key[8];
-        uint64_t kept[8];
-        int all = 0;
+      u64 key[kEach];
+      uint64_t kept[kEach];
+      int all = 0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int j = j0 + 64 * u + lane;
-          key[u] = j < count ? list[j] : 0;
-        }
+      for (int u = 0; u < kEach; ++u) {
+        const int j = j0 + 64 * u + lane;
+        key[u] = j < count ? list[j] : 0;
+      }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          kept[u] = __ballot(j0 + 64 * u + lane < count && order_value(key[u]) >= whole);
-          all += __popcll(kept[u]);
-        }
-        int base = 0;
-        if (lane == 0 && all) base = atomicAdd(&sh.count, all);
-        base = __builtin_amdgcn_readfirstlane(base);
+      for (int u = 0; u < kEach; ++u) {
+        kept[u] = __ballot(j0 + 64 * u + lane < count && order_value(key[u]) >= whole);
+        all += __popcll(kept[u]);
+      }
+      int base = 0;
+      if (lane == 0 && all) base = atomicAdd(&sh.count, all);
+      base = __builtin_amdgcn_readfirstlane(base);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (j0 + 64 * u >= count) break;
-          const bool keep = kept[u] >> lane & 1;
-          const u64 w = keep || (j0 + 64 * u + lane < count && rest_counts) ? row.mass(order_value(key[u])) : 0;
-          if (keep) {
-            const int at = base + __popcll(kept[u] & ((1ull << lane) - 1));
-            if (at < kCand) {
-              sh.key[at] = key[u];
-              sh.mass[at] = w;
-            }
-          } else {
-            below += w;
+      for (int u = 0; u < kEach; ++u) {
+        if (j0 + 64 * u >= count) break;
+        const bool keep = kept[u] >> lane & 1;
+        const u64 w = keep || (j0 + 64 * u + lane < count && rest_counts) ? row.mass(order_value(key[u])) : 0;
+        if (keep) {
+          const int at = base + __popcll(kept[u] & ((1ull << lane) - 1));
+          if (at < kCand) {
+            sh.key[at] = key[u];
+            sh.mass[at] = w;
           }
-          base += __popcll(kept[u]);
+        } else {
+          below += w;
         }
+        base += __popcll(kept[u]);
       }
     }
     if (rest_counts) below = block_reduce(below, sh, plus);
@@ -904,7 +919,7 @@ struct Plan {
 };
 inline Plan plan(int rows, int V, int vec) {
   Plan p;
-  const int per = vec * kSliceVecs * kSliceThreads;
+  const int per = vec * slice_vecs(vec) * kSliceThreads;
   p.S = (V + vec - 1 + per - 1) / per;
   p.cap = std::min(kCand, ((2 * kCand / p.S) + 63) & ~63);
   // The number of threads r whose maxima reach a bound that c tokens of a slice of random order reach:
