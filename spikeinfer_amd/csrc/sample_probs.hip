@@ -625,10 +625,10 @@ struct Row {
 // A cut over the whole row: the tokens' weights (by_count: 1 each; below `from`: none) in bins of
 // 1 / 64 of x below the largest, then the tokens of the bin that holds the cut as candidates; by
 // digits of the key where they are too many, or lie too far below.  share: target is one of the
-// weights' sum.
+// weights' sum; then `kept` is the kept tokens' weight (0 by digits, who do not have it).
 template <int DT>
 __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool by_count, u64 from, double target,
-                                       bool share) {
+                                       bool share, u64 &kept) {
   constexpr float kPerX = 64.f;
   const float top = static_cast<float>(row.m);
   auto bin = [&](float x) {  // (the largest, infinite or not, in the first)
@@ -649,7 +649,8 @@ __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool b
   if (share) {
     u64 z = 0;
     for (int b = threadIdx.x; b < kBins; b += kRowThreads) z += sh.hist[b];
-    target *= static_cast<double>(block_reduce(z, sh, plus));
+    kept = block_reduce(z, sh, plus);
+    target *= static_cast<double>(kept);
   }
   select_bin(sh, 0, target);
   const int digit = static_cast<int>(sh.digit);
@@ -668,10 +669,17 @@ __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool b
     if (n <= kCand) {
       for (int j = threadIdx.x; j < n; j += kRowThreads) sh.mass[j] = weight(order_value(sh.key[j]), order_index(sh.key[j]));
       __syncthreads();
-      return cand_cut(sh, n, by_count, from, above, target, INFINITY, 0.f);
+      const u64 cut = cand_cut(sh, n, by_count, from, above, target, INFINITY, 0.f);
+      if (share) {
+        u64 z = 0;
+        for (int j = threadIdx.x; j < n; j += kRowThreads) z += sh.key[j] >= cut ? sh.mass[j] : 0;
+        kept = above + block_reduce(z, sh, plus);
+      }
+      return cut;
     }
     __syncthreads();
   }
+  kept = 0;
   return radix_cut(sh, 0, order_key(top, 0), 0, target, [&](auto f) {
     row.each([&](int i, float v) {
       const float x = row.x(v);
@@ -683,28 +691,41 @@ __device__ __forceinline__ u64 row_cut(RowShared &sh, const Row<DT> &row, bool b
 // A row whose candidates do not decide it.
 template <int DT>
 __device__ __forceinline__ void long_way(RowShared &sh, const Row<DT> &row, const Ask &k, float *o) {
-  u64 cut = 0;
-  if (k.top_k) cut = row_cut(sh, row, true, 0, static_cast<double>(k.top_k), false);
-  if (k.open) cut = larger(cut, row_cut(sh, row, false, cut, static_cast<double>(k.top_p), true));
-  const float inv = 1.f / k.temp, top = static_cast<float>(row.m);
-  auto kept = [&](int i, float v) {
+  u64 cut = 0, weight = 0;
+  if (k.top_k) cut = row_cut(sh, row, true, 0, static_cast<double>(k.top_k), false, weight);
+  weight = 0;
+  if (k.open) cut = larger(cut, row_cut(sh, row, false, cut, static_cast<double>(k.top_p), true, weight));
+  // the kept tokens as numbers: x at least `lowest`, at or before the cut's
+  const float top = static_cast<float>(row.m), at = cut ? order_value(cut) : -INFINITY;
+  const int last = cut ? order_index(cut) : kMaxVocab;
+  float lowest = -INFINITY;
+  if (k.min_p > 0.f) {
+    lowest = static_cast<float>(row.m + row.low);
+    if (!row.alive(lowest)) lowest = nextafterf(lowest, INFINITY);
+    else if (row.alive(nextafterf(lowest, -INFINITY))) lowest = nextafterf(lowest, -INFINITY);
+  }
+  auto power_of = [&](int i, float v) {  // 0 if it is not kept
     const float x = row.x(v);
-    return row.alive(x) && order_key(x, i) >= cut;
+    return x >= lowest && (x > at || (x == at && i <= last)) ? expf(x == top ? 0.f : x - top) : 0.f;
   };
-  double z = 0.0;
-  row.each([&](int i, float v) { z += kept(i, v) ? static_cast<double>(power(v, k.temp, inv, top)) : 0.0; });
+  float scale = static_cast<float>(kMassScale / static_cast<double>(weight));
+  if (!weight) {
+    double z = 0.0;
+    row.each([&](int i, float v) { z += static_cast<double>(power_of(i, v)); });
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d);
-  double *part = reinterpret_cast<double *>(sh.wave);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = z;
-  __syncthreads();
-  z = 0.0;
+    for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d);
+    double *part = reinterpret_cast<double *>(sh.wave);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = z;
+    __syncthreads();
+    z = 0.0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / 64; ++w) z += part[w];
-  const float scale = static_cast<float>(1.0 / z);
-  row.each([&](int i, float v) {
-    if (kept(i, v)) o[i] = power(v, k.temp, inv, top) * scale;
+    for (int w = 0; w < kRowThreads / 64; ++w) z += part[w];
+    scale = static_cast<float>(1.0 / z);
+  }
+  row.each([&](int i, float v) {  // (the zeros are there)
+    const float e = power_of(i, v);
+    if (e > 0.f) o[i] = e * scale;
   });
 }
 
