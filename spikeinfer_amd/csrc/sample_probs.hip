@@ -863,6 +863,7 @@ __global__ __launch_bounds__(kRowThreads) __attribute__((amdgpu_waves_per_eu(4))
     if (rest_counts) below = block_reduce(below, sh, plus);
     __syncthreads();
     n = sh.count;
+    __syncthreads();  // (a cut counts in it anew)
     // of top_k's prefix every token is there, or every survivor of min_p
     known = n <= kCand && (rest_counts || (k.top_k && n >= k.top_k) || whole == -INFINITY ||
                            row.m + row.low >= static_cast<double>(whole));
