@@ -132,7 +132,8 @@ __device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
 // A workgroup 16 rows: their largest magnitudes, then the integers.  The waves share the row's
 // blocks and keep them in registers between the two (kKeep each; longer rows are read again).
 // WEIGHT: rows in the order of the groups of output channels.  Rows that do not exist become
-// zeros.  Bound by reading x and by the latency of the two passes.
+// zeros.  Bound by reading x and by the latency of the two passes: 16,384 rows of 4,864 in bf16 56 us
+// (239 MB read and written, 4.3 TB/s), 8,188 of 896 10 us, 64 of 896 4.5.
 template <int DT, bool WEIGHT>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int64_t stride, int64_t rows, int K, int KS,
                                                               v4i *packed, float *scales) {
@@ -236,11 +237,13 @@ struct Columns {
 // ---- few rows -----------------------------------------------------------------------
 // A workgroup TM tiles of 16 rows by one group of 64 columns; its eight waves share the steps
 // of K, each with its own blocks of both operands from memory, two steps ahead, and their sums
-// meet in LDS.  Bound by latency: a wave has few steps (K = 896: two).
+// meet in LDS.  Bound by latency: a wave has few steps (K = 896: two; 333 x 1,001 x 777 5.6 us).
 //
 // FUSED (at most 16 rows): x is quantised here.  A wave loads the blocks of x that it
 // multiplies, the waves exchange the rows' largest magnitudes, and the integers are the
 // instruction's operand where they are made; W's first blocks are on their way meanwhile.
+// 4 x 1,152 x 896 5.2 us in place of 4.1 and 4.5 in two launches, 16 x 9,728 x 896 5.6 of 4.0 and
+// 4.3, 16 x 896 x 4,864 19.3 of 15.1 and 7.2, each with a launch less to wait for.
 constexpr int kSplit = 8;
 
 // Adds up the waves' sums; wave i < TM has row tile i's afterwards.
@@ -372,16 +375,20 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
   if (wave == 0 && real) Columns(o, col).store<OT>(o, sum, sc.s, y, r16 * ystride, col);
 }
 
-// ---- few rows, many columns (the lm_head) ----------------------------------------------
-// A workgroup's four waves share up to 64 rows of x in LDS, each takes a group of 64 columns
-// over the whole K and streams its part of W three steps ahead.  Bound by reading W.
+// ---- a tile of rows, many columns (the lm_head) -----------------------------------------
+// A workgroup's four waves share up to 16 rows of x in LDS, each takes a group of 64 columns
+// over the whole K and streams its part of W three steps ahead.  Bound by reading W: 16 x
+// 151,936 x 896 24 us with W in the last-level cache and 29 without it (5.9 and 4.9 TB/s; large
+// tiles 26 and 31; with more rows in LDS the large tiles are faster: 64 rows 29 and 35 against
+// 37 and 43).  Loads that pass the caches by: 26 and 28.
 constexpr int kWideWaves = 4;
+constexpr int kWideColumns = 512;    // groups of columns from which on
 constexpr int kWideLds = 64 * 1024;  // two workgroups a CU
 constexpr int kAhead = 3;
-template <int TM, int OT>
+template <int OT>
 __global__ __launch_bounds__(64 * kWideWaves) void wide_kernel(const v4i *xq, const float *xs, const v4i *wq, Out o, void *y,
-                                                               int64_t ystride, int M, int KS, int MT, int NG) {
-  extern __shared__ v4i shx[];  // [MT][KS][64]
+                                                               int64_t ystride, int M, int KS, int NG) {
+  extern __shared__ v4i shx[];  // [KS][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
   const int g = blockIdx.x * kWideWaves + wave;
   const v4i *a = wq + static_cast<int64_t>(min(g, NG - 1)) * 4 * KS * 64 + lane;
@@ -389,40 +396,29 @@ __global__ __launch_bounds__(64 * kWideWaves) void wide_kernel(const v4i *xq, co
   auto load = [&](int ks, v4i (&av)[4]) {
     const int64_t at = min(ks, KS - 1);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) av[t] = __builtin_nontemporal_load(a + (t * static_cast<int64_t>(KS) + at) * 64);
+    for (int t = 0; t < 4; ++t) av[t] = a[(t * static_cast<int64_t>(KS) + at) * 64];
   };
 #pragma unroll
   for (int q = 0; q < kAhead; ++q) load(q, av[q]);
-  for (int i = threadIdx.x; i < MT * KS * 64; i += 64 * kWideWaves) shx[i] = xq[i];
+  for (int i = threadIdx.x; i < KS * 64; i += 64 * kWideWaves) shx[i] = xq[i];
   __syncthreads();
   if (g >= NG) return;
-  v4i acc[TM][4];
+  v4i acc[4];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  for (int j = 0; j < 4; ++j) acc[j] = v4i{0, 0, 0, 0};
   for (int k0 = 0; k0 < KS; k0 += kAhead) {
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       if (k0 + q < KS) {
-        v4i b[TM];
+        const v4i b = shx[(k0 + q) * 64 + lane];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) b[i] = shx[(min(i, MT - 1) * KS + k0 + q) * 64 + lane];
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[q][j], b[i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[q][j], b, acc[j], 0, 0, 0);
         load(k0 + q + kAhead, av[q]);
       }
     }
   }
   const int col = 64 * g + 16 * kq;
-  const Columns cols(o, col);
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = 16 * i + r16;
-    if (row < M) cols.store<OT>(o, acc[i], xs[row], y, row * ystride, col);
-  }
+  if (r16 < M) Columns(o, col).store<OT>(o, acc, xs[r16], y, r16 * ystride, col);
 }
 
 // ---- many rows ----------------------------------------------------------------------
@@ -431,7 +427,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void wide_kernel(const v4i *xq, co
 // the other's products.  The waves share x through LDS (a step's 8 KB, double-buffered, through
 // registers so that its loads are two steps ahead); each wave's part of W is its own and
 // goes from memory to registers, two steps ahead.  LDS then moves 40 KB a step of 512 cycles
-// of products, where both operands through it would take 72.
+// of products, where both operands through it would take 72.  8,192^3 491 us (2,239 TOP/s), 16,384 x
+// 896 x 4,864 69 (2,080), 8,188 x 9,728 x 896 86 (1,650: 14 steps, then 64 KB of stores).
 constexpr int kBM = 128, kBN = 256;
 constexpr int kTM = kBM / 16, kTN = 4;
 
@@ -556,18 +553,12 @@ void split(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y,
   split_kernel<TM, OT><<<static_cast<unsigned>((MT + TM - 1) / TM * NG), 64 * kSplit, 0, s>>>(xq, xs, wq, o, y, ystride, M,
                                                                                           KS, MT, NG);
 }
-template <int TM, int OT>
-void wide(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y, int64_t ystride, int M, int KS, int MT,
-          int NG, hipStream_t s) {
-  wide_kernel<TM, OT><<<(NG + kWideWaves - 1) / kWideWaves, 64 * kWideWaves, MT * KS * 1024, s>>>(xq, xs, wq, o, y, ystride,
-                                                                                             M, KS, MT, NG);
-}
-
 // The kernel for a size: the least of the times, in us, that fits to measurements give (64 to 2,048
 // rows, 512 to 9,728 columns, K = 896 and 4,864; within a fifth, near their borders).  Measured,
 // with one, two, four row tiles a workgroup of the split kernel and with large tiles: 64 x 896 x
 // 896 3.6, 4.1, 5.1, 9.1; 256 x 9,728 x 896 16.1, 12.5, 14.0, 12.4; 1,024 x 896 x 4,864 20.5,
-// 14.9, 12.9, 32.5; 2,048 x 4,864 x 896 57, 42, 44, 21.
+// 14.9, 12.9, 32.5; 2,048 x 4,864 x 896 57, 42, 44, 21.  From kWideColumns on large tiles whatever the
+// rows: 64 x 33,000 x 896 two row tiles 16, large tiles 12.
 enum Way { kSplit1, kSplit2, kSplit4, kTiles };
 constexpr double kMostThreads = 4294967295.0;  // of a launch
 inline Way way(int64_t M, int N, int KS, int out_bytes) {
@@ -591,13 +582,12 @@ void product(const v4i *xq, const float *xs, const v4i *wq, const float *ws, con
   const int64_t MT = row_tiles(M);
   const int NG = groups_of(N);
   const Out o{ws, bias, bias_dtype, N};
-  if (MT <= 4 && NG >= 512 && MT * KS * 1024 <= kWideLds) {
-    if (MT <= 1) wide<1, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
-    else if (MT <= 2) wide<2, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
-    else wide<4, OT>(xq, xs, wq, o, y, ystride, static_cast<int>(M), KS, static_cast<int>(MT), NG, s);
+  if (MT <= 1 && NG >= kWideColumns && KS * 1024 <= kWideLds) {
+    wide_kernel<OT><<<(NG + kWideWaves - 1) / kWideWaves, 64 * kWideWaves, KS * 1024, s>>>(xq, xs, wq, o, y, ystride,
+                                                                                       static_cast<int>(M), KS, NG);
     return;
   }
-  switch (way(M, N, KS, sizeof(typename Elem<OT>::T))) {
+  switch (NG >= kWideColumns ? kTiles : way(M, N, KS, sizeof(typename Elem<OT>::T))) {
     case kSplit1: split<1, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
     case kSplit2: split<2, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
     case kSplit4: split<4, OT>(xq, xs, wq, o, y, ystride, M, KS, MT, NG, s); break;
@@ -684,7 +674,7 @@ extern "C" int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, con
   i8::v4i *xq = static_cast<i8::v4i *>(workspace);
   float *xs = reinterpret_cast<float *>(static_cast<char *>(workspace) + i8::packed_bytes(M, K));
   const i8::v4i *wq = static_cast<const i8::v4i *>(packed);
-  if (M <= 16 && i8::groups_of(N) < 512) {
+  if (M <= 16 && i8::groups_of(N) < i8::kWideColumns) {
     if (y_dtype == SPK_F32) i8::fused<SPK_F32>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
     else if (y_dtype == SPK_F16) i8::fused<SPK_F16>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
     else i8::fused<SPK_BF16>(x, x_dtype, x_stride, wq, scales, bias, bias_dtype, y, y_stride, static_cast<int>(M), N, K, s);
