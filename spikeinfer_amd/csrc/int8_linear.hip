@@ -98,14 +98,16 @@ __device__ __forceinline__ Scale scale_of(uint32_t most) {
 }
 
 // rint(x / s) with the quotient rounded to fp32.  x inv is off by less than two steps of fp32
-// (1.5e-5 at 127), so where it lies further than that from a half its rounding is the same; only
-// where one of the sixteen is near a half are the quotients themselves needed (a division is ten
-// instructions, this is five).  Adding 1.5 2^23 rounds to an integer in the low bits.
+// (1.5e-5 at 127), so where it lies further than that from a half its rounding is the same
+// (adding 1.5 2^23 rounds to an integer in the low bits).  Near a half h = n + 1/2 the quotient rounds to
+// h itself where |x - h s| <= s ulp(h) / 2 (h has few bits, a tie is its), and to h's side
+// otherwise; x - h s is exact there.  A row whose largest magnitude is 127 times a power of two
+// has many halves: 64 rows of 4,864 with one such 5.7 us, 9.6 with divisions.
 template <int DT>
 __device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
   v4i out = {0, 0, 0, 0};
   if (!sc.some) return out;
-  constexpr float kMagic = 12582912.f;
+  constexpr float kMagic = 12582912.f, kNear = 0.5f - 6.2e-5f;
   uint32_t w[16];
   float far = 0.f;
 #pragma unroll
@@ -115,10 +117,19 @@ __device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
     far = fmaxf(far, fabsf(__builtin_fmaf(x, sc.inv, -(y - kMagic))));
     w[j] = __float_as_uint(y);
   }
-  if (far > 0.5f - 6.2e-5f || sc.tiny) {
+  if (far > kNear || sc.tiny) {
+    const float up = sc.tiny ? 0x1p100f : 1.f, inv = sc.tiny ? 1.f / (sc.s * up) : sc.inv, t = sc.s * up * 0x1p-24f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      w[j] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(elem_to_f32<DT>(b.e[j]) / sc.s), -127.f), 127.f)));
+    for (int j = 0; j < 16; ++j) {
+      const float x = elem_to_f32<DT>(b.e[j]) * up, y = __builtin_fmaf(x, inv, kMagic) - kMagic;
+      const float d = __builtin_fmaf(x, inv, -y);
+      if (fabsf(d) > kNear || sc.tiny) {
+        const float h = y + copysignf(0.5f, d), r = __builtin_fmaf(-h, sc.s * up, x);
+        const float ulp = __uint_as_float(__float_as_uint(h) & 0x7f800000u);  // (over 2^-23)
+        const float q = fabsf(r) <= ulp * t ? rintf(h) : h + copysignf(0.5f, r);
+        w[j] = __float_as_uint(fminf(fmaxf(q, -127.f), 127.f) + kMagic);
+      }
+    }
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -129,48 +140,54 @@ __device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
   return out;
 }
 
-// A workgroup 16 rows: their largest magnitudes, then the integers.  The waves share the row's
-// blocks and keep them in registers between the two (kKeep each; longer rows are read again).
-// WEIGHT: rows in the order of the groups of output channels.  Rows that do not exist become
-// zeros.  Bound by reading x and by the latency of the two passes: 16,384 rows of 4,864 in bf16 56 us
-// (239 MB read and written, 4.3 TB/s), 8,188 of 896 10 us, 64 of 896 4.5.
-template <int DT, bool WEIGHT>
+// A workgroup R rows of a tile (16 or 4): their largest magnitudes, then the integers.  A wave
+// takes 16 / R blocks at a time, in all R of their rows; the waves share the row's blocks and keep
+// them in registers between the two (kKeep times; longer rows are read again).  WEIGHT: rows in
+// the order of the groups of output channels.  Rows that do not exist become zeros.  Bound by
+// reading x and by the latency of the two passes: 16,384 rows of 4,864 in bf16 56 us (239 MB read
+// and written, 4.3 TB/s), 8,188 of 896 10 us.  Few tiles by four rows a workgroup: 1,000 rows of 896
+// 4.8 us (by 16 rows 8.5), 333 of 777 4.8 (8.9).
+template <int DT, bool WEIGHT, int R>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int64_t stride, int64_t rows, int K, int KS,
                                                               v4i *packed, float *scales) {
-  __shared__ uint32_t most[kRowWaves][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, r16 = lane & 15, kq = lane >> 4;
-  const int64_t tile = blockIdx.x;
+  constexpr int kBlocks = 16 / R;
+  __shared__ uint32_t most[kRowWaves][R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int r16 = static_cast<int>(blockIdx.x % kBlocks) * R + lane % R, kq = lane / R % 4;
+  const int64_t tile = blockIdx.x / kBlocks;
   const int64_t row = WEIGHT ? tile / 4 * 64 + 16 * (r16 >> 2) + 4 * (tile & 3) + (r16 & 3) : 16 * tile + r16;
   const bool real = row < rows;
   const char *p = static_cast<const char *>(x) + (real ? row : 0) * stride * static_cast<int64_t>(sizeof(typename Elem<DT>::T));
   const int Kr = real ? K : 0;
+  const int first = wave * kBlocks + lane / (4 * R), next = waves * kBlocks;
+  v4i *to = packed + tile * KS * 64 + kq * 16 + r16;
   Block<DT> v[kKeep];
 #pragma unroll
   for (int q = 0; q < kKeep; ++q)
-    if (wave + q * waves < KS) v[q].load(p, kStep * (wave + q * waves) + 8 * kq, Kr);
+    if (first + q * next < KS) v[q].load(p, kStep * (first + q * next) + 8 * kq, Kr);
   uint32_t m = 0;
 #pragma unroll
   for (int q = 0; q < kKeep; ++q)
-    if (wave + q * waves < KS) m = max(m, v[q].most());
-  for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
+    if (first + q * next < KS) m = max(m, v[q].most());
+  for (int ks = first + kKeep * next; ks < KS; ks += next) {
     Block<DT> a;
     a.load(p, kStep * ks + 8 * kq, Kr);
     m = max(m, a.most());
   }
-  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
-  m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
-  if (lane < 16) most[wave][lane] = m;
+#pragma unroll
+  for (int d = R; d < 64; d <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), d)));
+  if (lane < R) most[wave][lane] = m;
   __syncthreads();
-  for (int w = 0; w < waves; ++w) m = max(m, most[w][r16]);
+  for (int w = 0; w < waves; ++w) m = max(m, most[w][lane % R]);
   const Scale sc = scale_of(m);
-  if (threadIdx.x < 16) scales[row] = sc.s;
+  if (threadIdx.x < R) scales[row] = sc.s;
 #pragma unroll
   for (int q = 0; q < kKeep; ++q)
-    if (wave + q * waves < KS) packed[(tile * KS + wave + q * waves) * 64 + lane] = quantise16(v[q], sc);
-  for (int ks = wave + kKeep * waves; ks < KS; ks += waves) {
+    if (first + q * next < KS) to[(first + q * next) * 64] = quantise16(v[q], sc);
+  for (int ks = first + kKeep * next; ks < KS; ks += next) {
     Block<DT> a;
     a.load(p, kStep * ks + 8 * kq, Kr);
-    packed[(tile * KS + ks) * 64 + lane] = quantise16(a, sc);
+    to[ks * 64] = quantise16(a, sc);
   }
 }
 
@@ -242,12 +259,13 @@ struct Columns {
 // FUSED (at most 16 rows): x is quantised here.  A wave loads the blocks of x that it
 // multiplies, the waves exchange the rows' largest magnitudes, and the integers are the
 // instruction's operand where they are made; W's first blocks are on their way meanwhile.
-// 4 x 1,152 x 896 5.2 us in place of 4.1 and 4.5 in two launches, 16 x 9,728 x 896 5.6 of 4.0 and
-// 4.3, 16 x 896 x 4,864 19.3 of 15.1 and 7.2, each with a launch less to wait for.
+// 4 x 1,152 x 896 5.2 us in place of 3.8 and 4.4 in two launches, 16 x 9,728 x 896 5.6 of 4.0 and
+// 4.3, 4 x 896 x 4,864 11.4 of 4.0 and 7.8 (16 rows: 15.4 of 5.8 and 7.8), each with a launch less to
+// wait for.  Sixteen waves for more than two steps of eight (4 x 896 x 4,864: eight 12.6).
 constexpr int kSplit = 8;
 
 // Adds up the waves' sums; wave i < TM has row tile i's afterwards.
-template <int TM>
+template <int TM, int WAVES>
 __device__ __forceinline__ void join(v4i *sh, const v4i (&acc)[TM][4], v4i (&sum)[4]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -260,7 +278,7 @@ __device__ __forceinline__ void join(v4i *sh, const v4i (&acc)[TM][4], v4i (&sum
   for (int j = 0; j < 4; ++j) {
     sum[j] = sh[(wave * 4 + j) * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kSplit; ++w) sum[j] += sh[((w * TM + wave) * 4 + j) * 64 + lane];
+    for (int w = 1; w < WAVES; ++w) sum[j] += sh[((w * TM + wave) * 4 + j) * 64 + lane];
   }
 }
 
@@ -302,18 +320,18 @@ __global__ __launch_bounds__(64 * kSplit) void split_kernel(const v4i *xq, const
     load(ks + 3 * kSplit, av[1], bv[1]);
   }
   v4i sum[4];
-  join<TM>(sh, acc, sum);
+  join<TM, kSplit>(sh, acc, sum);
   const int64_t row = 16 * (m0 + wave) + r16;
   const int col = 64 * g + 16 * kq;
   if (wave < TM && row < M) Columns(o, col).store<OT>(o, sum, xs[row], y, row * ystride, col);
 }
 
 // HOLD: blocks of x that a wave holds; those of longer rows are read again.
-template <int DT, int HOLD, int OT>
-__global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64_t stride, const v4i *wq, Out o, void *y,
+template <int DT, int WAVES, int HOLD, int OT>
+__global__ __launch_bounds__(64 * WAVES) void fused_kernel(const void *x, int64_t stride, const v4i *wq, Out o, void *y,
                                                             int64_t ystride, int M, int K, int KS) {
-  __shared__ v4i sh[kSplit * 4 * 64];
-  __shared__ uint32_t most[kSplit][16];
+  __shared__ v4i sh[WAVES * 4 * 64];
+  __shared__ uint32_t most[WAVES][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4, g = blockIdx.x;
   const v4i *a = wq + static_cast<int64_t>(g) * 4 * KS * 64 + lane;
   const bool real = r16 < M;
@@ -327,13 +345,13 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
   };
   Block<DT> v[HOLD];
 #pragma unroll
-  for (int q = 0; q < HOLD; ++q) v[q].load(p, kStep * (wave + q * kSplit) + 8 * kq, Kr);
+  for (int q = 0; q < HOLD; ++q) v[q].load(p, kStep * (wave + q * WAVES) + 8 * kq, Kr);
   load(wave, av[0]);
-  load(wave + kSplit, av[1]);
+  load(wave + WAVES, av[1]);
   uint32_t m = 0;
 #pragma unroll
   for (int q = 0; q < HOLD; ++q) m = max(m, v[q].most());
-  for (int ks = wave + HOLD * kSplit; ks < KS; ks += kSplit) {
+  for (int ks = wave + HOLD * WAVES; ks < KS; ks += WAVES) {
     Block<DT> e;
     e.load(p, kStep * ks + 8 * kq, Kr);
     m = max(m, e.most());
@@ -343,7 +361,7 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
   if (lane < 16) most[wave][lane] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSplit; ++w) m = max(m, most[w][r16]);
+  for (int w = 0; w < WAVES; ++w) m = max(m, most[w][r16]);
   const Scale sc = scale_of(m);
   v4i acc[1][4];
 #pragma unroll
@@ -355,22 +373,22 @@ __global__ __launch_bounds__(64 * kSplit) void fused_kernel(const void *x, int64
   static_assert(HOLD % 2 == 0, "two buffers of W take turns");
 #pragma unroll
   for (int q = 0; q < HOLD; ++q) {
-    if (wave + q * kSplit < KS) products(av[q & 1], quantise16(v[q], sc));
-    load(wave + (q + 2) * kSplit, av[q & 1]);
+    if (wave + q * WAVES < KS) products(av[q & 1], quantise16(v[q], sc));
+    load(wave + (q + 2) * WAVES, av[q & 1]);
   }
-  for (int ks = wave + HOLD * kSplit; ks < KS; ks += 2 * kSplit) {
+  for (int ks = wave + HOLD * WAVES; ks < KS; ks += 2 * WAVES) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      if (ks + q * kSplit < KS) {
+      if (ks + q * WAVES < KS) {
         Block<DT> e;
-        e.load(p, kStep * (ks + q * kSplit) + 8 * kq, Kr);
+        e.load(p, kStep * (ks + q * WAVES) + 8 * kq, Kr);
         products(av[q], quantise16(e, sc));
-        load(ks + (q + 2) * kSplit, av[q]);
+        load(ks + (q + 2) * WAVES, av[q]);
       }
     }
   }
   v4i sum[4];
-  join<1>(sh, acc, sum);
+  join<1, WAVES>(sh, acc, sum);
   const int col = 64 * g + 16 * kq;
   if (wave == 0 && real) Columns(o, col).store<OT>(o, sum, sc.s, y, r16 * ystride, col);
 }
@@ -533,11 +551,11 @@ template <int DT>
 void launch_rows(const void *x, int64_t stride, int64_t rows, int K, bool weight, void *packed, float *scales,
                  hipStream_t s) {
   const int KS = static_cast<int>(k_steps(K));
-  const unsigned grid = static_cast<unsigned>(weight ? 4 * ((rows + 63) / 64) : row_tiles(rows));
-  const int waves = row_waves(KS);
+  const unsigned tiles = static_cast<unsigned>(weight ? 4 * ((rows + 63) / 64) : row_tiles(rows));
   v4i *to = static_cast<v4i *>(packed);
-  if (weight) rows_kernel<DT, true><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
-  else rows_kernel<DT, false><<<grid, 64 * waves, 0, s>>>(x, stride, rows, K, KS, to, scales);
+  if (weight) rows_kernel<DT, true, 16><<<tiles, 64 * row_waves(KS), 0, s>>>(x, stride, rows, K, KS, to, scales);
+  else if (tiles > 64) rows_kernel<DT, false, 16><<<tiles, 64 * row_waves(KS), 0, s>>>(x, stride, rows, K, KS, to, scales);
+  else rows_kernel<DT, false, 4><<<4 * tiles, 64 * row_waves((KS + 3) / 4), 0, s>>>(x, stride, rows, K, KS, to, scales);
 }
 
 void rows(const void *x, int dtype, int64_t stride, int64_t n, int K, bool weight, void *packed, float *scales,
@@ -605,8 +623,10 @@ template <int DT, int OT>
 void launch_fused(const void *x, int64_t stride, const v4i *wq, const Out &o, void *y, int64_t ystride, int M, int K,
                   hipStream_t s) {
   const int KS = static_cast<int>(k_steps(K)), NG = groups_of(o.N);
-  if (KS <= 2 * kSplit) fused_kernel<DT, 2, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
-  else fused_kernel<DT, 10, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  constexpr int kHold = DT == SPK_F32 ? 2 : 6;  // (of what 128 registers hold)
+  if (KS <= 2 * kSplit) fused_kernel<DT, kSplit, 2, OT><<<NG, 64 * kSplit, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  else if (KS <= 2 * 16) fused_kernel<DT, 16, 2, OT><<<NG, 64 * 16, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
+  else fused_kernel<DT, 16, kHold, OT><<<NG, 64 * 16, 0, s>>>(x, stride, wq, o, y, ystride, M, K, KS);
 }
 template <int OT>
 void fused(const void *x, int dtype, int64_t stride, const v4i *wq, const float *ws, const void *bias, int bias_dtype,
