@@ -8,7 +8,8 @@
 // largest): sums do not depend on the order they are made in, and a cut falls where exact
 // arithmetic has it unless two numbers agree to 11 digits.
 //
-// Two launches, both a workgroup a slice of a row.  Cuts keep few tokens as a rule, so:
+// Two launches, the first a workgroup a slice of a row, the second one a row (more where there are
+// no cuts).  Cuts keep few tokens as a rule, so:
 //   * the first (slice_kernel) holds its slice in registers, fills its part of the result with
 //     zeros and lists its candidates, the logits at or above a bound that so many of the
 //     threads' maxima reach, with the sum of the others' weights;
@@ -18,6 +19,9 @@
 //     where the cut could fall elsewhere within that bound, or below a slice's bound, the row
 //     goes the long way, through histograms of the weights over the row.
 // A row without cuts gets its sum from the first launch and its values from the second.
+// Many rows are bound by memory (320 of 151,936 in bf16: slices 64 us, 4.5 TB/s, rows 16), few by
+// the phases behind barriers (one row: 12 and 16 us, of which the weights in fp64 take 4 and 3).
+// The long way takes a workgroup about 190 us for 151,936 tokens.
 #include <algorithm>
 #include <cmath>
 

@@ -15,7 +15,8 @@
 // launch r follows each tree up to its r-th sum (the sums before it are there, so every
 // workgroup repeats the walk, in LDS), and its slices add up their share.  The last launch,
 // one workgroup a tree, follows the walk to its end, sums by itself where a tree needs more, and
-// draws.  Bound by reading the rows: 64 chains, 78 MB.  Sums and tests are fp64: a decision
+// draws.  Many trees are bound by reading the rows (64 chains of up to 8 nodes at 151,936 tokens:
+// slices 14.6 us, 5.3 TB/s, the last launch 11), few by latency (one chain 6.3 and 8.4).  Sums and tests are fp64: a decision
 // differs from exact arithmetic's only where the numbers are equal to 15 digits.
 #include <algorithm>
 
