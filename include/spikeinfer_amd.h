@@ -771,7 +771,7 @@ int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, const void *pa
  * zeros; a NaN has probability 0; of infinite logits all count the same, others nothing.
  *   logits   [rows, vocab] at row_stride, vocab stride 1, vocab <= 262144
  *   temperature float [rows]; top_k int32, top_p and min_p float [rows], or NULL: off
- *   probs    float [rows, vocab] at out_stride
+ *   probs    float [rows, vocab] at out_stride, not on the logits
  *   workspace spk_sample_probs_workspace_bytes(rows, vocab) bytes, 16-byte aligned (NULL
  *            when that is 0)
  */

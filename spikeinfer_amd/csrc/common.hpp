@@ -129,4 +129,15 @@ __device__ __forceinline__ void store_spike(void *p, int64_t i, int dtype, bool 
 inline bool valid_float_dtype(int d) { return d == SPK_F32 || d == SPK_F16 || d == SPK_BF16; }
 inline bool valid_any_dtype(int d) { return d >= SPK_F32 && d <= SPK_I32; }
 
+// Whether rows of n bytes at one distance lie on rows of m bytes at another (equal distances may
+// interleave).
+inline bool on_one_another(const void *a, int64_t stride_a, int64_t n, const void *b,
+                           int64_t stride_b, int64_t m, int64_t rows) {
+  const int64_t d = reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a);  // where b begins in a
+  if (d >= (rows - 1) * stride_a + n || d + (rows - 1) * stride_b + m <= 0) return false;
+  if (stride_a != stride_b || stride_a <= 0) return true;
+  const int64_t in = (d % stride_a + stride_a) % stride_a;
+  return in < n || in + m > stride_a;
+}
+
 }  // namespace spk

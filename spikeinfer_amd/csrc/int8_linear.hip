@@ -689,6 +689,9 @@ extern "C" int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, con
     return fail(SPK_EINVAL, "linear_int8: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if ((reinterpret_cast<uintptr_t>(packed) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return fail(SPK_EINVAL, "linear_int8: packed and workspace must be 16-byte aligned");
+  const int64_t xb = x_dtype == SPK_F32 ? 4 : 2, yb = y_dtype == SPK_F32 ? 4 : 2;
+  if (on_one_another(x, x_stride * xb, K * xb, y, y_stride * yb, N * yb, M))
+    return fail(SPK_EINVAL, "linear_int8: y lies on x");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int KS = static_cast<int>(i8::k_steps(K));
   i8::v4i *xq = static_cast<i8::v4i *>(workspace);

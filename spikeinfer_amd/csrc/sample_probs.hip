@@ -1005,10 +1005,14 @@ extern "C" int spk_sample_probs(const void *logits, int logits_dtype, int64_t ro
   if (static_cast<double>(rows) * probs::plan(1, vocab, 4).S * probs::kSliceThreads > 4294967295.0)
     return fail(SPK_EUNSUPPORTED, "sample_probs: more threads than a launch has, rows=%d vocab=%d", rows, vocab);
   if (!logits || !temperature || !probs_out) return fail(SPK_EINVAL, "sample_probs: null pointer");
+  const int64_t dtype_bytes = logits_dtype == SPK_F32 ? 4 : 2;
   const size_t need = spk_sample_probs_workspace_bytes(rows, vocab);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(SPK_EINVAL, "sample_probs: workspace of %zu bytes, %zu needed, aligned to 16",
                 workspace ? workspace_bytes : 0, need);
+  if (on_one_another(logits, row_stride * dtype_bytes, vocab * dtype_bytes, probs_out,
+                     out_stride * 4, vocab * int64_t{4}, rows))
+    return fail(SPK_EINVAL, "sample_probs: the output lies on the logits");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const probs::Args a{logits, row_stride, vocab, temperature, top_p, min_p, top_k, probs_out, out_stride, 0, 0, 0, 0,
                       0, nullptr, nullptr};

@@ -194,7 +194,7 @@ def sampling_probs(
     prefixes on the other side of a border, one token differs).  A greedy row is 1 at its first
     largest logit; a row with no logit above -infinity is all zeros; NaN has probability 0.
 
-    ``out``: optional ``float32 [rows, vocab]``, vocab contiguous; ``workspace``: optional ``uint8``
+    ``out``: optional ``float32 [rows, vocab]``, vocab contiguous, not on the logits; ``workspace``: optional ``uint8``
     scratch of :func:`sampling_probs_workspace_bytes` (calls that may run at once need one each).
     """
     native = _lib.native()

@@ -148,6 +148,17 @@ def test_strides_out_and_defaults(gpu):
     assert sampling_probs(torch.zeros((0, 5), device=gpu), torch.zeros(0, device=gpu)).shape == (0, 5)
 
 
+def test_rows_between_the_logits(gpu):
+    """Logits and probabilities in turn in one tensor; on one another they are refused."""
+    both = torch.randn((6, 2, 700), generator=torch.Generator().manual_seed(12)).to(gpu) * 3
+    logits, one = both[:, 0].clone(), torch.ones(6, device=gpu)
+    out = sampling_probs(both[:, 0], one, top_p=one * 0.8, out=both[:, 1])
+    assert torch.equal(both[:, 0], logits) and torch.equal(out, sampling_probs(logits, one, top_p=one * 0.8))
+    for bad in (both[:, 0], both.view(-1)[1:1 + 6 * 700].view(6, 700)):
+        with pytest.raises(ValueError, match="lies on the logits"):
+            sampling_probs(both[:, 0], one, out=bad)
+
+
 def test_offsets_past_32_bits(gpu):
     """A batch of more than 2^32 bytes of logits and of probabilities."""
     rows, V = 9000, 262144

@@ -32,6 +32,8 @@ def test_linear_refusals():
                    (dict(ws=None), 1), (dict(wsb=16), 1), (dict(ws=P + 4), 1), (dict(packed=P + 1), 1)):
         assert linear(**kw) == rc, kw
     assert linear(M=0) == _lib.SPK_OK
+    for kw in (dict(y=P), dict(y=P + 4 * 64 * 2), dict(y=P - 2 * 48 * 4), dict(x=P + 2 * 48 * 4, y=P)):
+        assert linear(**kw) == 1 and b"y lies on x" in lib.spk_last_error(), kw
     # more threads than a launch has
     assert linear(M=1 << 30, N=1 << 20, ys=1 << 20, wsb=1 << 62) == _lib.SPK_EUNSUPPORTED
     assert linear(M=1 << 30, K=4096, wsb=1 << 62) == _lib.SPK_EUNSUPPORTED and b"launch" in lib.spk_last_error()
@@ -54,6 +56,24 @@ def test_distribution_refusals():
                    (dict(ws=P + 8), 1)):
         assert probs(**kw) == rc, kw
     assert probs(rows=0) == _lib.SPK_OK
+
+
+def test_distributions_on_their_logits_are_refused():
+    """Whole, in part, at either end, rows of one between rows of the other."""
+    lib = _lib.load()
+    V, rows = 100, 3
+
+    def probs(out, os, dt=0, row_stride=V):
+        rc = lib.spk_sample_probs(1 << 20, dt, row_stride, rows, V, P, None, None, None, out, os, P, 1 << 40, None)
+        return rc, lib.spk_last_error()
+
+    base = 1 << 20
+    for out, os, dt, stride in ((base, V, 0, V), (base + 4, V, 0, V), (base + 4 * (rows * V - 1), V, 0, V),
+                                (base - 4 * (rows * V - 1), V, 0, V), (base, 2 * V, 0, V), (base + 2 * V, 2 * V, 2, V),
+                                (base + 4 * (V - 1), 2 * V, 0, 2 * V), (base + 4 * (V + 1), 2 * V, 0, 2 * V),
+                                (base, V, 0, 0), (base - 4 * V, 2 * V, 0, 0)):
+        rc, why = probs(out, os, dt, stride)
+        assert rc == 1 and b"lies on the logits" in why, (out - base, os, dt, stride)
 
 
 def test_verification_refusals():
