@@ -30,14 +30,15 @@ using draft::kMaxNodes;
 constexpr int kSliceThreads = 256;
 constexpr int kEndThreads = 1024;
 constexpr int kMaxSlices = 64;  // a lane each
-constexpr int kMaxRounds = 3;
+constexpr int kMaxRounds = 4;
 
 // Launches of slices.  A chain needs one sum, a tree one a rejected sibling, a few as a rule.
 // Those that are left to the last launch take one workgroup: 5 to 10 us each at 151,936 tokens,
 // 2 at 32,000; a launch that finds every tree done takes 2 to 3.  One launch against three, us:
 // 16 trees of 25 nodes at 151,936 tokens 56 and 36, 14 of 8 nodes with up to 3 siblings 52 and
 // 36, 64 chains of 8 nodes 27 and 30, one chain of 5 15 and 21; 7 trees of 13 nodes at 32,003
-// 20 and 28.  (Which of them it is the host does not know: few nodes are chains as a rule.)
+// 20 and 28.  (Which of them it is the host does not know: few nodes are chains as a rule.)  Three,
+// four and five over 25 draws of the 16 trees: 39.1, 37.8, 40.5, the slowest 59, 48, 51.
 inline int rounds_for(int max_nodes, int V) { return max_nodes > 8 && V >= 65536 ? kMaxRounds : 1; }
 
 struct Params {
