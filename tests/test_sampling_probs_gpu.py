@@ -148,6 +148,21 @@ def test_strides_out_and_defaults(gpu):
     assert sampling_probs(torch.zeros((0, 5), device=gpu), torch.zeros(0, device=gpu)).shape == (0, 5)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows_keep_their_counts(gpu, dtype):
+    """Thousands of rows whose top_k is decided among hundreds of candidates, all at once: each
+    keeps the first k of its order, every call."""
+    rows, V, k = 3000, 32003, 200
+    logits = (torch.randn((rows, V), generator=torch.Generator().manual_seed(13)) * 2).to(DTYPES[dtype]).to(gpu)
+    one, ks = torch.ones(rows, device=gpu), torch.full((rows,), k, dtype=torch.int32, device=gpu)
+    order = logits.float().sort(dim=1, descending=True, stable=True).indices[:, :k]
+    want = torch.zeros((rows, V), dtype=torch.bool, device=gpu).scatter_(1, order, True)
+    first = sampling_probs(logits, one, ks)
+    assert torch.equal(first > 0, want)
+    for _ in range(4):
+        assert torch.equal(sampling_probs(logits, one, ks), first)
+
+
 def test_rows_between_the_logits(gpu):
     """Logits and probabilities in turn in one tensor; on one another they are refused."""
     both = torch.randn((6, 2, 700), generator=torch.Generator().manual_seed(12)).to(gpu) * 3
