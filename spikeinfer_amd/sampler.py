@@ -308,7 +308,7 @@ class BatchSampler:
         need = [i for i, p in enumerate(self.params[:n]) if p.logit_bias or p.min_tokens]
         if not need:
             return logits
-        logits = logits.float()
+        logits = logits.to(torch.float32, copy=True)  # (fp32 logits are the caller's)
         lens = self.history_len[:n].tolist()  # host sync: only on this rare path
         for i in need:
             p = self.params[i]
