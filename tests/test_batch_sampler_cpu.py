@@ -15,7 +15,7 @@ def test_filters_leave_the_callers_logits(dtype):
     s.set_params([SamplingParams(logit_bias={1: 2.0, 3: -1.0}), SamplingParams(min_tokens=2, stop_token_ids=[0])])
     logits = torch.arange(12.0).reshape(2, 6).to(dtype)
     before = logits.clone()
-    want = before.float()
+    want = before.clone().float()
     want[0, 1] += 2.0
     want[0, 3] -= 1.0
     want[1, 0] = want[1, 4] = -torch.inf

@@ -16,7 +16,7 @@ def test_distributions_then_a_draw(gpu, dtype):
     n, V = 3, 700
     logits = torch.randn((n, V), generator=torch.Generator().manual_seed(0)).to(dtype).to(gpu)
     before = logits.clone()
-    changed = before.float()
+    changed = before.clone().float()
     changed[0, 5] += 6.0
     changed[1, 7] = -torch.inf
     changed[1, 9] = -torch.inf
