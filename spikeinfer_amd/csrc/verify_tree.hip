@@ -321,11 +321,12 @@ __global__ __launch_bounds__(kEndThreads) void end_kernel(Params P) {
     if (tid == (sh.found < kEndThreads ? sh.found : sh.last)) {
       double c = below + (inc - mine);
       int token = -1;
-      for (int x = x0; x < x1 && !(c > t); x += 4) {
+      // (where c is rounded up past t already, the first token with weight)
+      for (int x = x0; x < x1 && (token < 0 || !(c > t)); x += 4) {
         if (each > 4) w.weights(p, q, x, x1, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (v[j] > 0.0 && !(c > t)) {
+          if (v[j] > 0.0 && (token < 0 || !(c > t))) {
             token = x + j;
             c += v[j];
           }
