@@ -76,13 +76,15 @@ __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
 }
 
 // A logit over the temperature; what is finite stays finite (a mask of the type's lowest value
-// is no -infinity below a temperature of 1).  inv = 1 / temp in fp64: the quotient of two
+// is no -infinity below a temperature of 1), what is infinite stays infinite (over an infinite
+// temperature too, where every other logit is 0).  inv = 1 / temp in fp64: the quotient of two
 // fp32 numbers lies at least 2^-49 of itself from the middle between two fp32 numbers, and the
 // product is off by at most 2^-52, so its rounding is the quotient's (below 2^-126, where the
 // numbers have fewer bits, it may be the one beside it).
 __device__ __forceinline__ float quotient(float v, double inv) {
   const float x = static_cast<float>(static_cast<double>(v) * inv);
-  return fabsf(x) == INFINITY && fabsf(v) != INFINITY ? copysignf(kMost, v) : x;
+  if (fabsf(v) == INFINITY) return v;
+  return fabsf(x) == INFINITY ? copysignf(kMost, v) : x;
 }
 
 // A bound at or below every logit whose quotient is `x`, that of `bound`.
@@ -97,7 +99,7 @@ __device__ __forceinline__ float same_quotient(float bound, float x, float temp)
 __device__ __forceinline__ float power(float v, float temp, float inv, float x_most) {
   const float q = v * inv;
   float x = __builtin_fmaf(__builtin_fmaf(-q, temp, v), inv, q);
-  x = fabsf(q) < 1e30f ? x : quotient(v, 1.0 / static_cast<double>(temp));  // (and infinities, NaN)
+  x = fabsf(q) < 1e30f && temp < INFINITY ? x : quotient(v, 1.0 / static_cast<double>(temp));  // (and infinities, NaN)
   return x == x ? expf(x == x_most ? 0.f : x - x_most) : 0.f;
 }
 
@@ -352,7 +354,7 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
   bound = same_quotient(bound, whole, k.temp);
   if (k.min_p > 0.f) {  // those below ln min_p under this slice's largest are none of the row's
     const double x = static_cast<double>(x_most) + k.low;
-    const float least = x <= -static_cast<double>(kMost) ? -INFINITY : static_cast<float>(x * static_cast<double>(k.temp));
+    const float least = x <= -static_cast<double>(kMost) || !(k.temp < INFINITY) ? -INFINITY : static_cast<float>(x * static_cast<double>(k.temp));
     const float lower = fabsf(least) == INFINITY ? least : least - fabsf(least) * 0x1p-20f - k.temp * 0x1p-148f;
     if (lower > bound || !k.top_k) {
       bound = lower;
