@@ -744,8 +744,9 @@ int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_stri
  * Linear layer in 8-bit integers with a scale for every row of x and of W:
  *   s = max |x| / 127, q = rint(x / s) (both quotients rounded to fp32; s = 0: q = 0),
  *   y[m, n] = s_x[m] s_w[n] sum_k q_x[m, k] q_w[n, k] + bias[n]
- * The integer sum is exact; scales and bias are fp32, rounded once to y's type.  A row of x
- * that holds an infinity or a NaN gives a row of NaN, a row of W a column.
+ * The integer sum is exact; scales and bias are fp32, rounded once to y's type (s_x s_w is
+ * rounded as fp32 is, but has no smallest or largest value of its own).  A row of x that holds
+ * an infinity or a NaN gives a row of NaN, a row of W a column.
  *   w, x, bias, y  F32, F16 or BF16 each, channel stride 1, rows at their strides; rows of y
  *            must not lie on one another, nor y on x
  *   packed   spk_linear_int8_packed_bytes(N, K) bytes, 16-byte aligned, and scales float

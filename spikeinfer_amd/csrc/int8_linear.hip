@@ -192,7 +192,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int
 }
 
 // Sixteen columns of y from column `col` on, as a lane has them of a group's four tiles: the
-// channels' scales and biases, and the store of a row.
+// channels' scales and biases, and the store of a row.  Scales are mantissas and exponents: the
+// product of two may have no value in fp32 where y has one (large by large with a sum of 0, small by
+// small with a large one).  A power of two rounds nothing, so where it has, y's bits are those of sum *
+// (s_x * s_w) + bias (8,188 x 9,728 x 896 with x's rows 92 -> 94 us, K = 64 42.8 -> 44.1, others within 2 %).
 struct Out {
   const float *ws;
   const void *bias;
@@ -200,7 +203,8 @@ struct Out {
   int N;
 };
 struct Columns {
-  float s[16], b[16];
+  float s[16], b[16];  // mantissas, biases
+  int x[16];           // exponents
 
   __device__ __forceinline__ Columns(const Out &o, int col) {
     typedef float F4 __attribute__((ext_vector_type(4)));
@@ -208,7 +212,10 @@ struct Columns {
     for (int j = 0; j < 4; ++j) {
       const F4 v = *reinterpret_cast<const F4 *>(o.ws + col + 4 * j);  // (padded to 64)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[4 * j + e] = v[e];
+      for (int e = 0; e < 4; ++e) {
+        s[4 * j + e] = __builtin_amdgcn_frexp_mantf(v[e]);
+        x[4 * j + e] = __builtin_amdgcn_frexp_expf(v[e]);
+      }
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) b[e] = 0.f;
@@ -228,12 +235,24 @@ struct Columns {
     typedef typename Elem<OT>::T E;
     constexpr int W = Elem<OT>::kVec;
     typedef E Some __attribute__((ext_vector_type(W), aligned(sizeof(E))));  // (rows need no alignment)
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+    const float ms = __builtin_amdgcn_frexp_mantf(sx);
+    const int xs = __builtin_amdgcn_frexp_expf(sx);
+    float f[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      f[c] = __builtin_amdgcn_ldexpf(static_cast<float>(acc[c >> 2][c & 3]) * (ms * s[c]), xs + x[c]) + b[c];
     E v[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[4 * j + e] = f32_to_elem<OT>(static_cast<float>(acc[j][e]) * (sx * s[4 * j + e]) + b[4 * j + e]);
+    for (int c = 0; c < 16; c += 2) {
+      if constexpr (OT == SPK_BF16) {  // (two an instruction)
+        const uint32_t two = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{f[c], f[c + 1]}), B2));
+        v[c] = static_cast<E>(two), v[c + 1] = static_cast<E>(two >> 16);
+      } else {
+        v[c] = f32_to_elem<OT>(f[c]), v[c + 1] = f32_to_elem<OT>(f[c + 1]);
+      }
+    }
     E *out = static_cast<E *>(y) + at + col;
     if (col + 16 <= o.N) {
 #pragma unroll
