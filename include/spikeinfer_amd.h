@@ -748,7 +748,7 @@ int spk_evict(const SpkCacheLayer *layers, int nlayers, const int64_t cache_stri
  * rounded as fp32 is, but has no smallest or largest value of its own).  A row of x that holds
  * an infinity or a NaN gives a row of NaN, a row of W a column.
  *   w, x, bias, y  F32, F16 or BF16 each, channel stride 1, rows at their strides; rows of y
- *            must not lie on one another, nor y on x
+ *            must not lie on one another, nor y on x or bias (but one row of bias's type in place)
  *   packed   spk_linear_int8_packed_bytes(N, K) bytes, 16-byte aligned, and scales float
  *            [N rounded up to 64]: written by spk_linear_int8_pack, once per weight
  *   workspace spk_linear_int8_workspace_bytes(M, N, K) bytes, 16-byte aligned

@@ -140,4 +140,11 @@ inline bool on_one_another(const void *a, int64_t stride_a, int64_t n, const voi
   return in < n || in + m > stride_a;
 }
 
+// Whether n bytes lie on one of the rows of m bytes at one distance.
+inline bool on_rows(const void *a, int64_t n, const void *b, int64_t stride, int64_t m, int64_t rows) {
+  const int64_t d = reinterpret_cast<intptr_t>(a) - reinterpret_cast<intptr_t>(b);  // where a begins in b
+  if (d + n <= 0 || d >= (rows - 1) * stride + m) return false;
+  return stride <= 0 || d < 0 || d % stride < m || d % stride + n > stride;
+}
+
 }  // namespace spk

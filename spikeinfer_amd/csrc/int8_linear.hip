@@ -703,12 +703,16 @@ extern "C" int spk_linear_int8(const void *x, int x_dtype, int64_t x_stride, con
   if (!i8::launchable(M, N, static_cast<int>(i8::k_steps(K))))
     return fail(SPK_EUNSUPPORTED, "linear_int8: more threads than a launch has, M=%lld N=%d K=%d", (long long)M, N, K);
   if (!x || !packed || !scales || !y) return fail(SPK_EINVAL, "linear_int8: null pointer");
+  const int64_t yb = y_dtype == SPK_F32 ? 4 : 2, bb = bias_dtype == SPK_F32 ? 4 : 2;
+  // (one row in place is fine: a lane writes the columns whose biases it has read)
+  if (bias && !(M == 1 && bias == y && bias_dtype == y_dtype) && on_rows(bias, N * bb, y, y_stride * yb, N * yb, M))
+    return fail(SPK_EINVAL, "linear_int8: y lies on bias");
   const size_t need = spk_linear_int8_workspace_bytes(M, N, K);
   if (!workspace || workspace_bytes < need)
     return fail(SPK_EINVAL, "linear_int8: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if ((reinterpret_cast<uintptr_t>(packed) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return fail(SPK_EINVAL, "linear_int8: packed and workspace must be 16-byte aligned");
-  const int64_t xb = x_dtype == SPK_F32 ? 4 : 2, yb = y_dtype == SPK_F32 ? 4 : 2;
+  const int64_t xb = x_dtype == SPK_F32 ? 4 : 2;
   if (on_one_another(x, x_stride * xb, K * xb, y, y_stride * yb, N * yb, M))
     return fail(SPK_EINVAL, "linear_int8: y lies on x");
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -66,7 +66,8 @@ def linear_int8(x: torch.Tensor, w: Int8Weight, bias: torch.Tensor | None = None
         w: the weight, from :func:`pack_linear_int8`.
         bias: optional ``[N]`` of any of these types.
         out: optional ``[..., N]`` of any of these types, columns contiguous and rows one
-            distance apart; must not overlap x.  By default a new tensor of ``dtype`` (x's).
+            distance apart; must not overlap x, nor bias (but for one row in place). By default
+            a new tensor of ``dtype`` (x's).
         workspace: optional ``uint8`` scratch of :func:`linear_int8_workspace_bytes`; calls that
             may run at once need one each.
 
