@@ -796,7 +796,7 @@ int spk_sample_probs(const void *logits, int logits_dtype, int64_t row_stride, i
  *   uniforms float [rows] in [0, 1)
  *   targets  int64 [rows]: for rows of the path the token after them, as spk_accept_tree
  *            takes it, -1 for the other rows of a tree (and where p has no weight at all); rows
- *            of no sequence are left as they were
+ *            of no sequence are left as they were; the tokens themselves or apart from them
  *   workspace spk_verify_tree_workspace_bytes(N, V) bytes, 8-byte aligned
  * max_nodes <= 1024, N <= 65535.
  */

@@ -375,6 +375,9 @@ extern "C" int spk_verify_tree(const int64_t *tokens, const int32_t *parents, co
   if (N == 0 || rows == 0) return SPK_OK;
   if (!tokens || !parents || !target_probs || !draft_probs || !uniforms || !row_starts || !targets)
     return fail(SPK_EINVAL, "verify_tree: null pointer");
+  // (in place is fine: a tree's tokens are read before its targets are written)
+  if (targets != tokens && on_rows(targets, rows * 8, tokens, 0, rows * 8, 1))
+    return fail(SPK_EINVAL, "verify_tree: targets lie on other rows' tokens");
   const size_t need = spk_verify_tree_workspace_bytes(N, V);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
     return fail(SPK_EINVAL, "verify_tree: workspace of %zu bytes, %zu needed, aligned to 8", workspace ? workspace_bytes : 0,

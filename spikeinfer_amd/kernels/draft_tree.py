@@ -225,8 +225,8 @@ def verify_draft_tree(
             the token behind the path.
         distinct: a row's children were drawn without replacement (otherwise one independently of
             the other).
-        out: optional ``int64 [R]`` (needed for graph capture); rows of no sequence are left
-            as they were (-1 in a new tensor).
+        out: optional ``int64 [R]`` (needed for graph capture), ``tokens`` itself or apart from
+            them; rows of no sequence are left as they were (-1 in a new tensor).
         workspace: optional ``uint8`` scratch of :func:`verify_workspace_bytes`; calls that may run
             at once need one each.
 

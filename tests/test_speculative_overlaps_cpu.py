@@ -41,3 +41,19 @@ def test_the_result_on_its_bias(case):
 def test_a_bias_beside_the_result(case):
     rc, why = _linear(**case)
     assert rc == _lib.SPK_EINVAL and b"workspace" in why
+
+
+@pytest.mark.parametrize("shift", [1, 9, -1, -9])
+def test_targets_on_other_rows_tokens(shift):
+    lib = _lib.load()
+    rows = 10
+
+    def verify(out):
+        rc = lib.spk_verify_tree(P, 1 << 30, 1 << 31, 100, 1 << 32, 100, 1 << 33, 1 << 34, rows, 2, 8, 100, 0, out, P, 0, None)
+        return rc, lib.spk_last_error()
+
+    rc, why = verify(P + 8 * shift)
+    assert rc == _lib.SPK_EINVAL and b"targets lie on" in why
+    for beside in (P, P + 8 * rows, P - 8 * rows):
+        rc, why = verify(beside)
+        assert rc == _lib.SPK_EINVAL and b"workspace" in why

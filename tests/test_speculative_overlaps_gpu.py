@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from spikeinfer_amd.kernels import linear_int8, pack_linear_int8
+import speculative_ref as ref
+from spikeinfer_amd.kernels import linear_int8, pack_linear_int8, verify_draft_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +28,19 @@ def test_one_row_in_place_of_its_bias(gpu, N, K):
         rows[0, 1] = kept
         got = linear_int8(x, w8, rows[0, 1], out=rows[:, 0])
         assert torch.equal(got, linear_int8(x, w8, kept, dtype=dtype)) and torch.equal(rows[0, 1], kept)
+
+
+def test_targets_in_place_of_the_tokens(gpu):
+    """Hundreds of trees, each reading its own tokens only; shifted they are refused."""
+    case = ref.draft_case([7, 3, 12] * 200, 600, 5, 3)
+    d = {k: v.to(gpu) if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+    rows, used = len(case["tokens"]), int(case["row_starts"][-1])
+    want = verify_draft_tree(**d)
+    buffer = torch.zeros(rows + 5, dtype=torch.int64, device=gpu)
+    tokens = buffer[:rows]
+    tokens.copy_(d["tokens"])
+    with pytest.raises(ValueError, match="targets lie on"):
+        verify_draft_tree(**{**d, "tokens": tokens}, out=buffer[5:])
+    assert torch.equal(tokens, d["tokens"])
+    out = verify_draft_tree(**{**d, "tokens": tokens}, out=tokens)
+    assert torch.equal(out[:used], want[:used]) and torch.equal(out[used:], d["tokens"][used:])
