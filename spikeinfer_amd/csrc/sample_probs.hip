@@ -76,15 +76,18 @@ __device__ __forceinline__ u64 shfl_up_u64(u64 v, int d) {
 }
 
 // A logit over the temperature; what is finite stays finite (a mask of the type's lowest value
-// is no -infinity below a temperature of 1), what is infinite stays infinite (over an infinite
-// temperature too, where every other logit is 0).  inv = 1 / temp in fp64: the quotient of two
+// is no -infinity below a temperature of 1).  inv = inverse(temp): the quotient of two
 // fp32 numbers lies at least 2^-49 of itself from the middle between two fp32 numbers, and the
 // product is off by at most 2^-52, so its rounding is the quotient's (below 2^-126, where the
 // numbers have fewer bits, it may be the one beside it).
 __device__ __forceinline__ float quotient(float v, double inv) {
   const float x = static_cast<float>(static_cast<double>(v) * inv);
-  if (fabsf(v) == INFINITY) return v;
-  return fabsf(x) == INFINITY ? copysignf(kMost, v) : x;
+  return fabsf(x) == INFINITY && fabsf(v) != INFINITY ? copysignf(kMost, v) : x;
+}
+// 1 / temp in fp64; of an infinite temperature a number that makes every finite logit 0 in fp32
+// and leaves the infinite ones (0 would make them NaN).
+__device__ __forceinline__ double inverse(float temp) {
+  return temp < INFINITY ? 1.0 / static_cast<double>(temp) : 0x1p-400;
 }
 
 // A bound at or below every logit whose quotient is `x`, that of `bound`.
@@ -95,11 +98,12 @@ __device__ __forceinline__ float same_quotient(float bound, float x, float temp)
   return bound - fabsf(bound) * 0x1p-22f - temp * 0x1p-148f;
 }
 
-// exp(logit / temp - x_most) in fp32; the quotient with one correction (inv: fp32 of 1 / temp).
-__device__ __forceinline__ float power(float v, float temp, float inv, float x_most) {
+// exp(logit / temp - x_most) in fp32; the quotient with one correction (inv: fp32 of 1 / temp,
+// inv64 = inverse(temp)).
+__device__ __forceinline__ float power(float v, float temp, float inv, double inv64, float x_most) {
   const float q = v * inv;
   float x = __builtin_fmaf(__builtin_fmaf(-q, temp, v), inv, q);
-  x = fabsf(q) < 1e30f && temp < INFINITY ? x : quotient(v, 1.0 / static_cast<double>(temp));  // (and infinities, NaN)
+  x = fabsf(q) < 1e30f && temp < INFINITY ? x : quotient(v, inv64);  // (and infinities, NaN)
   return x == x ? expf(x == x_most ? 0.f : x - x_most) : 0.f;
 }
 
@@ -168,7 +172,7 @@ __device__ __forceinline__ Ask ask(const Args &a, int64_t r) {
   k.top_p = tp <= 0.f ? 0x1p-60f : tp;  // (the first token stays)
   const int tk = a.top_k ? a.top_k[r] : -1;
   k.top_k = tk > 0 && tk < a.V ? tk : 0;
-  k.inv = 1.0 / static_cast<double>(k.temp);
+  k.inv = inverse(k.temp);
   k.low = k.min_p > 0.f ? fmin(log(static_cast<double>(k.min_p)), 0.0) : -INFINITY;  // (the largest stays)
   k.open = k.top_p < 1.f;
   k.kind = !(k.temp >= kGreedyTemp) ? kGreedy : k.top_k || k.open || k.min_p > 0.f ? kCuts : kWhole;
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(kSliceThreads) void slice_kernel(Args a) {
   if (k.kind == kWhole) {
     const float inv = 1.f / k.temp;
     float z = 0.f;
-    each([&](int, float v) { z += power(v, k.temp, inv, x_most); });
+    each([&](int, float v) { z += power(v, k.temp, inv, k.inv, x_most); });
     const double all = sum(z);
     if (tid == 0) *head = Head{0, most, -INFINITY, all};
     return;
@@ -746,7 +750,7 @@ __device__ __forceinline__ void whole_row(const RowMem<DT> &mem, const Ask &k, f
   const int g0 = static_cast<int>(static_cast<int64_t>(groups) * part / parts);
   const int g1 = static_cast<int>(static_cast<int64_t>(groups) * (part + 1) / parts);
   const float inv = 1.f / k.temp;
-  auto value = [&](E e) { return power(elem_to_f32<DT>(e), k.temp, inv, x_most) * scale; };
+  auto value = [&](E e) { return power(elem_to_f32<DT>(e), k.temp, inv, k.inv, x_most) * scale; };
 #pragma unroll 4
   for (int g = g0 + static_cast<int>(threadIdx.x); g < g1; g += kRowThreads) {
     const E4 a = *reinterpret_cast<const E4 *>(mem.p + head + 4 * g);
