@@ -13,7 +13,7 @@
 // holds four columns of one row of y; a tile of W has four runs of four of a group of 64
 // output channels (tile j of a group: channels 16 q + 4 j + e in row 4 q + e), so that the
 // four tiles of a group give a lane 16 columns side by side, and a wave writes whole 128-byte
-// lines of y (8,188 x 9,728 of K = 64, nearly all stores: 67 -> 43 us).
+// lines of y (8,188 x 9,728 of K = 64, nearly all stores: 67 -> 43 us, 44 with any scales).
 #include <algorithm>
 #include <cmath>
 
@@ -145,8 +145,12 @@ __device__ __forceinline__ v4i quantise16(const Block<DT> &b, const Scale &sc) {
 // them in registers between the two (kKeep times; longer rows are read again).  WEIGHT: rows in
 // the order of the groups of output channels.  Rows that do not exist become zeros.  Bound by
 // reading x and by the latency of the two passes: 16,384 rows of 4,864 in bf16 56 us (239 MB read
-// and written, 4.3 TB/s), 8,188 of 896 10 us.  Few tiles by four rows a workgroup: 1,000 rows of 896
-// 4.8 us (by 16 rows 8.5), 333 of 777 4.8 (8.9).
+// and written, 4.3 TB/s), 8,188 of 896 9 us.  Up to 64 tiles by four rows a workgroup: 1,000 rows of 896
+// 4.8 us (by 16 rows 8.5), 333 of 777 4.8 (8.9).  The whole call with 896 columns by four and by
+// 16 rows, on both sides of that border, us: K = 896, 1,024 rows 12.2 and 12.7, 1,040 11.8 and
+// 12.5, 4,096 19.3 and 19.4, 16,384 34.9 and 35.8; K = 4,864, 64 rows 13.9 and 20.8, 1,024 22.0 and 28.2,
+// 1,040 22.9 and 28.1, 2,048 36.4 and 39.2, 4,096 53.9 and 52.1, 16,384 143 and 131: from 1,025 to about
+// 3,000 long rows the rule's side is the slower one, by up to 5 us.
 template <int DT, bool WEIGHT, int R>
 __global__ __launch_bounds__(64 * kRowWaves) void rows_kernel(const void *x, int64_t stride, int64_t rows, int K, int KS,
                                                               v4i *packed, float *scales) {
@@ -278,9 +282,10 @@ struct Columns {
 // FUSED (at most 16 rows): x is quantised here.  A wave loads the blocks of x that it
 // multiplies, the waves exchange the rows' largest magnitudes, and the integers are the
 // instruction's operand where they are made; W's first blocks are on their way meanwhile.
-// 4 x 1,152 x 896 5.2 us in place of 3.8 and 4.4 in two launches, 16 x 9,728 x 896 5.6 of 4.0 and
-// 4.3, 4 x 896 x 4,864 11.4 of 4.0 and 7.8 (16 rows: 15.4 of 5.8 and 7.8), each with a launch less to
-// wait for.  Sixteen waves for more than two steps of eight (4 x 896 x 4,864: eight 12.6).
+// 4 x 1,152 x 896 5.7 us in place of 3.8 and 4.4 in two launches, 16 x 9,728 x 896 5.9 of 4.0 and
+// 4.3, 4 x 896 x 4,864 12 of 4.0 and 7.8 (16 rows: 15.6 of 5.8 and 7.8), each with a launch less to
+// wait for.  With long rows few columns are few workgroups (14 for 896), which bounds these two.
+// Sixteen waves for more than two steps of eight (4 x 896 x 4,864: eight 12.6 where sixteen took 11.4).
 constexpr int kSplit = 8;
 
 // Adds up the waves' sums; wave i < TM has row tile i's afterwards.
@@ -591,7 +596,8 @@ void split(const v4i *xq, const float *xs, const v4i *wq, const Out &o, void *y,
                                                                                           KS, MT, NG);
 }
 // The kernel for a size: the least of the times, in us, that fits to measurements give (64 to 2,048
-// rows, 512 to 9,728 columns, K = 896 and 4,864; within a fifth, near their borders).  Measured,
+// rows, 512 to 9,728 columns, K = 896 and 4,864; within a fifth, near their borders; other sizes go by
+// the same lines, unmeasured).  Measured,
 // with one, two, four row tiles a workgroup of the split kernel and with large tiles: 64 x 896 x
 // 896 3.6, 4.1, 5.1, 9.1; 256 x 9,728 x 896 16.1, 12.5, 14.0, 12.4; 1,024 x 896 x 4,864 20.5,
 // 14.9, 12.9, 32.5; 2,048 x 4,864 x 896 57, 42, 44, 21.  From kWideColumns on large tiles whatever the

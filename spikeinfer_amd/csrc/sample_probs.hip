@@ -21,7 +21,15 @@
 // A row without cuts gets its sum from the first launch and its values from the second.
 // Many rows are bound by memory (320 of 151,936 in bf16: slices 64 us, 4.5 TB/s, rows 16), few by
 // the phases behind barriers (one row: 12 and 16 us, of which the weights in fp64 take 4 and 3).
-// The long way takes a workgroup about 190 us for 151,936 tokens.
+// The long way takes a workgroup 130 to 230 us for 151,936 tokens, and 750 and more where a cut has
+// to be found by digits.  Rows that go it, of bf16 logits:
+//   * nearly flat ones under top_p (a cut below the candidates), and top_k above kMostK;
+//   * masked ones, where fewer threads of a slice hold an allowed token than its bound asks for: the
+//     bound is the mask's value then, and every token of the slice is listed.  Five rows with 200 and
+//     2,000 tokens allowed: top_p 160 and 174 us, top_k of 50 242 and 17; with 20 allowed 158 and 763
+//     (fewer than top_k: the cut lies among the masked); with 20,000 25 and 19.  min_p escapes
+//     (13 to 18 us; with the type's lowest value as the mask and 20 allowed 65), rows without cuts too;
+//   * rows whose likely tokens lie in one slice: in descending order top_p 219 us, top_k of 50 253.
 #include <algorithm>
 #include <cmath>
 
@@ -524,11 +532,8 @@ __device__ __forceinline__ Place place(const u64 *key, const u64 *mass, int n) {
   return r;
 }
 
-// The cut as radix_cut finds it, among the n candidates in sh.key (sh.mass: their weights; by_count:
-// 1 each), of which those below `from` have none, x between `bottom` and `top` (where they are no
-// finite distance apart, the candidates are looked at).  Few are ranked one against the other.  Many go
-// into bins of equal width in x first, and those of the bin that holds the cut are ranked; where
-// that is too many as well (equal logits), by digits.
+// The cut as radix_cut finds it among at most kRank candidates, ranked one against the other; those
+// below `from` have no weight, by_count: 1 each.
 __device__ __forceinline__ u64 rank_cut(RowShared &sh, const u64 *key, const u64 *mass, int n, bool by_count, u64 from,
                                         u64 base, double target) {
   if (threadIdx.x == 0) sh.pick = 0;
@@ -542,6 +547,11 @@ __device__ __forceinline__ u64 rank_cut(RowShared &sh, const u64 *key, const u64
   __syncthreads();
   return sh.pick;
 }
+// The cut as radix_cut finds it, among the n candidates in sh.key (sh.mass: their weights; by_count:
+// 1 each), of which those below `from` have none, x between `bottom` and `top` (where they are no
+// finite distance apart, the candidates are looked at).  Few are ranked.  Many go into bins of equal
+// width in x first, and those of the bin that holds the cut are ranked; where that is too many as
+// well (equal logits), by digits.
 __device__ __forceinline__ u64 cand_cut(RowShared &sh, int n, bool by_count, u64 from, u64 base, double target, float top,
                                         float bottom) {
   if (n <= kRank) return rank_cut(sh, sh.key, sh.mass, n, by_count, from, base, target);
@@ -978,7 +988,8 @@ void launch(Args a, int rows, void *workspace, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>(rows) * p.S;
   slice_kernel<DT><<<grid, kSliceThreads, 0, s>>>(a);
   // Two workgroups a CU (256 CUs), which rows without cuts use, and two a row at least: 247 rows of
-  // 151,936 in bf16 88 us (103 with one, 93 with four a row), 320 rows 122 us (135 with one).
+  // 151,936 in bf16 88 us (103 with one, 93 with four a row), 320 rows 122 us (135 with one).  (Both before
+  // slices of 12,288 16-bit logits; with them 79 and 104.)
   a.groups = std::min(p.S, std::max(2, 512 / rows));
   row_kernel<DT><<<static_cast<unsigned>(rows) * a.groups, kRowThreads, 0, s>>>(a);
 }

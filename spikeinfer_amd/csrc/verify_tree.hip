@@ -34,11 +34,16 @@ constexpr int kMaxRounds = 4;
 
 // Launches of slices.  A chain needs one sum, a tree one a rejected sibling, a few as a rule.
 // Those that are left to the last launch take one workgroup: 5 to 10 us each at 151,936 tokens,
-// 2 at 32,000; a launch that finds every tree done takes 2 to 3.  One launch against three, us:
-// 16 trees of 25 nodes at 151,936 tokens 56 and 36, 14 of 8 nodes with up to 3 siblings 52 and
-// 36, 64 chains of 8 nodes 27 and 30, one chain of 5 15 and 21; 7 trees of 13 nodes at 32,003
-// 20 and 28.  (Which of them it is the host does not know: few nodes are chains as a rule.)  Three,
-// four and five over 25 draws of the 16 trees: 39.1, 37.8, 40.5, the slowest 59, 48, 51.
+// 2 at 32,000; a launch that finds every tree done takes 2 to 3.  One launch against four, us (medians
+// of five draws, in brackets the slowest), of 5, 8, 9, 12, 16 and 25 nodes alike:
+//   151,936 tokens: one chain 14 and 19; one tree with up to 3 siblings 14 (32) and 19 (32); 16 chains
+//   16-18 and 20-22, 16 trees 52-55 (73) and 34-37 (46); 64 chains 26-27 and 31-32, 64 trees 57-58
+//   (72) and 47-49 (61).
+//   32,000 tokens: one chain 14 and 19; 16 chains 15-16 and 20-21, 16 trees 26-27 (38) and 32-35 (48).
+// So siblings decide, and only over large vocabularies and in batches.  The host knows nodes alone:
+// above 8 it takes trees for granted.  Where that is wrong, batches of smaller trees lose 9 to 18 us,
+// longer chains and single trees 5.  Three, four and five launches over 25 draws of 16 trees of 25
+// nodes: 39.1, 37.8, 40.5, the slowest 59, 48, 51.
 inline int rounds_for(int max_nodes, int V) { return max_nodes > 8 && V >= 65536 ? kMaxRounds : 1; }
 
 struct Params {
